@@ -472,6 +472,134 @@ int safetensors_write_file_q4_0(const char *path, const jjo_host_tensor *tensors
 int safetensors_quantize_q4_0(const char *in_path, const char *out_path, const char *const *names, int num_names,
                               int num_threads);
 
+/* ------------------------------------------------------------------ MXFP4
+ * The OCP microscaling 4-bit floating point format beside Q4_0: the format that gfx950's
+ * matrix cores multiply directly.  No counterpart in the reference (its only quantized
+ * weights are block_q4_0, src/cuda/mm_q4_0_q8_1.cu:35-38).
+ *
+ * MXFP4 matrix [rows][cols], cols a multiple of 32, 16-byte aligned:
+ *     codes : rows*cols/2 bytes; element 2j of a row in the low nibble of its byte j,
+ *             element 2j+1 in the high one; e2m1: sign, then 0 0.5 1 1.5 2 3 4 6
+ *     scales: rows*cols/32 bytes behind them, [rows][cols/32], e8m0:
+ *             value = e2m1 * 2^(s - 127); s = 255: the block is NaN
+ * Stacked expert matrices are one matrix of E*rows rows.
+ * Conversion (the format's own rule): s = 2^(floor(log2 max|x|) - 2) over the block, at least
+ * 2^-127; x / s rounded to nearest even, at most 6 in magnitude.  A block that holds a NaN or
+ * an infinity gets s = 255 and zero codes.
+ * Activations and outputs are fp32, fp16 or bf16 (JJO_DTYPE_*), 16-byte aligned and contiguous
+ * unless a row stride is given; all sums are fp32, outputs rounded once.
+ */
+#define JJO_DTYPE_F32 0
+#define JJO_DTYPE_F16 1
+#define JJO_DTYPE_BF16 2
+
+/* Bytes of a [rows, cols] MXFP4 matrix (rows*cols/32*17); -1 unless rows > 0 and cols is a
+ * positive multiple of 32. */
+int64_t mxfp4_bytes(int64_t rows, int64_t cols);
+
+/*
+ * rows of `dtype` -> MXFP4 and back.  row_stride: elements from one row of x (or y) to the next,
+ * at least cols; with more than one row, row_stride * element size must be a multiple of 16.
+ * One launch, asynchronous on `stream`.  y receives the values rounded to `dtype` (nearest
+ * even); y's elements between the rows are not written.
+ */
+int quantize_mxfp4_device(void *stream, const void *x, int dtype, int64_t row_stride, void *out, int64_t rows,
+                          int64_t cols);
+int dequantize_mxfp4_device(void *stream, const void *q, void *y, int dtype, int64_t row_stride, int64_t rows,
+                            int64_t cols);
+
+/*
+ * y[t][n] = sum_k x[t][k] * w[n][k], both operands MXFP4 (x: [batch][ncols_k], w:
+ * [nrows_out][ncols_k]), y of y_dtype [batch][nrows_out]; the MXFP4 sibling of
+ * mat_mul_q4_0_q8_1_device.  No allocation, asynchronous.
+ */
+int mat_mul_mxfp4_device(const void *d_w, const void *d_x_mxfp4, void *d_y, int y_dtype, int ncols_k, int nrows_out,
+                         int batch, void *stream);
+
+/*
+ * Engine linear layer with MXFP4 weights, beside linear_q4_0_forward_device: quantizes the
+ * activation (num_tokens rows of in_dtype) to MXFP4 and multiplies; output of out_dtype.
+ * quant_workspace: linear_mxfp4_workspace_bytes(in_features, num_tokens) bytes of device memory,
+ * 16-byte aligned (may be NULL when that is 0: one token with in_features at most 16384, which is
+ * quantized inside the product).  in_features must be a multiple of 32.
+ */
+int64_t linear_mxfp4_workspace_bytes(int in_features, int num_tokens);
+int linear_mxfp4_forward_device(void *stream, void *quant_workspace, const void *input, int in_dtype,
+                                const void *weight, void *output, int out_dtype, int in_features, int out_features,
+                                int num_tokens);
+
+/*
+ * Grouped (MoE expert) products of rows sorted by expert, beside
+ * mat_mul_q4_0_q8_1_grouped_device: expert e's rows are expert_offsets[e]..expert_offsets[e+1]
+ * of x ([n_routes][ncols_k] MXFP4) and its weight is rows e*nrows_out.. of w.  Row r's output
+ * goes to row route_dst[r] of y (NULL: r).  expert_offsets (device, n_experts + 1 entries,
+ * non-decreasing, first 0) may end below n_routes: the rows behind the last expert's are not
+ * read and their outputs not written.  Ranges are clamped to [0, n_routes]; route_dst is not
+ * checked.
+ */
+int mat_mul_mxfp4_grouped_device(const void *d_w, const void *d_x_mxfp4, const int32_t *d_expert_offsets,
+                                 int n_experts, const int32_t *d_route_dst, void *d_y, int y_dtype, int ncols_k,
+                                 int nrows_out, int n_routes, void *stream);
+
+/*
+ * gate|up projection with SwiGLU and the MXFP4 conversion of its result in one grouped launch:
+ * mid [n_routes][intermediate_size] MXFP4 = silu(x . w_gate) * (x . w_up), beside
+ * moe_q4_0_gate_up_swiglu_q8_1_device.  Both sizes are multiples of 32.
+ */
+int moe_mxfp4_gate_up_swiglu_device(void *stream, const void *w_gate, const void *w_up, const void *x_mxfp4_permuted,
+                                    const int32_t *expert_offsets, int num_experts, void *mid_mxfp4, int hidden_size,
+                                    int intermediate_size, int n_routes);
+
+/*
+ * The whole MoE FFN with MXFP4 experts, beside moe_q4_0_ffn_forward_device: x, y of `dtype`
+ * [T][H], logits fp32 [T][E]; w_gate, w_up [E*I][H], w_down [E*H][I].  top_k <= min(32, E), E <= 1024,
+ * H and I multiples of 32.  `workspace` (256-byte aligned) holds every intermediate; it may be
+ * used again by the next call on the same stream.
+ */
+int64_t moe_mxfp4_ffn_workspace_bytes(int num_tokens, int hidden_size, int intermediate_size, int num_experts,
+                                      int top_k);
+int moe_mxfp4_ffn_forward_device(void *stream, const void *x, const float *logits, const void *w_gate,
+                                 const void *w_up, const void *w_down, void *y, int dtype, int num_tokens,
+                                 int hidden_size, int intermediate_size, int num_experts, int top_k, void *workspace,
+                                 int64_t workspace_bytes);
+
+/* ------------------------------------------------------------------ rows sorted by expert
+ * Token rows (fp32, fp16 or bf16) to their experts and back, with the gradients: the float
+ * siblings of moe_dispatch_q8_1_device and moe_combine_device.  R = num_tokens * top_k routes
+ * r = t*top_k + k.  A route whose expert id is outside [0, num_experts) is dropped (a padded
+ * token, an expert of another process): dst_of_route is -1, it has no sorted row.
+ * num_experts <= 1024, top_k <= 32; hidden_size is any positive number.
+ */
+
+/*
+ * Replaces the dispatch of fp32 rows (src/cuda/moe/moe_dispatch_sota.cu:45-95): expert_offsets
+ * [E+1], src_route[p] = the route at sorted row p, dst_of_route[r] = its row or -1, and
+ * x_sorted[p] = x[src_route[p] / top_k].  Rows and src_route entries behind expert_offsets[E]
+ * are left as they were.
+ */
+int moe_dispatch_rows_device(void *stream, const int32_t *expert_ids, const void *x, int dtype, int num_tokens,
+                             int top_k, int hidden_size, int num_experts, int32_t *expert_offsets,
+                             int32_t *src_route, int32_t *dst_of_route, void *x_sorted);
+/* grad_x[t] = sum over k of grad_sorted[dst_of_route[t, k]] (zero where every route is dropped). */
+int moe_dispatch_rows_backward_device(void *stream, const void *grad_sorted, int dtype, const int32_t *dst_of_route,
+                                      void *grad_x, int num_tokens, int hidden_size, int top_k);
+
+/*
+ * y[t] = sum over k of route_weights[t, k] * expert_out[dst_of_route[t, k]], in k order
+ * (src/cuda/moe/moe_combine_sota.cu:7-42); route_weights fp32.
+ */
+int moe_combine_rows_device(void *stream, const void *expert_out, int dtype, const int32_t *dst_of_route,
+                            const float *route_weights, void *y, int num_tokens, int hidden_size, int top_k);
+/*
+ * Its gradients: grad_expert_out[dst_of_route[t, k]] = route_weights[t, k] * grad_y[t] and
+ * grad_route_weights[t, k] = <grad_y[t], expert_out[dst_of_route[t, k]]> (fp32; 0 for a dropped
+ * route).  No two routes may share a row (as moe_dispatch_rows_device gives them); rows that no
+ * route has are left as they were.
+ */
+int moe_combine_rows_backward_device(void *stream, const void *grad_y, const void *expert_out, int dtype,
+                                     const int32_t *dst_of_route, const float *route_weights, void *grad_expert_out,
+                                     float *grad_route_weights, int num_tokens, int hidden_size, int top_k);
+
 #ifdef __cplusplus
 }
 #endif

@@ -82,7 +82,26 @@ EXPORTED_SYMBOLS = (
     "q4_0_to_split_device",
     "mat_mul_q4_0s_q8_1_device",
     "mat_mul_q4_0s_q8_1_f32_device",
+    "mxfp4_bytes",
+    "quantize_mxfp4_device",
+    "dequantize_mxfp4_device",
+    "mat_mul_mxfp4_device",
+    "linear_mxfp4_workspace_bytes",
+    "linear_mxfp4_forward_device",
+    "mat_mul_mxfp4_grouped_device",
+    "moe_mxfp4_gate_up_swiglu_device",
+    "moe_mxfp4_ffn_workspace_bytes",
+    "moe_mxfp4_ffn_forward_device",
+    "moe_dispatch_rows_device",
+    "moe_dispatch_rows_backward_device",
+    "moe_combine_rows_device",
+    "moe_combine_rows_backward_device",
 )
+
+DTYPE_F32 = 0
+DTYPE_F16 = 1
+DTYPE_BF16 = 2
+MX_BLOCK_BYTES = 17
 
 WEIGHT_DTYPE_F32 = 0
 WEIGHT_DTYPE_Q4_0 = 1
@@ -216,6 +235,34 @@ def lib() -> ctypes.CDLL:
         L.mat_mul_q4_0s_q8_1_device.argtypes = [vp, vp, vp, i32, i32, i32, vp]
         L.mat_mul_q4_0s_q8_1_f32_device.restype = i32
         L.mat_mul_q4_0s_q8_1_f32_device.argtypes = [vp, vp, vp, vp, i32, i32, i32, vp]
+        L.mxfp4_bytes.restype = i64
+        L.mxfp4_bytes.argtypes = [i64, i64]
+        L.quantize_mxfp4_device.restype = i32
+        L.quantize_mxfp4_device.argtypes = [vp, vp, i32, i64, vp, i64, i64]
+        L.dequantize_mxfp4_device.restype = i32
+        L.dequantize_mxfp4_device.argtypes = [vp, vp, vp, i32, i64, i64, i64]
+        L.mat_mul_mxfp4_device.restype = i32
+        L.mat_mul_mxfp4_device.argtypes = [vp, vp, vp, i32, i32, i32, i32, vp]
+        L.linear_mxfp4_workspace_bytes.restype = i64
+        L.linear_mxfp4_workspace_bytes.argtypes = [i32, i32]
+        L.linear_mxfp4_forward_device.restype = i32
+        L.linear_mxfp4_forward_device.argtypes = [vp, vp, vp, i32, vp, vp, i32, i32, i32, i32]
+        L.mat_mul_mxfp4_grouped_device.restype = i32
+        L.mat_mul_mxfp4_grouped_device.argtypes = [vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, vp]
+        L.moe_mxfp4_gate_up_swiglu_device.restype = i32
+        L.moe_mxfp4_gate_up_swiglu_device.argtypes = [vp, vp, vp, vp, vp, i32, vp, i32, i32, i32]
+        L.moe_mxfp4_ffn_workspace_bytes.restype = i64
+        L.moe_mxfp4_ffn_workspace_bytes.argtypes = [i32, i32, i32, i32, i32]
+        L.moe_mxfp4_ffn_forward_device.restype = i32
+        L.moe_mxfp4_ffn_forward_device.argtypes = [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, i64]
+        L.moe_dispatch_rows_device.restype = i32
+        L.moe_dispatch_rows_device.argtypes = [vp, vp, vp, i32, i32, i32, i32, i32, vp, vp, vp, vp]
+        L.moe_dispatch_rows_backward_device.restype = i32
+        L.moe_dispatch_rows_backward_device.argtypes = [vp, vp, i32, vp, vp, i32, i32, i32]
+        L.moe_combine_rows_device.restype = i32
+        L.moe_combine_rows_device.argtypes = [vp, vp, i32, vp, vp, vp, i32, i32, i32]
+        L.moe_combine_rows_backward_device.restype = i32
+        L.moe_combine_rows_backward_device.argtypes = [vp, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32]
         _lib = L
     return _lib
 
@@ -574,3 +621,236 @@ def moe_ffn(x, logits, w_gate, w_up, w_down, y, num_tokens: int, hidden: int, in
               _dev(w_down, "w_down"), _dev(y, "y"), num_tokens, hidden, inter, num_experts, top_k, _dev(ws, "ws"),
               ws.numel() * ws.element_size()),
            "moe_q4_0s_ffn_forward_device" if split else "moe_q4_0_ffn_forward_device")
+
+
+# ---------------------------------------------------------------- MXFP4 and sorted rows
+# The entries of csrc/bind_linear.cpp by their places in its table.
+(_QUANTIZE, _DEQUANTIZE, _MAT_MUL, _LINEAR, _GROUPED, _GATE_UP, _FFN, _DISPATCH, _DISPATCH_BACKWARD, _COMBINE,
+ _COMBINE_BACKWARD) = range(11)
+_entry_native = None
+_dtypes = None
+
+
+def _entry(which: int, where: str, stream, *args) -> None:
+    """A C entry through the native binding: tensors must be contiguous and on the current device."""
+    global _entry_native
+    if _entry_native is None:
+        lib()  # the same loud failure where nothing is built
+        from ._linear import entry
+        _entry_native = entry
+    rc = _entry_native(which, _current_stream, _current_device, stream, *args)
+    if rc != JJO_OK:
+        _check(rc, where)
+
+
+def _current_device() -> int:
+    return _torch.cuda.current_device()
+
+
+def _load_torch() -> None:
+    global _dtypes, _torch
+    import torch
+    _torch = torch
+    _dtypes = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
+
+
+def _dtype(t, name: str) -> int:
+    """JJO_DTYPE_* of a float32, float16 or bfloat16 tensor."""
+    if _dtypes is None:
+        _load_torch()
+    d = _dtypes.get(t.dtype)
+    if d is None:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16")
+    return d
+
+
+def _same_dtype(name: str, d: int, t) -> None:
+    if _dtypes.get(t.dtype) != d:
+        raise ValueError(f"{name} must have the dtype of the other rows")
+
+
+def _room(name: str, t, n: int) -> None:
+    """t holds at least n elements."""
+    if t.numel() < n:
+        raise ValueError(f"{name} is too small: {t.numel()} elements, need {n}")
+
+
+def _mx_room(name: str, t, rows: int, cols: int) -> None:
+    """t holds a [rows, cols] MXFP4 matrix (an invalid shape is the entry's to refuse)."""
+    if t.numel() * t.element_size() < rows * (cols // QK) * MX_BLOCK_BYTES:
+        raise ValueError(f"{name} is too small for a [{rows}, {cols}] MXFP4 matrix")
+
+
+def _typed(name: str, t, dtype, n: int) -> None:
+    if t.dtype != dtype or t.numel() < n:
+        raise ValueError(f"{name} must be {dtype} with {n} elements")
+
+
+def _rows_of(t, name: str, rows: int, cols: int):
+    """(argument, row stride) of rows x cols values: a contiguous tensor, or a 2-D one whose
+    rows are contiguous."""
+    if t.is_contiguous():
+        _room(name, t, rows * cols)
+        return t, cols
+    if t.dim() != 2 or t.stride(1) != 1 or t.shape[0] < rows or t.shape[1] < cols or (rows > 1 and t.stride(0) < cols):
+        raise ValueError(f"{name} must be contiguous, or [rows, cols] with contiguous rows that do not overlap")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    if t.get_device() != _current_device():
+        raise ValueError(f"{name} is on device {t.get_device()}, the current device is {_current_device()}")
+    return t.data_ptr(), t.stride(0)
+
+
+def mxfp4_bytes(rows: int, cols: int) -> int:
+    """Bytes of a [rows, cols] MXFP4 matrix; -1 if invalid."""
+    return int(lib().mxfp4_bytes(rows, cols))
+
+
+def quantize_mxfp4(x, out, rows: int, cols: int, stream=None) -> None:
+    """out = MXFP4 of x [rows, cols] (float32, float16 or bfloat16; rows may be strided)."""
+    d = _dtype(x, "x")
+    p, row_stride = _rows_of(x, "x", rows, cols)
+    _mx_room("out", out, rows, cols)
+    _entry(_QUANTIZE, "quantize_mxfp4_device", stream, p, d, row_stride, out, rows, cols)
+
+
+def dequantize_mxfp4(q, y, rows: int, cols: int, stream=None) -> None:
+    """y [rows, cols] (float32, float16 or bfloat16; rows may be strided) = the values of q."""
+    d = _dtype(y, "y")
+    p, row_stride = _rows_of(y, "y", rows, cols)
+    _mx_room("q", q, rows, cols)
+    _entry(_DEQUANTIZE, "dequantize_mxfp4_device", stream, q, p, d, row_stride, rows, cols)
+
+
+def mat_mul_mxfp4(w, xq, y, K: int, N: int, M: int, stream=None) -> None:
+    """y[M, N] = MXFP4 xq [M, K] . MXFP4 w [N, K]^T."""
+    d = _dtype(y, "y")
+    _room("y", y, M * N)
+    _mx_room("w", w, N, K)
+    _mx_room("xq", xq, M, K)
+    _entry(_MAT_MUL, "mat_mul_mxfp4_device", stream, w, xq, y, d, K, N, M)
+
+
+def linear_mxfp4_workspace_bytes(in_features: int, num_tokens: int) -> int:
+    return int(lib().linear_mxfp4_workspace_bytes(in_features, num_tokens))
+
+
+def linear_mxfp4(x, w, y, in_features: int, out_features: int, num_tokens: int, ws=None, stream=None) -> None:
+    """linear_mxfp4_forward_device: y [T, out] = MXFP4(x [T, in]) . w [out, in]^T; x and y in
+    float32, float16 or bfloat16, ws of linear_mxfp4_workspace_bytes."""
+    dx, dy = _dtype(x, "x"), _dtype(y, "y")
+    _room("x", x, num_tokens * in_features)
+    _room("y", y, num_tokens * out_features)
+    _mx_room("w", w, out_features, in_features)
+    if ws is not None and ws.numel() * ws.element_size() < lib().linear_mxfp4_workspace_bytes(in_features, num_tokens):
+        raise ValueError("ws is smaller than linear_mxfp4_workspace_bytes")
+    _entry(_LINEAR, "linear_mxfp4_forward_device", stream, ws, x, dx, w, y, dy, in_features, out_features, num_tokens)
+
+
+def grouped_mat_mul_mxfp4(w, xq, expert_offsets, y, K: int, N: int, n_routes: int, route_dst=None,
+                          stream=None) -> None:
+    """mat_mul_mxfp4_grouped_device: rows sorted by expert times their experts' weights."""
+    d = _dtype(y, "y")
+    n_experts = expert_offsets.numel() - 1
+    _typed("expert_offsets", expert_offsets, _torch.int32, 2)
+    if route_dst is not None:
+        _typed("route_dst", route_dst, _torch.int32, n_routes)
+    else:
+        _room("y", y, n_routes * N)
+    _mx_room("w", w, n_experts * N, K)
+    _mx_room("xq", xq, n_routes, K)
+    _entry(_GROUPED, "mat_mul_mxfp4_grouped_device", stream, w, xq, expert_offsets, n_experts, route_dst, y, d, K, N,
+           n_routes)
+
+
+def moe_gate_up_swiglu_mxfp4(w_gate, w_up, xq_perm, offsets, num_experts: int, mid_q, hidden: int, inter: int,
+                             n_routes: int, stream=None) -> None:
+    """mid_q [n_routes, inter] = MXFP4 of silu(x . w_gate) * (x . w_up) of rows sorted by expert."""
+    _mx_room("w_gate", w_gate, num_experts * inter, hidden)
+    _mx_room("w_up", w_up, num_experts * inter, hidden)
+    _mx_room("xq_perm", xq_perm, n_routes, hidden)
+    _mx_room("mid_q", mid_q, n_routes, inter)
+    if _dtypes is None:
+        _load_torch()
+    _typed("offsets", offsets, _torch.int32, num_experts + 1)
+    _entry(_GATE_UP, "moe_mxfp4_gate_up_swiglu_device", stream, w_gate, w_up, xq_perm, offsets, num_experts, mid_q,
+           hidden, inter, n_routes)
+
+
+def moe_ffn_mxfp4_workspace_bytes(num_tokens: int, hidden: int, inter: int, num_experts: int, top_k: int) -> int:
+    return int(lib().moe_mxfp4_ffn_workspace_bytes(num_tokens, hidden, inter, num_experts, top_k))
+
+
+def moe_ffn_mxfp4(x, logits, w_gate, w_up, w_down, y, num_tokens: int, hidden: int, inter: int, num_experts: int,
+                  top_k: int, ws, stream=None) -> None:
+    """The MoE FFN with MXFP4 experts: x and y [T, hidden] of one dtype, logits float32 [T, E]."""
+    d = _dtype(x, "x")
+    _same_dtype("y", d, y)
+    _room("x", x, num_tokens * hidden)
+    _room("y", y, num_tokens * hidden)
+    _typed("logits", logits, _torch.float32, num_tokens * num_experts)
+    _mx_room("w_gate", w_gate, num_experts * inter, hidden)
+    _mx_room("w_up", w_up, num_experts * inter, hidden)
+    _mx_room("w_down", w_down, num_experts * hidden, inter)
+    _entry(_FFN, "moe_mxfp4_ffn_forward_device", stream, x, logits, w_gate, w_up, w_down, y, d, num_tokens, hidden,
+           inter, num_experts, top_k, ws, ws.numel() * ws.element_size())
+
+
+def moe_dispatch_rows(ids, x, x_sorted, offsets, src_route, dst_of_route, num_tokens: int, top_k: int, hidden: int,
+                      num_experts: int, stream=None) -> None:
+    """Rows of x [T, hidden] to their experts: x_sorted[p] = x[src_route[p] // top_k], and the
+    tables; a route with an id outside [0, num_experts) is dropped (dst_of_route -1)."""
+    d = _dtype(x, "x")
+    _same_dtype("x_sorted", d, x_sorted)
+    r = num_tokens * top_k
+    i32 = _torch.int32
+    _typed("ids", ids, i32, r)
+    _typed("offsets", offsets, i32, num_experts + 1)
+    _typed("src_route", src_route, i32, r)
+    _typed("dst_of_route", dst_of_route, i32, r)
+    _room("x", x, num_tokens * hidden)
+    _room("x_sorted", x_sorted, r * hidden)
+    _entry(_DISPATCH, "moe_dispatch_rows_device", stream, ids, x, d, num_tokens, top_k, hidden, num_experts, offsets,
+           src_route, dst_of_route, x_sorted)
+
+
+def moe_dispatch_rows_backward(grad_sorted, dst_of_route, grad_x, num_tokens: int, hidden: int, top_k: int,
+                               stream=None) -> None:
+    """grad_x [T, hidden] = the sum of each token's sorted rows of grad_sorted."""
+    d = _dtype(grad_sorted, "grad_sorted")
+    _same_dtype("grad_x", d, grad_x)
+    _typed("dst_of_route", dst_of_route, _torch.int32, num_tokens * top_k)
+    _room("grad_sorted", grad_sorted, num_tokens * top_k * hidden)
+    _room("grad_x", grad_x, num_tokens * hidden)
+    _entry(_DISPATCH_BACKWARD, "moe_dispatch_rows_backward_device", stream, grad_sorted, d, dst_of_route, grad_x,
+           num_tokens, hidden, top_k)
+
+
+def moe_combine_rows(expert_out, dst_of_route, weights, y, num_tokens: int, hidden: int, top_k: int,
+                     stream=None) -> None:
+    """y [T, hidden] = sum over k of weights[t, k] * expert_out[dst_of_route[t, k]]."""
+    d = _dtype(expert_out, "expert_out")
+    _same_dtype("y", d, y)
+    _typed("dst_of_route", dst_of_route, _torch.int32, num_tokens * top_k)
+    _typed("weights", weights, _torch.float32, num_tokens * top_k)
+    _room("expert_out", expert_out, num_tokens * top_k * hidden)
+    _room("y", y, num_tokens * hidden)
+    _entry(_COMBINE, "moe_combine_rows_device", stream, expert_out, d, dst_of_route, weights, y, num_tokens, hidden,
+           top_k)
+
+
+def moe_combine_rows_backward(grad_y, expert_out, dst_of_route, weights, grad_expert_out, grad_weights,
+                              num_tokens: int, hidden: int, top_k: int, stream=None) -> None:
+    """The combine's gradients: grad_expert_out[dst] = weight * grad_y[t], grad_weights[t, k] = <grad_y[t], row>."""
+    d = _dtype(grad_y, "grad_y")
+    _same_dtype("expert_out", d, expert_out)
+    _same_dtype("grad_expert_out", d, grad_expert_out)
+    r = num_tokens * top_k
+    _typed("dst_of_route", dst_of_route, _torch.int32, r)
+    _typed("weights", weights, _torch.float32, r)
+    _typed("grad_weights", grad_weights, _torch.float32, r)
+    _room("grad_y", grad_y, num_tokens * hidden)
+    _room("expert_out", expert_out, r * hidden)
+    _room("grad_expert_out", grad_expert_out, r * hidden)
+    _entry(_COMBINE_BACKWARD, "moe_combine_rows_backward_device", stream, grad_y, expert_out, d, dst_of_route, weights,
+           grad_expert_out, grad_weights, num_tokens, hidden, top_k)

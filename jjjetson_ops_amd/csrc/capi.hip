@@ -342,6 +342,8 @@ __global__ __launch_bounds__(256) void read_floor_kernel(const uint4 *__restrict
 
 int device_cu_count() { return device_cus(); }
 
+int require_device() { return require_gfx950(); }
+
 hipError_t launch_block_sums(const void *w, const void *xq, int32_t *sumi, int K, int N, int M,
                              hipStream_t stream) {
     const int64_t total = (int64_t)M * N * (K / kQK);

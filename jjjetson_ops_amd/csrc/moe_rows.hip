@@ -1,0 +1,403 @@
+// Token rows (fp32, fp16, bf16) to their experts and back on gfx950, and the gradients.
+//
+//   sort      pos(r) = #{live r' : e(r') < e(r)} + #{live r' < r : e(r') = e(r)}, the order of
+//             moe_dispatch_kernel; a route whose id is outside [0, E) is dropped (dst -1)
+//   dispatch  rows[pos(r)] = x[r / top_k]
+//   its gradient          gx[t] = sum over k of g[dst(t, k)]
+//   combine   y[t] = sum over k of w(t, k) rows[dst(t, k)]
+//   its gradients         grows[dst(t, k)] = w(t, k) gy[t],  gw(t, k) = <gy[t], rows[dst(t, k)]>
+//
+// All of it is bound by HBM once there are some hundred rows and by latency below: a row is
+// moved in 16-byte pieces where its length allows, sums are fp32 in k order (one rounding, at
+// the store), and nothing is added with atomics, so a result does not depend on timing.
+#include <hip/hip_runtime.h>
+
+#include "mxfp4_common.hpp"
+
+namespace jjo {
+namespace {
+
+constexpr int kSortMax = 4096;  // routes that every workgroup of the dispatch counts by itself
+
+__device__ __forceinline__ bool live_id(int e, int n_experts) { return (unsigned)e < (unsigned)n_experts; }
+
+__device__ __forceinline__ int wave_total(int v) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+// Exclusive bases of the experts' counts in s_cnt[0..1023] (n_experts <= 1024), by 256 threads
+// of one workgroup: thread i takes entries 4i..4i+3.  s_part: four ints.
+__device__ __forceinline__ void expert_bases(int *s_cnt, int *s_part) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int c[4], tot = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tot += c[i] = s_cnt[4 * tid + i];
+    int incl = tot;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(incl, d);
+        if (lane >= d) incl += o;
+    }
+    if (lane == 63) s_part[wave] = incl;
+    __syncthreads();
+    int base = incl - tot;
+    for (int w = 0; w < wave; ++w) base += s_part[w];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        s_cnt[4 * tid + i] = base;
+        base += c[i];
+    }
+    __syncthreads();
+}
+
+// ---- dispatch of up to kSortMax routes in one launch.  Workgroup (t + 1, c) has its piece of
+// token t's row in flight, counts for each of the token's routes the routes that sort before
+// it (16 compares a thread and route at most) and stores the piece at each position;
+// workgroup 0 counts the experts' offsets.
+template <class U>
+__global__ __launch_bounds__(256) void dispatch_rows_kernel(const int32_t *__restrict__ ids, const U *__restrict__ x,
+                                                            int R, int top_k, int units, int n_experts,
+                                                            int32_t *__restrict__ offsets,
+                                                            int32_t *__restrict__ src_route,
+                                                            int32_t *__restrict__ dst_of_route, U *__restrict__ rows) {
+    constexpr int kIds = kSortMax / 256, kUnits = 4;
+    __shared__ int s_cnt[1024];
+    __shared__ int s_part[4][32];
+    __shared__ int s_pos[32];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (blockIdx.x == 0) {
+        if (blockIdx.y != 0) return;
+        for (int e = tid; e < 1024; e += 256) s_cnt[e] = 0;
+        __syncthreads();
+        for (int r = tid; r < R; r += 256) {
+            const int e = ids[r];
+            if (live_id(e, n_experts)) atomicAdd(&s_cnt[e], 1);
+        }
+        __syncthreads();
+        const int last = s_cnt[n_experts - 1];
+        expert_bases(s_cnt, s_part[0]);
+        for (int e = tid; e < n_experts; e += 256) offsets[e] = s_cnt[e];
+        if (tid == 0) offsets[n_experts] = s_cnt[n_experts - 1] + last;
+        return;
+    }
+    const int t = blockIdx.x - 1, u0 = blockIdx.y * (256 * kUnits);
+    const U *row = x + (size_t)t * units;
+    U v[kUnits];
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+        const int u = u0 + tid + 256 * i;
+        if (u < units) v[i] = row[u];
+    }
+    int key[kIds];  // expert * kSortMax + route; a dropped route sorts behind all
+#pragma unroll
+    for (int i = 0; i < kIds; ++i) {
+        const int r = tid + 256 * i;
+        const int e = r < R ? ids[r] : -1;
+        key[i] = live_id(e, n_experts) ? e * kSortMax + r : 0x7fffffff;
+    }
+    const int r_own = t * top_k + min(lane, top_k - 1);  // lane k: route k of the token
+    const int e_own = ids[r_own];
+    const int own_key = live_id(e_own, n_experts) ? e_own * kSortMax + r_own : -1;
+    for (int k = 0; k < top_k; ++k) {
+        const int own = __builtin_amdgcn_readlane(own_key, k);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kIds; ++i) n += key[i] < own;
+        n = wave_total(n);
+        if (lane == 0) s_part[wave][k] = own < 0 ? -1 : n;
+    }
+    __syncthreads();
+    if (tid < top_k) {
+        const int a = s_part[0][tid];
+        const int pos = a < 0 ? -1 : a + s_part[1][tid] + s_part[2][tid] + s_part[3][tid];
+        s_pos[tid] = pos;
+        if (blockIdx.y == 0) {
+            dst_of_route[t * top_k + tid] = pos;
+            if (pos >= 0) src_route[pos] = t * top_k + tid;
+        }
+    }
+    __syncthreads();
+    for (int k = 0; k < top_k; ++k) {
+        const int pos = s_pos[k];
+        if (pos < 0) continue;
+        U *out = rows + (size_t)pos * units;
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            const int u = u0 + tid + 256 * i;
+            if (u < units) out[u] = v[i];
+        }
+    }
+}
+
+// ---- sort of any number of routes.  Workgroup c places the routes of chunk c; it counts the
+// experts of every route itself (all, and those of the chunks before its own), so there is
+// no scratch and no second launch.  A wave's 64 ids are counted by one ballot per bit of the
+// id and one LDS add per distinct id.
+constexpr int kChunk = 1024;
+
+__global__ __launch_bounds__(256) void moe_sort_kernel(const int32_t *__restrict__ ids, int R, int n_experts,
+                                                       int32_t *__restrict__ offsets, int32_t *__restrict__ src_route,
+                                                       int32_t *__restrict__ dst_of_route) {
+    __shared__ int s_all[1024], s_before[1024];
+    __shared__ int s_wave[4][1024];  // the chunk's routes per wave, then each wave's next position
+    __shared__ int s_part[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int c0 = blockIdx.x * kChunk;
+    const int bits = 32 - __builtin_clz(n_experts);
+    for (int e = tid; e < 1024; e += 256) {
+        s_all[e] = s_before[e] = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) s_wave[w][e] = 0;
+    }
+    __syncthreads();
+    // lanes of the wave with the same live id as this one
+    auto same = [&](int e, bool live) {
+        uint64_t grp = __ballot(live);
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t one = __ballot((e >> b) & 1);
+            grp &= (e >> b) & 1 ? one : ~one;
+        }
+        return grp;
+    };
+    for (int r0 = 64 * wave; r0 < R; r0 += 256) {  // c0 is a multiple of 64: a step is before it or not
+        const int r = r0 + lane;
+        const int e = r < R ? ids[r] : -1;
+        const bool live = live_id(e, n_experts);
+        const uint64_t grp = same(e, live);
+        if (live && lane == 63 - __builtin_clzll(grp)) {
+            const int n = __builtin_popcountll(grp);
+            atomicAdd(&s_all[e], n);
+            if (r0 < c0) atomicAdd(&s_before[e], n);
+        }
+    }
+    // the chunk's own routes: wave w has [c0 + 256 w, c0 + 256 (w + 1))
+    int *mine = s_wave[wave];
+    const int w0 = c0 + (kChunk / 4) * wave;
+    for (int i = 0; i < kChunk / 4; i += 64) {
+        const int r = w0 + i + lane;
+        const int e = r < R ? ids[r] : -1;
+        const bool live = live_id(e, n_experts);
+        const uint64_t grp = same(e, live);
+        if (live && lane == 63 - __builtin_clzll(grp)) mine[e] += __builtin_popcountll(grp);
+    }
+    __syncthreads();
+    const int last = s_all[n_experts - 1];
+    __syncthreads();
+    expert_bases(s_all, s_part);
+    if (blockIdx.x == 0) {
+        for (int e = tid; e < n_experts; e += 256) offsets[e] = s_all[e];
+        if (tid == 0) offsets[n_experts] = s_all[n_experts - 1] + last;
+    }
+    for (int e = tid; e < n_experts; e += 256) {
+        int base = s_all[e] + s_before[e];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int n = s_wave[w][e];
+            s_wave[w][e] = base;
+            base += n;
+        }
+    }
+    __syncthreads();
+    for (int i = 0; i < kChunk / 4; i += 64) {
+        const int r = w0 + i + lane;
+        const int e = r < R ? ids[r] : -1;
+        const bool live = live_id(e, n_experts);
+        const uint64_t grp = same(e, live);
+        int pos = -1;
+        if (live) {
+            pos = mine[e] + __builtin_popcountll(grp & ((1ull << lane) - 1ull));
+            src_route[pos] = r;
+        }
+        if (r < R) dst_of_route[r] = pos;
+        if (live && lane == 63 - __builtin_clzll(grp)) mine[e] = pos + 1;  // after every lane's read: one wave
+    }
+}
+
+// rows[dst(t, k)] = x[t], a thread per piece of a token's row.
+template <class U>
+__global__ __launch_bounds__(256) void scatter_rows_kernel(const U *__restrict__ x,
+                                                           const int32_t *__restrict__ dst_of_route, int R, int top_k,
+                                                           int units, U *__restrict__ rows) {
+    const int t = blockIdx.x, u = blockIdx.y * 256 + threadIdx.x;
+    if (u >= units) return;
+    const U v = x[(size_t)t * units + u];
+    for (int k = 0; k < top_k; ++k) {
+        const int pos = dst_of_route[t * top_k + k];
+        if ((unsigned)pos < (unsigned)R) rows[(size_t)pos * units + u] = v;
+    }
+}
+
+// ---- sums over a token's routes (combine; the dispatch's gradient without weights)
+template <class TI, class TO, int VEC, bool WEIGHTED>
+__global__ __launch_bounds__(256) void join_rows_kernel(const TI *__restrict__ rows,
+                                                        const int32_t *__restrict__ dst_of_route,
+                                                        const float *__restrict__ weights, int R, int top_k, int H,
+                                                        TO *__restrict__ y) {
+    const int t = blockIdx.x, h = (blockIdx.y * 256 + threadIdx.x) * VEC;
+    if (h >= H) return;
+    float acc[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+    for (int k0 = 0; k0 < top_k; k0 += 4) {
+        MxVec<TI, VEC> v[4];
+        int pos[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            pos[j] = k0 + j < top_k ? dst_of_route[t * top_k + k0 + j] : -1;
+            if ((unsigned)pos[j] < (unsigned)R)
+                v[j] = *reinterpret_cast<const MxVec<TI, VEC> *>(rows + (size_t)pos[j] * H + h);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if ((unsigned)pos[j] < (unsigned)R) {
+                const float w = WEIGHTED ? weights[t * top_k + k0 + j] : 1.0f;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w, (float)v[j].v[i], acc[i]);
+            }
+    }
+    MxVec<TO, VEC> o;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o.v[i] = (TO)acc[i];
+    *reinterpret_cast<MxVec<TO, VEC> *>(y + (size_t)t * H + h) = o;
+}
+
+// ---- gradients of the combine: a workgroup per token, its gradient row read once per route
+// from the cache, the routes' dot products reduced in a fixed order.
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void combine_rows_backward_kernel(
+    const T *__restrict__ grad_y, const T *__restrict__ rows, const int32_t *__restrict__ dst_of_route,
+    const float *__restrict__ weights, int R, int top_k, int H, T *__restrict__ grad_rows,
+    float *__restrict__ grad_weights) {
+    __shared__ float s_dot[32][4];
+    const int t = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const T *g = grad_y + (size_t)t * H;
+    for (int k = 0; k < top_k; ++k) {
+        const int pos = dst_of_route[t * top_k + k];
+        float dot = 0.0f;
+        if ((unsigned)pos < (unsigned)R) {
+            const float w = weights[t * top_k + k];
+            const T *e = rows + (size_t)pos * H;
+            T *ge = grad_rows + (size_t)pos * H;
+            for (int h = threadIdx.x * VEC; h < H; h += 256 * VEC) {
+                const MxVec<T, VEC> gv = *reinterpret_cast<const MxVec<T, VEC> *>(g + h);
+                const MxVec<T, VEC> ev = *reinterpret_cast<const MxVec<T, VEC> *>(e + h);
+                MxVec<T, VEC> o;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    dot = fmaf((float)gv.v[i], (float)ev.v[i], dot);
+                    o.v[i] = (T)(w * (float)gv.v[i]);
+                }
+                *reinterpret_cast<MxVec<T, VEC> *>(ge + h) = o;
+            }
+        }
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) dot += __shfl_xor(dot, d);
+        if (lane == 0) s_dot[k][wave] = dot;
+    }
+    __syncthreads();
+    if (threadIdx.x < top_k) {
+        const float *d = s_dot[threadIdx.x];
+        grad_weights[t * top_k + threadIdx.x] = (d[0] + d[1]) + (d[2] + d[3]);
+    }
+}
+
+bool aligned_to(const void *a, const void *b, size_t n) { return (((uintptr_t)a | (uintptr_t)b) & (n - 1)) == 0; }
+
+template <class U>
+hipError_t run_dispatch(const int32_t *ids, const void *x, int T, int top_k, size_t row_bytes, int E, int32_t *offsets,
+                        int32_t *src_route, int32_t *dst_of_route, void *rows, hipStream_t stream) {
+    const int R = T * top_k, units = (int)(row_bytes / sizeof(U));
+    if (R <= kSortMax) {
+        const dim3 grid((unsigned)T + 1, (unsigned)((units + 1023) / 1024));
+        hipLaunchKernelGGL(dispatch_rows_kernel<U>, grid, dim3(256), 0, stream, ids, (const U *)x, R, top_k, units, E,
+                           offsets, src_route, dst_of_route, (U *)rows);
+        return hipGetLastError();
+    }
+    const hipError_t e = launch_moe_sort(ids, R, E, offsets, src_route, dst_of_route, stream);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(scatter_rows_kernel<U>, dim3((unsigned)T, (unsigned)((units + 255) / 256)), dim3(256), 0, stream,
+                       (const U *)x, dst_of_route, R, top_k, units, (U *)rows);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_moe_sort(const int32_t *ids, int n_routes, int n_experts, int32_t *offsets, int32_t *src_route,
+                           int32_t *dst_of_route, hipStream_t stream) {
+    hipLaunchKernelGGL(moe_sort_kernel, dim3((unsigned)((n_routes + kChunk - 1) / kChunk)), dim3(256), 0, stream, ids,
+                       n_routes, n_experts, offsets, src_route, dst_of_route);
+    return hipGetLastError();
+}
+
+hipError_t launch_moe_dispatch_rows(const int32_t *ids, const void *x, int elem_bytes, int T, int top_k, int H, int E,
+                                    int32_t *offsets, int32_t *src_route, int32_t *dst_of_route, void *rows,
+                                    hipStream_t stream) {
+    const size_t bytes = (size_t)H * elem_bytes;
+    if (bytes % 16 == 0 && aligned_to(x, rows, 16))
+        return run_dispatch<uint4>(ids, x, T, top_k, bytes, E, offsets, src_route, dst_of_route, rows, stream);
+    if (bytes % 4 == 0 && aligned_to(x, rows, 4))
+        return run_dispatch<uint32_t>(ids, x, T, top_k, bytes, E, offsets, src_route, dst_of_route, rows, stream);
+    return run_dispatch<uint16_t>(ids, x, T, top_k, bytes, E, offsets, src_route, dst_of_route, rows, stream);
+}
+
+namespace {
+template <class TI, class TO, int VEC>
+hipError_t run_join(const void *rows, const int32_t *dst, const float *weights, void *y, int T, int H, int top_k,
+                    hipStream_t stream) {
+    const dim3 grid((unsigned)T, (unsigned)((H / VEC + 255) / 256));
+    if (weights != nullptr)
+        hipLaunchKernelGGL((join_rows_kernel<TI, TO, VEC, true>), grid, dim3(256), 0, stream, (const TI *)rows, dst,
+                           weights, T * top_k, top_k, H, (TO *)y);
+    else
+        hipLaunchKernelGGL((join_rows_kernel<TI, TO, VEC, false>), grid, dim3(256), 0, stream, (const TI *)rows, dst,
+                           weights, T * top_k, top_k, H, (TO *)y);
+    return hipGetLastError();
+}
+
+template <class TI, class TO>
+hipError_t run_join_types(const void *rows, const int32_t *dst, const float *weights, void *y, int T, int H, int top_k,
+                          hipStream_t stream) {
+    constexpr int kWide = 16 / sizeof(TI);
+    if (H % kWide == 0 && aligned_to(rows, y, 16)) return run_join<TI, TO, kWide>(rows, dst, weights, y, T, H, top_k, stream);
+    if (sizeof(TI) == 2 && H % 2 == 0 && aligned_to(rows, y, 4))
+        return run_join<TI, TO, 2>(rows, dst, weights, y, T, H, top_k, stream);
+    return run_join<TI, TO, 1>(rows, dst, weights, y, T, H, top_k, stream);
+}
+}  // namespace
+
+hipError_t launch_moe_join_rows(const void *rows, int rows_dtype, const int32_t *dst_of_route, const float *weights,
+                                void *y, int dtype, int T, int H, int top_k, hipStream_t stream) {
+    return mx_by_dtype(rows_dtype, [&](auto in) {
+        using TI = typename decltype(in)::type;
+        if (rows_dtype == dtype) return run_join_types<TI, TI>(rows, dst_of_route, weights, y, T, H, top_k, stream);
+        if (rows_dtype != JJO_DTYPE_F32) return hipErrorInvalidValue;
+        return dtype == JJO_DTYPE_F16
+                   ? run_join_types<float, _Float16>(rows, dst_of_route, weights, y, T, H, top_k, stream)
+                   : run_join_types<float, __bf16>(rows, dst_of_route, weights, y, T, H, top_k, stream);
+    });
+}
+
+hipError_t launch_moe_combine_rows_backward(const void *grad_y, const void *rows, int dtype,
+                                            const int32_t *dst_of_route, const float *weights, void *grad_rows,
+                                            float *grad_weights, int T, int H, int top_k, hipStream_t stream) {
+    return mx_by_dtype(dtype, [&](auto tag) {
+        using E = typename decltype(tag)::type;
+        constexpr int kWide = 16 / sizeof(E);
+        const bool a16 = aligned_to(grad_y, rows, 16) && aligned_to(grad_rows, grad_rows, 16);
+        const bool a4 = aligned_to(grad_y, rows, 4) && aligned_to(grad_rows, grad_rows, 4);
+        auto run = [&](auto vec) {
+            constexpr int V = decltype(vec)::value;
+            hipLaunchKernelGGL((combine_rows_backward_kernel<E, V>), dim3((unsigned)T), dim3(256), 0, stream,
+                               (const E *)grad_y, (const E *)rows, dst_of_route, weights, T * top_k, top_k, H,
+                               (E *)grad_rows, grad_weights);
+            return hipGetLastError();
+        };
+        if (H % kWide == 0 && a16) return run(std::integral_constant<int, kWide>{});
+        if (sizeof(E) == 2 && H % 2 == 0 && a4) return run(std::integral_constant<int, 2>{});
+        return run(std::integral_constant<int, 1>{});
+    });
+}
+
+}  // namespace jjo

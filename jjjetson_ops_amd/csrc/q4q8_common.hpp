@@ -32,6 +32,9 @@ int hip_fail(hipError_t e, const char *what);
 // thread-safely; later calls with the same or a smaller size cost a lookup.
 hipError_t ensure_dynamic_lds(const void *kernel, size_t bytes);
 
+// JJO_OK if the current device is a gfx950 (checked once per device), else the error, set.
+int require_device();
+
 // Compute units of the current device (256 on MI355X; the value found when the
 // C ABI checked the device).
 int device_cu_count();
