@@ -139,12 +139,15 @@ int mat_mul_mxfp4_device(const void *d_w, const void *d_x_mxfp4, void *d_y, int 
     clear_error();
     int rc = check_mm("mat_mul_mxfp4", d_w, d_x_mxfp4, d_y, y_dtype, ncols_k, nrows_out, batch);
     if (rc != JJO_OK || (rc = require_device()) != JJO_OK) return rc;
-    return launched(launch_mxfp4_direct(d_w, d_x_mxfp4, d_y, y_dtype, ncols_k, nrows_out, batch, MxGroups{},
+    return launched(launch_mxfp4_mm(d_w, d_x_mxfp4, d_y, y_dtype, ncols_k, nrows_out, batch, MxGroups{},
                                         (hipStream_t)stream),
                     "mat_mul_mxfp4 launch");
 }
 
-int64_t linear_mxfp4_workspace_bytes(int in_features, int num_tokens) { return mxfp4_bytes(num_tokens, in_features); }
+int64_t linear_mxfp4_workspace_bytes(int in_features, int num_tokens) {
+    const int64_t bytes = mxfp4_bytes(num_tokens, in_features);
+    return bytes >= 0 && num_tokens == 1 && in_features <= kMxFusedMaxK ? 0 : bytes;
+}
 
 int linear_mxfp4_forward_device(void *stream, void *quant_workspace, const void *input, int in_dtype,
                                 const void *weight, void *output, int out_dtype, int in_features, int out_features,
@@ -153,13 +156,17 @@ int linear_mxfp4_forward_device(void *stream, void *quant_workspace, const void 
     int rc = check_mm("linear_mxfp4", weight, input, output, out_dtype, in_features, out_features, num_tokens);
     if (rc != JJO_OK) return rc;
     if (!dtype_ok(in_dtype)) return set_error(JJO_ERR_INVALID_ARG, "linear_mxfp4: unknown dtype %d", in_dtype);
-    if (quant_workspace == nullptr || !aligned(quant_workspace, 16))
+    const bool fused = num_tokens == 1 && in_features <= kMxFusedMaxK;
+    if (!fused && (quant_workspace == nullptr || !aligned(quant_workspace, 16)))
         return set_error(JJO_ERR_INVALID_ARG, "linear_mxfp4: a 16-byte aligned workspace is required");
     if ((rc = require_device()) != JJO_OK) return rc;
     hipStream_t s = (hipStream_t)stream;
+    if (fused)
+        return launched(launch_mxfp4_gemv(weight, input, in_dtype, output, out_dtype, in_features, out_features, s),
+                        "linear_mxfp4 launch");
     const hipError_t e = launch_quantize_mxfp4(input, in_dtype, in_features, quant_workspace, num_tokens, in_features, s);
     if (e != hipSuccess) return launched(e, "linear_mxfp4 quantize");
-    return launched(launch_mxfp4_direct(weight, quant_workspace, output, out_dtype, in_features, out_features,
+    return launched(launch_mxfp4_mm(weight, quant_workspace, output, out_dtype, in_features, out_features,
                                         num_tokens, MxGroups{}, s),
                     "linear_mxfp4 launch");
 }
@@ -174,7 +181,7 @@ int mat_mul_mxfp4_grouped_device(const void *d_w, const void *d_x_mxfp4, const i
         return rc;
     MxGroups g;
     g.offsets = d_expert_offsets, g.n_experts = n_experts, g.route_dst = d_route_dst;
-    return launched(launch_mxfp4_direct(d_w, d_x_mxfp4, d_y, y_dtype, ncols_k, nrows_out, n_routes, g,
+    return launched(launch_mxfp4_mm(d_w, d_x_mxfp4, d_y, y_dtype, ncols_k, nrows_out, n_routes, g,
                                         (hipStream_t)stream),
                     "mat_mul_mxfp4_grouped launch");
 }
@@ -192,7 +199,7 @@ int moe_mxfp4_gate_up_swiglu_device(void *stream, const void *w_gate, const void
     if ((rc = require_device()) != JJO_OK) return rc;
     MxGroups g;
     g.offsets = expert_offsets, g.n_experts = num_experts;
-    return launched(launch_mxfp4_direct_swiglu(w_gate, w_up, x_mxfp4_permuted, mid_mxfp4, hidden_size,
+    return launched(launch_mxfp4_swiglu(w_gate, w_up, x_mxfp4_permuted, mid_mxfp4, hidden_size,
                                                intermediate_size, n_routes, g, (hipStream_t)stream),
                     who);
 }
@@ -233,10 +240,10 @@ int moe_mxfp4_ffn_forward_device(void *stream, const void *x, const float *logit
     if (e == hipSuccess) e = launch_quantize_mxfp4(x, dtype, H, ws.xq, T, H, s);
     if (e != hipSuccess) return launched(e, "moe_mxfp4_ffn routing");
     g.src_route = ws.src_route, g.top_k = top_k, g.x_rows = T;
-    if ((e = launch_mxfp4_direct_swiglu(w_gate, w_up, ws.xq, ws.midq, H, I, R, g, s)) != hipSuccess)
+    if ((e = launch_mxfp4_swiglu(w_gate, w_up, ws.xq, ws.midq, H, I, R, g, s)) != hipSuccess)
         return launched(e, "moe_mxfp4_ffn gate|up");
     g.src_route = nullptr;
-    if ((e = launch_mxfp4_direct(w_down, ws.midq, ws.eout, JJO_DTYPE_F32, I, H, R, g, s)) != hipSuccess)
+    if ((e = launch_mxfp4_mm(w_down, ws.midq, ws.eout, JJO_DTYPE_F32, I, H, R, g, s)) != hipSuccess)
         return launched(e, "moe_mxfp4_ffn down");
     return launched(launch_moe_join_rows(ws.eout, JJO_DTYPE_F32, ws.dst_of_route, ws.route_w, y, dtype, T, H, top_k, s),
                     "moe_mxfp4_ffn combine");

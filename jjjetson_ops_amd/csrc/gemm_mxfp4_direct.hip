@@ -15,6 +15,8 @@
 namespace jjo {
 namespace {
 
+constexpr int kFusedMaxK = kMxFusedMaxK;
+
 struct MxProblem {
     const uint8_t *w, *w2, *x;  // w2: the up matrix (SwiGLU)
     void *y;                    // outputs, or the MXFP4 rows of the SwiGLU form
@@ -24,12 +26,81 @@ struct MxProblem {
     MxGroups g;
 };
 
-// RT tiles of 16 weight rows x TT tiles of 16 tokens, W waves over K, U steps of 128 loaded ahead.
-// SWIGLU: RT = 4, two tiles of gate rows and the two of the same up rows.
-template <int RT, int TT, int W, int U, bool GROUPED, bool SWIGLU>
+// Operands of U steps of TILES tiles of 16 rows.  A row's scale bytes of the U steps are one load:
+// dword u holds the bytes of step u's four lane groups.  Rows shorter than that (and only
+// they) fetch each byte where it is used.
+template <int TILES, int U>
+struct MxChunk {
+    u32x4v v[U][TILES];
+    uint32_t s[TILES][U];
+};
+template <int TILES, int U>
+__device__ __forceinline__ void load_chunk(MxChunk<TILES, U> &c, const uint8_t *const (&rows)[TILES],
+                                           const uint8_t *const (&scales)[TILES], int step, int nb) {
+    const int q = (threadIdx.x & 63) >> 4;
+    if (nb >= 4 * U) {
+        const int at = min(4 * step, nb - 4 * U);  // the last chunk's bytes end with the row
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) __builtin_memcpy(c.s[t], scales[t] + at, 4 * U);  // whatever the alignment
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int blk = min(4 * (step + u) + q, nb - 1);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) c.v[u][t] = *reinterpret_cast<const u32x4v *>(rows[t] + (size_t)blk * 16);
+    }
+}
+// The chunk's scale bytes to their places: shifted where the row ends inside the chunk (zeros
+// behind it), or fetched.
+template <int TILES, int U>
+__device__ __forceinline__ void place_scales(MxChunk<TILES, U> &c, const uint8_t *const (&scales)[TILES], int step,
+                                             int nb) {
+    const int over = 4 * step + 4 * U - nb;  // uniform
+    if (over <= 0) return;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        if (nb >= 4 * U) {
+            unsigned __int128 b = 0;
+            __builtin_memcpy(&b, c.s[t], 4 * U);
+            b >>= 8 * over;
+            __builtin_memcpy(c.s[t], &b, 4 * U);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                c.s[t][u] = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    c.s[t][u] |= (uint32_t)scales[t][min(4 * (step + u) + k, nb - 1)] << (8 * k);
+            }
+        }
+    }
+}
+
+// One wave's 1024 values of the fused activation, 16 a lane, to codes and scales in LDS.
+template <class T>
+__device__ __forceinline__ void load16(const T *p, float *x) {
+    constexpr int kVec = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 16 / kVec; ++i) {
+        const MxVec<T, kVec> a = reinterpret_cast<const MxVec<T, kVec> *>(p)[i];
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) x[kVec * i + k] = (float)a.v[k];
+    }
+}
+
+// RT tiles of 16 weight rows x TT tiles of 16 tokens, W waves over K, U steps of 128 in registers
+// and U more in flight.  SWIGLU: RT = 4, two tiles of gate rows and the two of the same up
+// rows.  XT: void (x is MXFP4), or the type of the one token's row, which every wave quantizes
+// for its own slice of K.
+template <int RT, int TT, int W, int U, bool GROUPED, bool SWIGLU, class XT>
 __global__ __launch_bounds__(64 * W) void mxfp4_direct_kernel(MxProblem p) {
+    constexpr bool kFused = !std::is_void_v<XT>;
+    constexpr int kPieces = 2;  // of 1024 values in a wave's slice of the fused form
     __shared__ f32x4v part[W][RT * TT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+    __shared__ u32x4v x_codes[kFused ? W : 1][kFused ? 32 * kPieces : 1];
+    __shared__ uint8_t x_scales[kFused ? W : 1][kFused ? 32 * kPieces : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r16 = lane & 15, q = lane >> 4;
     const int tile_t = (int)(blockIdx.x % (unsigned)p.token_tiles), tile_n = (int)(blockIdx.x / (unsigned)p.token_tiles);
     int expert = 0, first = tile_t * 16 * TT, end = p.M;
     if constexpr (GROUPED) {
@@ -52,13 +123,15 @@ __global__ __launch_bounds__(64 * W) void mxfp4_direct_kernel(MxProblem p) {
         ws[rt] = m + all * half + row * nb;
     }
     const uint8_t *xr[TT], *xs[TT];
-    const size_t x_rows = p.g.src_route != nullptr ? p.g.x_rows : p.M;
+    if constexpr (!kFused) {
+        const size_t x_rows = p.g.src_route != nullptr ? p.g.x_rows : p.M;
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-        int t = min(first + 16 * tt + r16, end - 1);
-        if (GROUPED && p.g.src_route != nullptr) t = min(max(p.g.src_route[t] / p.g.top_k, 0), p.g.x_rows - 1);
-        xr[tt] = p.x + (size_t)t * half;
-        xs[tt] = p.x + x_rows * half + (size_t)t * nb;
+        for (int tt = 0; tt < TT; ++tt) {
+            int t = min(first + 16 * tt + r16, end - 1);
+            if (GROUPED && p.g.src_route != nullptr) t = min(max(p.g.src_route[t] / p.g.top_k, 0), p.g.x_rows - 1);
+            xr[tt] = p.x + (size_t)t * half;
+            xs[tt] = p.x + x_rows * half + (size_t)t * nb;
+        }
     }
     f32x4v acc[RT][TT];
 #pragma unroll
@@ -66,33 +139,77 @@ __global__ __launch_bounds__(64 * W) void mxfp4_direct_kernel(MxProblem p) {
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = f32x4v{0.f, 0.f, 0.f, 0.f};
 
+    MxChunk<RT, U> w;
+    MxChunk<TT, U> x;
+    if constexpr (kFused) {
+        // The token's values are asked for before the weights: loads return in order.
+        typedef std::conditional_t<kFused, XT, float> T;
+        const T *src = (const T *)p.x + 128 * (size_t)s_beg;
+        const int live = min(128 * (s_end - s_beg), p.K - 128 * s_beg);  // a multiple of 32
+        float v[kPieces][16];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+            if (1024 * i + 16 * lane < live) load16(src + 1024 * i + 16 * lane, v[i]);
+        if (s_beg < s_end) load_chunk(w, wr, ws, s_beg, nb);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            if (1024 * i >= 128 * (s_end - s_beg)) break;
+            const bool in = 1024 * i + 16 * lane < live;
+            uint32_t m = 0;
+            if (in) {
+                m = mx_amax8(v[i]);
+                const uint32_t o = mx_amax8(v[i] + 8);
+                m = o > m ? o : m;
+            }
+            const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, true);  // lane ^ 1
+            m = o > m ? o : m;
+            const uint32_t s = mx_scale_byte(m);
+            uint2 c = make_uint2(0u, 0u);
+            if (in) c = make_uint2(mx_codes8(v[i], s), mx_codes8(v[i] + 8, s));
+            reinterpret_cast<uint2 *>(&x_codes[wave][32 * i])[lane] = c;
+            if ((lane & 1) == 0) x_scales[wave][32 * i + (lane >> 1)] = (uint8_t)s;
+        }
+    } else if (s_beg < s_end) {
+        load_chunk(w, wr, ws, s_beg, nb);
+        load_chunk(x, xr, xs, s_beg, nb);
+    }
     for (int s = s_beg; s < s_end; s += U) {
-        u32x4v a[U][RT], b[U][TT];
-        uint32_t sa[U][RT], sb[U][TT];
+        MxChunk<RT, U> w_next;
+        MxChunk<TT, U> x_next;
+        if (s + U < s_end) {
+            load_chunk(w_next, wr, ws, s + U, nb);
+            if constexpr (!kFused) load_chunk(x_next, xr, xs, s + U, nb);
+        }
+        place_scales(w, ws, s, nb);
+        if constexpr (!kFused) place_scales(x, xs, s, nb);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int blk = 4 * min(s + u, s_end - 1) + q, at = min(blk, nb - 1);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                a[u][rt] = *reinterpret_cast<const u32x4v *>(wr[rt] + (size_t)at * 16);
-                sa[u][rt] = ws[rt][at];
-                if (blk >= nb) a[u][rt] = u32x4v{0u, 0u, 0u, 0u};  // behind the row's end (K % 128)
-            }
-#pragma unroll
-            for (int tt = 0; tt < TT; ++tt) {
-                b[u][tt] = *reinterpret_cast<const u32x4v *>(xr[tt] + (size_t)at * 16);
-                sb[u][tt] = xs[tt][at];
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (s + u < s_end) {
+            if (s + u >= s_end) break;
+            if (4 * (s + u) + 4 > nb) {  // the row ends inside the step (K % 128)
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int tt = 0; tt < TT; ++tt)
-                        acc[rt][tt] = mx_mfma(a[u][rt], b[u][tt], acc[rt][tt], sa[u][rt], sb[u][tt]);
+                    if (4 * (s + u) + q >= nb) w.v[u][rt] = u32x4v{0u, 0u, 0u, 0u};
             }
+            u32x4v xv[TT];
+            uint32_t sx[TT];
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) {
+                if constexpr (kFused) {
+                    xv[tt] = x_codes[wave][4 * (s + u - s_beg) + q];
+                    sx[tt] = x_scales[wave][4 * (s + u - s_beg) + q];
+                } else {
+                    xv[tt] = x.v[u][tt];
+                    sx[tt] = x.s[tt][u] >> (8 * q);
+                }
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt)
+                    acc[rt][tt] = mx_mfma(w.v[u][rt], xv[tt], acc[rt][tt], w.s[rt][u] >> (8 * q), sx[tt]);
+        }
+        w = w_next;
+        if constexpr (!kFused) x = x_next;
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
@@ -125,19 +242,20 @@ __global__ __launch_bounds__(64 * W) void mxfp4_direct_kernel(MxProblem p) {
     }
 }
 
-template <int RT, int TT, int W, int U, bool SWIGLU>
+template <int RT, int TT, int W, int U, bool SWIGLU, class XT = void>
 hipError_t run_direct(MxProblem p, hipStream_t stream) {
     const int rows = SWIGLU ? 32 : 16 * RT;
     // token tiles of M rows, and one more for each expert that can have a rest
     p.token_tiles = (p.M + 16 * TT - 1) / (16 * TT) + (p.g.offsets != nullptr ? std::min(p.g.n_experts, p.M) : 0);
     const int64_t wgs = (int64_t)p.token_tiles * ((p.N + rows - 1) / rows);
     if (wgs * 64 * W >= 1LL << 32) return hipErrorInvalidConfiguration;
-    if (p.g.offsets != nullptr)
-        hipLaunchKernelGGL((mxfp4_direct_kernel<RT, TT, W, U, true, SWIGLU>), dim3((unsigned)wgs), dim3(64 * W), 0,
-                           stream, p);
+    const dim3 grid((unsigned)wgs), block(64 * W);
+    if constexpr (!std::is_void_v<XT>)
+        hipLaunchKernelGGL((mxfp4_direct_kernel<RT, TT, W, U, false, false, XT>), grid, block, 0, stream, p);
+    else if (p.g.offsets != nullptr)
+        hipLaunchKernelGGL((mxfp4_direct_kernel<RT, TT, W, U, true, SWIGLU, void>), grid, block, 0, stream, p);
     else if constexpr (!SWIGLU)
-        hipLaunchKernelGGL((mxfp4_direct_kernel<RT, TT, W, U, false, false>), dim3((unsigned)wgs), dim3(64 * W), 0,
-                           stream, p);
+        hipLaunchKernelGGL((mxfp4_direct_kernel<RT, TT, W, U, false, false, void>), grid, block, 0, stream, p);
     else
         return hipErrorInvalidValue;
     return hipGetLastError();
@@ -155,18 +273,27 @@ int mean_rows(int M, const MxGroups &g) {
 hipError_t launch_mxfp4_direct(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
                                const MxGroups &groups, hipStream_t stream) {
     const MxProblem p{(const uint8_t *)w, nullptr, (const uint8_t *)xq, y, dtype, K, N, M, 0, groups};
-    const int mean = mean_rows(M, groups);
-    if (mean <= 16) return run_direct<1, 1, 4, 8, false>(p, stream);
-    if (mean <= 32) return run_direct<2, 2, 4, 4, false>(p, stream);
-    return run_direct<4, 4, 4, 2, false>(p, stream);
+    const int mean = mean_rows(M, groups), steps = (K + 127) / 128;
+    if (mean <= 16) return steps >= 64 ? run_direct<1, 1, 8, 4, false>(p, stream) : run_direct<1, 1, 4, 4, false>(p, stream);
+    if (mean <= 32) return steps >= 64 ? run_direct<1, 2, 8, 4, false>(p, stream) : run_direct<1, 2, 4, 4, false>(p, stream);
+    return run_direct<2, 4, 4, 2, false>(p, stream);
 }
 
 hipError_t launch_mxfp4_direct_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I,
                                       int M, const MxGroups &groups, hipStream_t stream) {
     const MxProblem p{(const uint8_t *)w_gate, (const uint8_t *)w_up, (const uint8_t *)xq, mid, JJO_DTYPE_F32, K, I, M,
                       0, groups};
-    if (mean_rows(M, groups) <= 16) return run_direct<4, 1, 4, 4, true>(p, stream);
-    return run_direct<4, 4, 4, 2, true>(p, stream);
+    if (mean_rows(M, groups) <= 16) return run_direct<4, 1, 4, 2, true>(p, stream);
+    return run_direct<4, 2, 4, 2, true>(p, stream);
+}
+
+hipError_t launch_mxfp4_gemv(const void *w, const void *x, int x_dtype, void *y, int y_dtype, int K, int N,
+                             hipStream_t stream) {
+    const MxProblem p{(const uint8_t *)w, nullptr, (const uint8_t *)x, y, y_dtype, K, N, 1, 0, MxGroups{}};
+    return mx_by_dtype(x_dtype, [&](auto tag) {
+        using T = typename decltype(tag)::type;
+        return K > 8192 ? run_direct<1, 1, 8, 4, false, T>(p, stream) : run_direct<1, 1, 4, 4, false, T>(p, stream);
+    });
 }
 
 }  // namespace jjo

@@ -118,9 +118,24 @@ struct MxGroups {
 };
 hipError_t launch_mxfp4_direct(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
                                const MxGroups &groups, hipStream_t stream);
+// One token whose row is quantized inside the product (K <= kMxFusedMaxK).
+constexpr int kMxFusedMaxK = 16384;
+hipError_t launch_mxfp4_gemv(const void *w, const void *x, int x_dtype, void *y, int y_dtype, int K, int N,
+                             hipStream_t stream);
 // mid = MXFP4 of silu(x . w_gate) * (x . w_up), [M][I] (I % 32 == 0), of grouped rows.
 hipError_t launch_mxfp4_direct_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I,
                                       int M, const MxGroups &groups, hipStream_t stream);
+// The same products on LDS tiles of `tile` (256 or 128) rows and tokens, where accepted.
+bool mxfp4_tiled_accepts(int K, const MxGroups &groups);
+hipError_t launch_mxfp4_tiled(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
+                              const MxGroups &groups, int tile, hipStream_t stream);
+hipError_t launch_mxfp4_tiled_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I,
+                                     int M, const MxGroups &groups, int tile, hipStream_t stream);
+// The products on the kernel chosen for the shape.
+hipError_t launch_mxfp4_mm(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
+                           const MxGroups &groups, hipStream_t stream);
+hipError_t launch_mxfp4_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I, int M,
+                               const MxGroups &groups, hipStream_t stream);
 
 // Rows to their experts and back (moe_rows.hip).
 hipError_t launch_moe_sort(const int32_t *ids, int n_routes, int n_experts, int32_t *offsets, int32_t *src_route,

@@ -62,14 +62,14 @@ __device__ __forceinline__ bool mx_expert_tile(const int32_t *__restrict__ offse
         }
         const uint64_t past = __ballot(base + incl > tile);
         if (past != 0) {
-            const int l = __builtin_ctzll(past);
-            const int t0 = base + __shfl(incl - mine, l);
-            expert = e0 + l;
-            first = __shfl(beg, l) + (tile - t0) * rows;
-            end = __shfl(fin, l);
+            const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
+            const int t0 = base + __builtin_amdgcn_readlane(incl - mine, l);
+            expert = e0 + l;  // scalars: the row addresses below are
+            first = __builtin_amdgcn_readlane(beg, l) + (tile - t0) * rows;
+            end = __builtin_amdgcn_readlane(fin, l);
             return true;
         }
-        base += __shfl(incl, 63);
+        base += __builtin_amdgcn_readlane(incl, 63);
     }
     return false;
 }

@@ -122,7 +122,8 @@ def test_quantize_strided(dtype, dev):
 # -------------------------------------------------------------------------- products
 SHAPES = [(32, 1, 1), (32, 16, 1), (128, 5, 2), (160, 33, 3), (4096, 96, 1), (4096, 100, 4), (1056, 130, 16),
           (992, 64, 17), (2048, 256, 24), (11008, 48, 7), (512, 200, 33), (1024, 257, 64), (160, 70, 65),
-          (640, 300, 100), (4096, 256, 129), (256, 1000, 255), (1312, 520, 300), (2048, 512, 600)]
+          (640, 300, 100), (4096, 256, 129), (256, 1000, 255), (1312, 520, 300), (2048, 512, 600), (288, 8300, 2050),
+          (800, 4200, 4111)]
 
 
 @pytest.mark.parametrize("K,N,M", SHAPES)
@@ -188,7 +189,7 @@ def _offsets(rng, E, R, skew):
 
 GROUPED = [(3, 64, 40, 1, "even"), (8, 256, 96, 5, "skewed"), (8, 512, 130, 40, "even"), (5, 160, 64, 100, "one"),
            (70, 128, 32, 200, "skewed"), (4, 1056, 256, 300, "even"), (8, 512, 160, 1000, "skewed"),
-           (300, 64, 32, 64, "even")]
+           (300, 64, 32, 64, "even"), (64, 288, 1056, 9500, "even"), (64, 256, 1030, 9500, "skewed")]
 
 
 @pytest.mark.parametrize("E,K,N,R,skew", GROUPED)
@@ -235,7 +236,8 @@ def _check_swiglu(mid, g, u, dg, du):
 
 @pytest.mark.parametrize("E,K,I,R,skew", [(3, 64, 32, 1, "even"), (8, 512, 96, 12, "skewed"), (4, 160, 160, 50, "even"),
                                           (4, 1056, 128, 300, "even"), (8, 512, 224, 1000, "skewed"),
-                                          (70, 128, 32, 200, "skewed")])
+                                          (70, 128, 32, 200, "skewed"), (64, 288, 544, 9500, "even"),
+                                          (64, 256, 512, 9500, "skewed")])
 def test_gate_up_swiglu(E, K, I, R, skew, dev):
     note(f"gate_up E={E} K={K} I={I} R={R}")
     rng = np.random.default_rng(E + K + R + I)
