@@ -16,26 +16,24 @@ __device__ __forceinline__ f32x4v mx_mfma(u32x4v w, u32x4v x, f32x4v acc, uint32
 }
 
 // Four consecutive outputs of one row (the first `live` of them), in y's type.  `vec`: the row
-// and y are aligned for one access.
-__device__ __forceinline__ void mx_store4(void *y, int dtype, size_t at, f32x4v v, int live, bool vec) {
-    if (dtype == JJO_DTYPE_F32) {
-        float *p = (float *)y + at;
-        if (vec && live >= 4) *reinterpret_cast<f32x4v *>(p) = v;
-        else
-            for (int i = 0; i < live && i < 4; ++i) p[i] = v[i];
-    } else if (dtype == JJO_DTYPE_F16) {
-        MxVec<_Float16, 4> o = {{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]}};
-        _Float16 *p = (_Float16 *)y + at;
-        if (vec && live >= 4) *reinterpret_cast<MxVec<_Float16, 4> *>(p) = o;
-        else
-            for (int i = 0; i < live && i < 4; ++i) p[i] = o.v[i];
+// and y are aligned for one access.  Every index is a constant: an indexed copy would be moved to
+// LDS, addressed by the workgroup size of the launch packet, which lies in host memory (14 us more
+// for a decode step).
+template <class T>
+__device__ __forceinline__ void mx_store4_as(T *p, f32x4v v, int live, bool vec) {
+    if (vec && live >= 4) {
+        *reinterpret_cast<MxVec<T, 4> *>(p) = MxVec<T, 4>{{(T)v[0], (T)v[1], (T)v[2], (T)v[3]}};
     } else {
-        MxVec<__bf16, 4> o = {{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]}};
-        __bf16 *p = (__bf16 *)y + at;
-        if (vec && live >= 4) *reinterpret_cast<MxVec<__bf16, 4> *>(p) = o;
-        else
-            for (int i = 0; i < live && i < 4; ++i) p[i] = o.v[i];
+        p[0] = (T)v[0];
+        if (live > 1) p[1] = (T)v[1];
+        if (live > 2) p[2] = (T)v[2];
+        if (live > 3) p[3] = (T)v[3];
     }
+}
+__device__ __forceinline__ void mx_store4(void *y, int dtype, size_t at, f32x4v v, int live, bool vec) {
+    if (dtype == JJO_DTYPE_F32) mx_store4_as((float *)y + at, v, live, vec);
+    else if (dtype == JJO_DTYPE_F16) mx_store4_as((_Float16 *)y + at, v, live, vec);
+    else mx_store4_as((__bf16 *)y + at, v, live, vec);
 }
 
 // The tile-th tile of `rows` sorted rows, counted over the experts in order: its expert, its
