@@ -43,15 +43,50 @@ struct MxTile {
     static constexpr int kDma = kRows / 8 / kWaves;  // instructions a wave and stage
     static constexpr int kScaleRows = (kRows + kThreads - 1) / kThreads;  // rows a thread
     static constexpr int kStage = kRows * 128;
-    static constexpr int kLds = 2 * (kStage + kRows * 8);
-    static_assert(kRows % (8 * kWaves) == 0 && kRowsN % 8 == 0, "whole DMA instructions");
+    static constexpr int kLds = 2 * (kStage + kRows * 16) + kRows * 4;
+    static_assert(kRows % (8 * kWaves) == 0 && kRowsN % 8 == 0 && kDma % 2 == 0, "whole DMA instructions");
 };
+
+// A wave's outputs (from weight row n, token t on) through its own 4 KB of LDS, 16 tokens at a time:
+// the matrix instruction leaves 4 consecutive outputs of a token in a lane, 32 bytes of a row in
+// an instruction; read back a row is 16 RT outputs in whole 128-byte lines.  N % 8 == 0.
+template <class T, int RT, int TT>
+__device__ __forceinline__ void store_rows(T *__restrict__ y, const f32x4v (&acc)[RT][TT], uint8_t *stage, int n,
+                                           int t, int end, int N, const int32_t *__restrict__ route_dst) {
+    constexpr int kVec = 16 / sizeof(T), kChunks = 16 * RT / kVec, kRowsAtOnce = 64 / kChunks;
+    const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
+    const int row = lane / kChunks, chunk = lane % kChunks;
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int at = 16 * rt + 4 * q;
+            MxVec<T, 4> v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v.v[i] = (T)acc[rt][tt][i];
+            *reinterpret_cast<MxVec<T, 4> *>(stage + r16 * (kChunks * 16) + 16 * ((at / kVec) ^ (r16 % kChunks)) +
+                                             at % kVec * sizeof(T)) = v;
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < 16 / kRowsAtOnce; ++k) {
+            const int r = kRowsAtOnce * k + row, token = t + 16 * tt + r;
+            const u32x4v v = *reinterpret_cast<const u32x4v *>(stage + r * (kChunks * 16) + 16 * (chunk ^ (r % kChunks)));
+            if (token < end && n + chunk * kVec < N) {
+                const size_t to = route_dst != nullptr ? route_dst[token] : token;
+                *reinterpret_cast<u32x4v *>(y + to * N + n + chunk * kVec) = v;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
 
 template <class Tile, bool GROUPED, bool SWIGLU>
 __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) {
     constexpr int RT = Tile::RT, TT = Tile::TT;
     extern __shared__ __align__(16) uint8_t lds[];
     uint8_t *const lds_scales = lds + 2 * Tile::kStage;
+    uint32_t *const lds_rows = reinterpret_cast<uint32_t *>(lds_scales + 2 * Tile::kRows * 16);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, q = lane >> 4;
     const int wn = wave % Tile::WN, wt = wave / Tile::WN;
@@ -85,23 +120,16 @@ __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) 
     const size_t w_first = (size_t)expert * p.N, w_all = (size_t)(GROUPED ? p.g.n_experts : 1) * p.N;
     const size_t x_all = p.g.src_route != nullptr ? p.g.x_rows : p.M;
 
-    // ---- this lane's part of the DMA: rows 8 * i + lane / 8, piece (lane % 8) ^ (lane / 8)
-    const uint8_t *base[Tile::kDma];  // uniform
-    uint32_t off[Tile::kDma];
-    const uint32_t piece = 16 * ((lane & 7) ^ (lane >> 3));
-#pragma unroll
-    for (int i = 0; i < Tile::kDma; ++i) {
-        const int row8 = 8 * (wave * Tile::kDma + i), row = row8 + (lane >> 3);
-        if (row8 < Tile::kRowsN) {
-            base[i] = (is_up(row8) ? p.w2 : p.w) + w_first * half;
-            base[i] += (size_t)n0 * half;
-            off[i] = (uint32_t)(weight_row(row) - n0) * half + piece;
-        } else {
-            const int t0 = GROUPED && p.g.src_route != nullptr ? 0 : first;
-            base[i] = p.x + (size_t)t0 * half;
-            off[i] = (uint32_t)(token_row(row - Tile::kRowsN) - t0) * half + piece;
-        }
-    }
+    // ---- the DMA: instruction i of a wave takes rows 8 * i + lane / 8, piece (lane % 8) ^ (lane / 8).  The
+    // rows' offsets stand in LDS: kept in registers they would spill, and a reload from scratch
+    // waits for every DMA before it.
+    const int t0 = GROUPED && p.g.src_route != nullptr ? 0 : first;
+    for (int row = threadIdx.x; row < Tile::kRows; row += Tile::kThreads)
+        lds_rows[row] = row < Tile::kRowsN ? (uint32_t)(weight_row(row) - n0) * half
+                                           : (uint32_t)(token_row(row - Tile::kRowsN) - t0) * half;
+    const uint8_t *const w_base = p.w + (w_first + n0) * (size_t)half, *const x_base = p.x + (size_t)t0 * half;
+    const uint8_t *const w2_base = SWIGLU ? p.w2 + (w_first + n0) * (size_t)half : nullptr;
+    const uint32_t piece = 16 * ((lane & 7) ^ ((lane >> 4) & 3));
     // ---- and of the scales: one row, or kScaleRows
     const uint8_t *srow[Tile::kScaleRows];
 #pragma unroll
@@ -112,31 +140,46 @@ __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) 
         else
             srow[i] = p.x + x_all * half + (size_t)token_row(row - Tile::kRowsN) * nb;
     }
-    uint64_t sv[Tile::kScaleRows];
-    auto load_scales = [&](int st) {  // the last stage's bytes end with the row (nb >= 8)
+    // A pair of stages at a time: 16 bytes of each row are one request.
+    uint32_t sv[Tile::kScaleRows][4];
+    auto load_scales = [&](int pair) {  // the last pair's bytes end with the row (nb >= 16)
 #pragma unroll
-        for (int i = 0; i < Tile::kScaleRows; ++i) __builtin_memcpy(&sv[i], srow[i] + min(8 * st, nb - 8), 8);
+        for (int i = 0; i < Tile::kScaleRows; ++i) __builtin_memcpy(sv[i], srow[i] + min(16 * pair, nb - 16), 16);
     };
-    auto store_scales = [&](int st) {
-        const int over = max(8 * st + 8 - nb, 0);  // zeros behind the row's end
+    auto store_scales = [&](int pair) {
+        const int over = 16 * pair + 16 - nb;
 #pragma unroll
         for (int i = 0; i < Tile::kScaleRows; ++i) {
+            if (over > 0) {  // zeros behind the row's end
+                unsigned __int128 v;
+                __builtin_memcpy(&v, sv[i], 16);
+                v >>= 8 * over;
+                __builtin_memcpy(sv[i], &v, 16);
+            }
             const int row = threadIdx.x + i * Tile::kThreads;
-            if (row < Tile::kRows)
-                *reinterpret_cast<uint64_t *>(lds_scales + (st & 1) * (Tile::kRows * 8) + row * 8) = sv[i] >> (8 * over);
+            uint8_t *to = lds_scales + (pair & 1) * (Tile::kRows * 16) + row * 8;
+            if (row < Tile::kRows) {
+                *reinterpret_cast<uint2 *>(to) = make_uint2(sv[i][0], sv[i][1]);
+                *reinterpret_cast<uint2 *>(to + Tile::kRows * 8) = make_uint2(sv[i][2], sv[i][3]);
+            }
         }
     };
     const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
-    auto dma = [&](int st) {
+    auto dma = [&](int st, int buffer) {
         const uint32_t left = 16u * (uint32_t)(nb - 8 * st);  // bytes of the row from the stage on
-        const uint32_t back = piece + 16 > left ? piece + 16 - left : 0;
+        const uint32_t most = left >= 128u ? 112u : left - 16u;
+        const uint32_t at[2] = {(uint32_t)min(piece, most), (uint32_t)min(piece ^ 64u, most)};  // rows of an even, an odd instruction
+        uint32_t off[Tile::kDma];
+#pragma unroll
+        for (int i = 0; i < Tile::kDma; ++i) off[i] = lds_rows[8 * (wave * Tile::kDma + i) + (lane >> 3)] + at[i & 1];
 #pragma unroll
         for (int i = 0; i < Tile::kDma; ++i) {
-            const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds0 + (st & 1) * Tile::kStage +
-                                                                1024 * (wave * Tile::kDma + i));
+            const int row8 = 8 * (wave * Tile::kDma + i);
+            const uint8_t *base = row8 >= Tile::kRowsN ? x_base : is_up(row8) ? w2_base : w_base;
+            const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds0 + buffer * Tile::kStage + 128 * row8);
             asm volatile("global_load_lds_dwordx4 %0, %1"
                          :
-                         : "v"(off[i] - back), "s"(base[i] + (size_t)st * 128), "{m0}"(m0v)
+                         : "v"(off[i]), "s"(base + (size_t)st * 128), "{m0}"(m0v)
                          : "memory");
         }
     };
@@ -148,19 +191,27 @@ __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) 
         for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = f32x4v{0.f, 0.f, 0.f, 0.f};
 
     load_scales(0);
-    dma(0);
+    __syncthreads();
+    dma(0, 0);
     const uint32_t w_at = (uint32_t)(16 * RT * wn + r16), x_at = (uint32_t)(Tile::kRowsN + 16 * TT * wt + r16);
-    const uint32_t sw0 = 16u * ((2 * q) ^ (r16 & 7)), sw1 = 16u * ((2 * q + 1) ^ (r16 & 7));
+    const uint32_t sw0 = 16u * ((2 * q) ^ (r16 >> 1)), sw1 = 16u * ((2 * q + 1) ^ (r16 >> 1));
     for (int st = 0; st < stages; ++st) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // stage st has landed
-        store_scales(st);
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (st + 1 < stages) {
-            load_scales(st + 1);
-            dma(st + 1);
+        if ((st & 1) == 0) store_scales(st >> 1);
+        if (const int over = 8 * st + 8 - nb; over > 0) {  // the row ends inside the stage: zero weights behind it
+            asm volatile("s_barrier" ::: "memory");
+            for (int i = threadIdx.x; i < Tile::kRowsN * 8; i += Tile::kThreads)
+                if ((i & 7) >= 8 - over)
+                    *reinterpret_cast<u32x4v *>(lds + (st & 1) * Tile::kStage + (i >> 3) * 128 + 16 * ((i & 7) ^ ((i >> 4) & 7))) =
+                        u32x4v{0u, 0u, 0u, 0u};
         }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        // The next stage on its way; behind the last one, the last again (nothing reads it).
+        const int next = min(st + 1, stages - 1);
+        if ((st & 1) == 0) load_scales(min((st >> 1) + 1, (stages - 1) >> 1));
+        dma(next, (st + 1) & 1);
         const uint8_t *buf = lds + (st & 1) * Tile::kStage;
-        const uint8_t *sbuf = lds_scales + (st & 1) * (Tile::kRows * 8);
+        const uint8_t *sbuf = lds_scales + (st & 3) * (Tile::kRows * 8);
         uint32_t sw[RT], sx[TT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) sw[rt] = *reinterpret_cast<const uint16_t *>(sbuf + (w_at + 16 * rt) * 8 + 2 * q);
@@ -168,28 +219,21 @@ __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) 
         for (int tt = 0; tt < TT; ++tt) sx[tt] = *reinterpret_cast<const uint16_t *>(sbuf + (x_at + 16 * tt) * 8 + 2 * q);
         auto step = [&](auto u_tag) {
             constexpr int U = decltype(u_tag)::value;
-            const uint32_t sw_off = U == 0 ? sw0 : sw1;
-            u32x4v a[RT], b[TT];
+            const uint8_t *at = buf + (U == 0 ? sw0 : sw1);
+            u32x4v a[RT];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-                a[rt] = *reinterpret_cast<const u32x4v *>(buf + (w_at + 16 * rt) * 128 + sw_off);
+            for (int rt = 0; rt < RT; ++rt) a[rt] = *reinterpret_cast<const u32x4v *>(at + (w_at + 16 * rt) * 128);
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
-                b[tt] = *reinterpret_cast<const u32x4v *>(buf + (x_at + 16 * tt) * 128 + sw_off);
-            if (8 * st + 8 > nb) {  // the row ends inside the stage
+            for (int tt = 0; tt < TT; ++tt) {
+                const u32x4v b = *reinterpret_cast<const u32x4v *>(at + (x_at + 16 * tt) * 128);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-                    if (8 * st + 2 * q + U >= nb) a[rt] = u32x4v{0u, 0u, 0u, 0u};
+                for (int rt = 0; rt < RT; ++rt) acc[rt][tt] = mx_mfma_step<U>(a[rt], b, acc[rt][tt], sw[rt], sx[tt]);
             }
-#pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-                    acc[rt][tt] = mx_mfma_step<U>(a[rt], b[tt], acc[rt][tt], sw[rt], sx[tt]);
         };
         step(std::integral_constant<int, 0>{});
         step(std::integral_constant<int, 1>{});
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outlives the workgroup's LDS
 
     if constexpr (SWIGLU) {
         static_assert(!SWIGLU || RT == 4, "a wave holds 32 gate rows and the same 32 up rows");
@@ -204,6 +248,17 @@ __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) 
             mx_swiglu_store(gate, up, codes + row * (p.N / 2) + n / 2, scales + row * (p.N / kQK) + n / kQK, t < end);
         }
     } else {
+        if (p.N % 8 == 0) {
+            __syncthreads();  // no wave reads a stage any more
+            uint8_t *stage = lds + wave * 4096;
+            const int nw = n0 + 16 * RT * wn, tw = first + 16 * TT * wt;
+            const int32_t *route_dst = GROUPED ? p.g.route_dst : nullptr;
+            if (p.dtype == JJO_DTYPE_F32) store_rows<float, RT, TT>((float *)p.y, acc, stage, nw, tw, end, p.N, route_dst);
+            else if (p.dtype == JJO_DTYPE_F16)
+                store_rows<_Float16, RT, TT>((_Float16 *)p.y, acc, stage, nw, tw, end, p.N, route_dst);
+            else store_rows<__bf16, RT, TT>((__bf16 *)p.y, acc, stage, nw, tw, end, p.N, route_dst);
+            return;
+        }
         const bool vec = p.N % 4 == 0;  // y is 16-byte aligned
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
@@ -243,9 +298,9 @@ typedef MxTile<4, 4, 2, 2> Tile128;  // 128 x 128, 4 waves
 
 }  // namespace
 
-// Rows of at least one stage; byte offsets inside a tile (and of gathered rows) fit 32 bits.
+// Rows of at least two stages; byte offsets inside a tile (and of gathered rows) fit 32 bits.
 bool mxfp4_tiled_accepts(int K, const MxGroups &g) {
-    return K >= 256 && K <= 1 << 23 && (g.src_route == nullptr || (int64_t)g.x_rows * (K / 2) < 1LL << 32);
+    return K >= 512 && K <= 1 << 23 && (g.src_route == nullptr || (int64_t)g.x_rows * (K / 2) < 1LL << 32);
 }
 
 hipError_t launch_mxfp4_tiled(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
