@@ -231,13 +231,12 @@ int moe_mxfp4_ffn_forward_device(void *stream, const void *x, const float *logit
                          (long long)workspace_bytes, (long long)ws.bytes);
     if ((rc = require_device()) != JJO_OK) return rc;
     hipStream_t s = (hipStream_t)stream;
-    // 1) top-k, 2) sort, 3) x -> MXFP4 once per token (the products fetch a route's row by its token),
-    // 4) gate|up with SwiGLU, 5) down, 6) weighted sum back to token order
+    // 1) top-k, sort, and x to MXFP4 once per token (the products fetch a route's row by its token),
+    // 2) gate|up with SwiGLU, 3) down, 4) weighted sum back to token order
     MxGroups g;
     g.offsets = ws.offsets, g.n_experts = E;
-    hipError_t e = launch_moe_top_k(logits, ws.route_w, ws.ids, T, E, top_k, s);
-    if (e == hipSuccess) e = launch_moe_sort(ws.ids, R, E, ws.offsets, ws.src_route, ws.dst_of_route, s);
-    if (e == hipSuccess) e = launch_quantize_mxfp4(x, dtype, H, ws.xq, T, H, s);
+    hipError_t e = launch_mxfp4_route(x, dtype, logits, T, H, E, top_k, ws.route_w, ws.ids, ws.offsets, ws.src_route,
+                                      ws.dst_of_route, ws.xq, s);
     if (e != hipSuccess) return launched(e, "moe_mxfp4_ffn routing");
     g.src_route = ws.src_route, g.top_k = top_k, g.x_rows = T;
     if ((e = launch_mxfp4_swiglu(w_gate, w_up, ws.xq, ws.midq, H, I, R, g, s)) != hipSuccess)

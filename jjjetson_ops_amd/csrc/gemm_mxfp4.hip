@@ -26,14 +26,6 @@ struct MxTiled {
     MxGroups g;
 };
 
-// acc += W . X^T of step U of a stage: byte U of the scale registers.
-template <int U>
-__device__ __forceinline__ f32x4v mx_mfma_step(u32x4v w, u32x4v x, f32x4v acc, uint32_t sw, uint32_t sx) {
-    const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-    const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, U, (int)sw, U, (int)sx);
-}
-
 // WN x WT waves of RT tiles of 16 weight rows x TT tiles of 16 tokens each.
 template <int RT_, int TT_, int WN_, int WT_>
 struct MxTile {
@@ -44,7 +36,7 @@ struct MxTile {
     static constexpr int kScaleRows = (kRows + kThreads - 1) / kThreads;  // rows a thread
     static constexpr int kStage = kRows * 128;
     static constexpr int kLds = 2 * (kStage + kRows * 16) + kRows * 4;
-    static_assert(kRows % (8 * kWaves) == 0 && kRowsN % 8 == 0 && kDma % 2 == 0, "whole DMA instructions");
+    static_assert(kRows % (8 * kWaves) == 0 && kRowsN % 8 == 0, "whole DMA instructions");
 };
 
 // A wave's outputs (from weight row n, token t on) through its own 4 KB of LDS, 16 tokens at a time:
@@ -120,16 +112,17 @@ __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) 
     const size_t w_first = (size_t)expert * p.N, w_all = (size_t)(GROUPED ? p.g.n_experts : 1) * p.N;
     const size_t x_all = p.g.src_route != nullptr ? p.g.x_rows : p.M;
 
-    // ---- the DMA: instruction i of a wave takes rows 8 * i + lane / 8, piece (lane % 8) ^ (lane / 8).  The
+    // ---- the DMA: instruction i of a wave takes run kDma * wave + i of 8 rows, a lane piece (lane % 8) ^ (row / 2 % 8) of
+    // row lane / 8.  The
     // rows' offsets stand in LDS: kept in registers they would spill, and a reload from scratch
     // waits for every DMA before it.
     const int t0 = GROUPED && p.g.src_route != nullptr ? 0 : first;
     for (int row = threadIdx.x; row < Tile::kRows; row += Tile::kThreads)
         lds_rows[row] = row < Tile::kRowsN ? (uint32_t)(weight_row(row) - n0) * half
                                            : (uint32_t)(token_row(row - Tile::kRowsN) - t0) * half;
-    const uint8_t *const w_base = p.w + (w_first + n0) * (size_t)half, *const x_base = p.x + (size_t)t0 * half;
-    const uint8_t *const w2_base = SWIGLU ? p.w2 + (w_first + n0) * (size_t)half : nullptr;
-    const uint32_t piece = 16 * ((lane & 7) ^ ((lane >> 4) & 3));
+    const uint64_t x_base = (uint64_t)p.x + (uint64_t)t0 * half, w_at0 = (uint64_t)(w_first + n0) * half;
+    const uint64_t w_base = (uint64_t)p.w + w_at0, w2_base = SWIGLU ? (uint64_t)p.w2 + w_at0 : w_base;
+    const uint32_t piece = 16 * ((lane & 7) ^ ((lane >> 4) & 3));  // of an even run of 8 rows; ^ 64 for an odd one
     // ---- and of the scales: one row, or kScaleRows
     const uint8_t *srow[Tile::kScaleRows];
 #pragma unroll
@@ -168,18 +161,23 @@ __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) 
     auto dma = [&](int st, int buffer) {
         const uint32_t left = 16u * (uint32_t)(nb - 8 * st);  // bytes of the row from the stage on
         const uint32_t most = left >= 128u ? 112u : left - 16u;
-        const uint32_t at[2] = {(uint32_t)min(piece, most), (uint32_t)min(piece ^ 64u, most)};  // rows of an even, an odd instruction
+        const uint32_t even = min((uint32_t)piece, most), odd = min((uint32_t)piece ^ 64u, most);
         uint32_t off[Tile::kDma];
 #pragma unroll
-        for (int i = 0; i < Tile::kDma; ++i) off[i] = lds_rows[8 * (wave * Tile::kDma + i) + (lane >> 3)] + at[i & 1];
+        for (int i = 0; i < Tile::kDma; ++i)
+            off[i] = lds_rows[8 * (wave * Tile::kDma + i) + (lane >> 3)] + ((wave * Tile::kDma + i) & 1 ? odd : even);
 #pragma unroll
         for (int i = 0; i < Tile::kDma; ++i) {
             const int row8 = 8 * (wave * Tile::kDma + i);
-            const uint8_t *base = row8 >= Tile::kRowsN ? x_base : is_up(row8) ? w2_base : w_base;
             const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds0 + buffer * Tile::kStage + 128 * row8);
-            asm volatile("global_load_lds_dwordx4 %0, %1"
+            // Masks, not branches: a choice among captured addresses would go through scratch.
+            const uint64_t up = -(uint64_t)is_up(row8), x = -(uint64_t)(row8 >= Tile::kRowsN);
+            const uint64_t from = (x_base & x) + ((w_base + (up & (w2_base - w_base))) & ~x) + (uint64_t)st * 128;
+            // Five wait states: an SGPR that a VALU instruction wrote is not read by a load before, nor M0 in the
+            // next cycle, and the compiler does not count them for an asm statement.
+            asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
                          :
-                         : "v"(off[i]), "s"(base + (size_t)st * 128), "{m0}"(m0v)
+                         : "v"(off[i]), "s"(from), "{m0}"(m0v)
                          : "memory");
         }
     };
@@ -227,7 +225,7 @@ __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) 
             for (int tt = 0; tt < TT; ++tt) {
                 const u32x4v b = *reinterpret_cast<const u32x4v *>(at + (x_at + 16 * tt) * 128);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) acc[rt][tt] = mx_mfma_step<U>(a[rt], b, acc[rt][tt], sw[rt], sx[tt]);
+                for (int rt = 0; rt < RT; ++rt) acc[rt][tt] = mx_mfma<U, U>(a[rt], b, acc[rt][tt], sw[rt], sx[tt]);
             }
         };
         step(std::integral_constant<int, 0>{});
@@ -293,8 +291,19 @@ hipError_t run_tiled(MxTiled p, hipStream_t stream) {
     return hipErrorInvalidValue;
 }
 
-typedef MxTile<4, 8, 4, 2> Tile256;  // 256 rows x 256 tokens, 8 waves
-typedef MxTile<4, 4, 2, 2> Tile128;  // 128 x 128, 4 waves
+// Tiles of `tokens` tokens: 128 weight rows on four waves up to 128 tokens, 256 on eight above.
+template <bool SWIGLU>
+hipError_t run_tile(const MxTiled &p, int tokens, hipStream_t stream) {
+    switch (tokens) {
+        case 32: return run_tiled<MxTile<4, 1, 2, 2>, SWIGLU>(p, stream);
+        case 64: return run_tiled<MxTile<4, 2, 2, 2>, SWIGLU>(p, stream);
+        case 96: return run_tiled<MxTile<4, 3, 2, 2>, SWIGLU>(p, stream);
+        case 128: return run_tiled<MxTile<4, 4, 2, 2>, SWIGLU>(p, stream);
+        case 192: return run_tiled<MxTile<4, 6, 4, 2>, SWIGLU>(p, stream);
+        case 256: return run_tiled<MxTile<4, 8, 4, 2>, SWIGLU>(p, stream);
+    }
+    return hipErrorInvalidValue;
+}
 
 }  // namespace
 
@@ -306,14 +315,14 @@ bool mxfp4_tiled_accepts(int K, const MxGroups &g) {
 hipError_t launch_mxfp4_tiled(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
                               const MxGroups &groups, int tile, hipStream_t stream) {
     const MxTiled p{(const uint8_t *)w, nullptr, (const uint8_t *)xq, y, dtype, K, N, M, 0, 0, groups};
-    return tile == 256 ? run_tiled<Tile256, false>(p, stream) : run_tiled<Tile128, false>(p, stream);
+    return run_tile<false>(p, tile, stream);
 }
 
 hipError_t launch_mxfp4_tiled_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I,
                                      int M, const MxGroups &groups, int tile, hipStream_t stream) {
     const MxTiled p{(const uint8_t *)w_gate, (const uint8_t *)w_up, (const uint8_t *)xq, mid, JJO_DTYPE_F32, K, I, M,
                     0, 0, groups};
-    return tile == 256 ? run_tiled<Tile256, true>(p, stream) : run_tiled<Tile128, true>(p, stream);
+    return run_tile<true>(p, tile, stream);
 }
 
 namespace {

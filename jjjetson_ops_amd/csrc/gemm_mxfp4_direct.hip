@@ -3,11 +3,20 @@
 //
 //     y[t][n] = sum over blocks b of 2^(sw[n,b] + sx[t,b] - 254) * sum_j cw[n,b,j] * cx[t,b,j]
 //
-// One v_mfma_scale_f32_16x16x128 takes 16 rows x 16 tokens x four blocks: a lane's operand is
-// one block, 16 bytes as they lie in the matrix, and its scale operand that block's byte, so
-// nothing is unpacked.  Sums are fp32.  Bound by reading the weights (17/32 byte a value): a
-// workgroup's waves cut K between them, so that a small output still fills the chip with
-// loads in flight; the slices are added through LDS in slice order.
+// Bound by reading the weights (17/32 byte a value).  What that takes:
+//   * Addresses.  The instruction's operand has 16 rows in neighbouring lanes, so loading it as it is
+//     touches four rows in every four lanes, 64 cache tags a load instead of 16; with the
+//     activation's loads beside the weights' that was what the kernel waited for (114688 x 4096, 4
+//     tokens: 54 us, of which 13 the activation's loads and 10 the scales').  Here the 16 rows of an operand
+//     are 4 weight rows x 4 neighbouring blocks: lane 16 j + 4 a + b has row a, block 4 j + b of a chunk of 16
+//     blocks, so a load is 4 rows x 256 contiguous bytes.  The activation is held alike (4
+//     tokens x 4 blocks), and of the 16 x 16 products the ones wanted are those whose weight and
+//     activation blocks agree, a quarter: sum over b of acc[(a, b)][(t, b)].  The matrix cores idle
+//     anyway; the diagonal is summed once, at the end.
+//   * Loads in flight: a wave asks for all chunks of its slice (NC) before it multiplies the first; KW
+//     waves cut K between them, so that a small output still fills the chip.  Sums are fp32, the
+//     slices' added through LDS in slice order.
+//   * Scales: 16 bytes a lane, once per NC chunks, through the wave's own LDS.
 #include <hip/hip_runtime.h>
 
 #include "mxfp4_mm.hpp"
@@ -15,68 +24,16 @@
 namespace jjo {
 namespace {
 
-constexpr int kFusedMaxK = kMxFusedMaxK;
-
 struct MxProblem {
     const uint8_t *w, *w2, *x;  // w2: the up matrix (SwiGLU)
     void *y;                    // outputs, or the MXFP4 rows of the SwiGLU form
     int dtype;
     int K, N, M;
-    int token_tiles;  // of the launch; workgroup i has token tile i % token_tiles
+    int tiles_n;  // row tiles of the launch
     MxGroups g;
 };
 
-// Operands of U steps of TILES tiles of 16 rows.  A row's scale bytes of the U steps are one load:
-// dword u holds the bytes of step u's four lane groups.  Rows shorter than that (and only
-// they) fetch each byte where it is used.
-template <int TILES, int U>
-struct MxChunk {
-    u32x4v v[U][TILES];
-    uint32_t s[TILES][U];
-};
-template <int TILES, int U>
-__device__ __forceinline__ void load_chunk(MxChunk<TILES, U> &c, const uint8_t *const (&rows)[TILES],
-                                           const uint8_t *const (&scales)[TILES], int step, int nb) {
-    const int q = (threadIdx.x & 63) >> 4;
-    if (nb >= 4 * U) {
-        const int at = min(4 * step, nb - 4 * U);  // the last chunk's bytes end with the row
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) __builtin_memcpy(c.s[t], scales[t] + at, 4 * U);  // whatever the alignment
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int blk = min(4 * (step + u) + q, nb - 1);
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) c.v[u][t] = *reinterpret_cast<const u32x4v *>(rows[t] + (size_t)blk * 16);
-    }
-}
-// The chunk's scale bytes to their places: shifted where the row ends inside the chunk (zeros
-// behind it), or fetched.
-template <int TILES, int U>
-__device__ __forceinline__ void place_scales(MxChunk<TILES, U> &c, const uint8_t *const (&scales)[TILES], int step,
-                                             int nb) {
-    const int over = 4 * step + 4 * U - nb;  // uniform
-    if (over <= 0) return;
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-        if (nb >= 4 * U) {
-            unsigned __int128 b = 0;
-            __builtin_memcpy(&b, c.s[t], 4 * U);
-            b >>= 8 * over;
-            __builtin_memcpy(c.s[t], &b, 4 * U);
-        } else {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                c.s[t][u] = 0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    c.s[t][u] |= (uint32_t)scales[t][min(4 * (step + u) + k, nb - 1)] << (8 * k);
-            }
-        }
-    }
-}
-
-// One wave's 1024 values of the fused activation, 16 a lane, to codes and scales in LDS.
+// 16 consecutive values of the fused activation.
 template <class T>
 __device__ __forceinline__ void load16(const T *p, float *x) {
     constexpr int kVec = 16 / sizeof(T);
@@ -88,174 +45,232 @@ __device__ __forceinline__ void load16(const T *p, float *x) {
     }
 }
 
-// RT tiles of 16 weight rows x TT tiles of 16 tokens, W waves over K, U steps of 128 in registers
-// and U more in flight.  SWIGLU: RT = 4, two tiles of gate rows and the two of the same up
-// rows.  XT: void (x is MXFP4), or the type of the one token's row, which every wave quantizes
-// for its own slice of K.
-template <int RT, int TT, int W, int U, bool GROUPED, bool SWIGLU, class XT>
-__global__ __launch_bounds__(64 * W) void mxfp4_direct_kernel(MxProblem p) {
+__device__ __forceinline__ float quad_sum(float v) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xb1, 0xf, 0xf, true));  // lane ^ 1
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4e, 0xf, 0xf, true));  // lane ^ 2
+    return v;
+}
+
+// A wave has 16 weight rows (4 operands of 4 rows) x TG operands of 4 tokens and NC chunks of 512 values at
+// once; KW waves cut K between them, RW have rows of their own.  SWIGLU: RW = 4, two times 16 gate
+// rows and the two times 16 up rows beside them.  XT: void (x is MXFP4), or the type of the one
+// token's row, which every wave quantizes for its own slice of K.
+template <int TG, int KW, int RW, int NC, bool GROUPED, bool SWIGLU, class XT>
+__global__ __launch_bounds__(64 * KW * RW) void mxfp4_direct_kernel(MxProblem p) {
     constexpr bool kFused = !std::is_void_v<XT>;
-    constexpr int kPieces = 2;  // of 1024 values in a wave's slice of the fused form
-    __shared__ f32x4v part[W][RT * TT][64];
-    __shared__ u32x4v x_codes[kFused ? W : 1][kFused ? 32 * kPieces : 1];
-    __shared__ uint8_t x_scales[kFused ? W : 1][kFused ? 32 * kPieces : 1];
+    constexpr int W = KW * RW, kTokens = 4 * TG;
+    constexpr int kPieces = NC == 1 ? 1 : NC == 2 ? 2 : 4;  // of 16 scale bytes a row
+    constexpr int kScaleRows = kFused ? 16 : 16 + kTokens, kAtOnce = 64 / kPieces;  // rows a load instruction
+    constexpr int kScaleLoads = (kScaleRows + kAtOnce - 1) / kAtOnce;
+    __shared__ __align__(16) uint8_t s_scales[W][kScaleLoads * kAtOnce][16 * kPieces];
+    __shared__ __align__(16) uint8_t x_codes[kFused ? W : 1][kFused ? 256 * NC : 16];
+    __shared__ uint8_t x_scales[kFused ? W : 1][kFused ? 16 * NC : 1];
+    __shared__ float part[W][TG][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r16 = lane & 15, q = lane >> 4;
-    const int tile_t = (int)(blockIdx.x % (unsigned)p.token_tiles), tile_n = (int)(blockIdx.x / (unsigned)p.token_tiles);
-    int expert = 0, first = tile_t * 16 * TT, end = p.M;
+    const int kw = wave % KW, rw = wave / KW;
+    const int la = lane >> 2 & 3, lb = lane & 3, lj = lane >> 4, blk0 = 4 * lj + lb;
+    // Row tiles vary fastest: the eight XCDs, which take workgroups in turn, then have the same
+    // share of the token tiles that exist.
+    const int tile_t = (int)(blockIdx.x / (unsigned)p.tiles_n), tile_n = (int)(blockIdx.x % (unsigned)p.tiles_n);
+    int expert = 0, first = tile_t * kTokens, end = p.M;
     if constexpr (GROUPED) {
-        if (!mx_expert_tile(p.g.offsets, p.g.n_experts, p.M, 16 * TT, tile_t, expert, first, end)) return;
+        if (!mx_expert_tile(p.g.offsets, p.g.n_experts, p.M, kTokens, tile_t, expert, first, end)) return;
     }
-    constexpr int kRows = SWIGLU ? 32 : 16 * RT;  // weight rows of one matrix
-    const int n0 = tile_n * kRows;
-    const int nb = p.K / kQK, steps = (nb + 3) / 4;
-    const int s_beg = (int)((int64_t)steps * wave / W), s_end = (int)((int64_t)steps * (wave + 1) / W);
+    static_assert(!SWIGLU || RW == 4, "32 gate rows and the same 32 up rows");
+    const int n0 = SWIGLU ? 32 * tile_n + 16 * (rw & 1) : 16 * (tile_n * RW + rw);
+    const int nb = p.K / kQK, chunks = (nb + 15) / 16;
+    const int c_beg = chunks * kw / KW, c_end = chunks * (kw + 1) / KW;
     const size_t half = (size_t)p.K / 2;
 
-    const uint8_t *wr[RT], *ws[RT];
+    const uint8_t *const w = SWIGLU && rw >= 2 ? p.w2 : p.w;
+    const size_t w_first = (size_t)expert * p.N, w_all = (size_t)(GROUPED ? p.g.n_experts : 1) * p.N;
+    const uint8_t *w_row[4];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const uint8_t *m = SWIGLU && rt >= 2 ? p.w2 : p.w;
-        const int tile = SWIGLU ? rt & 1 : rt;
-        const size_t row = (size_t)expert * p.N + min(n0 + 16 * tile + r16, p.N - 1);
-        const size_t all = (size_t)(GROUPED ? p.g.n_experts : 1) * p.N;
-        wr[rt] = m + row * half;
-        ws[rt] = m + all * half + row * nb;
-    }
-    const uint8_t *xr[TT], *xs[TT];
+    for (int g = 0; g < 4; ++g) w_row[g] = w + (w_first + min(n0 + 4 * g + la, p.N - 1)) * half;
+    // The token of row `r` of the tile, and x's rows.
+    const bool routed = GROUPED && p.g.src_route != nullptr;
+    const size_t x_all = routed ? p.g.x_rows : p.M;
+    auto token = [&](int r) {
+        const int t = min(first + r, end - 1);
+        return routed ? min(max(p.g.src_route[t] / p.g.top_k, 0), p.g.x_rows - 1) : t;
+    };
+    const uint8_t *x_row[TG], *s_row[kScaleLoads];
     if constexpr (!kFused) {
-        const size_t x_rows = p.g.src_route != nullptr ? p.g.x_rows : p.M;
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-            int t = min(first + 16 * tt + r16, end - 1);
-            if (GROUPED && p.g.src_route != nullptr) t = min(max(p.g.src_route[t] / p.g.top_k, 0), p.g.x_rows - 1);
-            xr[tt] = p.x + (size_t)t * half;
-            xs[tt] = p.x + x_rows * half + (size_t)t * nb;
-        }
+        for (int t = 0; t < TG; ++t) x_row[t] = p.x + (size_t)token(4 * t + la) * half;
     }
-    f32x4v acc[RT][TT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < kScaleLoads; ++i) {
+        const int r = i * kAtOnce + lane / kPieces;
+        if (kFused || r < 16) s_row[i] = w + w_all * half + (w_first + min(n0 + min(r, 15), p.N - 1)) * nb;
+        else s_row[i] = p.x + x_all * half + (size_t)token(min(r - 16, kTokens - 1)) * nb;
+    }
 
-    MxChunk<RT, U> w;
-    MxChunk<TT, U> x;
-    if constexpr (kFused) {
-        // The token's values are asked for before the weights: loads return in order.
-        typedef std::conditional_t<kFused, XT, float> T;
-        const T *src = (const T *)p.x + 128 * (size_t)s_beg;
-        const int live = min(128 * (s_end - s_beg), p.K - 128 * s_beg);  // a multiple of 32
-        float v[kPieces][16];
+    f32x4v acc[4][TG];
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i)
-            if (1024 * i + 16 * lane < live) load16(src + 1024 * i + 16 * lane, v[i]);
-        if (s_beg < s_end) load_chunk(w, wr, ws, s_beg, nb);
+    for (int g = 0; g < 4; ++g)
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            if (1024 * i >= 128 * (s_end - s_beg)) break;
-            const bool in = 1024 * i + 16 * lane < live;
-            uint32_t m = 0;
-            if (in) {
-                m = mx_amax8(v[i]);
-                const uint32_t o = mx_amax8(v[i] + 8);
+        for (int t = 0; t < TG; ++t) acc[g][t] = f32x4v{0.f, 0.f, 0.f, 0.f};
+
+    for (int c0 = c_beg; c0 < c_end; c0 += NC) {
+        // ---- everything of NC chunks is asked for, in the order of its use (loads return in order);
+        // chunks behind the slice are its last one again
+        float v[kFused ? (NC + 1) / 2 : 1][16];
+        if constexpr (kFused) {  // 16 values a lane; behind the row's end its last ones (they meet zero weights)
+            typedef std::conditional_t<kFused, XT, float> T;
+#pragma unroll
+            for (int i = 0; i < (NC + 1) / 2; ++i)
+                load16((const T *)p.x + min(512 * c0 + 1024 * i + 16 * lane, p.K - 32 + 16 * (lane & 1)), v[i]);
+        }
+        u32x4v sv[kScaleLoads], a[NC][4], b[NC][TG];
+        const int piece = lane % kPieces, s_at = min(16 * (c0 + piece), nb - 16);
+        // The last 16 bytes of a row where it ends earlier: behind codes, so also before a short row's start.
+#pragma unroll
+        for (int i = 0; i < kScaleLoads; ++i) __builtin_memcpy(&sv[i], s_row[i] + s_at, 16);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const size_t at = 16 * (size_t)min(16 * min(c0 + c, c_end - 1) + blk0, nb - 1);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) a[c][g] = *reinterpret_cast<const u32x4v *>(w_row[g] + at);
+            if constexpr (!kFused) {
+#pragma unroll
+                for (int t = 0; t < TG; ++t) b[c][t] = *reinterpret_cast<const u32x4v *>(x_row[t] + at);
+            }
+        }
+        // ---- scales, and the fused activation, to the wave's LDS
+        if constexpr (kFused) {
+#pragma unroll
+            for (int i = 0; i < (NC + 1) / 2; ++i) {
+                uint32_t m = mx_amax8(v[i]), o = mx_amax8(v[i] + 8);
                 m = o > m ? o : m;
+                o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, true);  // lane ^ 1
+                m = o > m ? o : m;
+                const uint32_t s = mx_scale_byte(m);
+                if (NC % 2 == 0 || 1024 * i + 16 * lane < 512 * NC) {
+                    *reinterpret_cast<uint2 *>(&x_codes[wave][512 * i + 8 * lane]) =
+                        make_uint2(mx_codes8(v[i], s), mx_codes8(v[i] + 8, s));
+                    if ((lane & 1) == 0) x_scales[wave][32 * i + (lane >> 1)] = (uint8_t)s;
+                }
             }
-            const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, true);  // lane ^ 1
-            m = o > m ? o : m;
-            const uint32_t s = mx_scale_byte(m);
-            uint2 c = make_uint2(0u, 0u);
-            if (in) c = make_uint2(mx_codes8(v[i], s), mx_codes8(v[i] + 8, s));
-            reinterpret_cast<uint2 *>(&x_codes[wave][32 * i])[lane] = c;
-            if ((lane & 1) == 0) x_scales[wave][32 * i + (lane >> 1)] = (uint8_t)s;
         }
-    } else if (s_beg < s_end) {
-        load_chunk(w, wr, ws, s_beg, nb);
-        load_chunk(x, xr, xs, s_beg, nb);
-    }
-    for (int s = s_beg; s < s_end; s += U) {
-        MxChunk<RT, U> w_next;
-        MxChunk<TT, U> x_next;
-        if (s + U < s_end) {
-            load_chunk(w_next, wr, ws, s + U, nb);
-            if constexpr (!kFused) load_chunk(x_next, xr, xs, s + U, nb);
-        }
-        place_scales(w, ws, s, nb);
-        if constexpr (!kFused) place_scales(x, xs, s, nb);
+        const int over = 16 * (c0 + piece) + 16 - nb;  // zeros behind the row's end
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (s + u >= s_end) break;
-            if (4 * (s + u) + 4 > nb) {  // the row ends inside the step (K % 128)
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-                    if (4 * (s + u) + q >= nb) w.v[u][rt] = u32x4v{0u, 0u, 0u, 0u};
+        for (int i = 0; i < kScaleLoads; ++i) {
+            if (16 * (c0 + kPieces) > nb) {
+                unsigned __int128 s;
+                __builtin_memcpy(&s, &sv[i], 16);
+                s = over >= 16 ? 0 : s >> (8 * max(over, 0));
+                __builtin_memcpy(&sv[i], &s, 16);
             }
-            u32x4v xv[TT];
-            uint32_t sx[TT];
+            *reinterpret_cast<u32x4v *>(&s_scales[wave][i * kAtOnce + lane / kPieces][16 * piece]) = sv[i];
+        }
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt) {
+        for (int c = 0; c < NC; ++c) {
+            if (c0 + c >= c_end) break;
+            if (16 * (c0 + c) + 16 > nb) {  // the row ends inside the chunk: zero weights behind it
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    if (16 * (c0 + c) + blk0 >= nb) a[c][g] = u32x4v{0u, 0u, 0u, 0u};
+            }
+            uint32_t sw[4], sx[TG];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) sw[g] = s_scales[wave][4 * g + la][16 * c + blk0];
+#pragma unroll
+            for (int t = 0; t < TG; ++t) {
                 if constexpr (kFused) {
-                    xv[tt] = x_codes[wave][4 * (s + u - s_beg) + q];
-                    sx[tt] = x_scales[wave][4 * (s + u - s_beg) + q];
+                    b[c][t] = *reinterpret_cast<const u32x4v *>(&x_codes[wave][16 * (16 * c + blk0)]);
+                    sx[t] = x_scales[wave][16 * c + blk0];
                 } else {
-                    xv[tt] = x.v[u][tt];
-                    sx[tt] = x.s[tt][u] >> (8 * q);
+                    sx[t] = s_scales[wave][16 + 4 * t + la][16 * c + blk0];
                 }
             }
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
+            for (int g = 0; g < 4; ++g)
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
-                    acc[rt][tt] = mx_mfma(w.v[u][rt], xv[tt], acc[rt][tt], w.s[rt][u] >> (8 * q), sx[tt]);
+                for (int t = 0; t < TG; ++t) acc[g][t] = mx_mfma<0, 0>(a[c][g], b[c][t], acc[g][t], sw[g], sx[t]);
         }
-        w = w_next;
-        if constexpr (!kFused) x = x_next;
+        __builtin_amdgcn_wave_barrier();
     }
+
+    // ---- acc[g][t] of lane 16 q + 4 t' + b' has (row 4 g + q, block group i) in register i for token 4 t + t',
+    // block group b': register b' of it, summed over the four lanes of b', is the output.  Lane 16 q + 4 t' + b' keeps
+    // row 4 b' + q.
+    float r[TG];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int t = 0; t < TG; ++t) {
+        float s[4];
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt) part[wave][rt * TT + tt][lane] = acc[rt][tt];
-    __syncthreads();
-    auto total = [&](int tile) {
-        f32x4v v = part[0][tile][lane];
+        for (int g = 0; g < 4; ++g) {
+            const f32x4v d = acc[g][t];
+            s[g] = quad_sum(lb == 0 ? d[0] : lb == 1 ? d[1] : lb == 2 ? d[2] : d[3]);
+        }
+        r[t] = lb == 0 ? s[0] : lb == 1 ? s[1] : lb == 2 ? s[2] : s[3];
+    }
+    if constexpr (W > 1) {
 #pragma unroll
-        for (int k = 1; k < W; ++k) v += part[k][tile][lane];
-        return v;
+        for (int t = 0; t < TG; ++t) part[wave][t][lane] = r[t];
+        __syncthreads();
+    }
+    auto total = [&](int row_wave, int t) {
+        float s = part[row_wave * KW][t][lane];
+#pragma unroll
+        for (int k = 1; k < KW; ++k) s += part[row_wave * KW + k][t][lane];
+        return s;
     };
+    const int row = 4 * lb + lj;
     if constexpr (SWIGLU) {
+        // A block of 32 values of a token is two values each of 16 lanes (all but bits 2, 3 of the lane).
         uint8_t *codes = (uint8_t *)p.y, *scales = codes + (size_t)p.M * (p.N / 2);
-        for (int tt = wave; tt < TT; tt += W) {
-            const f32x4v gate[2] = {total(tt), total(TT + tt)}, up[2] = {total(2 * TT + tt), total(3 * TT + tt)};
-            const int t = first + 16 * tt + r16;
-            const size_t row = min(t, p.M - 1);
-            mx_swiglu_store(gate, up, codes + row * (p.N / 2) + n0 / 2, scales + row * (p.N / kQK) + n0 / kQK, t < end);
+        const int n = 32 * tile_n;
+        for (int t = wave; t < TG; t += W) {
+            const int tok = first + 4 * t + la;
+            float h[8] = {mx_silu_mul(total(0, t), total(2, t)), mx_silu_mul(total(1, t), total(3, t)), 0, 0, 0, 0, 0, 0};
+            uint32_t m = mx_amax8(h);
+#pragma unroll
+            for (int d : {1, 2, 16, 32}) {
+                const uint32_t o = (uint32_t)__shfl_xor((int)m, d);
+                m = o > m ? o : m;
+            }
+            const uint32_t s = mx_scale_byte(m);
+            uint32_t c = mx_codes8(h, s);
+            c |= (uint32_t)__shfl_xor((int)c, 16) << 8;  // of row ^ 1: bits 8..15
+            if (tok >= end || (lj & 1) != 0) continue;
+            uint8_t *to = codes + (size_t)tok * (p.N / 2) + n / 2 + row / 2;
+            to[0] = (uint8_t)((c & 15u) | (c >> 8 & 15u) << 4);
+            to[8] = (uint8_t)((c >> 4 & 15u) | (c >> 12 & 15u) << 4);
+            if (row == 0) scales[(size_t)tok * (p.N / kQK) + n / kQK] = (uint8_t)s;
         }
     } else {
-        const bool vec = p.N % 4 == 0;  // y is 16-byte aligned
-        for (int tile = wave; tile < RT * TT; tile += W) {
-            const f32x4v v = total(tile);
-            const int t = first + 16 * (tile % TT) + r16, n = n0 + 16 * (tile / TT) + 4 * q;
-            if (t >= end || n >= p.N) continue;
-            const int row = GROUPED && p.g.route_dst != nullptr ? p.g.route_dst[t] : t;
-            mx_store4(p.y, p.dtype, (size_t)row * p.N + n, v, p.N - n, vec);
+#pragma unroll
+        for (int t = 0; t < TG; ++t) {
+            if (t % KW != kw) continue;
+            const float out = W > 1 ? total(rw, t) : r[t];
+            const int tok = first + 4 * t + la, n = n0 + row;
+            if (tok >= end || n >= p.N) continue;
+            const size_t to = (size_t)(GROUPED && p.g.route_dst != nullptr ? p.g.route_dst[tok] : tok) * p.N + n;
+            if (p.dtype == JJO_DTYPE_F32) ((float *)p.y)[to] = out;
+            else if (p.dtype == JJO_DTYPE_F16) ((_Float16 *)p.y)[to] = (_Float16)out;
+            else ((__bf16 *)p.y)[to] = (__bf16)out;
         }
     }
 }
 
-template <int RT, int TT, int W, int U, bool SWIGLU, class XT = void>
+template <int TG, int KW, int RW, int NC, bool SWIGLU, class XT = void>
 hipError_t run_direct(MxProblem p, hipStream_t stream) {
-    const int rows = SWIGLU ? 32 : 16 * RT;
+    constexpr int rows = SWIGLU ? 32 : 16 * RW, threads = 64 * KW * RW;
     // token tiles of M rows, and one more for each expert that can have a rest
-    p.token_tiles = (p.M + 16 * TT - 1) / (16 * TT) + (p.g.offsets != nullptr ? std::min(p.g.n_experts, p.M) : 0);
-    const int64_t wgs = (int64_t)p.token_tiles * ((p.N + rows - 1) / rows);
-    if (wgs * 64 * W >= 1LL << 32) return hipErrorInvalidConfiguration;
-    const dim3 grid((unsigned)wgs), block(64 * W);
+    const int64_t token_tiles = (p.M + 4 * TG - 1) / (4 * TG) + (p.g.offsets != nullptr ? std::min(p.g.n_experts, p.M) : 0);
+    p.tiles_n = (p.N + rows - 1) / rows;
+    const int64_t wgs = token_tiles * p.tiles_n;
+    if (wgs * threads >= 1LL << 32) return hipErrorInvalidConfiguration;
+    const dim3 grid((unsigned)wgs), block(threads);
     if constexpr (!std::is_void_v<XT>)
-        hipLaunchKernelGGL((mxfp4_direct_kernel<RT, TT, W, U, false, false, XT>), grid, block, 0, stream, p);
+        hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, NC, false, false, XT>), grid, block, 0, stream, p);
     else if (p.g.offsets != nullptr)
-        hipLaunchKernelGGL((mxfp4_direct_kernel<RT, TT, W, U, true, SWIGLU, void>), grid, block, 0, stream, p);
+        hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, NC, true, SWIGLU, void>), grid, block, 0, stream, p);
     else if constexpr (!SWIGLU)
-        hipLaunchKernelGGL((mxfp4_direct_kernel<RT, TT, W, U, false, false, void>), grid, block, 0, stream, p);
+        hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, NC, false, false, void>), grid, block, 0, stream, p);
     else
         return hipErrorInvalidValue;
     return hipGetLastError();
@@ -270,21 +285,41 @@ int mean_rows(int M, const MxGroups &g) {
 
 }  // namespace
 
+int form = 0;
+
 hipError_t launch_mxfp4_direct(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
                                const MxGroups &groups, hipStream_t stream) {
     const MxProblem p{(const uint8_t *)w, nullptr, (const uint8_t *)xq, y, dtype, K, N, M, 0, groups};
-    const int mean = mean_rows(M, groups), steps = (K + 127) / 128;
-    if (mean <= 16) return steps >= 64 ? run_direct<1, 1, 8, 4, false>(p, stream) : run_direct<1, 1, 4, 4, false>(p, stream);
-    if (mean <= 32) return steps >= 64 ? run_direct<1, 2, 8, 4, false>(p, stream) : run_direct<1, 2, 4, 4, false>(p, stream);
-    return run_direct<2, 4, 4, 2, false>(p, stream);
+    const int mean = mean_rows(M, groups);
+    switch (form) {
+#define F(n, ...) case n: return run_direct<__VA_ARGS__, false>(p, stream);
+        F(1, 1, 4, 1, 2) F(2, 1, 8, 1, 2) F(3, 1, 2, 2, 2) F(4, 1, 1, 4, 4) F(5, 1, 8, 1, 4) F(6, 1, 4, 1, 4) F(7, 1, 2, 4, 4) F(8, 1, 4, 2, 2) F(9, 1, 2, 2, 4)
+        F(11, 4, 4, 1, 2) F(12, 4, 8, 1, 2) F(13, 4, 2, 2, 2) F(14, 4, 1, 4, 3) F(15, 4, 8, 1, 3)  F(16, 4, 4, 1, 4) F(17, 4, 1, 4, 2) F(18, 4, 4, 2, 2) F(19, 4, 1, 2, 3)
+        F(21, 6, 4, 1, 2) F(22, 6, 8, 1, 2) F(23, 6, 8, 1, 1) F(24, 6, 4, 2, 1) F(25, 6, 4, 2, 2) F(26, 6, 8, 2, 1)
+        F(31, 2, 4, 1, 2) F(32, 2, 8, 1, 2) F(33, 2, 4, 2, 2) F(34, 2, 4, 1, 1)
+        F(41, 8, 4, 1, 1) F(42, 8, 8, 1, 1) F(43, 8, 8, 1, 2) F(44, 8, 4, 2, 1)
+#undef F
+    }
+    if (mean <= 4) return run_direct<1, 4, 1, 2, false>(p, stream);
+    if (mean <= 16) return run_direct<4, 4, 1, 2, false>(p, stream);
+    return run_direct<8, 4, 1, 1, false>(p, stream);
 }
 
 hipError_t launch_mxfp4_direct_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I,
                                       int M, const MxGroups &groups, hipStream_t stream) {
     const MxProblem p{(const uint8_t *)w_gate, (const uint8_t *)w_up, (const uint8_t *)xq, mid, JJO_DTYPE_F32, K, I, M,
                       0, groups};
-    if (mean_rows(M, groups) <= 16) return run_direct<4, 1, 4, 2, true>(p, stream);
-    return run_direct<4, 2, 4, 2, true>(p, stream);
+    const int mean = mean_rows(M, groups);
+    switch (form) {
+#define F(n, ...) case n: return run_direct<__VA_ARGS__, true>(p, stream);
+        F(1, 1, 2, 4, 2) F(2, 1, 4, 4, 2) F(3, 1, 2, 4, 4) F(4, 1, 1, 4, 2) F(5, 1, 1, 4, 4) F(6, 1, 4, 4, 1)
+        F(11, 4, 2, 4, 2) F(12, 4, 4, 4, 2) F(13, 4, 1, 4, 2) F(14, 4, 1, 4, 4) F(15, 4, 4, 4, 1) F(16, 4, 2, 4, 1)
+        F(21, 6, 2, 4, 2) F(22, 6, 1, 4, 2) F(23, 6, 2, 4, 1) F(24, 8, 1, 4, 1) F(25, 8, 2, 4, 1)
+#undef F
+    }
+    if (mean <= 4) return run_direct<1, 2, 4, 2, true>(p, stream);
+    if (mean <= 16) return run_direct<4, 2, 4, 2, true>(p, stream);
+    return run_direct<8, 2, 4, 1, true>(p, stream);
 }
 
 hipError_t launch_mxfp4_gemv(const void *w, const void *x, int x_dtype, void *y, int y_dtype, int K, int N,
@@ -292,7 +327,12 @@ hipError_t launch_mxfp4_gemv(const void *w, const void *x, int x_dtype, void *y,
     const MxProblem p{(const uint8_t *)w, nullptr, (const uint8_t *)x, y, y_dtype, K, N, 1, 0, MxGroups{}};
     return mx_by_dtype(x_dtype, [&](auto tag) {
         using T = typename decltype(tag)::type;
-        return K > 8192 ? run_direct<1, 1, 8, 4, false, T>(p, stream) : run_direct<1, 1, 4, 4, false, T>(p, stream);
+        switch (form) {
+#define F(n, ...) case n: return run_direct<__VA_ARGS__, false, T>(p, stream);
+        F(1, 1, 4, 1, 2) F(2, 1, 8, 1, 2) F(3, 1, 8, 1, 1) F(4, 1, 2, 1, 4) F(5, 1, 2, 2, 4) F(6, 1, 4, 2, 2) F(7, 1, 8, 1, 3) F(8, 1, 8, 1, 4) F(9, 1, 4, 1, 4)
+#undef F
+        }
+        return run_direct<1, 4, 1, 2, false, T>(p, stream);
     });
 }
 

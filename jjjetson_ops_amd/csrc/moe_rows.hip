@@ -12,6 +12,7 @@
 // the store), and nothing is added with atomics, so a result does not depend on timing.
 #include <hip/hip_runtime.h>
 
+#include "moe_top_k.hpp"
 #include "mxfp4_common.hpp"
 
 namespace jjo {
@@ -137,14 +138,14 @@ __global__ __launch_bounds__(256) void dispatch_rows_kernel(const int32_t *__res
 // id and one LDS add per distinct id.
 constexpr int kChunk = 1024;
 
-__global__ __launch_bounds__(256) void moe_sort_kernel(const int32_t *__restrict__ ids, int R, int n_experts,
-                                                       int32_t *__restrict__ offsets, int32_t *__restrict__ src_route,
-                                                       int32_t *__restrict__ dst_of_route) {
+__device__ __forceinline__ void sort_chunk(int chunk, const int32_t *__restrict__ ids, int R, int n_experts,
+                                           int32_t *__restrict__ offsets, int32_t *__restrict__ src_route,
+                                           int32_t *__restrict__ dst_of_route) {
     __shared__ int s_all[1024], s_before[1024];
     __shared__ int s_wave[4][1024];  // the chunk's routes per wave, then each wave's next position
     __shared__ int s_part[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int c0 = blockIdx.x * kChunk;
+    const int c0 = chunk * kChunk;
     const int bits = 32 - __builtin_clz(n_experts);
     for (int e = tid; e < 1024; e += 256) {
         s_all[e] = s_before[e] = 0;
@@ -184,9 +185,8 @@ __global__ __launch_bounds__(256) void moe_sort_kernel(const int32_t *__restrict
     }
     __syncthreads();
     const int last = s_all[n_experts - 1];
-    __syncthreads();
     expert_bases(s_all, s_part);
-    if (blockIdx.x == 0) {
+    if (chunk == 0) {
         for (int e = tid; e < n_experts; e += 256) offsets[e] = s_all[e];
         if (tid == 0) offsets[n_experts] = s_all[n_experts - 1] + last;
     }
@@ -212,6 +212,73 @@ __global__ __launch_bounds__(256) void moe_sort_kernel(const int32_t *__restrict
         }
         if (r < R) dst_of_route[r] = pos;
         if (live && lane == 63 - __builtin_clzll(grp)) mine[e] = pos + 1;  // after every lane's read: one wave
+    }
+}
+
+__global__ __launch_bounds__(256) void moe_sort_kernel(const int32_t *__restrict__ ids, int R, int n_experts,
+                                                       int32_t *__restrict__ offsets, int32_t *__restrict__ src_route,
+                                                       int32_t *__restrict__ dst_of_route) {
+    sort_chunk(blockIdx.x, ids, R, n_experts, offsets, src_route, dst_of_route);
+}
+
+// The sort and the quantizer of x (n8 groups of eight values) in one launch: neither needs the other.
+template <class T>
+__global__ __launch_bounds__(256) void sort_quantize_kernel(const int32_t *__restrict__ ids, int R, int n_experts,
+                                                            int32_t *__restrict__ offsets,
+                                                            int32_t *__restrict__ src_route,
+                                                            int32_t *__restrict__ dst_of_route, int chunks,
+                                                            const T *__restrict__ x, int64_t n8,
+                                                            uint8_t *__restrict__ xq) {
+    if ((int)blockIdx.x < chunks) {
+        sort_chunk(blockIdx.x, ids, R, n_experts, offsets, src_route, dst_of_route);
+        return;
+    }
+    const int64_t i = (int64_t)(blockIdx.x - chunks) * 256 + threadIdx.x;
+    if (i < n8) mx_quantize8(x + 8 * i, i, n8, xq);
+}
+
+// Few routes: workgroup 0 selects every token's experts (a wave per token) and places the routes, each
+// thread counting those before its own; the other workgroups quantize x meanwhile.
+constexpr int kRouteOne = 512;
+
+template <class T, int PER>
+__global__ __launch_bounds__(1024) void route_quantize_kernel(const float *__restrict__ logits, int num_tokens,
+                                                              int num_experts, int top_k, float *__restrict__ route_w,
+                                                              int32_t *__restrict__ ids, int32_t *__restrict__ offsets,
+                                                              int32_t *__restrict__ src_route,
+                                                              int32_t *__restrict__ dst_of_route,
+                                                              const T *__restrict__ x, int64_t n8,
+                                                              uint8_t *__restrict__ xq) {
+    if (blockIdx.x > 0) {
+        const int64_t i = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x;
+        if (i < n8) mx_quantize8(x + 8 * i, i, n8, xq);
+        return;
+    }
+    __shared__ int s_ids[kRouteOne];
+    __shared__ float s_w[kRouteOne];
+    const int R = num_tokens * top_k, tid = threadIdx.x, wave = tid >> 6;
+    for (int t = wave; t < num_tokens; t += 16)
+        top_k_token<PER>(logits + (size_t)t * num_experts, num_experts, top_k, s_w + t * top_k, s_ids + t * top_k,
+                         tid & 63);
+    __syncthreads();
+    // Threads 0..511: the routes; 512..: the experts' offsets.
+    if (tid < R) {
+        const int e = s_ids[tid];
+        int pos = 0;
+        for (int j = 0; j < R; ++j) {
+            const int o = s_ids[j];
+            pos += (o < e) | ((o == e) & (j < tid));
+        }
+        dst_of_route[tid] = pos;
+        src_route[pos] = tid;
+        route_w[tid] = s_w[tid];
+        ids[tid] = e;
+    }
+    for (int e = tid - kRouteOne; e <= num_experts; e += 512) {
+        if (e < 0) break;
+        int c = 0;
+        for (int j = 0; j < R; ++j) c += s_ids[j] < e;
+        offsets[e] = c;
     }
 }
 
@@ -329,6 +396,34 @@ hipError_t launch_moe_sort(const int32_t *ids, int n_routes, int n_experts, int3
     hipLaunchKernelGGL(moe_sort_kernel, dim3((unsigned)((n_routes + kChunk - 1) / kChunk)), dim3(256), 0, stream, ids,
                        n_routes, n_experts, offsets, src_route, dst_of_route);
     return hipGetLastError();
+}
+
+hipError_t launch_mxfp4_route(const void *x, int dtype, const float *logits, int T, int H, int E, int top_k,
+                              float *route_w, int32_t *ids, int32_t *offsets, int32_t *src_route,
+                              int32_t *dst_of_route, void *xq, hipStream_t stream) {
+    const int R = T * top_k;
+    const int64_t n8 = (int64_t)T * (H / 8);
+    return mx_by_dtype(dtype, [&](auto tag) {
+        using X = typename decltype(tag)::type;
+        if (R <= kRouteOne) {
+            const dim3 grid((unsigned)(1 + (n8 + 1023) / 1024));
+            auto go = [&](auto per) {
+                hipLaunchKernelGGL((route_quantize_kernel<X, decltype(per)::value>), grid, dim3(1024), 0, stream, logits,
+                                   T, E, top_k, route_w, ids, offsets, src_route, dst_of_route, (const X *)x, n8,
+                                   (uint8_t *)xq);
+                return hipGetLastError();
+            };
+            if (E <= 64) return go(std::integral_constant<int, 1>{});
+            if (E <= 256) return go(std::integral_constant<int, 4>{});
+            return go(std::integral_constant<int, 16>{});
+        }
+        const hipError_t e = launch_moe_top_k(logits, route_w, ids, T, E, top_k, stream);
+        if (e != hipSuccess) return e;
+        const int chunks = (R + kChunk - 1) / kChunk;
+        hipLaunchKernelGGL(sort_quantize_kernel<X>, dim3((unsigned)(chunks + (n8 + 255) / 256)), dim3(256), 0, stream,
+                           ids, R, E, offsets, src_route, dst_of_route, chunks, (const X *)x, n8, (uint8_t *)xq);
+        return hipGetLastError();
+    });
 }
 
 hipError_t launch_moe_dispatch_rows(const int32_t *ids, const void *x, int elem_bytes, int T, int top_k, int H, int E,

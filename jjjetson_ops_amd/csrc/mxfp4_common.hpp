@@ -99,6 +99,30 @@ __device__ __forceinline__ uint32_t mx_max_quad(uint32_t m) {
     return o > m ? o : m;
 }
 
+// Eight consecutive values, one 16-byte load or two.
+template <class T>
+__device__ __forceinline__ void mx_load8(const T *p, float *x) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+        const MxVec<T, 8> a = *reinterpret_cast<const MxVec<T, 8> *>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (float)a.v[i];
+    }
+}
+
+// Group `i` of eight values of a matrix of n8 of them, by a quad of lanes per block (n8 % 4 == 0): its
+// codes and, from one lane of four, the scale.
+template <class T>
+__device__ __forceinline__ void mx_quantize8(const T *p, int64_t i, int64_t n8, uint8_t *__restrict__ out) {
+    float v[8];
+    mx_load8(p, v);
+    const uint32_t s = mx_scale_byte(mx_max_quad(mx_amax8(v)));
+    reinterpret_cast<uint32_t *>(out)[i] = mx_codes8(v, s);
+    if ((threadIdx.x & 3) == 0) out[4 * n8 + (i >> 2)] = (uint8_t)s;
+}
+
 // ---- launchers (asynchronous on `stream`; arguments validated by the C ABI)
 hipError_t launch_quantize_mxfp4(const void *x, int dtype, int64_t row_stride, void *out, int64_t rows, int64_t cols,
                                  hipStream_t stream);
@@ -143,6 +167,10 @@ hipError_t launch_moe_sort(const int32_t *ids, int n_routes, int n_experts, int3
 hipError_t launch_moe_dispatch_rows(const int32_t *ids, const void *x, int elem_bytes, int T, int top_k, int H, int E,
                                     int32_t *offsets, int32_t *src_route, int32_t *dst_of_route, void *rows,
                                     hipStream_t stream);
+// Routing of the MXFP4 FFN: top-k, sort, and x to MXFP4, in one launch (up to kMxRouteOne routes) or two.
+hipError_t launch_mxfp4_route(const void *x, int dtype, const float *logits, int T, int H, int E, int top_k,
+                              float *route_w, int32_t *ids, int32_t *offsets, int32_t *src_route,
+                              int32_t *dst_of_route, void *xq, hipStream_t stream);
 // y[t] = sum over k of weights[t, k] * rows[dst(t, k)] (weights nullptr: 1), routes with dst outside
 // [0, T * top_k) left out.
 hipError_t launch_moe_join_rows(const void *rows, int rows_dtype, const int32_t *dst_of_route, const float *weights,

@@ -7,12 +7,13 @@
 namespace jjo {
 
 // acc[16 weights][16 tokens] += W[16][128] . X[16][128]^T.  Lane l holds row l % 16 of either
-// operand and of it the block l / 16 (32 values, 16 bytes) with that block's scale byte; of
-// acc it holds weights 4 * (l / 16) + 0..3 of token l % 16.
+// operand and of it the block l / 16 (32 values, 16 bytes) with that block's scale byte, byte BW (BX)
+// of its scale register; of acc it holds weights 4 * (l / 16) + 0..3 of token l % 16.
+template <int BW, int BX>
 __device__ __forceinline__ f32x4v mx_mfma(u32x4v w, u32x4v x, f32x4v acc, uint32_t sw, uint32_t sx) {
     const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
     const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, 0, (int)sw, 0, (int)sx);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, BW, (int)sw, BX, (int)sx);
 }
 
 // Four consecutive outputs of one row (the first `live` of them), in y's type.  `vec`: the row
@@ -36,6 +37,18 @@ __device__ __forceinline__ void mx_store4(void *y, int dtype, size_t at, f32x4v 
     else mx_store4_as((__bf16 *)y + at, v, live, vec);
 }
 
+// Inclusive sums over the wave's lanes: row shifts inside the rows of 16, then row_bcast15 and
+// row_bcast31; a lane without a source takes 0.
+__device__ __forceinline__ int mx_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
 // The tile-th tile of `rows` sorted rows, counted over the experts in order: its expert, its
 // first row and the end of its expert's rows; false behind the last.  Ranges are clamped to
 // [0, M], so a malformed table drops rows instead of leaving the buffers.  All lanes of a
@@ -52,12 +65,7 @@ __device__ __forceinline__ bool mx_expert_tile(const int32_t *__restrict__ offse
             fin = min(max(offsets[e + 1], beg), M);
         }
         const int mine = (fin - beg + rows - 1) / rows;
-        int incl = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(incl, d);
-            if (lane >= d) incl += o;
-        }
+        const int incl = mx_scan(mine);
         const uint64_t past = __ballot(base + incl > tile);
         if (past != 0) {
             const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));

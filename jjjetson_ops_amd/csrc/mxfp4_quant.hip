@@ -15,18 +15,6 @@
 namespace jjo {
 namespace {
 
-template <class T>
-__device__ __forceinline__ void load8(const T *p, float *x) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-        const MxVec<T, 8> a = *reinterpret_cast<const MxVec<T, 8> *>(p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (float)a.v[i];
-    }
-}
-
 // n8: groups of eight values in all, per_row of them in a row.
 template <class T, bool STRIDED>
 __global__ __launch_bounds__(256) void quantize_mxfp4_kernel(const T *__restrict__ x, int64_t row_stride,
@@ -35,11 +23,7 @@ __global__ __launch_bounds__(256) void quantize_mxfp4_kernel(const T *__restrict
     if (i >= n8) return;  // n8 % 4 == 0: quads leave as a whole
     const T *p = x + 8 * i;
     if constexpr (STRIDED) p = x + (i / per_row) * row_stride + 8 * (i % per_row);
-    float v[8];
-    load8(p, v);
-    const uint32_t s = mx_scale_byte(mx_max_quad(mx_amax8(v)));
-    reinterpret_cast<uint32_t *>(out)[i] = mx_codes8(v, s);
-    if ((threadIdx.x & 3) == 0) out[4 * n8 + (i >> 2)] = (uint8_t)s;
+    mx_quantize8(p, i, n8, out);
 }
 
 template <class T, bool STRIDED>
