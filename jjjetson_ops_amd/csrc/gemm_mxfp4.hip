@@ -4,12 +4,18 @@
 //     y[t][n] = sum over blocks b of 2^(sw[n,b] + sx[t,b] - 254) * sum_j cw[n,b,j] * cx[t,b,j]
 //
 // A stage is 256 values (128 bytes) of every weight row and token row of the tile, two steps of the
-// matrix instruction.  The codes go to LDS by DMA, 8 rows an instruction, the 16-byte pieces of a
-// row permuted by its row number (piece ^ row % 8) so that the 8 lanes that LDS serves at a time
-// fall in different banks; of the stage's 8 blocks lane group q of a step u takes block 2q + u,
+// matrix instruction.  The codes go to LDS by DMA, 8 rows of 128 bytes an instruction, the 16-byte pieces of a
+// row permuted by its row number (piece ^ row / 2 % 8) so that the 16 lanes that LDS serves at a time
+// fall in its 64 banks once; of the stage's 8 blocks lane group q of a step u takes block 2q + u,
 // so that a lane's two scale bytes are one 16-bit read and the instruction picks the byte.  The
-// scales (8 bytes a row and stage, of any alignment) go through a register of one thread per row.
-// While a stage is computed the next one lands in the other buffer; one barrier per stage.
+// scales (8 bytes a row and stage, of any alignment) go through a register of one thread per row, two
+// stages at a time.  While a stage is computed the next one lands in the other buffer; one barrier per stage.
+//
+// What bounds it: for prompts the matrix instruction and LDS together (2047 x 14336 x 4096: 79 us, 3.0 Pflop/s;
+// the instruction alone on random data in registers reaches 6.2, a library product of 8192 cubed 3.1); a
+// small product a stage's latency, about 1 us.  There the tiles are cut along K as well (KG), into groups of
+// waves with stages of their own, so that two or three stages are in flight: 4096 x 4096 and 256 tokens 13.4
+// us, 17.3 without.
 #include <hip/hip_runtime.h>
 
 #include "mxfp4_mm.hpp"
@@ -26,17 +32,19 @@ struct MxTiled {
     MxGroups g;
 };
 
-// WN x WT waves of RT tiles of 16 weight rows x TT tiles of 16 tokens each.
-template <int RT_, int TT_, int WN_, int WT_>
+// WN x WT waves of RT tiles of 16 weight rows x TT tiles of 16 tokens each; KG groups of such waves
+// cut K between them, each with stages of its own.
+template <int RT_, int TT_, int WN_, int WT_, int KG_ = 1>
 struct MxTile {
-    static constexpr int RT = RT_, TT = TT_, WN = WN_, WT = WT_;
-    static constexpr int kWaves = WN * WT, kThreads = 64 * kWaves;
+    static constexpr int RT = RT_, TT = TT_, WN = WN_, WT = WT_, KG = KG_;
+    static constexpr int kWaves = WN * WT, kThreads = 64 * kWaves;  // of a group
     static constexpr int kRowsN = 16 * RT * WN, kRowsT = 16 * TT * WT, kRows = kRowsN + kRowsT;
     static constexpr int kDma = kRows / 8 / kWaves;  // instructions a wave and stage
     static constexpr int kScaleRows = (kRows + kThreads - 1) / kThreads;  // rows a thread
-    static constexpr int kStage = kRows * 128;
-    static constexpr int kLds = 2 * (kStage + kRows * 16) + kRows * 4;
+    static constexpr int kStage = kRows * 128, kGroupLds = 2 * (kStage + kRows * 16);
+    static constexpr int kLds = KG * kGroupLds + kRows * 4;
     static_assert(kRows % (8 * kWaves) == 0 && kRowsN % 8 == 0, "whole DMA instructions");
+    static_assert(kLds <= 160 * 1024 && (KG == 1 || kThreads * RT * TT * 16 <= kGroupLds), "a group's sums fit its stages");
 };
 
 // A wave's outputs (from weight row n, token t on) through its own 4 KB of LDS, 16 tokens at a time:
@@ -74,12 +82,15 @@ __device__ __forceinline__ void store_rows(T *__restrict__ y, const f32x4v (&acc
 }
 
 template <class Tile, bool GROUPED, bool SWIGLU>
-__global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) {
+__global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) {
     constexpr int RT = Tile::RT, TT = Tile::TT;
-    extern __shared__ __align__(16) uint8_t lds[];
-    uint8_t *const lds_scales = lds + 2 * Tile::kStage;
-    uint32_t *const lds_rows = reinterpret_cast<uint32_t *>(lds_scales + 2 * Tile::kRows * 16);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int KG = Tile::KG;
+    extern __shared__ __align__(16) uint8_t lds_all[];
+    const int lane = threadIdx.x & 63, any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kg = KG == 1 ? 0 : any_wave / Tile::kWaves, wave = KG == 1 ? any_wave : any_wave % Tile::kWaves;
+    const int tid = KG == 1 ? (int)threadIdx.x : 64 * wave + lane;  // in the group
+    uint8_t *const lds = lds_all + kg * Tile::kGroupLds, *const lds_scales = lds + 2 * Tile::kStage;
+    uint32_t *const lds_rows = reinterpret_cast<uint32_t *>(lds_all + KG * Tile::kGroupLds);
     const int r16 = lane & 15, q = lane >> 4;
     const int wn = wave % Tile::WN, wt = wave / Tile::WN;
 
@@ -117,7 +128,7 @@ __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) 
     // rows' offsets stand in LDS: kept in registers they would spill, and a reload from scratch
     // waits for every DMA before it.
     const int t0 = GROUPED && p.g.src_route != nullptr ? 0 : first;
-    for (int row = threadIdx.x; row < Tile::kRows; row += Tile::kThreads)
+    for (int row = threadIdx.x; row < Tile::kRows; row += KG * Tile::kThreads)
         lds_rows[row] = row < Tile::kRowsN ? (uint32_t)(weight_row(row) - n0) * half
                                            : (uint32_t)(token_row(row - Tile::kRowsN) - t0) * half;
     const uint64_t x_base = (uint64_t)p.x + (uint64_t)t0 * half, w_at0 = (uint64_t)(w_first + n0) * half;
@@ -127,7 +138,7 @@ __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) 
     const uint8_t *srow[Tile::kScaleRows];
 #pragma unroll
     for (int i = 0; i < Tile::kScaleRows; ++i) {
-        const int row = min((int)threadIdx.x + i * Tile::kThreads, Tile::kRows - 1);
+        const int row = min(tid + i * Tile::kThreads, Tile::kRows - 1);
         if (row < Tile::kRowsN)
             srow[i] = (is_up(row) ? p.w2 : p.w) + w_all * half + (w_first + weight_row(row)) * nb;
         else
@@ -149,7 +160,7 @@ __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) 
                 v >>= 8 * over;
                 __builtin_memcpy(sv[i], &v, 16);
             }
-            const int row = threadIdx.x + i * Tile::kThreads;
+            const int row = tid + i * Tile::kThreads;
             uint8_t *to = lds_scales + (pair & 1) * (Tile::kRows * 16) + row * 8;
             if (row < Tile::kRows) {
                 *reinterpret_cast<uint2 *>(to) = make_uint2(sv[i][0], sv[i][1]);
@@ -188,26 +199,35 @@ __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) 
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = f32x4v{0.f, 0.f, 0.f, 0.f};
 
-    load_scales(0);
+    // A group takes whole pairs of stages.  All run as many rounds as the longest (barriers).
+    const int pairs = (stages + 1) / 2, p_beg = pairs * kg / KG, p_end = pairs * (kg + 1) / KG;
+    const int s_beg = 2 * p_beg, s_end = min(2 * p_end, stages);
+    const int rounds = KG == 1 ? stages : 2 * ((pairs + KG - 1) / KG);
+    const int cut = nb % 8 != 0 ? stages - 1 - 2 * (pairs * (KG - 1) / KG) : -1;  // the last group's last round
+    load_scales(p_beg);
     __syncthreads();
-    dma(0, 0);
+    dma(s_beg, 0);
     const uint32_t w_at = (uint32_t)(16 * RT * wn + r16), x_at = (uint32_t)(Tile::kRowsN + 16 * TT * wt + r16);
     const uint32_t sw0 = 16u * ((2 * q) ^ (r16 >> 1)), sw1 = 16u * ((2 * q + 1) ^ (r16 >> 1));
-    for (int st = 0; st < stages; ++st) {
+    for (int round = 0; round < rounds; ++round) {
+        const int st = s_beg + round;  // s_beg is even
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // stage st has landed
-        if ((st & 1) == 0) store_scales(st >> 1);
-        if (const int over = 8 * st + 8 - nb; over > 0) {  // the row ends inside the stage: zero weights behind it
+        if ((st & 1) == 0 && (KG == 1 || st < s_end)) store_scales(st >> 1);
+        if (round == cut) {  // the row ends inside the last stage: zero weights behind it
             asm volatile("s_barrier" ::: "memory");
-            for (int i = threadIdx.x; i < Tile::kRowsN * 8; i += Tile::kThreads)
-                if ((i & 7) >= 8 - over)
-                    *reinterpret_cast<u32x4v *>(lds + (st & 1) * Tile::kStage + (i >> 3) * 128 + 16 * ((i & 7) ^ ((i >> 4) & 7))) =
-                        u32x4v{0u, 0u, 0u, 0u};
+            const int over = 8 * stages - nb;
+            if (kg == KG - 1)
+                for (int i = tid; i < Tile::kRowsN * 8; i += Tile::kThreads)
+                    if ((i & 7) >= 8 - over)
+                        *reinterpret_cast<u32x4v *>(lds + (st & 1) * Tile::kStage + (i >> 3) * 128 +
+                                                    16 * ((i & 7) ^ ((i >> 4) & 7))) = u32x4v{0u, 0u, 0u, 0u};
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         // The next stage on its way; behind the last one, the last again (nothing reads it).
-        const int next = min(st + 1, stages - 1);
-        if ((st & 1) == 0) load_scales(min((st >> 1) + 1, (stages - 1) >> 1));
+        const int next = min(st + 1, s_end - 1);
+        if ((st & 1) == 0) load_scales(min((st >> 1) + 1, p_end - 1));
         dma(next, (st + 1) & 1);
+        if (KG > 1 && st >= s_end) continue;
         const uint8_t *buf = lds + (st & 1) * Tile::kStage;
         const uint8_t *sbuf = lds_scales + (st & 3) * (Tile::kRows * 8);
         uint32_t sw[RT], sx[TT];
@@ -233,6 +253,22 @@ __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) 
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outlives the workgroup's LDS
 
+    if constexpr (KG > 1) {  // the other groups' sums, in their order
+        f32x4v *const sums = reinterpret_cast<f32x4v *>(lds_all) + tid;
+        __syncthreads();  // no wave reads a stage any more
+        if (kg > 0) {
+#pragma unroll
+            for (int i = 0; i < RT * TT; ++i)
+                sums[(kg * Tile::kGroupLds / 16) + i * Tile::kThreads] = acc[i / TT][i % TT];
+        }
+        __syncthreads();
+        if (kg > 0) return;
+#pragma unroll
+        for (int k = 1; k < KG; ++k)
+#pragma unroll
+            for (int i = 0; i < RT * TT; ++i) acc[i / TT][i % TT] += sums[(k * Tile::kGroupLds / 16) + i * Tile::kThreads];
+    }
+
     if constexpr (SWIGLU) {
         static_assert(!SWIGLU || RT == 4, "a wave holds 32 gate rows and the same 32 up rows");
         uint8_t *codes = (uint8_t *)p.y, *scales = codes + (size_t)p.M * (p.N / 2);
@@ -247,7 +283,7 @@ __global__ __launch_bounds__(Tile::kThreads) void mxfp4_tiled_kernel(MxTiled p) 
         }
     } else {
         if (p.N % 8 == 0) {
-            __syncthreads();  // no wave reads a stage any more
+            if constexpr (KG == 1) __syncthreads();  // no wave reads a stage any more
             uint8_t *stage = lds + wave * 4096;
             const int nw = n0 + 16 * RT * wn, tw = first + 16 * TT * wt;
             const int32_t *route_dst = GROUPED ? p.g.route_dst : nullptr;
@@ -278,8 +314,8 @@ hipError_t run_tiled(MxTiled p, hipStream_t stream) {
     p.tiles_n = (p.N + kOutN - 1) / kOutN;
     p.tiles_t = (p.M + Tile::kRowsT - 1) / Tile::kRowsT + (p.g.offsets != nullptr ? std::min(p.g.n_experts, p.M) : 0);
     const int64_t wgs = (int64_t)p.tiles_n * p.tiles_t;
-    if (wgs * Tile::kThreads >= 1LL << 32) return hipErrorInvalidConfiguration;
-    const dim3 grid((unsigned)wgs), block(Tile::kThreads);
+    if (wgs * Tile::KG * Tile::kThreads >= 1LL << 32) return hipErrorInvalidConfiguration;
+    const dim3 grid((unsigned)wgs), block(Tile::KG * Tile::kThreads);
     auto go = [&](auto kernel) {
         const hipError_t e = ensure_dynamic_lds((const void *)kernel, Tile::kLds);
         if (e != hipSuccess) return e;
@@ -291,10 +327,24 @@ hipError_t run_tiled(MxTiled p, hipStream_t stream) {
     return hipErrorInvalidValue;
 }
 
-// Tiles of `tokens` tokens: 128 weight rows on four waves up to 128 tokens, 256 on eight above.
+struct MxTileChoice {
+    int tokens;  // 0: the direct kernel
+    bool split;  // K cut inside the workgroup
+};
+
+// 128 weight rows on four waves up to 128 tokens, 256 on eight above.
 template <bool SWIGLU>
-hipError_t run_tile(const MxTiled &p, int tokens, hipStream_t stream) {
-    switch (tokens) {
+hipError_t run_tile(const MxTiled &p, const MxTileChoice &tile, hipStream_t stream) {
+    if (tile.split) {
+        switch (tile.tokens) {
+            case 32: return run_tiled<MxTile<4, 1, 2, 2, 3>, SWIGLU>(p, stream);
+            case 64: return run_tiled<MxTile<4, 2, 2, 2, 2>, SWIGLU>(p, stream);
+            case 96: return run_tiled<MxTile<4, 3, 2, 2, 2>, SWIGLU>(p, stream);
+            case 128: return run_tiled<MxTile<4, 4, 2, 2, 2>, SWIGLU>(p, stream);
+        }
+        return hipErrorInvalidValue;
+    }
+    switch (tile.tokens) {
         case 32: return run_tiled<MxTile<4, 1, 2, 2>, SWIGLU>(p, stream);
         case 64: return run_tiled<MxTile<4, 2, 2, 2>, SWIGLU>(p, stream);
         case 96: return run_tiled<MxTile<4, 3, 2, 2>, SWIGLU>(p, stream);
@@ -305,56 +355,65 @@ hipError_t run_tile(const MxTiled &p, int tokens, hipStream_t stream) {
     return hipErrorInvalidValue;
 }
 
-}  // namespace
-
 // Rows of at least two stages; byte offsets inside a tile (and of gathered rows) fit 32 bits.
-bool mxfp4_tiled_accepts(int K, const MxGroups &g) {
+bool tiles_accept(int K, const MxGroups &g) {
     return K >= 512 && K <= 1 << 23 && (g.src_route == nullptr || (int64_t)g.x_rows * (K / 2) < 1LL << 32);
 }
 
-hipError_t launch_mxfp4_tiled(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
-                              const MxGroups &groups, int tile, hipStream_t stream) {
-    const MxTiled p{(const uint8_t *)w, nullptr, (const uint8_t *)xq, y, dtype, K, N, M, 0, 0, groups};
-    return run_tile<false>(p, tile, stream);
+// The kernel of a product with N weight rows in all (gate and up together).
+//
+// The direct kernel is bound by its workgroups' work, a tile by the latency of its stages, which is
+// the same for any output up to a tile per CU: 4096 x 4096 and 64 / 128 / 256 tokens 7.6 / 11.7 /
+// 18.8 us direct against 13.5 / 13.3 / 13.4 us on split tiles, 8192 x 14336 and 64 / 96 tokens 36 / 52 against 38 /
+// 38 us.  They meet at 8 workgroups of 16 rows x 16 tokens a CU (4 where K < 2048: 32768 x 1024 and 12
+// tokens, 8 a CU, 8.4 against 7.2 us).  Behind that the matrix itself is the bound: up to 16 tokens the direct
+// kernel reads it as fast from K = 4096 on (131072 x 4096, 16 tokens: 59 against 63 us).
+//
+// Split tiles where the smallest tile that leaves at most one workgroup a CU can do it (4096 x 4096, 256
+// tokens: 13.4 against 17.3 us; 14336 x 4096, 256: 20.4 against 21.9; 4096 x 11008, 512: 27.6 against 34).
+// Otherwise the tile whose rounds over the CUs cost least; kCost is a round's time in us at K =
+// 4096 with each CU's share of workgroups in flight (14336 x 4096: 96 tokens' tiles 22 us for 384 tokens, 128 27
+// for 512, 192 34 for 768, 256 42 for 1024, and each of the others there is slower).
+MxTileChoice tile_for(int K, int64_t N, int M, const MxGroups &g) {
+    const int64_t experts = mx_experts(M, g), rows = mx_rows(M, g), cus = device_cu_count();
+    const int64_t mean = (M + experts - 1) / experts;
+    const int64_t small = experts * ((N + 15) / 16) * ((rows + 15) / 16);
+    const int most = g.offsets == nullptr ? 16 : 10;  // an uneven share of 10 rows is 16 and more for some
+    if (!tiles_accept(K, g) || mean <= 4 || small <= (K < 2048 ? 4 : 8) * cus || (mean <= most && K >= 4096)) return {0, false};
+    auto rounds = [&](int tokens) {
+        const int64_t n = tokens <= 128 ? 128 : 256;
+        return (experts * ((rows + tokens - 1) / tokens) * ((N + n - 1) / n) + cus - 1) / cus;
+    };
+    if (K >= 2048)
+        for (int tokens : {32, 64, 96, 128})
+            if (rounds(tokens) == 1) return {tokens, true};
+    constexpr struct {
+        int tokens;
+        float cost;
+    } kCost[] = {{32, 9.f}, {64, 10.f}, {96, 11.5f}, {128, 14.f}, {192, 32.f}, {256, 40.f}};
+    int best = 0;
+    for (int i = 1; i < 6; ++i)
+        if (rounds(kCost[i].tokens) * kCost[i].cost < rounds(kCost[best].tokens) * kCost[best].cost) best = i;
+    return {kCost[best].tokens, false};
 }
 
-hipError_t launch_mxfp4_tiled_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I,
-                                     int M, const MxGroups &groups, int tile, hipStream_t stream) {
-    const MxTiled p{(const uint8_t *)w_gate, (const uint8_t *)w_up, (const uint8_t *)xq, mid, JJO_DTYPE_F32, K, I, M,
-                    0, 0, groups};
-    return run_tile<true>(p, tile, stream);
-}
-
-namespace {
-// Rows per expert expected (of M rows in all), or M.
-int mean_rows(int M, const MxGroups &g) {
-    if (g.offsets == nullptr) return M;
-    const int active = std::min(g.n_experts, M);
-    return (M + active - 1) / active;
-}
-
-// Tile of the staged kernel (256 or 128), or 0 for the direct one.
-int tile_for(int K, int N, int M, const MxGroups &g) {
-    const int mean = mean_rows(M, g);
-    if (mean <= 48 || !mxfp4_tiled_accepts(K, g)) return 0;
-    const int64_t groups = g.offsets == nullptr ? 1 : std::min(g.n_experts, M);
-    const int64_t t256 = groups * ((mean + 255) / 256) * ((N + 255) / 256);
-    return mean > 128 && t256 >= device_cu_count() ? 256 : 128;
-}
 }  // namespace
 
 hipError_t launch_mxfp4_mm(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
                            const MxGroups &groups, hipStream_t stream) {
-    const int tile = tile_for(K, N, M, groups);
-    return tile != 0 ? launch_mxfp4_tiled(w, xq, y, dtype, K, N, M, groups, tile, stream)
-                     : launch_mxfp4_direct(w, xq, y, dtype, K, N, M, groups, stream);
+    const MxTileChoice tile = tile_for(K, N, M, groups);
+    if (tile.tokens == 0) return launch_mxfp4_direct(w, xq, y, dtype, K, N, M, groups, stream);
+    const MxTiled p{(const uint8_t *)w, nullptr, (const uint8_t *)xq, y, dtype, K, N, M, 0, 0, groups};
+    return run_tile<false>(p, tile, stream);
 }
 
 hipError_t launch_mxfp4_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I, int M,
                                const MxGroups &groups, hipStream_t stream) {
-    const int tile = tile_for(K, 2 * I, M, groups);
-    return tile != 0 ? launch_mxfp4_tiled_swiglu(w_gate, w_up, xq, mid, K, I, M, groups, tile, stream)
-                     : launch_mxfp4_direct_swiglu(w_gate, w_up, xq, mid, K, I, M, groups, stream);
+    const MxTileChoice tile = tile_for(K, 2 * (int64_t)I, M, groups);
+    if (tile.tokens == 0) return launch_mxfp4_direct_swiglu(w_gate, w_up, xq, mid, K, I, M, groups, stream);
+    const MxTiled p{(const uint8_t *)w_gate, (const uint8_t *)w_up, (const uint8_t *)xq, mid, JJO_DTYPE_F32, K, I, M,
+                    0, 0, groups};
+    return run_tile<true>(p, tile, stream);
 }
 
 }  // namespace jjo

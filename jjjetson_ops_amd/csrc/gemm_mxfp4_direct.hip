@@ -51,15 +51,19 @@ __device__ __forceinline__ float quad_sum(float v) {
     return v;
 }
 
+// Chunks of 512 values that a wave asks for at once: 3 and 4 cost registers and gain nothing on average
+// (one token, K = 4096, N = 11008: 6.6 us with 2, 6.5 with 4; K = 11008, N = 4096: 7.4 and 7.0).
+constexpr int kMxChunks = 2;
+
 // A wave has 16 weight rows (4 operands of 4 rows) x TG operands of 4 tokens and NC chunks of 512 values at
 // once; KW waves cut K between them, RW have rows of their own.  SWIGLU: RW = 4, two times 16 gate
 // rows and the two times 16 up rows beside them.  XT: void (x is MXFP4), or the type of the one
 // token's row, which every wave quantizes for its own slice of K.
-template <int TG, int KW, int RW, int NC, bool GROUPED, bool SWIGLU, class XT>
+template <int TG, int KW, int RW, bool GROUPED, bool SWIGLU, class XT>
 __global__ __launch_bounds__(64 * KW * RW) void mxfp4_direct_kernel(MxProblem p) {
     constexpr bool kFused = !std::is_void_v<XT>;
     constexpr int W = KW * RW, kTokens = 4 * TG;
-    constexpr int kPieces = NC == 1 ? 1 : NC == 2 ? 2 : 4;  // of 16 scale bytes a row
+    constexpr int NC = kMxChunks, kPieces = NC;  // of 16 scale bytes a row
     constexpr int kScaleRows = kFused ? 16 : 16 + kTokens, kAtOnce = 64 / kPieces;  // rows a load instruction
     constexpr int kScaleLoads = (kScaleRows + kAtOnce - 1) / kAtOnce;
     __shared__ __align__(16) uint8_t s_scales[W][kScaleLoads * kAtOnce][16 * kPieces];
@@ -115,12 +119,10 @@ __global__ __launch_bounds__(64 * KW * RW) void mxfp4_direct_kernel(MxProblem p)
     for (int c0 = c_beg; c0 < c_end; c0 += NC) {
         // ---- everything of NC chunks is asked for, in the order of its use (loads return in order);
         // chunks behind the slice are its last one again
-        float v[kFused ? (NC + 1) / 2 : 1][16];
+        float v[16];
         if constexpr (kFused) {  // 16 values a lane; behind the row's end its last ones (they meet zero weights)
             typedef std::conditional_t<kFused, XT, float> T;
-#pragma unroll
-            for (int i = 0; i < (NC + 1) / 2; ++i)
-                load16((const T *)p.x + min(512 * c0 + 1024 * i + 16 * lane, p.K - 32 + 16 * (lane & 1)), v[i]);
+            load16((const T *)p.x + min(512 * c0 + 16 * lane, p.K - 32 + 16 * (lane & 1)), v);
         }
         u32x4v sv[kScaleLoads], a[NC][4], b[NC][TG];
         const int piece = lane % kPieces, s_at = min(16 * (c0 + piece), nb - 16);
@@ -139,19 +141,13 @@ __global__ __launch_bounds__(64 * KW * RW) void mxfp4_direct_kernel(MxProblem p)
         }
         // ---- scales, and the fused activation, to the wave's LDS
         if constexpr (kFused) {
-#pragma unroll
-            for (int i = 0; i < (NC + 1) / 2; ++i) {
-                uint32_t m = mx_amax8(v[i]), o = mx_amax8(v[i] + 8);
-                m = o > m ? o : m;
-                o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, true);  // lane ^ 1
-                m = o > m ? o : m;
-                const uint32_t s = mx_scale_byte(m);
-                if (NC % 2 == 0 || 1024 * i + 16 * lane < 512 * NC) {
-                    *reinterpret_cast<uint2 *>(&x_codes[wave][512 * i + 8 * lane]) =
-                        make_uint2(mx_codes8(v[i], s), mx_codes8(v[i] + 8, s));
-                    if ((lane & 1) == 0) x_scales[wave][32 * i + (lane >> 1)] = (uint8_t)s;
-                }
-            }
+            uint32_t m = mx_amax8(v), o = mx_amax8(v + 8);
+            m = o > m ? o : m;
+            o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, true);  // lane ^ 1
+            m = o > m ? o : m;
+            const uint32_t s = mx_scale_byte(m);
+            *reinterpret_cast<uint2 *>(&x_codes[wave][8 * lane]) = make_uint2(mx_codes8(v, s), mx_codes8(v + 8, s));
+            if ((lane & 1) == 0) x_scales[wave][lane >> 1] = (uint8_t)s;
         }
         const int over = 16 * (c0 + piece) + 16 - nb;  // zeros behind the row's end
 #pragma unroll
@@ -207,11 +203,9 @@ __global__ __launch_bounds__(64 * KW * RW) void mxfp4_direct_kernel(MxProblem p)
         }
         r[t] = lb == 0 ? s[0] : lb == 1 ? s[1] : lb == 2 ? s[2] : s[3];
     }
-    if constexpr (W > 1) {
 #pragma unroll
-        for (int t = 0; t < TG; ++t) part[wave][t][lane] = r[t];
-        __syncthreads();
-    }
+    for (int t = 0; t < TG; ++t) part[wave][t][lane] = r[t];
+    __syncthreads();
     auto total = [&](int row_wave, int t) {
         float s = part[row_wave * KW][t][lane];
 #pragma unroll
@@ -245,7 +239,7 @@ __global__ __launch_bounds__(64 * KW * RW) void mxfp4_direct_kernel(MxProblem p)
 #pragma unroll
         for (int t = 0; t < TG; ++t) {
             if (t % KW != kw) continue;
-            const float out = W > 1 ? total(rw, t) : r[t];
+            const float out = total(rw, t);
             const int tok = first + 4 * t + la, n = n0 + row;
             if (tok >= end || n >= p.N) continue;
             const size_t to = (size_t)(GROUPED && p.g.route_dst != nullptr ? p.g.route_dst[tok] : tok) * p.N + n;
@@ -256,7 +250,7 @@ __global__ __launch_bounds__(64 * KW * RW) void mxfp4_direct_kernel(MxProblem p)
     }
 }
 
-template <int TG, int KW, int RW, int NC, bool SWIGLU, class XT = void>
+template <int TG, int KW, int RW, bool SWIGLU, class XT = void>
 hipError_t run_direct(MxProblem p, hipStream_t stream) {
     constexpr int rows = SWIGLU ? 32 : 16 * RW, threads = 64 * KW * RW;
     // token tiles of M rows, and one more for each expert that can have a rest
@@ -266,60 +260,43 @@ hipError_t run_direct(MxProblem p, hipStream_t stream) {
     if (wgs * threads >= 1LL << 32) return hipErrorInvalidConfiguration;
     const dim3 grid((unsigned)wgs), block(threads);
     if constexpr (!std::is_void_v<XT>)
-        hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, NC, false, false, XT>), grid, block, 0, stream, p);
+        hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, false, false, XT>), grid, block, 0, stream, p);
     else if (p.g.offsets != nullptr)
-        hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, NC, true, SWIGLU, void>), grid, block, 0, stream, p);
+        hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, true, SWIGLU, void>), grid, block, 0, stream, p);
     else if constexpr (!SWIGLU)
-        hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, NC, false, false, void>), grid, block, 0, stream, p);
+        hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, false, false, void>), grid, block, 0, stream, p);
     else
         return hipErrorInvalidValue;
     return hipGetLastError();
 }
 
-// Rows per expert expected (of M rows in all), or M.
-int mean_rows(int M, const MxGroups &g) {
-    if (g.offsets == nullptr) return M;
-    const int active = std::min(g.n_experts, M);
-    return (M + active - 1) / active;
-}
-
 }  // namespace
 
-int form = 0;
-
+// Tokens at once, of the mean rows of an expert: an uneven share of 3 rows is mostly up to 4 for one expert, and
+// more operands than tokens cost what they would with tokens (K = 4096, N = 14336: 7.4 us for 4 tokens on one
+// operand, 7.9 for 7 on two, 9.6 for 16 on four).  More than 16 tokens are more tiles of 16: operands for 24
+// and 32 took longer at every size (4096 x 4096, 32 tokens: 7.6 against 5.9 us).
 hipError_t launch_mxfp4_direct(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
                                const MxGroups &groups, hipStream_t stream) {
     const MxProblem p{(const uint8_t *)w, nullptr, (const uint8_t *)xq, y, dtype, K, N, M, 0, groups};
-    const int mean = mean_rows(M, groups);
-    switch (form) {
-#define F(n, ...) case n: return run_direct<__VA_ARGS__, false>(p, stream);
-        F(1, 1, 4, 1, 2) F(2, 1, 8, 1, 2) F(3, 1, 2, 2, 2) F(4, 1, 1, 4, 4) F(5, 1, 8, 1, 4) F(6, 1, 4, 1, 4) F(7, 1, 2, 4, 4) F(8, 1, 4, 2, 2) F(9, 1, 2, 2, 4)
-        F(11, 4, 4, 1, 2) F(12, 4, 8, 1, 2) F(13, 4, 2, 2, 2) F(14, 4, 1, 4, 3) F(15, 4, 8, 1, 3)  F(16, 4, 4, 1, 4) F(17, 4, 1, 4, 2) F(18, 4, 4, 2, 2) F(19, 4, 1, 2, 3)
-        F(21, 6, 4, 1, 2) F(22, 6, 8, 1, 2) F(23, 6, 8, 1, 1) F(24, 6, 4, 2, 1) F(25, 6, 4, 2, 2) F(26, 6, 8, 2, 1)
-        F(31, 2, 4, 1, 2) F(32, 2, 8, 1, 2) F(33, 2, 4, 2, 2) F(34, 2, 4, 1, 1)
-        F(41, 8, 4, 1, 1) F(42, 8, 8, 1, 1) F(43, 8, 8, 1, 2) F(44, 8, 4, 2, 1)
-#undef F
-    }
-    if (mean <= 4) return run_direct<1, 4, 1, 2, false>(p, stream);
-    if (mean <= 16) return run_direct<4, 4, 1, 2, false>(p, stream);
-    return run_direct<8, 4, 1, 1, false>(p, stream);
+    const bool grouped = groups.offsets != nullptr;
+    const int64_t experts = mx_experts(M, groups), rows = mx_rows(M, groups), mean = (M + experts - 1) / experts;
+    if (mean <= (grouped ? 3 : 4)) return run_direct<1, 4, 1, false>(p, stream);
+    if (rows <= 8) return run_direct<2, 4, 1, false>(p, stream);
+    // Two row tiles a workgroup and half as many slices of K once there are three workgroups a CU
+    // (4096 x 4096: 32 tokens 5.9 us on four slices, 6.5 on two; 96 tokens 10.6 and 9.2).
+    if (experts * ((N + 15) / 16) * ((rows + 15) / 16) > 3 * device_cu_count())
+        return run_direct<4, 2, 2, false>(p, stream);
+    return run_direct<4, 4, 1, false>(p, stream);
 }
 
 hipError_t launch_mxfp4_direct_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I,
                                       int M, const MxGroups &groups, hipStream_t stream) {
     const MxProblem p{(const uint8_t *)w_gate, (const uint8_t *)w_up, (const uint8_t *)xq, mid, JJO_DTYPE_F32, K, I, M,
                       0, groups};
-    const int mean = mean_rows(M, groups);
-    switch (form) {
-#define F(n, ...) case n: return run_direct<__VA_ARGS__, true>(p, stream);
-        F(1, 1, 2, 4, 2) F(2, 1, 4, 4, 2) F(3, 1, 2, 4, 4) F(4, 1, 1, 4, 2) F(5, 1, 1, 4, 4) F(6, 1, 4, 4, 1)
-        F(11, 4, 2, 4, 2) F(12, 4, 4, 4, 2) F(13, 4, 1, 4, 2) F(14, 4, 1, 4, 4) F(15, 4, 4, 4, 1) F(16, 4, 2, 4, 1)
-        F(21, 6, 2, 4, 2) F(22, 6, 1, 4, 2) F(23, 6, 2, 4, 1) F(24, 8, 1, 4, 1) F(25, 8, 2, 4, 1)
-#undef F
-    }
-    if (mean <= 4) return run_direct<1, 2, 4, 2, true>(p, stream);
-    if (mean <= 16) return run_direct<4, 2, 4, 2, true>(p, stream);
-    return run_direct<8, 2, 4, 1, true>(p, stream);
+    const int experts = mx_experts(M, groups), mean = (M + experts - 1) / experts;
+    if (mean <= 3) return run_direct<1, 1, 4, true>(p, stream);
+    return run_direct<4, 1, 4, true>(p, stream);
 }
 
 hipError_t launch_mxfp4_gemv(const void *w, const void *x, int x_dtype, void *y, int y_dtype, int K, int N,
@@ -327,12 +304,7 @@ hipError_t launch_mxfp4_gemv(const void *w, const void *x, int x_dtype, void *y,
     const MxProblem p{(const uint8_t *)w, nullptr, (const uint8_t *)x, y, y_dtype, K, N, 1, 0, MxGroups{}};
     return mx_by_dtype(x_dtype, [&](auto tag) {
         using T = typename decltype(tag)::type;
-        switch (form) {
-#define F(n, ...) case n: return run_direct<__VA_ARGS__, false, T>(p, stream);
-        F(1, 1, 4, 1, 2) F(2, 1, 8, 1, 2) F(3, 1, 8, 1, 1) F(4, 1, 2, 1, 4) F(5, 1, 2, 2, 4) F(6, 1, 4, 2, 2) F(7, 1, 8, 1, 3) F(8, 1, 8, 1, 4) F(9, 1, 4, 1, 4)
-#undef F
-        }
-        return run_direct<1, 4, 1, 2, false, T>(p, stream);
+        return run_direct<1, 4, 1, false, T>(p, stream);
     });
 }
 

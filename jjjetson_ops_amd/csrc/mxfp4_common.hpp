@@ -12,6 +12,7 @@
 #include <hip/hip_fp16.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "q4q8_common.hpp"
@@ -140,6 +141,15 @@ struct MxGroups {
     int top_k = 1;
     int x_rows = 0;  // rows of x where src_route is given
 };
+// Experts with rows, of M rows in all, as far as it is known without reading the offsets ...
+inline int mx_experts(int M, const MxGroups &g) { return g.offsets == nullptr ? 1 : std::min(g.n_experts, M); }
+// ... and the rows of one that has many: the mean and two standard deviations of a random share.
+inline int mx_rows(int M, const MxGroups &g) {
+    if (g.offsets == nullptr) return M;
+    const double mean = (double)M / mx_experts(M, g);
+    return std::min(M, (int)std::ceil(mean + 2 * std::sqrt(mean)));
+}
+// The products on the direct kernel (any shape) ...
 hipError_t launch_mxfp4_direct(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
                                const MxGroups &groups, hipStream_t stream);
 // One token whose row is quantized inside the product (K <= kMxFusedMaxK).
@@ -149,13 +159,7 @@ hipError_t launch_mxfp4_gemv(const void *w, const void *x, int x_dtype, void *y,
 // mid = MXFP4 of silu(x . w_gate) * (x . w_up), [M][I] (I % 32 == 0), of grouped rows.
 hipError_t launch_mxfp4_direct_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I,
                                       int M, const MxGroups &groups, hipStream_t stream);
-// The same products on LDS tiles of `tile` (256 or 128) rows and tokens, where accepted.
-bool mxfp4_tiled_accepts(int K, const MxGroups &groups);
-hipError_t launch_mxfp4_tiled(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
-                              const MxGroups &groups, int tile, hipStream_t stream);
-hipError_t launch_mxfp4_tiled_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I,
-                                     int M, const MxGroups &groups, int tile, hipStream_t stream);
-// The products on the kernel chosen for the shape.
+// ... and on the kernel chosen for the shape.
 hipError_t launch_mxfp4_mm(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
                            const MxGroups &groups, hipStream_t stream);
 hipError_t launch_mxfp4_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I, int M,

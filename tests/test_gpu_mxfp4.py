@@ -325,6 +325,102 @@ def test_ffn_same_expert_for_all_and_for_none(dev):
     _check_ffn((wg, wu, wd), x, logits, T, H, I, E, k, "f32", dev)
 
 
+# ------------------------------------------------- large products, every tile; the oracle on the GPU
+def _bytes(gen, rows, cols, dev):
+    """Random codes under scales of seven magnitudes, and their values in fp64."""
+    half = rows * cols // 2
+    q = torch.randint(0, 256, (rows * cols // 32 * 17,), dtype=torch.uint8, device=dev, generator=gen)
+    q[half:] = 119 + q[half:] % 7
+    table = torch.from_numpy(mx.values(np.arange(16, dtype=np.uint8))).to(dev)
+    b = q[:half].view(rows, cols // 2).int()
+    v = torch.stack([table[b & 15], table[b >> 4]], 2).view(rows, cols // 32, 32)
+    v *= torch.exp2(q[half:].view(rows, cols // 32, 1).double() - 127)
+    return q, v.view(rows, cols)
+
+
+def _product(x, w):
+    """x . w^T and the bound of its fp32 sum (sum_bound)."""
+    return x @ w.t().contiguous(), (x.shape[1] // 32 + 8) * 2.0 ** -23 * (x.abs() @ w.abs().t().contiguous())
+
+
+def _close_dev(got, exp, bound):
+    bad = ~((got.double() - exp).abs() <= bound)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist(), (got.double() - exp).abs().max().item())
+
+
+# With 256 CUs: tiles of 32, 64, 96 and 128 tokens cut along K, then whole, then 192 and 256; a last block, a
+# last pair of stages and row and token tiles that are not full.
+@pytest.mark.parametrize("K,N,M", [(2080, 8264, 50), (2336, 16424, 33), (2080, 16424, 70), (2048, 16420, 100),
+                                   (544, 16424, 16), (1056, 16424, 50), (608, 16420, 90), (768, 16424, 127),
+                                   (544, 14344, 700), (800, 14340, 1000)])
+def test_mat_mul_tiles(K, N, M, dev):
+    note(f"mat_mul tiles K={K} N={N} M={M}")
+    gen = torch.Generator(device=dev).manual_seed(K + N + M)
+    w, wv = _bytes(gen, N, K, dev)
+    x, xv = _bytes(gen, M, K, dev)
+    exp, bound = _product(xv, wv)
+    for dtype in DT:
+        y = torch.full((M * N + 8,), 3.0, dtype=DT[dtype], device=dev)
+        capi.mat_mul_mxfp4(w, x, y, K, N, M)
+        assert (y[M * N:] == 3.0).all()
+        _close_dev(y[:M * N].view(M, N), exp, bound + mx.HALF_STEP[dtype] * (exp.abs() + bound) + mx.TINY[dtype])
+
+
+# (E, K, values a row of the two matrices together, rows): the same tiles for an expert's rows.
+TILES = [(4, 2080, 4160, 48), (4, 2336, 4160, 160), (4, 2080, 4160, 256), (4, 2048, 4160, 400), (4, 544, 4160, 48),
+         (4, 1056, 4160, 160), (4, 608, 4160, 256), (4, 768, 4160, 400), (8, 544, 8192, 1200), (8, 800, 8192, 1600),
+         (4, 2080, 4160, 16)]
+
+
+def _uneven(E, R):
+    """Ranges of rows: one expert has none, one the most, and some rows belong to no expert."""
+    share = np.full(E, (R - R // 16) // E)
+    share[1] += share[2] - share[2] // 2
+    share[2] //= 2
+    share[3] += share[0]
+    share[0] = 0
+    return np.concatenate([[0], np.cumsum(share)])
+
+
+@pytest.mark.parametrize("E,K,N,R", TILES)
+def test_grouped_tiles(E, K, N, R, dev):
+    note(f"grouped tiles E={E} K={K} N={N} R={R}")
+    gen = torch.Generator(device=dev).manual_seed(K + N + R)
+    w, wv = _bytes(gen, E * N, K, dev)
+    x, xv = _bytes(gen, R, K, dev)
+    off = _uneven(E, R)
+    exp, bound = torch.full((R, N), 5.0, dtype=torch.float64, device=dev), torch.zeros(R, N, dtype=torch.float64, device=dev)
+    for e in range(E):
+        r = slice(off[e], off[e + 1])
+        exp[r], bound[r] = _product(xv[r], wv[e * N:(e + 1) * N])
+    od = torch.from_numpy(off.astype(np.int32)).to(dev)
+    y = torch.full((R, N), 5.0, device=dev)
+    capi.grouped_mat_mul_mxfp4(w, x, od, y, K, N, R)
+    _close_dev(y, exp, bound)
+
+
+@pytest.mark.parametrize("E,K,N,R", TILES)
+def test_gate_up_swiglu_tiles(E, K, N, R, dev):
+    I = N // 2
+    note(f"gate_up tiles E={E} K={K} I={I} R={R}")
+    gen = torch.Generator(device=dev).manual_seed(K + N + R)
+    (wg, wgv), (wu, wuv) = (_bytes(gen, E * I, K, dev) for _ in range(2))
+    x, xv = _bytes(gen, R, K, dev)
+    off = _uneven(E, R)
+    live = off[-1]
+    g, u, dg, du = (torch.zeros(live, I, dtype=torch.float64, device=dev) for _ in range(4))
+    for e in range(E):
+        r, we = slice(off[e], off[e + 1]), slice(e * I, (e + 1) * I)
+        g[r], dg[r] = _product(xv[r], wgv[we])
+        u[r], du[r] = _product(xv[r], wuv[we])
+    mid = torch.full((capi.mxfp4_bytes(R, I) + 16,), 0x5A, dtype=torch.uint8, device=dev)
+    capi.moe_gate_up_swiglu_mxfp4(wg, wu, x, torch.from_numpy(off.astype(np.int32)).to(dev), E, mid, K, I, R)
+    got = mid.cpu().numpy()
+    code, s = mx.unpack(got, R, I)
+    assert (got[-16:] == 0x5A).all() and (s[live:] == 0x5A).all()  # rows of no expert stay
+    _check_swiglu(mx.pack(code[:live], s[:live]), *(t.cpu().numpy() for t in (g, u, dg, du)))
+
+
 # ---------------------------------------------------------------- graphs and streams
 def _replays_match(fn, outs, dev, n=3):
     fn()
