@@ -39,11 +39,10 @@ struct MxTile {
     static constexpr int RT = RT_, TT = TT_, WN = WN_, WT = WT_, KG = KG_;
     static constexpr int kWaves = WN * WT, kThreads = 64 * kWaves;  // of a group
     static constexpr int kRowsN = 16 * RT * WN, kRowsT = 16 * TT * WT, kRows = kRowsN + kRowsT;
-    static constexpr int kDma = kRows / 8 / kWaves;  // instructions a wave and stage
+    static constexpr int kRuns = kRows / 8, kDma = (kRuns + kWaves - 1) / kWaves;  // DMA instructions; a wave's
     static constexpr int kScaleRows = (kRows + kThreads - 1) / kThreads;  // rows a thread
     static constexpr int kStage = kRows * 128, kGroupLds = 2 * (kStage + kRows * 16);
     static constexpr int kLds = KG * kGroupLds + kRows * 4;
-    static_assert(kRows % (8 * kWaves) == 0 && kRowsN % 8 == 0, "whole DMA instructions");
     static_assert(kLds <= 160 * 1024 && (KG == 1 || kThreads * RT * TT * 16 <= kGroupLds), "a group's sums fit its stages");
 };
 
@@ -173,13 +172,16 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
         const uint32_t left = 16u * (uint32_t)(nb - 8 * st);  // bytes of the row from the stage on
         const uint32_t most = left >= 128u ? 112u : left - 16u;
         const uint32_t even = min((uint32_t)piece, most), odd = min((uint32_t)piece ^ 64u, most);
+        auto run = [&](int i) {  // of 8 rows; the last one again where they do not divide
+            const int at = wave * Tile::kDma + i;
+            return Tile::kRuns % Tile::kWaves == 0 ? at : min(at, Tile::kRuns - 1);
+        };
         uint32_t off[Tile::kDma];
 #pragma unroll
-        for (int i = 0; i < Tile::kDma; ++i)
-            off[i] = lds_rows[8 * (wave * Tile::kDma + i) + (lane >> 3)] + ((wave * Tile::kDma + i) & 1 ? odd : even);
+        for (int i = 0; i < Tile::kDma; ++i) off[i] = lds_rows[8 * run(i) + (lane >> 3)] + (run(i) & 1 ? odd : even);
 #pragma unroll
         for (int i = 0; i < Tile::kDma; ++i) {
-            const int row8 = 8 * (wave * Tile::kDma + i);
+            const int row8 = 8 * run(i);
             const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds0 + buffer * Tile::kStage + 128 * row8);
             // Masks, not branches: a choice among captured addresses would go through scratch.
             const uint64_t up = -(uint64_t)is_up(row8), x = -(uint64_t)(row8 >= Tile::kRowsN);
@@ -349,6 +351,7 @@ hipError_t run_tile(const MxTiled &p, const MxTileChoice &tile, hipStream_t stre
         case 64: return run_tiled<MxTile<4, 2, 2, 2>, SWIGLU>(p, stream);
         case 96: return run_tiled<MxTile<4, 3, 2, 2>, SWIGLU>(p, stream);
         case 128: return run_tiled<MxTile<4, 4, 2, 2>, SWIGLU>(p, stream);
+        case 160: return run_tiled<MxTile<4, 5, 4, 2>, SWIGLU>(p, stream);
         case 192: return run_tiled<MxTile<4, 6, 4, 2>, SWIGLU>(p, stream);
         case 256: return run_tiled<MxTile<4, 8, 4, 2>, SWIGLU>(p, stream);
     }
@@ -372,8 +375,9 @@ bool tiles_accept(int K, const MxGroups &g) {
 // Split tiles where the smallest tile that leaves at most one workgroup a CU can do it (4096 x 4096, 256
 // tokens: 13.4 against 17.3 us; 14336 x 4096, 256: 20.4 against 21.9; 4096 x 11008, 512: 27.6 against 34).
 // Otherwise the tile whose rounds over the CUs cost least; kCost is a round's time in us at K =
-// 4096 with each CU's share of workgroups in flight (14336 x 4096: 96 tokens' tiles 22 us for 384 tokens, 128 27
-// for 512, 192 34 for 768, 256 42 for 1024, and each of the others there is slower).
+// 4096 with each CU's share of workgroups in flight (14336 x 4096: 96 tokens' tiles 22 us for 384 tokens, 128 26
+// for 512, 160 31 for 640, 192 34 for 768, 256 41 for 1024, and each of the others there is slower; 8 experts of 28672 rows
+// with 128 tokens each: 160 158 us, 192 165, 128 193).
 MxTileChoice tile_for(int K, int64_t N, int M, const MxGroups &g) {
     const int64_t experts = mx_experts(M, g), rows = mx_rows(M, g), cus = device_cu_count();
     const int64_t mean = (M + experts - 1) / experts;
@@ -390,9 +394,9 @@ MxTileChoice tile_for(int K, int64_t N, int M, const MxGroups &g) {
     constexpr struct {
         int tokens;
         float cost;
-    } kCost[] = {{32, 9.f}, {64, 10.f}, {96, 11.5f}, {128, 14.f}, {192, 32.f}, {256, 40.f}};
+    } kCost[] = {{32, 9.f}, {64, 10.f}, {96, 11.5f}, {128, 14.f}, {160, 28.5f}, {192, 31.f}, {256, 39.5f}};
     int best = 0;
-    for (int i = 1; i < 6; ++i)
+    for (int i = 1; i < 7; ++i)
         if (rounds(kCost[i].tokens) * kCost[i].cost < rounds(kCost[best].tokens) * kCost[best].cost) best = i;
     return {kCost[best].tokens, false};
 }

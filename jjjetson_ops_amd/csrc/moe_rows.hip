@@ -132,56 +132,73 @@ __global__ __launch_bounds__(256) void dispatch_rows_kernel(const int32_t *__res
     }
 }
 
-// ---- sort of any number of routes.  Workgroup c places the routes of chunk c; it counts the
-// experts of every route itself (all, and those of the chunks before its own), so there is
-// no scratch and no second launch.  A wave's 64 ids are counted by one ballot per bit of the
-// id and one LDS add per distinct id.
-constexpr int kChunk = 1024;
+// ---- sort of any number of routes.  Workgroup c places the routes of chunk c, whose ids it keeps
+// in registers; it counts the experts of every other chunk itself (those before its own apart
+// from those behind), so there is no scratch and no second launch.  A wave's 64 ids are
+// counted by one ballot per bit of the id and one LDS add per distinct id.  Bound by latency: ids
+// are asked for four loads at a time (800 routes of 64 experts: KSORT us, 9.0 with a load at a time and the own chunk
+// read three times).
+constexpr int kChunk = 1024, kOwn = kChunk / 256;
 
 __device__ __forceinline__ void sort_chunk(int chunk, const int32_t *__restrict__ ids, int R, int n_experts,
                                            int32_t *__restrict__ offsets, int32_t *__restrict__ src_route,
                                            int32_t *__restrict__ dst_of_route) {
-    __shared__ int s_all[1024], s_before[1024];
+    __shared__ int s_all[1024], s_other[2][1024];  // other chunks: before this one, behind it
     __shared__ int s_wave[4][1024];  // the chunk's routes per wave, then each wave's next position
     __shared__ int s_part[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int c0 = chunk * kChunk;
     const int bits = 32 - __builtin_clz(n_experts);
-    for (int e = tid; e < 1024; e += 256) {
-        s_all[e] = s_before[e] = 0;
+    // 256 routes from r0 on, 64 at a time
+    auto load = [&](int r0, int (&e)[kOwn]) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) s_wave[w][e] = 0;
-    }
-    __syncthreads();
+        for (int i = 0; i < kOwn; ++i) {
+            const int r = r0 + 64 * i + lane;
+            e[i] = r < R ? ids[r] : -1;
+        }
+    };
     // lanes of the wave with the same live id as this one
-    auto same = [&](int e, bool live) {
-        uint64_t grp = __ballot(live);
+    auto same = [&](int e) {
+        uint64_t grp = __ballot(live_id(e, n_experts));
         for (int b = 0; b < bits; ++b) {
             const uint64_t one = __ballot((e >> b) & 1);
             grp &= (e >> b) & 1 ? one : ~one;
         }
         return grp;
     };
-    for (int r0 = 64 * wave; r0 < R; r0 += 256) {  // c0 is a multiple of 64: a step is before it or not
-        const int r = r0 + lane;
-        const int e = r < R ? ids[r] : -1;
-        const bool live = live_id(e, n_experts);
-        const uint64_t grp = same(e, live);
-        if (live && lane == 63 - __builtin_clzll(grp)) {
-            const int n = __builtin_popcountll(grp);
-            atomicAdd(&s_all[e], n);
-            if (r0 < c0) atomicAdd(&s_before[e], n);
-        }
+    auto count = [&](int e, uint64_t grp, int *to) {
+        if (live_id(e, n_experts) && lane == 63 - __builtin_clzll(grp)) atomicAdd(&to[e], __builtin_popcountll(grp));
+    };
+    int own[kOwn], *const mine = s_wave[wave];
+    const int w0 = chunk * kChunk + 256 * wave;
+    load(w0, own);
+    for (int e = tid; e < n_experts; e += 256) {
+        s_other[0][e] = s_other[1][e] = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) s_wave[w][e] = 0;
     }
-    // the chunk's own routes: wave w has [c0 + 256 w, c0 + 256 (w + 1))
-    int *mine = s_wave[wave];
-    const int w0 = c0 + (kChunk / 4) * wave;
-    for (int i = 0; i < kChunk / 4; i += 64) {
-        const int r = w0 + i + lane;
-        const int e = r < R ? ids[r] : -1;
-        const bool live = live_id(e, n_experts);
-        const uint64_t grp = same(e, live);
-        if (live && lane == 63 - __builtin_clzll(grp)) mine[e] += __builtin_popcountll(grp);
+    __syncthreads();
+    uint64_t grp[kOwn];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+        grp[i] = same(own[i]);
+        count(own[i], grp[i], mine);
+    }
+    for (int r0 = 256 * wave; r0 < R; r0 += kChunk) {
+        if (r0 == w0) continue;
+        int e[kOwn];
+        load(r0, e);
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) count(e[i], same(e[i]), s_other[r0 > w0]);
+    }
+    __syncthreads();
+    for (int e = tid; e < 1024; e += 256) {
+        int n = 0;
+        if (e < n_experts) {
+            n = s_other[0][e] + s_other[1][e];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) n += s_wave[w][e];
+        }
+        s_all[e] = n;
     }
     __syncthreads();
     const int last = s_all[n_experts - 1];
@@ -191,7 +208,7 @@ __device__ __forceinline__ void sort_chunk(int chunk, const int32_t *__restrict_
         if (tid == 0) offsets[n_experts] = s_all[n_experts - 1] + last;
     }
     for (int e = tid; e < n_experts; e += 256) {
-        int base = s_all[e] + s_before[e];
+        int base = s_all[e] + s_other[0][e];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const int n = s_wave[w][e];
@@ -200,18 +217,17 @@ __device__ __forceinline__ void sort_chunk(int chunk, const int32_t *__restrict_
         }
     }
     __syncthreads();
-    for (int i = 0; i < kChunk / 4; i += 64) {
-        const int r = w0 + i + lane;
-        const int e = r < R ? ids[r] : -1;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+        const int r = w0 + 64 * i + lane, e = own[i];
         const bool live = live_id(e, n_experts);
-        const uint64_t grp = same(e, live);
         int pos = -1;
         if (live) {
-            pos = mine[e] + __builtin_popcountll(grp & ((1ull << lane) - 1ull));
+            pos = mine[e] + __builtin_popcountll(grp[i] & ((1ull << lane) - 1ull));
             src_route[pos] = r;
         }
         if (r < R) dst_of_route[r] = pos;
-        if (live && lane == 63 - __builtin_clzll(grp)) mine[e] = pos + 1;  // after every lane's read: one wave
+        if (live && lane == 63 - __builtin_clzll(grp[i])) mine[e] = pos + 1;  // after every lane's read: one wave
     }
 }
 
