@@ -638,13 +638,17 @@ def _entry(which: int, where: str, stream, *args) -> None:
         lib()  # the same loud failure where nothing is built
         from ._linear import entry
         _entry_native = entry
-    rc = _entry_native(which, _current_stream, _current_device, stream, *args)
+    rc = _entry_native(which, _stream_of, _current_device, stream, *args)
     if rc != JJO_OK:
         _check(rc, where)
 
 
 def _current_device() -> int:
     return _torch.cuda.current_device()
+
+
+def _stream_of(device: int) -> int:
+    return _torch._C._cuda_getCurrentRawStream(device)
 
 
 def _load_torch() -> None:

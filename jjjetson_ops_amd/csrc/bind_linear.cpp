@@ -10,7 +10,7 @@
 // linear(split, current_stream, x, w, y, in_features, out_features, num_tokens, ws, stream)
 //   -> status code of linear_q4_0_forward_device / linear_q4_0s_forward_device, or None if a
 //      size or an address is no int (the caller then leaves the conversion to ctypes)
-// entry(which, current_stream, current_device, stream, arguments...) -> status code of the
+// entry(which, stream_of_device, current_device, stream, arguments...) -> status code of the
 //      which-th entry of kEntries, its arguments in the C order without the stream.  Tensors must be
 //      contiguous and on the current device; an address (int) is taken as it is.
 #define PY_SSIZE_T_CLEAN
@@ -68,11 +68,12 @@ int device_ptr(PyObject *t, const char *name, void **out) {
     return rc;
 }
 
-// None: the current stream; an int: a hipStream_t; anything else: its cuda_stream.
-int stream_ptr(PyObject *stream, PyObject *current_stream, void **out) {
+// None: the current stream (of `device`, where the callable takes one); an int: a hipStream_t; anything
+// else: its cuda_stream.
+int stream_ptr(PyObject *stream, PyObject *current_stream, PyObject *device, void **out) {
     PyObject *r;
     if (stream == Py_None)
-        r = PyObject_CallNoArgs(current_stream);
+        r = device == nullptr ? PyObject_CallNoArgs(current_stream) : PyObject_CallOneArg(current_stream, device);
     else if (PyLong_Check(stream))
         r = Py_NewRef(stream);
     else
@@ -92,7 +93,7 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (split < 0) return nullptr;
     void *stream, *ws = nullptr, *x, *w, *y;
     int in, out, tokens;
-    int rc = stream_ptr(a[9], a[1], &stream);
+    int rc = stream_ptr(a[9], a[1], nullptr, &stream);
     if (rc > 0 && a[8] != Py_None) rc = device_ptr(a[8], "ws", &ws);
     if (rc > 0) rc = device_ptr(a[2], "x", &x);
     if (rc > 0) rc = device_ptr(a[3], "w", &w);
@@ -252,10 +253,9 @@ PyObject *entry(PyObject *, PyObject *const *a, Py_ssize_t n) {
     PyObject *r = PyObject_CallNoArgs(a[2]);
     if (r == nullptr) return nullptr;
     const long device = PyLong_AsLong(r);
-    Py_DECREF(r);
-    if (device == -1 && PyErr_Occurred()) return nullptr;
     void *stream;
-    int rc = stream_ptr(a[3], a[1], &stream);
+    int rc = device == -1 && PyErr_Occurred() ? 0 : stream_ptr(a[3], a[1], r, &stream);
+    Py_DECREF(r);
     if (rc == 0) return nullptr;
     if (rc < 0) {
         PyErr_SetString(PyExc_TypeError, "stream must be a stream, its address or None");
