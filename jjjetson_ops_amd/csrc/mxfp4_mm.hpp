@@ -70,10 +70,11 @@ __device__ __forceinline__ bool mx_expert_tile(const int32_t *__restrict__ offse
         if (past != 0) {
             const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
             const int t0 = base + __builtin_amdgcn_readlane(incl - mine, l);
+            const int begin = __builtin_amdgcn_readlane(beg, l);
             expert = e0 + l;  // scalars: the row addresses below are
-            first = __builtin_amdgcn_readlane(beg, l) + (tile - t0) * rows;
+            first = begin + (tile - t0) * rows;
             end = __builtin_amdgcn_readlane(fin, l);
-            return true;
+            return first >= begin && first < end;  // only sums of a malformed table that overflowed fail it
         }
         base += __builtin_amdgcn_readlane(incl, 63);
     }

@@ -218,3 +218,25 @@ def test_graph(dev):
             torch.cuda.synchronize()
             for a, b in zip(outs, eager):
                 assert torch.equal(a, b)
+
+
+def test_rows_beyond_32_bits(dev):
+    """Sorted rows of 4.6 GB, there and back: with one expert's rows behind the other's, the sum of
+    a token's eight equal rows is exact."""
+    T, k, H, E = 70_000, 8, 4096, 16
+    note(f"rows offsets T={T} k={k} H={H}")
+    gen = torch.Generator(device=dev).manual_seed(1)
+    R = T * k
+    x = torch.randn(T, H, device=dev, dtype=torch.bfloat16, generator=gen)
+    ids = torch.argsort(torch.rand(T, E, device=dev, generator=gen), 1)[:, :k].int().contiguous()
+    rows = torch.empty(R, H, dtype=torch.bfloat16, device=dev)
+    off, src, dst = (torch.empty(n, dtype=torch.int32, device=dev) for n in (E + 1, R, R))
+    capi.moe_dispatch_rows(ids, x, rows, off, src, dst, T, k, H, E)
+    want = torch.argsort(ids.view(-1).long() * R + torch.arange(R, device=dev))
+    assert torch.equal(src.long(), want)
+    assert torch.equal(off.long(), torch.searchsorted(ids.view(-1).sort()[0].long(), torch.arange(E + 1, device=dev)))
+    for p in range(0, R, 70_000):
+        assert torch.equal(rows[p:p + 70_000], x[want[p:p + 70_000] // k])
+    back = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
+    capi.moe_dispatch_rows_backward(rows, dst, back, T, H, k)
+    assert torch.equal(back, x * 8)

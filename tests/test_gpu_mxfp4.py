@@ -421,6 +421,27 @@ def test_gate_up_swiglu_tiles(E, K, N, R, dev):
     _check_swiglu(mx.pack(code[:live], s[:live]), *(t.cpu().numpy() for t in (g, u, dg, du)))
 
 
+@pytest.mark.parametrize("M", [1, 7, 40])
+def test_mat_mul_offsets_beyond_32_bits(M, dev):
+    """A weight of 4.7 GB: its first and last rows."""
+    K, N = 16384, 540_000
+    note(f"mat_mul offsets K={K} N={N} M={M}")
+    gen = torch.Generator(device=dev).manual_seed(M)
+    half = N * (K // 2)
+    w = torch.randint(0, 256, (N * (K // 32) * 17,), dtype=torch.uint8, device=dev, generator=gen)
+    w[half:] = 119 + w[half:] % 7
+    x, xv = _bytes(gen, M, K, dev)
+    y = torch.full((M, N), float("nan"), device=dev)
+    capi.mat_mul_mxfp4(w, x, y, K, N, M)
+    rows = 64
+    for n0 in (0, N - rows):
+        codes, scales = w[n0 * (K // 2):(n0 + rows) * (K // 2)], w[half + n0 * (K // 32):half + (n0 + rows) * (K // 32)]
+        wv = mx.dequantize(torch.cat([codes, scales]).cpu().numpy(), rows, K)
+        exp, bound = _product(xv, torch.from_numpy(wv).to(dev))
+        _close_dev(y[:, n0:n0 + rows], exp, bound)
+    assert not y.isnan().any()
+
+
 # ---------------------------------------------------------------- graphs and streams
 def _replays_match(fn, outs, dev, n=3):
     fn()
