@@ -81,6 +81,7 @@ struct MxFfnWs {
     int32_t *ids, *offsets, *src_route, *dst_of_route;
     uint8_t *xq, *midq;
     float *eout;
+    int slices;  // of the down product, each R rows of eout
     int64_t bytes;
 };
 
@@ -100,7 +101,8 @@ MxFfnWs ffn_layout(uint8_t *base, int T, int H, int I, int E, int top_k) {
     w.dst_of_route = (int32_t *)take(R * 4);
     w.xq = take(mx_bytes(T, H));
     w.midq = take(mx_bytes(R, I));
-    w.eout = (float *)take(R * H * 4);
+    w.slices = mxfp4_down_slices(I, H, (int)R, E);
+    w.eout = (float *)take(w.slices * R * H * 4);
     w.bytes = off;
     return w;
 }
@@ -249,9 +251,10 @@ int moe_mxfp4_ffn_forward_device(void *stream, const void *x, const float *logit
     if ((e = launch_mxfp4_swiglu(w_gate, w_up, ws.xq, ws.midq, H, I, R, g, s)) != hipSuccess)
         return launched(e, "moe_mxfp4_ffn gate|up");
     g.src_route = nullptr;
-    if ((e = launch_mxfp4_mm(w_down, ws.midq, ws.eout, JJO_DTYPE_F32, I, H, R, g, s)) != hipSuccess)
+    if ((e = launch_mxfp4_mm(w_down, ws.midq, ws.eout, JJO_DTYPE_F32, I, H, R, g, s, ws.slices)) != hipSuccess)
         return launched(e, "moe_mxfp4_ffn down");
-    return launched(launch_moe_join_rows(ws.eout, JJO_DTYPE_F32, ws.dst_of_route, ws.route_w, y, dtype, T, H, top_k, s),
+    return launched(launch_moe_join_rows(ws.eout, JJO_DTYPE_F32, ws.dst_of_route, ws.route_w, y, dtype, T, H, top_k, s,
+                                         ws.slices),
                     "moe_mxfp4_ffn combine");
 }
 

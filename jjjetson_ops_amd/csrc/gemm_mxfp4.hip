@@ -29,6 +29,7 @@ struct MxTiled {
     int dtype;
     int K, N, M;
     int tiles_n, tiles_t;  // of the launch
+    int slices;            // of K, each with its own rows of y
     MxGroups g;
 };
 
@@ -201,11 +202,13 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = f32x4v{0.f, 0.f, 0.f, 0.f};
 
-    // A group takes whole pairs of stages.  All run as many rounds as the longest (barriers).
-    const int pairs = (stages + 1) / 2, p_beg = pairs * kg / KG, p_end = pairs * (kg + 1) / KG;
+    // A slice, and in it a group, takes whole pairs of stages.  All run as many rounds as the longest (barriers).
+    const int pairs = (stages + 1) / 2, parts = p.slices * KG, part = (int)blockIdx.y * KG + kg;
+    const int p_beg = pairs * part / parts, p_end = pairs * (part + 1) / parts;
     const int s_beg = 2 * p_beg, s_end = min(2 * p_end, stages);
-    const int rounds = KG == 1 ? stages : 2 * ((pairs + KG - 1) / KG);
-    const int cut = nb % 8 != 0 ? stages - 1 - 2 * (pairs * (KG - 1) / KG) : -1;  // the last group's last round
+    const int rounds = KG == 1 ? s_end - s_beg : 2 * ((pairs + parts - 1) / parts);
+    // The last part's last round, where the row ends inside its stage.
+    const int cut = nb % 8 != 0 && (int)blockIdx.y == p.slices - 1 ? stages - 1 - 2 * (pairs * (parts - 1) / parts) : -1;
     load_scales(p_beg);
     __syncthreads();
     dma(s_beg, 0);
@@ -289,7 +292,9 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
             uint8_t *stage = lds + wave * 4096;
             const int nw = n0 + 16 * RT * wn, tw = first + 16 * TT * wt;
             const int32_t *route_dst = GROUPED ? p.g.route_dst : nullptr;
-            if (p.dtype == JJO_DTYPE_F32) store_rows<float, RT, TT>((float *)p.y, acc, stage, nw, tw, end, p.N, route_dst);
+            if (p.dtype == JJO_DTYPE_F32)
+                store_rows<float, RT, TT>((float *)p.y + (size_t)blockIdx.y * p.M * p.N, acc, stage, nw, tw, end, p.N,
+                                          route_dst);
             else if (p.dtype == JJO_DTYPE_F16)
                 store_rows<_Float16, RT, TT>((_Float16 *)p.y, acc, stage, nw, tw, end, p.N, route_dst);
             else store_rows<__bf16, RT, TT>((__bf16 *)p.y, acc, stage, nw, tw, end, p.N, route_dst);
@@ -317,7 +322,7 @@ hipError_t run_tiled(MxTiled p, hipStream_t stream) {
     p.tiles_t = (p.M + Tile::kRowsT - 1) / Tile::kRowsT + (p.g.offsets != nullptr ? std::min(p.g.n_experts, p.M) : 0);
     const int64_t wgs = (int64_t)p.tiles_n * p.tiles_t;
     if (wgs * Tile::KG * Tile::kThreads >= 1LL << 32) return hipErrorInvalidConfiguration;
-    const dim3 grid((unsigned)wgs), block(Tile::KG * Tile::kThreads);
+    const dim3 grid((unsigned)wgs, (unsigned)p.slices), block(Tile::KG * Tile::kThreads);
     auto go = [&](auto kernel) {
         const hipError_t e = ensure_dynamic_lds((const void *)kernel, Tile::kLds);
         if (e != hipSuccess) return e;
@@ -332,6 +337,7 @@ hipError_t run_tiled(MxTiled p, hipStream_t stream) {
 struct MxTileChoice {
     int tokens;  // 0: the direct kernel
     bool split;  // K cut inside the workgroup
+    float cost;  // of a whole tile's rounds: us at K = 4096
 };
 
 // 128 weight rows on four waves up to 128 tokens, 256 on eight above.
@@ -378,45 +384,67 @@ bool tiles_accept(int K, const MxGroups &g) {
 // 4096 with each CU's share of workgroups in flight (14336 x 4096: 96 tokens' tiles 22 us for 384 tokens, 128 26
 // for 512, 160 31 for 640, 192 34 for 768, 256 41 for 1024, and each of the others there is slower; 8 experts of 28672 rows
 // with 128 tokens each: 160 158 us, 192 165, 128 193).
-MxTileChoice tile_for(int K, int64_t N, int M, const MxGroups &g) {
-    const int64_t experts = mx_experts(M, g), rows = mx_rows(M, g), cus = device_cu_count();
+MxTileChoice tile_for(int K, int64_t N, int M, const MxGroups &g, int64_t cus) {
+    const int64_t experts = mx_experts(M, g), rows = mx_rows(M, g);
     const int64_t mean = (M + experts - 1) / experts;
     const int64_t small = experts * ((N + 15) / 16) * ((rows + 15) / 16);
     const int most = g.offsets == nullptr ? 16 : 10;  // an uneven share of 10 rows is 16 and more for some
-    if (!tiles_accept(K, g) || mean <= 4 || small <= (K < 2048 ? 4 : 8) * cus || (mean <= most && K >= 4096)) return {0, false};
+    if (!tiles_accept(K, g) || mean <= 4 || small <= (K < 2048 ? 4 : 8) * cus || (mean <= most && K >= 4096))
+        return {0, false, 0.f};
     auto rounds = [&](int tokens) {
         const int64_t n = tokens <= 128 ? 128 : 256;
         return (experts * ((rows + tokens - 1) / tokens) * ((N + n - 1) / n) + cus - 1) / cus;
     };
     if (K >= 2048)
         for (int tokens : {32, 64, 96, 128})
-            if (rounds(tokens) == 1) return {tokens, true};
+            if (rounds(tokens) == 1) return {tokens, true, 0.f};
+    MxTileChoice best{0, false, 0.f};
     constexpr struct {
         int tokens;
         float cost;
     } kCost[] = {{32, 9.f}, {64, 10.f}, {96, 11.5f}, {128, 14.f}, {160, 28.5f}, {192, 31.f}, {256, 39.5f}};
-    int best = 0;
-    for (int i = 1; i < 7; ++i)
-        if (rounds(kCost[i].tokens) * kCost[i].cost < rounds(kCost[best].tokens) * kCost[best].cost) best = i;
-    return {kCost[best].tokens, false};
+    for (const auto &c : kCost) {
+        const float cost = (float)rounds(c.tokens) * c.cost;
+        if (best.tokens == 0 || cost < best.cost) best = {c.tokens, false, cost};
+    }
+    return best;
 }
 
 }  // namespace
 
+// Two slices of K (fp32 outputs, N % 8 == 0, added by the reader) for experts whose whole tiles leave CUs without
+// work: the cheapest tile for half the length on twice the workgroups, against the cheapest for all of it (of the
+// difference 0.4 to 0.5 was measured) and the second slice's way through memory, 4 bytes an output at 5 TB/s.  8
+// experts, K = 14336 to 4096: of 128 rows each 66 us on tiles of 160 rows in two slices, 80 on two tiles of 96 rows
+// an expert; of 225 rows 84 and 99, of 512 199 and 225.  The workspace depends on it, so the rule takes the chip's
+// 256 CUs and not the device's.
+constexpr int64_t kMxCus = 256;
+int mxfp4_down_slices(int K, int N, int M, int n_experts) {
+    MxGroups g;
+    static const int32_t grouped = 0;
+    g.offsets = &grouped, g.n_experts = n_experts;
+    const MxTileChoice one = tile_for(K, N, M, g, kMxCus);
+    if (one.tokens == 0 || one.split || K < 4096 || N % 8 != 0) return 1;
+    const MxTileChoice two = tile_for(K, N, M, g, kMxCus / 2);  // tiles as well, and whole ones: fewer CUs
+    return 0.4f * (one.cost - 0.5f * two.cost) * (float)K / 4096.f > (float)M * (float)N * 4.f / 5e6f ? 2 : 1;
+}
+
 hipError_t launch_mxfp4_mm(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
-                           const MxGroups &groups, hipStream_t stream) {
-    const MxTileChoice tile = tile_for(K, N, M, groups);
-    if (tile.tokens == 0) return launch_mxfp4_direct(w, xq, y, dtype, K, N, M, groups, stream);
-    const MxTiled p{(const uint8_t *)w, nullptr, (const uint8_t *)xq, y, dtype, K, N, M, 0, 0, groups};
+                           const MxGroups &groups, hipStream_t stream, int slices) {
+    // A tile for half the length costs half, on twice the workgroups: as if there were half the CUs.
+    const MxTileChoice tile = tile_for(K, N, M, groups, slices == 1 ? device_cu_count() : kMxCus / slices);
+    if (tile.tokens == 0)
+        return slices == 1 ? launch_mxfp4_direct(w, xq, y, dtype, K, N, M, groups, stream) : hipErrorInvalidValue;
+    const MxTiled p{(const uint8_t *)w, nullptr, (const uint8_t *)xq, y, dtype, K, N, M, 0, 0, slices, groups};
     return run_tile<false>(p, tile, stream);
 }
 
 hipError_t launch_mxfp4_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I, int M,
                                const MxGroups &groups, hipStream_t stream) {
-    const MxTileChoice tile = tile_for(K, 2 * (int64_t)I, M, groups);
+    const MxTileChoice tile = tile_for(K, 2 * (int64_t)I, M, groups, device_cu_count());
     if (tile.tokens == 0) return launch_mxfp4_direct_swiglu(w_gate, w_up, xq, mid, K, I, M, groups, stream);
     const MxTiled p{(const uint8_t *)w_gate, (const uint8_t *)w_up, (const uint8_t *)xq, mid, JJO_DTYPE_F32, K, I, M,
-                    0, 0, groups};
+                    0, 0, 1, groups};
     return run_tile<true>(p, tile, stream);
 }
 

@@ -161,7 +161,9 @@ hipError_t launch_mxfp4_direct_swiglu(const void *w_gate, const void *w_up, cons
                                       int M, const MxGroups &groups, hipStream_t stream);
 // ... and on the kernel chosen for the shape.
 hipError_t launch_mxfp4_mm(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
-                           const MxGroups &groups, hipStream_t stream);
+                           const MxGroups &groups, hipStream_t stream, int slices = 1);
+// Slices of K (1 or 2) that a grouped product whose reader adds them is best cut into: y holds slices of M rows.
+int mxfp4_down_slices(int K, int N, int M, int n_experts);
 hipError_t launch_mxfp4_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I, int M,
                                const MxGroups &groups, hipStream_t stream);
 
@@ -176,9 +178,9 @@ hipError_t launch_mxfp4_route(const void *x, int dtype, const float *logits, int
                               float *route_w, int32_t *ids, int32_t *offsets, int32_t *src_route,
                               int32_t *dst_of_route, void *xq, hipStream_t stream);
 // y[t] = sum over k of weights[t, k] * rows[dst(t, k)] (weights nullptr: 1), routes with dst outside
-// [0, T * top_k) left out.
+// [0, T * top_k) left out; fp32 rows may be the sum of two slices (T * top_k rows apart).
 hipError_t launch_moe_join_rows(const void *rows, int rows_dtype, const int32_t *dst_of_route, const float *weights,
-                                void *y, int dtype, int T, int H, int top_k, hipStream_t stream);
+                                void *y, int dtype, int T, int H, int top_k, hipStream_t stream, int slices = 1);
 hipError_t launch_moe_combine_rows_backward(const void *grad_y, const void *rows, int dtype,
                                             const int32_t *dst_of_route, const float *weights, void *grad_rows,
                                             float *grad_weights, int T, int H, int top_k, hipStream_t stream);

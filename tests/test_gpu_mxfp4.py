@@ -326,16 +326,22 @@ def test_ffn_same_expert_for_all_and_for_none(dev):
 
 
 # ------------------------------------------------- large products, every tile; the oracle on the GPU
-def _bytes(gen, rows, cols, dev):
+def _values(q, rows, cols):
+    """The values of an MXFP4 matrix without NaN blocks, in fp64."""
+    half = rows * cols // 2
+    table = torch.from_numpy(mx.values(np.arange(16, dtype=np.uint8))).to(q.device)
+    b = q[:half].view(rows, cols // 2).int()
+    v = torch.stack([table[b & 15], table[b >> 4]], 2).view(rows, cols // 32, 32)
+    v *= torch.exp2(q[half:rows * cols // 32 * 17].view(rows, cols // 32, 1).double() - 127)
+    return v.view(rows, cols)
+
+
+def _bytes(gen, rows, cols, dev, scale=119):
     """Random codes under scales of seven magnitudes, and their values in fp64."""
     half = rows * cols // 2
     q = torch.randint(0, 256, (rows * cols // 32 * 17,), dtype=torch.uint8, device=dev, generator=gen)
-    q[half:] = 119 + q[half:] % 7
-    table = torch.from_numpy(mx.values(np.arange(16, dtype=np.uint8))).to(dev)
-    b = q[:half].view(rows, cols // 2).int()
-    v = torch.stack([table[b & 15], table[b >> 4]], 2).view(rows, cols // 32, 32)
-    v *= torch.exp2(q[half:].view(rows, cols // 32, 1).double() - 127)
-    return q, v.view(rows, cols)
+    q[half:] = scale + q[half:] % 7
+    return q, _values(q, rows, cols)
 
 
 def _product(x, w):
@@ -419,6 +425,45 @@ def test_gate_up_swiglu_tiles(E, K, N, R, dev):
     code, s = mx.unpack(got, R, I)
     assert (got[-16:] == 0x5A).all() and (s[live:] == 0x5A).all()  # rows of no expert stay
     _check_swiglu(mx.pack(code[:live], s[:live]), *(t.cpu().numpy() for t in (g, u, dg, du)))
+
+
+@pytest.mark.parametrize("T,H,I,E,k,dtype", [(500, 4096, 4096, 8, 2, "bf16"), (400, 4096, 8224, 6, 2, "f32"),
+                                             (1100, 2048, 5600, 12, 2, "f16")])
+def test_ffn_down_in_slices(T, H, I, E, k, dtype, dev):
+    """Experts with many rows and few tiles: the down product in two slices of K, added by the
+    combine, against fp64 from the intermediate on."""
+    note(f"ffn slices T={T} H={H} I={I} E={E} k={k} {dtype}")
+    gen = torch.Generator(device=dev).manual_seed(T)
+    R = T * k
+    wg, wu = (_bytes(gen, E * I, H, dev, 116)[0] for _ in range(2))
+    wd = _bytes(gen, E * H, I, dev)[0]
+    x = torch.randn(T, H, device=dev, generator=gen).to(DT[dtype])
+    logits = torch.randn(T, E, device=dev, generator=gen)
+    n = capi.moe_ffn_mxfp4_workspace_bytes(T, H, I, E, k)
+    assert n > 2 * R * H * 4 + capi.mxfp4_bytes(T, H) + capi.mxfp4_bytes(R, I)  # two slices
+    ws = torch.full((n,), 0xFF, dtype=torch.uint8, device=dev)
+    y = torch.full((T, H), float("nan"), dtype=DT[dtype], device=dev)
+    capi.moe_ffn_mxfp4(x, logits, wg, wu, wd, y, T, H, I, E, k, ws)
+
+    i32 = dict(dtype=torch.int32, device=dev)
+    share, ids, off = torch.empty(T, k, device=dev), torch.empty(T, k, **i32), torch.empty(E + 1, **i32)
+    src, dst = torch.empty(R, **i32), torch.empty(R, **i32)
+    rows = torch.empty(R, H, dtype=DT[dtype], device=dev)
+    xq = torch.empty(capi.mxfp4_bytes(R, H), dtype=torch.uint8, device=dev)
+    mid = torch.empty(capi.mxfp4_bytes(R, I), dtype=torch.uint8, device=dev)
+    capi.moe_top_k(logits, share, ids, T, E, k)
+    capi.moe_dispatch_rows(ids, x, rows, off, src, dst, T, k, H, E)
+    capi.quantize_mxfp4(rows, xq, R, H)
+    capi.moe_gate_up_swiglu_mxfp4(wg, wu, xq, off, E, mid, H, I, R)
+    o, midv, wdv = off.tolist(), _values(mid, R, I), _values(wd, E * H, I)
+    eo, eb = (torch.zeros(R, H, dtype=torch.float64, device=dev) for _ in range(2))
+    for e in range(E):
+        q = slice(o[e], o[e + 1])
+        eo[q], eb[q] = _product(midv[q], wdv[e * H:(e + 1) * H])
+    d, w = dst.long().view(T, k), share.double()[..., None]
+    exp = (w * eo[d]).sum(1)
+    bound = (w * (eb[d] + k * 2.0 ** -23 * eo[d].abs())).sum(1)
+    _close_dev(y, exp, bound + mx.HALF_STEP[dtype] * (exp.abs() + bound) + mx.TINY[dtype])
 
 
 @pytest.mark.parametrize("M", [1, 7, 40])
