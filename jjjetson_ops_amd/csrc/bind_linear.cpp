@@ -293,7 +293,8 @@ extern "C" __attribute__((visibility("default"))) PyObject *PyInit__linear(void)
     s_data_ptr = PyUnicode_InternFromString("data_ptr");
     s_cuda_stream = PyUnicode_InternFromString("cuda_stream");
     s_get_device = PyUnicode_InternFromString("get_device");
-    if (s_get_device == nullptr || s_is_cuda == nullptr || s_is_contiguous == nullptr || s_data_ptr == nullptr || s_cuda_stream == nullptr)
+    if (s_get_device == nullptr || s_is_cuda == nullptr || s_is_contiguous == nullptr || s_data_ptr == nullptr ||
+        s_cuda_stream == nullptr)
         return nullptr;
     return PyModule_Create(&module);
 }

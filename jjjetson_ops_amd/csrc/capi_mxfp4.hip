@@ -15,7 +15,8 @@ int elem_bytes(int d) { return d == JJO_DTYPE_F32 ? 4 : 2; }
 // A launch's status; a shape whose tiles do not fit one grid is the caller's error.
 int launched(hipError_t e, const char *what) {
     if (e == hipSuccess) return JJO_OK;
-    if (e == hipErrorInvalidConfiguration) return set_error(JJO_ERR_INVALID_ARG, "%s: the shape exceeds one launch", what);
+    if (e == hipErrorInvalidConfiguration)
+        return set_error(JJO_ERR_INVALID_ARG, "%s: the shape exceeds one launch", what);
     return hip_fail(e, what);
 }
 
@@ -31,8 +32,9 @@ int check_rows(const char *who, const void *x, int dtype, int64_t row_stride, co
     if (!aligned(x, 16) || !aligned(q, 16))
         return set_error(JJO_ERR_INVALID_ARG, "%s: 16-byte aligned buffers required", who);
     if (rows > 1 && (row_stride < cols || row_stride > (1LL << 40) || row_stride * elem_bytes(dtype) % 16 != 0))
-        return set_error(JJO_ERR_INVALID_ARG, "%s: row_stride=%lld must be at least cols=%lld and keep rows 16-byte aligned",
-                         who, (long long)row_stride, (long long)cols);
+        return set_error(JJO_ERR_INVALID_ARG,
+                         "%s: row_stride=%lld must be at least cols=%lld and keep rows 16-byte aligned", who,
+                         (long long)row_stride, (long long)cols);
     return JJO_OK;
 }
 
@@ -59,7 +61,8 @@ int check_experts(const char *who, const void *offsets, int n_experts) {
 
 int check_routes(const char *who, int dtype, int T, int H, int E, int top_k) {
     if (!dtype_ok(dtype)) return set_error(JJO_ERR_INVALID_ARG, "%s: unknown dtype %d", who, dtype);
-    if (T <= 0 || H <= 0) return set_error(JJO_ERR_INVALID_ARG, "%s: num_tokens=%d hidden_size=%d must be positive", who, T, H);
+    if (T <= 0 || H <= 0)
+        return set_error(JJO_ERR_INVALID_ARG, "%s: num_tokens=%d hidden_size=%d must be positive", who, T, H);
     if (E <= 0 || E > 1024 || top_k <= 0 || top_k > 32)
         return set_error(JJO_ERR_INVALID_ARG, "%s: need 1 <= top_k <= 32 and 1 <= num_experts <= 1024 (got top_k=%d "
                          "num_experts=%d)", who, top_k, E);
@@ -72,7 +75,8 @@ int check_routes(const char *who, int dtype, int T, int H, int E, int top_k) {
 // Every chunk of the sort counts all routes: quadratic in their number.
 int check_sort(const char *who, int T, int top_k) {
     if ((int64_t)T * top_k > 1 << 24)
-        return set_error(JJO_ERR_INVALID_ARG, "%s: num_tokens=%d * top_k=%d: at most 2^24 routes are sorted", who, T, top_k);
+        return set_error(JJO_ERR_INVALID_ARG, "%s: num_tokens=%d * top_k=%d: at most 2^24 routes are sorted", who, T,
+                         top_k);
     return JJO_OK;
 }
 

@@ -4,18 +4,19 @@
 //     y[t][n] = sum over blocks b of 2^(sw[n,b] + sx[t,b] - 254) * sum_j cw[n,b,j] * cx[t,b,j]
 //
 // A stage is 256 values (128 bytes) of every weight row and token row of the tile, two steps of the
-// matrix instruction.  The codes go to LDS by DMA, 8 rows of 128 bytes an instruction, the 16-byte pieces of a
-// row permuted by its row number (piece ^ row / 2 % 8) so that the 16 lanes that LDS serves at a time
-// fall in its 64 banks once; of the stage's 8 blocks lane group q of a step u takes block 2q + u,
-// so that a lane's two scale bytes are one 16-bit read and the instruction picks the byte.  The
-// scales (8 bytes a row and stage, of any alignment) go through a register of one thread per row, two
-// stages at a time.  While a stage is computed the next one lands in the other buffer; one barrier per stage.
+// matrix instruction.  The codes go to LDS by DMA, 8 rows of 128 bytes an instruction, the 16-byte
+// pieces of a row permuted by its row number (piece ^ row / 2 % 8) so that the 16 lanes that LDS
+// serves at a time fall in its 64 banks once; of the stage's 8 blocks lane group q of a step u takes
+// block 2q + u, so that a lane's two scale bytes are one 16-bit read and the instruction picks the
+// byte.  The scales (8 bytes a row and stage, of any alignment) go through a register of one thread
+// per row, two stages at a time.  While a stage is computed the next one lands in the other buffer;
+// one barrier per stage.
 //
-// What bounds it: for prompts the matrix instruction and LDS together (2047 x 14336 x 4096: 79 us, 3.0 Pflop/s;
-// the instruction alone on random data in registers reaches 6.2, a library product of 8192 cubed 3.1); a
-// small product a stage's latency, about 1 us.  There the tiles are cut along K as well (KG), into groups of
-// waves with stages of their own, so that two or three stages are in flight: 4096 x 4096 and 256 tokens 13.4
-// us, 17.3 without.
+// What bounds it: for prompts the matrix instruction and LDS together (2047 tokens, 14336 x 4096:
+// 79 us, 3.0 Pflop/s; 66 without any load; the instruction alone on random data in registers
+// reaches 6.2 Pflop/s, a library product of 8192 cubed 3.1); a small product a stage's latency, about
+// 1 us.  There the tiles are cut along K as well (KG), into groups of waves with stages of their
+// own, so that two or three stages are in flight: 4096 x 4096 and 256 tokens 13.4 us, 17.3 without.
 #include <hip/hip_runtime.h>
 
 #include "mxfp4_mm.hpp"
@@ -44,7 +45,8 @@ struct MxTile {
     static constexpr int kScaleRows = (kRows + kThreads - 1) / kThreads;  // rows a thread
     static constexpr int kStage = kRows * 128, kGroupLds = 2 * (kStage + kRows * 16);
     static constexpr int kLds = KG * kGroupLds + kRows * 4;
-    static_assert(kLds <= 160 * 1024 && (KG == 1 || kThreads * RT * TT * 16 <= kGroupLds), "a group's sums fit its stages");
+    static_assert(kLds <= 160 * 1024, "LDS of a CU");
+    static_assert(KG == 1 || kThreads * RT * TT * 16 <= kGroupLds, "a group's sums fit its stages");
 };
 
 // A wave's outputs (from weight row n, token t on) through its own 4 KB of LDS, 16 tokens at a time:
@@ -71,7 +73,8 @@ __device__ __forceinline__ void store_rows(T *__restrict__ y, const f32x4v (&acc
 #pragma unroll
         for (int k = 0; k < 16 / kRowsAtOnce; ++k) {
             const int r = kRowsAtOnce * k + row, token = t + 16 * tt + r;
-            const u32x4v v = *reinterpret_cast<const u32x4v *>(stage + r * (kChunks * 16) + 16 * (chunk ^ (r % kChunks)));
+            const u32x4v v =
+                *reinterpret_cast<const u32x4v *>(stage + r * (kChunks * 16) + 16 * (chunk ^ (r % kChunks)));
             if (token < end && n + chunk * kVec < N) {
                 const size_t to = route_dst != nullptr ? route_dst[token] : token;
                 *reinterpret_cast<u32x4v *>(y + to * N + n + chunk * kVec) = v;
@@ -123,10 +126,9 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
     const size_t w_first = (size_t)expert * p.N, w_all = (size_t)(GROUPED ? p.g.n_experts : 1) * p.N;
     const size_t x_all = p.g.src_route != nullptr ? p.g.x_rows : p.M;
 
-    // ---- the DMA: instruction i of a wave takes run kDma * wave + i of 8 rows, a lane piece (lane % 8) ^ (row / 2 % 8) of
-    // row lane / 8.  The
-    // rows' offsets stand in LDS: kept in registers they would spill, and a reload from scratch
-    // waits for every DMA before it.
+    // ---- the DMA: instruction i of a wave takes run kDma * wave + i of 8 rows, a lane piece
+    // (lane % 8) ^ (row / 2 % 8) of row lane / 8.  The rows' offsets stand in LDS: kept in registers
+    // they would spill, and a reload from scratch waits for every DMA before it.
     const int t0 = GROUPED && p.g.src_route != nullptr ? 0 : first;
     for (int row = threadIdx.x; row < Tile::kRows; row += KG * Tile::kThreads)
         lds_rows[row] = row < Tile::kRowsN ? (uint32_t)(weight_row(row) - n0) * half
@@ -208,7 +210,8 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
     const int s_beg = 2 * p_beg, s_end = min(2 * p_end, stages);
     const int rounds = KG == 1 ? s_end - s_beg : 2 * ((pairs + parts - 1) / parts);
     // The last part's last round, where the row ends inside its stage.
-    const int cut = nb % 8 != 0 && (int)blockIdx.y == p.slices - 1 ? stages - 1 - 2 * (pairs * (parts - 1) / parts) : -1;
+    const bool ends = nb % 8 != 0 && (int)blockIdx.y == p.slices - 1;
+    const int cut = ends ? stages - 1 - 2 * (pairs * (parts - 1) / parts) : -1;
     load_scales(p_beg);
     __syncthreads();
     dma(s_beg, 0);
@@ -237,9 +240,11 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
         const uint8_t *sbuf = lds_scales + (st & 3) * (Tile::kRows * 8);
         uint32_t sw[RT], sx[TT];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) sw[rt] = *reinterpret_cast<const uint16_t *>(sbuf + (w_at + 16 * rt) * 8 + 2 * q);
+        for (int rt = 0; rt < RT; ++rt)
+            sw[rt] = *reinterpret_cast<const uint16_t *>(sbuf + (w_at + 16 * rt) * 8 + 2 * q);
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt) sx[tt] = *reinterpret_cast<const uint16_t *>(sbuf + (x_at + 16 * tt) * 8 + 2 * q);
+        for (int tt = 0; tt < TT; ++tt)
+            sx[tt] = *reinterpret_cast<const uint16_t *>(sbuf + (x_at + 16 * tt) * 8 + 2 * q);
         auto step = [&](auto u_tag) {
             constexpr int U = decltype(u_tag)::value;
             const uint8_t *at = buf + (U == 0 ? sw0 : sw1);
@@ -271,7 +276,8 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
 #pragma unroll
         for (int k = 1; k < KG; ++k)
 #pragma unroll
-            for (int i = 0; i < RT * TT; ++i) acc[i / TT][i % TT] += sums[(k * Tile::kGroupLds / 16) + i * Tile::kThreads];
+            for (int i = 0; i < RT * TT; ++i)
+                acc[i / TT][i % TT] += sums[(k * Tile::kGroupLds / 16) + i * Tile::kThreads];
     }
 
     if constexpr (SWIGLU) {
@@ -372,18 +378,19 @@ bool tiles_accept(int K, const MxGroups &g) {
 // The kernel of a product with N weight rows in all (gate and up together).
 //
 // The direct kernel is bound by its workgroups' work, a tile by the latency of its stages, which is
-// the same for any output up to a tile per CU: 4096 x 4096 and 64 / 128 / 256 tokens 7.6 / 11.7 /
-// 18.8 us direct against 13.5 / 13.3 / 13.4 us on split tiles, 8192 x 14336 and 64 / 96 tokens 36 / 52 against 38 /
-// 38 us.  They meet at 8 workgroups of 16 rows x 16 tokens a CU (4 where K < 2048: 32768 x 1024 and 12
-// tokens, 8 a CU, 8.4 against 7.2 us).  Behind that the matrix itself is the bound: up to 16 tokens the direct
-// kernel reads it as fast from K = 4096 on (131072 x 4096, 16 tokens: 59 against 63 us).
+// the same for any output up to a tile per CU: 4096 x 4096 (N x K) and 64 / 128 / 256 tokens 7.6 /
+// 11.7 / 18.8 us direct against 13.5 / 13.3 / 13.4 us on split tiles, 8192 x 14336 and 64 / 96 tokens
+// 36 / 52 against 38 / 38 us.  They meet at 8 workgroups of 16 rows x 16 tokens a CU (4 where K <
+// 2048: 32768 x 1024 and 12 tokens, 8 a CU, 8.4 against 7.2 us).  Behind that the matrix itself is the
+// bound: up to 16 tokens the direct kernel reads it as fast from K = 4096 on (131072 x 4096, 16
+// tokens: 59 against 63 us).
 //
-// Split tiles where the smallest tile that leaves at most one workgroup a CU can do it (4096 x 4096, 256
-// tokens: 13.4 against 17.3 us; 14336 x 4096, 256: 20.4 against 21.9; 4096 x 11008, 512: 27.6 against 34).
-// Otherwise the tile whose rounds over the CUs cost least; kCost is a round's time in us at K =
-// 4096 with each CU's share of workgroups in flight (14336 x 4096: 96 tokens' tiles 22 us for 384 tokens, 128 26
-// for 512, 160 31 for 640, 192 34 for 768, 256 41 for 1024, and each of the others there is slower; 8 experts of 28672 rows
-// with 128 tokens each: 160 158 us, 192 165, 128 193).
+// Split tiles where the smallest tile that leaves at most one workgroup a CU can do it (4096 x 4096,
+// 256 tokens: 13.4 against 17.3 us; 14336 x 4096, 256: 20.4 against 21.9; 4096 x 11008, 512: 27.6
+// against 34).  Otherwise the tile whose rounds over the CUs cost least; kCost is a round's time in
+// us at K = 4096 with each CU's share of workgroups in flight (14336 x 4096: tiles of 96 take 22 us
+// for 384 tokens, 128 26 for 512, 160 31 for 640, 192 34 for 768, 256 41 for 1024, and each of the
+// others there is slower; 8 experts of 28672 rows with 128 tokens each: 160 158 us, 192 165, 128 193).
 MxTileChoice tile_for(int K, int64_t N, int M, const MxGroups &g, int64_t cus) {
     const int64_t experts = mx_experts(M, g), rows = mx_rows(M, g);
     const int64_t mean = (M + experts - 1) / experts;
@@ -412,12 +419,13 @@ MxTileChoice tile_for(int K, int64_t N, int M, const MxGroups &g, int64_t cus) {
 
 }  // namespace
 
-// Two slices of K (fp32 outputs, N % 8 == 0, added by the reader) for experts whose whole tiles leave CUs without
-// work: the cheapest tile for half the length on twice the workgroups, against the cheapest for all of it (of the
-// difference 0.4 to 0.5 was measured) and the second slice's way through memory, 4 bytes an output at 5 TB/s.  8
-// experts, K = 14336 to 4096: of 128 rows each 66 us on tiles of 160 rows in two slices, 80 on two tiles of 96 rows
-// an expert; of 225 rows 84 and 99, of 512 199 and 225.  The workspace depends on it, so the rule takes the chip's
-// 256 CUs and not the device's.
+// Two slices of K (fp32 outputs, N % 8 == 0, added by the reader) for experts whose whole tiles leave
+// CUs without work: the cheapest tile for half the length on twice the workgroups, against the
+// cheapest for all of it (of the difference 0.4 to 0.5 was measured) and the second slice's way
+// through memory, 4 bytes an output at 5 TB/s.  8 experts, K = 14336 to 4096: of 128 rows each 66 us on
+// tiles of 160 rows in two slices, 80 on two tiles of 96 rows an expert; of 225 rows 84 and 99, of 512
+// 199 and 225.  The workspace depends on it, so the rule takes the chip's 256 CUs and not the
+// device's.
 constexpr int64_t kMxCus = 256;
 int mxfp4_down_slices(int K, int N, int M, int n_experts) {
     MxGroups g;

@@ -254,7 +254,8 @@ template <int TG, int KW, int RW, bool SWIGLU, class XT = void>
 hipError_t run_direct(MxProblem p, hipStream_t stream) {
     constexpr int rows = SWIGLU ? 32 : 16 * RW, threads = 64 * KW * RW;
     // token tiles of M rows, and one more for each expert that can have a rest
-    const int64_t token_tiles = (p.M + 4 * TG - 1) / (4 * TG) + (p.g.offsets != nullptr ? std::min(p.g.n_experts, p.M) : 0);
+    const int64_t rests = p.g.offsets != nullptr ? std::min(p.g.n_experts, p.M) : 0;
+    const int64_t token_tiles = (p.M + 4 * TG - 1) / (4 * TG) + rests;
     p.tiles_n = (p.N + rows - 1) / rows;
     const int64_t wgs = token_tiles * p.tiles_n;
     if (wgs * threads >= 1LL << 32) return hipErrorInvalidConfiguration;

@@ -332,7 +332,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const TI *__restrict__ r
             if ((unsigned)pos[j] < (unsigned)R)
                 v[j] = *reinterpret_cast<const MxVec<TI, VEC> *>(rows + (size_t)pos[j] * H + h);
             if (SLICES == 2 && (unsigned)pos[j] < (unsigned)R)
-                v2[SLICES == 2 ? j : 0] = *reinterpret_cast<const MxVec<TI, VEC> *>(rows + ((size_t)R + pos[j]) * H + h);
+                v2[SLICES == 2 ? j : 0] =
+                    *reinterpret_cast<const MxVec<TI, VEC> *>(rows + ((size_t)R + pos[j]) * H + h);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -340,7 +341,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const TI *__restrict__ r
                 const float w = WEIGHTED ? weights[t * top_k + k0 + j] : 1.0f;
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    const float e = SLICES == 2 ? (float)v[j].v[i] + (float)v2[SLICES == 2 ? j : 0].v[i] : (float)v[j].v[i];
+                    float e = (float)v[j].v[i];
+                    if constexpr (SLICES == 2) e += (float)v2[j].v[i];
                     acc[i] = fmaf(w, e, acc[i]);
                 }
             }
@@ -465,8 +467,8 @@ hipError_t run_join(const void *rows, const int32_t *dst, const float *weights, 
     const dim3 grid((unsigned)T, (unsigned)((H / VEC + 255) / 256));
     if (slices == 2) {
         if constexpr (sizeof(TI) == 4 && VEC == 4) {  // the FFN's: H % 32 == 0
-            hipLaunchKernelGGL((join_rows_kernel<TI, TO, VEC, true, 2>), grid, dim3(256), 0, stream, (const TI *)rows, dst,
-                               weights, T * top_k, top_k, H, (TO *)y);
+            hipLaunchKernelGGL((join_rows_kernel<TI, TO, VEC, true, 2>), grid, dim3(256), 0, stream, (const TI *)rows,
+                               dst, weights, T * top_k, top_k, H, (TO *)y);
             return hipGetLastError();
         }
         return hipErrorInvalidValue;
@@ -484,7 +486,8 @@ template <class TI, class TO>
 hipError_t run_join_types(const void *rows, const int32_t *dst, const float *weights, void *y, int T, int H, int top_k,
                           hipStream_t stream, int slices) {
     constexpr int kWide = 16 / sizeof(TI);
-    if (H % kWide == 0 && aligned_to(rows, y, 16)) return run_join<TI, TO, kWide>(rows, dst, weights, y, T, H, top_k, stream, slices);
+    if (H % kWide == 0 && aligned_to(rows, y, 16))
+        return run_join<TI, TO, kWide>(rows, dst, weights, y, T, H, top_k, stream, slices);
     if (sizeof(TI) == 2 && H % 2 == 0 && aligned_to(rows, y, 4))
         return run_join<TI, TO, 2>(rows, dst, weights, y, T, H, top_k, stream, slices);
     return run_join<TI, TO, 1>(rows, dst, weights, y, T, H, top_k, stream, slices);
@@ -495,7 +498,8 @@ hipError_t launch_moe_join_rows(const void *rows, int rows_dtype, const int32_t 
                                 void *y, int dtype, int T, int H, int top_k, hipStream_t stream, int slices) {
     return mx_by_dtype(rows_dtype, [&](auto in) {
         using TI = typename decltype(in)::type;
-        if (rows_dtype == dtype) return run_join_types<TI, TI>(rows, dst_of_route, weights, y, T, H, top_k, stream, slices);
+        if (rows_dtype == dtype)
+            return run_join_types<TI, TI>(rows, dst_of_route, weights, y, T, H, top_k, stream, slices);
         if (rows_dtype != JJO_DTYPE_F32) return hipErrorInvalidValue;
         return dtype == JJO_DTYPE_F16
                    ? run_join_types<float, _Float16>(rows, dst_of_route, weights, y, T, H, top_k, stream, slices)

@@ -374,8 +374,8 @@ def test_mat_mul_tiles(K, N, M, dev):
 
 # (E, K, values a row of the two matrices together, rows): the same tiles for an expert's rows.
 TILES = [(4, 2080, 4160, 48), (4, 2336, 4160, 160), (4, 2080, 4160, 256), (4, 2048, 4160, 400), (4, 544, 4160, 48),
-         (4, 1056, 4160, 160), (4, 608, 4160, 256), (4, 768, 4160, 400), (8, 544, 8192, 1030), (8, 544, 8192, 1240), (8, 800, 8192, 1600),
-         (4, 2080, 4160, 16)]
+         (4, 1056, 4160, 160), (4, 608, 4160, 256), (4, 768, 4160, 400), (8, 544, 8192, 1030), (8, 544, 8192, 1240),
+         (8, 800, 8192, 1600), (4, 2080, 4160, 16)]
 
 
 def _uneven(E, R):
@@ -395,7 +395,8 @@ def test_grouped_tiles(E, K, N, R, dev):
     w, wv = _bytes(gen, E * N, K, dev)
     x, xv = _bytes(gen, R, K, dev)
     off = _uneven(E, R)
-    exp, bound = torch.full((R, N), 5.0, dtype=torch.float64, device=dev), torch.zeros(R, N, dtype=torch.float64, device=dev)
+    exp = torch.full((R, N), 5.0, dtype=torch.float64, device=dev)
+    bound = torch.zeros_like(exp)
     for e in range(E):
         r = slice(off[e], off[e + 1])
         exp[r], bound[r] = _product(xv[r], wv[e * N:(e + 1) * N])
@@ -522,6 +523,45 @@ def test_graph(T, dev):
         capi.linear_mxfp4(y, wg, z, H, E * I, T, ws=lw)
 
     _replays_match(step, [y, z], dev)
+
+
+@pytest.mark.parametrize("T,H,I", [(300, 544, 576), (500, 4096, 4096)])
+def test_graph_tiles(T, H, I, dev):
+    """The tiled kernels, the two-launch routing and the sliced down product; two graphs of one
+    workspace, replayed in turn."""
+    note(f"mxfp4 graph tiles T={T} H={H}")
+    E, k = 8, 2
+    gen = torch.Generator(device=dev).manual_seed(T)
+    wg, wu, wd = (_bytes(gen, rows, cols, dev, 116)[0] for rows, cols in ((E * I, H), (E * I, H), (E * H, I)))
+    xs = [torch.randn(T, H, device=dev, generator=gen).bfloat16() for _ in range(2)]
+    logits = torch.randn(T, E, device=dev, generator=gen)
+    ws = torch.empty(capi.moe_ffn_mxfp4_workspace_bytes(T, H, I, E, k), dtype=torch.uint8, device=dev)
+    lw = torch.empty(capi.linear_mxfp4_workspace_bytes(H, T), dtype=torch.uint8, device=dev)
+    ys, zs = [torch.empty_like(x) for x in xs], [torch.empty(T, E * I, device=dev) for _ in xs]
+
+    def step(i):
+        capi.moe_ffn_mxfp4(xs[i], logits, wg, wu, wd, ys[i], T, H, I, E, k, ws)
+        capi.linear_mxfp4(ys[i], wg, zs[i], H, E * I, T, ws=lw)
+
+    for i in range(2):
+        step(i)
+    torch.cuda.synchronize()
+    eager = [t.clone() for t in ys + zs]
+    s, graphs = torch.cuda.Stream(), []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=s):
+            step(i)
+    for _ in range(3):
+        for t in ys + zs:
+            t.zero_()
+        ws.fill_(0xFF)
+        torch.cuda.synchronize()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(ys + zs, eager):
+            assert torch.equal(a, b)
 
 
 def test_streams(dev):
