@@ -35,18 +35,21 @@ struct MxTiled {
 };
 
 // WN x WT waves of RT tiles of 16 weight rows x TT tiles of 16 tokens each; KG groups of such waves
-// cut K between them, each with stages of its own.
-template <int RT_, int TT_, int WN_, int WT_, int KG_ = 1>
+// cut K between them, each with stages of its own; NW stages of weights in LDS (and two of x).
+template <int RT_, int TT_, int WN_, int WT_, int KG_ = 1, int NW_ = 2>
 struct MxTile {
-    static constexpr int RT = RT_, TT = TT_, WN = WN_, WT = WT_, KG = KG_;
+    static constexpr int RT = RT_, TT = TT_, WN = WN_, WT = WT_, KG = KG_, NW = NW_;
     static constexpr int kWaves = WN * WT, kThreads = 64 * kWaves;  // of a group
     static constexpr int kRowsN = 16 * RT * WN, kRowsT = 16 * TT * WT, kRows = kRowsN + kRowsT;
-    static constexpr int kRuns = kRows / 8, kDma = (kRuns + kWaves - 1) / kWaves;  // DMA instructions; a wave's
+    static constexpr int kRunsN = kRowsN / 8, kRunsT = kRowsT / 8;  // DMA instructions a stage, and a wave's
+    static constexpr int kDmaN = (kRunsN + kWaves - 1) / kWaves, kDmaT = (kRunsT + kWaves - 1) / kWaves;
     static constexpr int kScaleRows = (kRows + kThreads - 1) / kThreads;  // rows a thread
-    static constexpr int kStage = kRows * 128, kGroupLds = 2 * (kStage + kRows * 16);
+    static constexpr int kStageN = kRowsN * 128, kStageT = kRowsT * 128;
+    static constexpr int kGroupLds = NW * kStageN + 2 * kStageT + 2 * kRows * 16;
     static constexpr int kLds = KG * kGroupLds + kRows * 4;
     static_assert(kLds <= 160 * 1024, "LDS of a CU");
     static_assert(KG == 1 || kThreads * RT * TT * 16 <= kGroupLds, "a group's sums fit its stages");
+    static_assert(NW == 2 || (NW == 3 && KG == 1), "weights one stage ahead or two");
 };
 
 // A wave's outputs (from weight row n, token t on) through its own 4 KB of LDS, 16 tokens at a time:
@@ -92,7 +95,8 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
     const int lane = threadIdx.x & 63, any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kg = KG == 1 ? 0 : any_wave / Tile::kWaves, wave = KG == 1 ? any_wave : any_wave % Tile::kWaves;
     const int tid = KG == 1 ? (int)threadIdx.x : 64 * wave + lane;  // in the group
-    uint8_t *const lds = lds_all + kg * Tile::kGroupLds, *const lds_scales = lds + 2 * Tile::kStage;
+    uint8_t *const lds = lds_all + kg * Tile::kGroupLds, *const lds_x = lds + Tile::NW * Tile::kStageN;
+    uint8_t *const lds_scales = lds_x + 2 * Tile::kStageT;
     uint32_t *const lds_rows = reinterpret_cast<uint32_t *>(lds_all + KG * Tile::kGroupLds);
     const int r16 = lane & 15, q = lane >> 4;
     const int wn = wave % Tile::WN, wt = wave / Tile::WN;
@@ -170,25 +174,29 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
             }
         }
     };
-    const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
-    auto dma = [&](int st, int buffer) {
+    // The weights' (or x's) part of stage st to its `buffer`-th place.
+    auto dma = [&](auto x_tag, int st, int buffer) {
+        constexpr bool X = decltype(x_tag)::value;
+        constexpr int kRuns = X ? Tile::kRunsT : Tile::kRunsN, kMine = X ? Tile::kDmaT : Tile::kDmaN;
+        const uint32_t to = X ? (uint32_t)(uintptr_t)lds_x + buffer * Tile::kStageT
+                              : (uint32_t)(uintptr_t)lds + buffer * Tile::kStageN;
         const uint32_t left = 16u * (uint32_t)(nb - 8 * st);  // bytes of the row from the stage on
         const uint32_t most = left >= 128u ? 112u : left - 16u;
         const uint32_t even = min((uint32_t)piece, most), odd = min((uint32_t)piece ^ 64u, most);
         auto run = [&](int i) {  // of 8 rows; the last one again where they do not divide
-            const int at = wave * Tile::kDma + i;
-            return Tile::kRuns % Tile::kWaves == 0 ? at : min(at, Tile::kRuns - 1);
+            const int at = wave * kMine + i;
+            return kRuns % Tile::kWaves == 0 ? at : min(at, kRuns - 1);
         };
-        uint32_t off[Tile::kDma];
+        uint32_t off[kMine];
 #pragma unroll
-        for (int i = 0; i < Tile::kDma; ++i) off[i] = lds_rows[8 * run(i) + (lane >> 3)] + (run(i) & 1 ? odd : even);
+        for (int i = 0; i < kMine; ++i)
+            off[i] = lds_rows[(X ? Tile::kRowsN : 0) + 8 * run(i) + (lane >> 3)] + (run(i) & 1 ? odd : even);
 #pragma unroll
-        for (int i = 0; i < Tile::kDma; ++i) {
-            const int row8 = 8 * run(i);
-            const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds0 + buffer * Tile::kStage + 128 * row8);
-            // Masks, not branches: a choice among captured addresses would go through scratch.
-            const uint64_t up = -(uint64_t)is_up(row8), x = -(uint64_t)(row8 >= Tile::kRowsN);
-            const uint64_t from = (x_base & x) + ((w_base + (up & (w2_base - w_base))) & ~x) + (uint64_t)st * 128;
+        for (int i = 0; i < kMine; ++i) {
+            const uint32_t m0v = __builtin_amdgcn_readfirstlane(to + 1024 * run(i));
+            // A mask, not a branch: a choice among captured addresses would go through scratch.
+            const uint64_t up = -(uint64_t)is_up(8 * run(i));
+            const uint64_t from = (X ? x_base : w_base + (up & (w2_base - w_base))) + (uint64_t)st * 128;
             // Five wait states: an SGPR that a VALU instruction wrote is not read by a load before, nor M0 in the
             // next cycle, and the compiler does not count them for an asm statement.
             asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
@@ -197,6 +205,8 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
                          : "memory");
         }
     };
+    constexpr std::integral_constant<bool, false> kW{};
+    constexpr std::integral_constant<bool, true> kX{};
 
     f32x4v acc[RT][TT];
 #pragma unroll
@@ -214,12 +224,16 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
     const int cut = ends ? stages - 1 - 2 * (pairs * (parts - 1) / parts) : -1;
     load_scales(p_beg);
     __syncthreads();
-    dma(s_beg, 0);
-    const uint32_t w_at = (uint32_t)(16 * RT * wn + r16), x_at = (uint32_t)(Tile::kRowsN + 16 * TT * wt + r16);
+    dma(kW, s_beg, 0);
+    dma(kX, s_beg, 0);
+    if constexpr (Tile::NW == 3) dma(kW, min(s_beg + 1, s_end - 1), 1);
+    const uint32_t w_at = (uint32_t)(16 * RT * wn + r16), x_at = (uint32_t)(16 * TT * wt + r16);
+    int w_buffer = 0;
     const uint32_t sw0 = 16u * ((2 * q) ^ (r16 >> 1)), sw1 = 16u * ((2 * q + 1) ^ (r16 >> 1));
     for (int round = 0; round < rounds; ++round) {
         const int st = s_beg + round;  // s_beg is even
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // stage st has landed
+        // Stage st has landed: loads return in order, the last ones are the next stage's weights (NW == 3).
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(Tile::NW == 3 ? Tile::kDmaN : 0) : "memory");
         if ((st & 1) == 0 && (KG == 1 || st < s_end)) store_scales(st >> 1);
         if (round == cut) {  // the row ends inside the last stage: zero weights behind it
             asm volatile("s_barrier" ::: "memory");
@@ -227,16 +241,19 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
             if (kg == KG - 1)
                 for (int i = tid; i < Tile::kRowsN * 8; i += Tile::kThreads)
                     if ((i & 7) >= 8 - over)
-                        *reinterpret_cast<u32x4v *>(lds + (st & 1) * Tile::kStage + (i >> 3) * 128 +
+                        *reinterpret_cast<u32x4v *>(lds + w_buffer * Tile::kStageN + (i >> 3) * 128 +
                                                     16 * ((i & 7) ^ ((i >> 4) & 7))) = u32x4v{0u, 0u, 0u, 0u};
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         // The next stage on its way; behind the last one, the last again (nothing reads it).
-        const int next = min(st + 1, s_end - 1);
         if ((st & 1) == 0) load_scales(min((st >> 1) + 1, p_end - 1));
-        dma(next, (st + 1) & 1);
+        const int w_next = w_buffer == Tile::NW - 1 ? 0 : w_buffer + 1;
+        if constexpr (Tile::NW == 2) dma(kW, min(st + 1, s_end - 1), w_next);
+        dma(kX, min(st + 1, s_end - 1), (st + 1) & 1);
+        if constexpr (Tile::NW == 3) dma(kW, min(st + 2, s_end - 1), w_next == 2 ? 0 : w_next + 1);
+        const uint8_t *wbuf = lds + w_buffer * Tile::kStageN, *xbuf = lds_x + (st & 1) * Tile::kStageT;
+        w_buffer = w_next;
         if (KG > 1 && st >= s_end) continue;
-        const uint8_t *buf = lds + (st & 1) * Tile::kStage;
         const uint8_t *sbuf = lds_scales + (st & 3) * (Tile::kRows * 8);
         uint32_t sw[RT], sx[TT];
 #pragma unroll
@@ -244,16 +261,16 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
             sw[rt] = *reinterpret_cast<const uint16_t *>(sbuf + (w_at + 16 * rt) * 8 + 2 * q);
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt)
-            sx[tt] = *reinterpret_cast<const uint16_t *>(sbuf + (x_at + 16 * tt) * 8 + 2 * q);
+            sx[tt] = *reinterpret_cast<const uint16_t *>(sbuf + (Tile::kRowsN + x_at + 16 * tt) * 8 + 2 * q);
         auto step = [&](auto u_tag) {
             constexpr int U = decltype(u_tag)::value;
-            const uint8_t *at = buf + (U == 0 ? sw0 : sw1);
+            const uint32_t at = U == 0 ? sw0 : sw1;
             u32x4v a[RT];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) a[rt] = *reinterpret_cast<const u32x4v *>(at + (w_at + 16 * rt) * 128);
+            for (int rt = 0; rt < RT; ++rt) a[rt] = *reinterpret_cast<const u32x4v *>(wbuf + at + (w_at + 16 * rt) * 128);
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt) {
-                const u32x4v b = *reinterpret_cast<const u32x4v *>(at + (x_at + 16 * tt) * 128);
+                const u32x4v b = *reinterpret_cast<const u32x4v *>(xbuf + at + (x_at + 16 * tt) * 128);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) acc[rt][tt] = mx_mfma<U, U>(a[rt], b, acc[rt][tt], sw[rt], sx[tt]);
             }
@@ -346,7 +363,9 @@ struct MxTileChoice {
     float cost;  // of a whole tile's rounds: us at K = 4096
 };
 
-// 128 weight rows on four waves up to 128 tokens, 256 on eight above.
+// 128 weight rows on four waves up to 128 tokens, 256 on eight above; there the weights come two stages
+// ahead where LDS has room (8 experts of 28672 rows, 128 tokens each: 152 us on tiles of 160, 159
+// with one stage ahead; no difference where several token tiles read the same weights).
 template <bool SWIGLU>
 hipError_t run_tile(const MxTiled &p, const MxTileChoice &tile, hipStream_t stream) {
     if (tile.split) {
@@ -363,8 +382,8 @@ hipError_t run_tile(const MxTiled &p, const MxTileChoice &tile, hipStream_t stre
         case 64: return run_tiled<MxTile<4, 2, 2, 2>, SWIGLU>(p, stream);
         case 96: return run_tiled<MxTile<4, 3, 2, 2>, SWIGLU>(p, stream);
         case 128: return run_tiled<MxTile<4, 4, 2, 2>, SWIGLU>(p, stream);
-        case 160: return run_tiled<MxTile<4, 5, 4, 2>, SWIGLU>(p, stream);
-        case 192: return run_tiled<MxTile<4, 6, 4, 2>, SWIGLU>(p, stream);
+        case 160: return run_tiled<MxTile<4, 5, 4, 2, 1, 3>, SWIGLU>(p, stream);
+        case 192: return run_tiled<MxTile<4, 6, 4, 2, 1, 3>, SWIGLU>(p, stream);
         case 256: return run_tiled<MxTile<4, 8, 4, 2>, SWIGLU>(p, stream);
     }
     return hipErrorInvalidValue;
@@ -390,7 +409,7 @@ bool tiles_accept(int K, const MxGroups &g) {
 // against 34).  Otherwise the tile whose rounds over the CUs cost least; kCost is a round's time in
 // us at K = 4096 with each CU's share of workgroups in flight (14336 x 4096: tiles of 96 take 22 us
 // for 384 tokens, 128 26 for 512, 160 31 for 640, 192 34 for 768, 256 41 for 1024, and each of the
-// others there is slower; 8 experts of 28672 rows with 128 tokens each: 160 158 us, 192 165, 128 193).
+// others there is slower; 8 experts of 28672 rows with 128 tokens each: 160 152 us, 192 163, 128 191).
 MxTileChoice tile_for(int K, int64_t N, int M, const MxGroups &g, int64_t cus) {
     const int64_t experts = mx_experts(M, g), rows = mx_rows(M, g);
     const int64_t mean = (M + experts - 1) / experts;
