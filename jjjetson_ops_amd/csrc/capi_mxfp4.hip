@@ -27,7 +27,7 @@ int check_rows(const char *who, const void *x, int dtype, int64_t row_stride, co
     if (mxfp4_bytes(rows, cols) < 0)
         return set_error(JJO_ERR_INVALID_ARG, "%s: rows=%lld must be positive and cols=%lld a positive multiple of %d",
                          who, (long long)rows, (long long)cols, kQK);
-    if (rows > (1LL << 41) / cols)  // a grid of 2^32 threads
+    if (rows * (cols / 8) > kMxMaxGroups)
         return set_error(JJO_ERR_INVALID_ARG, "%s: %lld x %lld exceeds one launch", who, (long long)rows, (long long)cols);
     if (!aligned(x, 16) || !aligned(q, 16))
         return set_error(JJO_ERR_INVALID_ARG, "%s: 16-byte aligned buffers required", who);

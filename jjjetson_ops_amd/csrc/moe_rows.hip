@@ -426,6 +426,7 @@ hipError_t launch_mxfp4_route(const void *x, int dtype, const float *logits, int
                               int32_t *dst_of_route, void *xq, hipStream_t stream) {
     const int R = T * top_k;
     const int64_t n8 = (int64_t)T * (H / 8);
+    if (n8 > kMxMaxGroups) return hipErrorInvalidConfiguration;
     return mx_by_dtype(dtype, [&](auto tag) {
         using X = typename decltype(tag)::type;
         if (R <= kRouteOne) {

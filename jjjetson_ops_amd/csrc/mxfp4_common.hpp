@@ -124,6 +124,9 @@ __device__ __forceinline__ void mx_quantize8(const T *p, int64_t i, int64_t n8, 
     if ((threadIdx.x & 3) == 0) out[4 * n8 + (i >> 2)] = (uint8_t)s;
 }
 
+// Groups of eight values of one quantizer launch, a thread each: a grid has fewer than 2^32 threads.
+constexpr int64_t kMxMaxGroups = (1LL << 32) - (1 << 20);
+
 // ---- launchers (asynchronous on `stream`; arguments validated by the C ABI)
 hipError_t launch_quantize_mxfp4(const void *x, int dtype, int64_t row_stride, void *out, int64_t rows, int64_t cols,
                                  hipStream_t stream);

@@ -62,6 +62,7 @@ __global__ __launch_bounds__(256) void dequantize_mxfp4_kernel(const uint8_t *__
 hipError_t launch_quantize_mxfp4(const void *x, int dtype, int64_t row_stride, void *out, int64_t rows, int64_t cols,
                                  hipStream_t stream) {
     const int64_t n8 = rows * (cols / 8);
+    if (n8 > kMxMaxGroups) return hipErrorInvalidConfiguration;
     const dim3 grid((unsigned)((n8 + 255) / 256));
     return mx_by_dtype(dtype, [&](auto tag) {
         using T = typename decltype(tag)::type;
@@ -78,6 +79,7 @@ hipError_t launch_quantize_mxfp4(const void *x, int dtype, int64_t row_stride, v
 hipError_t launch_dequantize_mxfp4(const void *q, void *y, int dtype, int64_t row_stride, int64_t rows, int64_t cols,
                                    hipStream_t stream) {
     const int64_t n8 = rows * (cols / 8);
+    if (n8 > kMxMaxGroups) return hipErrorInvalidConfiguration;
     const dim3 grid((unsigned)((n8 + 255) / 256));
     return mx_by_dtype(dtype, [&](auto tag) {
         using T = typename decltype(tag)::type;

@@ -42,6 +42,8 @@ def _calls():
         "q null": lambda: q(None, None, f32, 32, A, 1, 32),
         "q dtype": lambda: q(None, A, bad, 32, A, 1, 32),
         "q cols": lambda: q(None, A, f32, 48, A, 1, 48),
+        "q one launch": lambda: q(None, A, f32, 1 << 15, A, 1 << 20, 1 << 15),
+        "dq one launch": lambda: d(None, A, A, f32, 1 << 15, 1 << 20, 1 << 15),
         "q rows": lambda: q(None, A, f32, 32, A, 0, 32),
         "q aligned": lambda: q(None, A8, f32, 32, A, 1, 32),
         "q stride below": lambda: q(None, A, f32, 28, A, 2, 32),
