@@ -72,14 +72,6 @@ int check_routes(const char *who, int dtype, int T, int H, int E, int top_k) {
     return JJO_OK;
 }
 
-// Every chunk of the sort counts all routes: quadratic in their number.
-int check_sort(const char *who, int T, int top_k) {
-    if ((int64_t)T * top_k > 1 << 24)
-        return set_error(JJO_ERR_INVALID_ARG, "%s: num_tokens=%d * top_k=%d: at most 2^24 routes are sorted", who, T,
-                         top_k);
-    return JJO_OK;
-}
-
 struct MxFfnWs {
     float *route_w;
     int32_t *ids, *offsets, *src_route, *dst_of_route;
@@ -112,8 +104,8 @@ MxFfnWs ffn_layout(uint8_t *base, int T, int H, int I, int E, int top_k) {
 }
 
 int check_ffn(int T, int H, int I, int E, int top_k) {
-    int rc = check_routes("moe_mxfp4_ffn", JJO_DTYPE_F32, T, H, E, top_k);
-    if (rc != JJO_OK || (rc = check_sort("moe_mxfp4_ffn", T, top_k)) != JJO_OK) return rc;
+    const int rc = check_routes("moe_mxfp4_ffn", JJO_DTYPE_F32, T, H, E, top_k);
+    if (rc != JJO_OK) return rc;
     if (H % kQK != 0 || I <= 0 || I % kQK != 0 || I > 1 << 28 || top_k > E)
         return set_error(JJO_ERR_INVALID_ARG, "moe_mxfp4_ffn: hidden_size=%d and intermediate_size=%d must be positive "
                          "multiples of %d, top_k=%d at most num_experts=%d", H, I, kQK, top_k, E);
@@ -267,7 +259,7 @@ int moe_dispatch_rows_device(void *stream, const int32_t *expert_ids, const void
                              int32_t *src_route, int32_t *dst_of_route, void *x_sorted) {
     clear_error();
     int rc = check_routes("moe_dispatch_rows", dtype, num_tokens, hidden_size, num_experts, top_k);
-    if (rc != JJO_OK || (rc = check_sort("moe_dispatch_rows", num_tokens, top_k)) != JJO_OK) return rc;
+    if (rc != JJO_OK) return rc;
     if (expert_ids == nullptr || x == nullptr || expert_offsets == nullptr || src_route == nullptr ||
         dst_of_route == nullptr || x_sorted == nullptr)
         return set_error(JJO_ERR_INVALID_ARG, "moe_dispatch_rows: null pointer argument");

@@ -132,13 +132,43 @@ __global__ __launch_bounds__(256) void dispatch_rows_kernel(const int32_t *__res
     }
 }
 
-// ---- sort of any number of routes.  Workgroup c places the routes of chunk c, whose ids it keeps
+// ---- sort of up to kSortOne routes in one launch.  Workgroup c places the routes of chunk c, whose ids it keeps
 // in registers; it counts the experts of every other chunk itself (those before its own apart
 // from those behind), so there is no scratch and no second launch.  A wave's 64 ids are
 // counted by one ballot per bit of the id and one LDS add per distinct id.  Bound by latency: ids
 // are asked for four loads at a time (800 routes of 64 experts: 5.0 us, 9.0 with a load at a time and the own chunk
 // read three times).
 constexpr int kChunk = 1024, kOwn = kChunk / 256;
+constexpr int kSortOne = 4096;
+
+// Lanes of the wave with the same live id as this one, of `bits` bits.
+__device__ __forceinline__ uint64_t same_id(int e, int n_experts, int bits) {
+    uint64_t grp = __ballot(live_id(e, n_experts));
+    for (int b = 0; b < bits; ++b) {
+        const uint64_t one = __ballot((e >> b) & 1);
+        grp &= (e >> b) & 1 ? one : ~one;
+    }
+    return grp;
+}
+
+__device__ __forceinline__ void count_ids(int e, int n_experts, uint64_t grp, int *to) {
+    const int lane = threadIdx.x & 63;
+    if (live_id(e, n_experts) && lane == 63 - __builtin_clzll(grp)) atomicAdd(&to[e], __builtin_popcountll(grp));
+}
+
+// Route r (up to `end`) to its position, `next` of its wave and expert and the lanes before it.
+__device__ __forceinline__ void place_id(int e, int n_experts, uint64_t grp, int r, int end, int *next,
+                                         int32_t *__restrict__ src_route, int32_t *__restrict__ dst_of_route) {
+    const int lane = threadIdx.x & 63;
+    const bool live = live_id(e, n_experts);
+    int pos = -1;
+    if (live) {
+        pos = next[e] + __builtin_popcountll(grp & ((1ull << lane) - 1ull));
+        src_route[pos] = r;
+    }
+    if (r < end) dst_of_route[r] = pos;
+    if (live && lane == 63 - __builtin_clzll(grp)) next[e] = pos + 1;  // after every lane's read: one wave
+}
 
 __device__ __forceinline__ void sort_chunk(int chunk, const int32_t *__restrict__ ids, int R, int n_experts,
                                            int32_t *__restrict__ offsets, int32_t *__restrict__ src_route,
@@ -156,18 +186,6 @@ __device__ __forceinline__ void sort_chunk(int chunk, const int32_t *__restrict_
             e[i] = r < R ? ids[r] : -1;
         }
     };
-    // lanes of the wave with the same live id as this one
-    auto same = [&](int e) {
-        uint64_t grp = __ballot(live_id(e, n_experts));
-        for (int b = 0; b < bits; ++b) {
-            const uint64_t one = __ballot((e >> b) & 1);
-            grp &= (e >> b) & 1 ? one : ~one;
-        }
-        return grp;
-    };
-    auto count = [&](int e, uint64_t grp, int *to) {
-        if (live_id(e, n_experts) && lane == 63 - __builtin_clzll(grp)) atomicAdd(&to[e], __builtin_popcountll(grp));
-    };
     int own[kOwn], *const mine = s_wave[wave];
     const int w0 = chunk * kChunk + 256 * wave;
     load(w0, own);
@@ -180,15 +198,15 @@ __device__ __forceinline__ void sort_chunk(int chunk, const int32_t *__restrict_
     uint64_t grp[kOwn];
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-        grp[i] = same(own[i]);
-        count(own[i], grp[i], mine);
+        grp[i] = same_id(own[i], n_experts, bits);
+        count_ids(own[i], n_experts, grp[i], mine);
     }
     for (int r0 = 256 * wave; r0 < R; r0 += kChunk) {
         if (r0 == w0) continue;
         int e[kOwn];
         load(r0, e);
 #pragma unroll
-        for (int i = 0; i < kOwn; ++i) count(e[i], same(e[i]), s_other[r0 > w0]);
+        for (int i = 0; i < kOwn; ++i) count_ids(e[i], n_experts, same_id(e[i], n_experts, bits), s_other[r0 > w0]);
     }
     __syncthreads();
     for (int e = tid; e < 1024; e += 256) {
@@ -218,23 +236,137 @@ __device__ __forceinline__ void sort_chunk(int chunk, const int32_t *__restrict_
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-        const int r = w0 + 64 * i + lane, e = own[i];
-        const bool live = live_id(e, n_experts);
-        int pos = -1;
-        if (live) {
-            pos = mine[e] + __builtin_popcountll(grp[i] & ((1ull << lane) - 1ull));
-            src_route[pos] = r;
+    for (int i = 0; i < kOwn; ++i)
+        place_id(own[i], n_experts, grp[i], w0 + 64 * i + lane, R, mine, src_route, dst_of_route);
+}
+
+// ---- sort of many routes, in three launches, linear in their number.  dst_of_route is the scratch: a
+// chunk's part of it (at least kChunk entries, as many as there can be experts; the last chunk is up
+// to twice as long) holds the chunk's counts, then its first positions, then its results.
+
+__global__ __launch_bounds__(256) void sort_count_kernel(const int32_t *__restrict__ ids, int R, int n_experts,
+                                                         int chunks, int32_t *__restrict__ dst_of_route) {
+    __shared__ int s_cnt[1024];
+    for (int e = threadIdx.x; e < n_experts; e += 256) s_cnt[e] = 0;
+    __syncthreads();
+    const int beg = blockIdx.x * kChunk, end = (int)blockIdx.x == chunks - 1 ? R : beg + kChunk;
+    for (int r0 = beg; r0 < end; r0 += 1024) {
+        int e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = r0 + 256 * i + threadIdx.x;
+            e[i] = r < end ? ids[r] : -1;
         }
-        if (r < R) dst_of_route[r] = pos;
-        if (live && lane == 63 - __builtin_clzll(grp[i])) mine[e] = pos + 1;  // after every lane's read: one wave
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (live_id(e[i], n_experts)) atomicAdd(&s_cnt[e[i]], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < n_experts; e += 256) dst_of_route[beg + e] = s_cnt[e];
+}
+
+// One workgroup: counts to first positions.  Thread (g, e) has expert e in the g-th part of the chunks;
+// eight loads in flight.
+__global__ __launch_bounds__(1024) void sort_scan_kernel(int n_experts, int wide, int chunks,
+                                                         int32_t *__restrict__ dst_of_route,
+                                                         int32_t *__restrict__ offsets) {
+    constexpr int kAhead = 8;
+    __shared__ int s_sum[1024], s_base[1024], s_part[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int e = tid % wide, g = tid / wide, groups = 1024 / wide;  // wide: n_experts up to a power of two, at least 16
+    const int beg = (int)((int64_t)chunks * g / groups);
+    const int end = e < n_experts ? (int)((int64_t)chunks * (g + 1) / groups) : beg;
+    int32_t *const at = dst_of_route + e;
+    int sum = 0;
+    for (int i = beg; i < end; i += kAhead) {
+        int v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) v[k] = i + k < end ? at[(size_t)(i + k) * kChunk] : 0;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) sum += v[k];
+    }
+    s_sum[tid] = sum;
+    __syncthreads();
+    int before = 0, total = 0;  // of expert e: in the groups before this one, in all
+    for (int k = 0; k < groups; ++k) {
+        const int v = s_sum[k * wide + e];
+        if (k < g) before += v;
+        total += v;
+    }
+    // exclusive sum of the totals over the experts: the first `wide` threads
+    int incl = tid < wide ? total : 0;
+    const int mine = incl;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(incl, d);
+        if (lane >= d) incl += o;
+    }
+    if (lane == 63) s_part[wave] = incl;
+    __syncthreads();
+    int base = incl - mine;
+    for (int w = 0; w < wave; ++w) base += s_part[w];
+    if (tid < wide) s_base[tid] = base;
+    if (tid < n_experts) offsets[tid] = base;
+    if (tid == n_experts - 1) offsets[n_experts] = base + mine;
+    __syncthreads();
+    int pos = s_base[e] + before;
+    for (int i = beg; i < end; i += kAhead) {
+        int v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) v[k] = i + k < end ? at[(size_t)(i + k) * kChunk] : 0;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            if (i + k < end) at[(size_t)(i + k) * kChunk] = pos;
+            pos += v[k];
+        }
     }
 }
 
-__global__ __launch_bounds__(256) void moe_sort_kernel(const int32_t *__restrict__ ids, int R, int n_experts,
-                                                       int32_t *__restrict__ offsets, int32_t *__restrict__ src_route,
-                                                       int32_t *__restrict__ dst_of_route) {
-    sort_chunk(blockIdx.x, ids, R, n_experts, offsets, src_route, dst_of_route);
+__global__ __launch_bounds__(256) void sort_place_kernel(const int32_t *__restrict__ ids, int R, int n_experts,
+                                                         int chunks, int32_t *__restrict__ src_route,
+                                                         int32_t *__restrict__ dst_of_route) {
+    __shared__ int s_base[1024];
+    __shared__ int s_wave[4][1024];  // 1024 routes' counts per wave, then each wave's next position
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int bits = 32 - __builtin_clz(n_experts);
+    const int beg = blockIdx.x * kChunk, end = (int)blockIdx.x == chunks - 1 ? R : beg + kChunk;
+    for (int e = tid; e < n_experts; e += 256) s_base[e] = dst_of_route[beg + e];
+    for (int r0 = beg; r0 < end; r0 += kChunk) {
+        for (int e = tid; e < n_experts; e += 256) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) s_wave[w][e] = 0;
+        }
+        int own[kOwn], *const mine = s_wave[wave];
+        uint64_t grp[kOwn];
+        const int w0 = r0 + 256 * wave;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            const int r = w0 + 64 * i + lane;
+            own[i] = r < end ? ids[r] : -1;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            grp[i] = same_id(own[i], n_experts, bits);
+            count_ids(own[i], n_experts, grp[i], mine);
+        }
+        __syncthreads();
+        for (int e = tid; e < n_experts; e += 256) {
+            int base = s_base[e];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int n = s_wave[w][e];
+                s_wave[w][e] = base;
+                base += n;
+            }
+            s_base[e] = base;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            place_id(own[i], n_experts, grp[i], w0 + 64 * i + lane, end, mine, src_route, dst_of_route);
+        __syncthreads();  // the counts are cleared
+    }
 }
 
 // The sort and the quantizer of x (n8 groups of eight values) in one launch: neither needs the other.
@@ -298,13 +430,24 @@ __global__ __launch_bounds__(1024) void route_quantize_kernel(const float *__res
     }
 }
 
+// Threads of a workgroup that share a row of `pieces`: up to a power of two, so that short rows
+// leave none idle (32768 tokens of 64 values, 8 routes each: the combine 9.0 us, 35.7 with a workgroup a row).
+inline int log2_threads(int pieces) {
+    int n = 0;
+    while (n < 8 && (1 << n) < pieces) ++n;
+    return n;
+}
+
 // rows[dst(t, k)] = x[t], a thread per piece of a token's row.
-template <class U>
+template <class U, bool PACKED>
 __global__ __launch_bounds__(256) void scatter_rows_kernel(const U *__restrict__ x,
-                                                           const int32_t *__restrict__ dst_of_route, int R, int top_k,
-                                                           int units, U *__restrict__ rows) {
-    const int t = blockIdx.x, u = blockIdx.y * 256 + threadIdx.x;
-    if (u >= units) return;
+                                                           const int32_t *__restrict__ dst_of_route, int T, int top_k,
+                                                           int units, int log2_row, U *__restrict__ rows) {
+    const int R = T * top_k;
+    // A row a workgroup (the usual case): t is a scalar, and so are the rows' addresses.
+    const int t = PACKED ? (blockIdx.x * 256 + threadIdx.x) >> log2_row : blockIdx.x;
+    const int u = PACKED ? threadIdx.x & ((1 << log2_row) - 1) : blockIdx.y * 256 + threadIdx.x;
+    if (t >= T || u >= units) return;
     const U v = x[(size_t)t * units + u];
     for (int k = 0; k < top_k; ++k) {
         const int pos = dst_of_route[t * top_k + k];
@@ -313,13 +456,14 @@ __global__ __launch_bounds__(256) void scatter_rows_kernel(const U *__restrict__
 }
 
 // ---- sums over a token's routes (combine; the dispatch's gradient without weights)
-template <class TI, class TO, int VEC, bool WEIGHTED, int SLICES>
+template <class TI, class TO, int VEC, bool WEIGHTED, int SLICES, bool PACKED>
 __global__ __launch_bounds__(256) void join_rows_kernel(const TI *__restrict__ rows,
                                                         const int32_t *__restrict__ dst_of_route,
-                                                        const float *__restrict__ weights, int R, int top_k, int H,
-                                                        TO *__restrict__ y) {
-    const int t = blockIdx.x, h = (blockIdx.y * 256 + threadIdx.x) * VEC;
-    if (h >= H) return;
+                                                        const float *__restrict__ weights, int T, int top_k, int H,
+                                                        int log2_row, TO *__restrict__ y) {
+    const int t = PACKED ? (blockIdx.x * 256 + threadIdx.x) >> log2_row : blockIdx.x, R = T * top_k;
+    const int h = (PACKED ? threadIdx.x & ((1 << log2_row) - 1) : blockIdx.y * 256 + threadIdx.x) * VEC;
+    if (t >= T || h >= H) return;
     float acc[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
@@ -407,8 +551,14 @@ hipError_t run_dispatch(const int32_t *ids, const void *x, int T, int top_k, siz
     }
     const hipError_t e = launch_moe_sort(ids, R, E, offsets, src_route, dst_of_route, stream);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(scatter_rows_kernel<U>, dim3((unsigned)T, (unsigned)((units + 255) / 256)), dim3(256), 0, stream,
-                       (const U *)x, dst_of_route, R, top_k, units, (U *)rows);
+    const int log2_row = log2_threads(units), tokens = 256 >> log2_row;
+    const dim3 grid((unsigned)((T + tokens - 1) / tokens), (unsigned)((units + 255) / 256));
+    if (log2_row == 8)
+        hipLaunchKernelGGL((scatter_rows_kernel<U, false>), grid, dim3(256), 0, stream, (const U *)x, dst_of_route, T,
+                           top_k, units, log2_row, (U *)rows);
+    else
+        hipLaunchKernelGGL((scatter_rows_kernel<U, true>), grid, dim3(256), 0, stream, (const U *)x, dst_of_route, T,
+                           top_k, units, log2_row, (U *)rows);
     return hipGetLastError();
 }
 
@@ -416,8 +566,15 @@ hipError_t run_dispatch(const int32_t *ids, const void *x, int T, int top_k, siz
 
 hipError_t launch_moe_sort(const int32_t *ids, int n_routes, int n_experts, int32_t *offsets, int32_t *src_route,
                            int32_t *dst_of_route, hipStream_t stream) {
-    hipLaunchKernelGGL(moe_sort_kernel, dim3((unsigned)((n_routes + kChunk - 1) / kChunk)), dim3(256), 0, stream, ids,
-                       n_routes, n_experts, offsets, src_route, dst_of_route);
+    const int chunks = n_routes / kChunk;
+    int wide = 16;
+    while (wide < n_experts) wide *= 2;
+    hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)chunks), dim3(256), 0, stream, ids, n_routes, n_experts,
+                       chunks, dst_of_route);
+    hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, stream, n_experts, wide, chunks, dst_of_route,
+                       offsets);
+    hipLaunchKernelGGL(sort_place_kernel, dim3((unsigned)chunks), dim3(256), 0, stream, ids, n_routes, n_experts,
+                       chunks, src_route, dst_of_route);
     return hipGetLastError();
 }
 
@@ -443,6 +600,10 @@ hipError_t launch_mxfp4_route(const void *x, int dtype, const float *logits, int
         }
         const hipError_t e = launch_moe_top_k(logits, route_w, ids, T, E, top_k, stream);
         if (e != hipSuccess) return e;
+        if (R > kSortOne) {
+            const hipError_t q = launch_quantize_mxfp4(x, dtype, H, xq, T, H, stream);
+            return q != hipSuccess ? q : launch_moe_sort(ids, R, E, offsets, src_route, dst_of_route, stream);
+        }
         const int chunks = (R + kChunk - 1) / kChunk;
         hipLaunchKernelGGL(sort_quantize_kernel<X>, dim3((unsigned)(chunks + (n8 + 255) / 256)), dim3(256), 0, stream,
                            ids, R, E, offsets, src_route, dst_of_route, chunks, (const X *)x, n8, (uint8_t *)xq);
@@ -462,25 +623,30 @@ hipError_t launch_moe_dispatch_rows(const int32_t *ids, const void *x, int elem_
 }
 
 namespace {
-template <class TI, class TO, int VEC>
+template <class TI, class TO, int VEC, bool PACKED>
 hipError_t run_join(const void *rows, const int32_t *dst, const float *weights, void *y, int T, int H, int top_k,
                     hipStream_t stream, int slices) {
-    const dim3 grid((unsigned)T, (unsigned)((H / VEC + 255) / 256));
+    const int log2_row = log2_threads(H / VEC), tokens = 256 >> log2_row;
+    const dim3 grid((unsigned)((T + tokens - 1) / tokens), (unsigned)((H / VEC + 255) / 256));
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, (const TI *)rows, dst, weights, T, top_k, H, log2_row,
+                           (TO *)y);
+        return hipGetLastError();
+    };
     if (slices == 2) {
-        if constexpr (sizeof(TI) == 4 && VEC == 4) {  // the FFN's: H % 32 == 0
-            hipLaunchKernelGGL((join_rows_kernel<TI, TO, VEC, true, 2>), grid, dim3(256), 0, stream, (const TI *)rows,
-                               dst, weights, T * top_k, top_k, H, (TO *)y);
-            return hipGetLastError();
-        }
+        if constexpr (sizeof(TI) == 4 && VEC == 4)  // the FFN's: H % 32 == 0
+            return go(join_rows_kernel<TI, TO, VEC, true, 2, PACKED>);
         return hipErrorInvalidValue;
     }
-    if (weights != nullptr)
-        hipLaunchKernelGGL((join_rows_kernel<TI, TO, VEC, true, 1>), grid, dim3(256), 0, stream, (const TI *)rows, dst,
-                           weights, T * top_k, top_k, H, (TO *)y);
-    else
-        hipLaunchKernelGGL((join_rows_kernel<TI, TO, VEC, false, 1>), grid, dim3(256), 0, stream, (const TI *)rows, dst,
-                           weights, T * top_k, top_k, H, (TO *)y);
-    return hipGetLastError();
+    return weights != nullptr ? go(join_rows_kernel<TI, TO, VEC, true, 1, PACKED>)
+                              : go(join_rows_kernel<TI, TO, VEC, false, 1, PACKED>);
+}
+
+template <class TI, class TO, int VEC>
+hipError_t run_join_rows(const void *rows, const int32_t *dst, const float *weights, void *y, int T, int H, int top_k,
+                         hipStream_t stream, int slices) {
+    return H / VEC > 128 ? run_join<TI, TO, VEC, false>(rows, dst, weights, y, T, H, top_k, stream, slices)
+                         : run_join<TI, TO, VEC, true>(rows, dst, weights, y, T, H, top_k, stream, slices);
 }
 
 template <class TI, class TO>
@@ -488,10 +654,10 @@ hipError_t run_join_types(const void *rows, const int32_t *dst, const float *wei
                           hipStream_t stream, int slices) {
     constexpr int kWide = 16 / sizeof(TI);
     if (H % kWide == 0 && aligned_to(rows, y, 16))
-        return run_join<TI, TO, kWide>(rows, dst, weights, y, T, H, top_k, stream, slices);
+        return run_join_rows<TI, TO, kWide>(rows, dst, weights, y, T, H, top_k, stream, slices);
     if (sizeof(TI) == 2 && H % 2 == 0 && aligned_to(rows, y, 4))
-        return run_join<TI, TO, 2>(rows, dst, weights, y, T, H, top_k, stream, slices);
-    return run_join<TI, TO, 1>(rows, dst, weights, y, T, H, top_k, stream, slices);
+        return run_join_rows<TI, TO, 2>(rows, dst, weights, y, T, H, top_k, stream, slices);
+    return run_join_rows<TI, TO, 1>(rows, dst, weights, y, T, H, top_k, stream, slices);
 }
 }  // namespace
 

@@ -74,8 +74,6 @@ def _calls():
         "dispatch top_k": lambda: dis(None, A, A, f32, 4, 33, 32, 64, A, A, A, A),
         "dispatch experts": lambda: dis(None, A, A, f32, 4, 2, 32, 1025, A, A, A, A),
         "dispatch tokens": lambda: dis(None, A, A, f32, 0, 2, 32, 8, A, A, A, A),
-        "dispatch sorted routes": lambda: dis(None, A, A, f32, (1 << 19) + 1, 32, 32, 64, A, A, A, A),
-        "ffn sorted routes": lambda: ffn(None, A, A, A, A, A, A, f32, (1 << 19) + 1, 32, 32, 64, 32, W, 1 << 40),
         "dispatch routes": lambda: dis(None, A, A, f32, 1 << 23, 32, 32, 64, A, A, A, A),
         "dispatch_backward": lambda: disb(None, A, f32, A, None, 4, 32, 2),
         "combine hidden": lambda: com(None, A, f32, A, A, A, 4, 0, 2),
