@@ -53,17 +53,33 @@ __device__ __forceinline__ void expert_bases(int *s_cnt, int *s_part) {
     __syncthreads();
 }
 
+// A row of any length in pieces of 16 bytes, whatever its alignment (a load or store of a wave then
+// touches a line more): the last piece ends with the row and overlaps the one before, which is
+// the same values once more.  Rows shorter than a piece go by single elements.  8192 tokens top-2 of
+// 4095 bf16 values: the combine ODD us, 71 by single elements (30 for 4096).
+template <class V>
+__device__ __forceinline__ V load_any(const void *p) {
+    V v;
+    __builtin_memcpy(&v, p, sizeof(V));
+    return v;
+}
+template <class V>
+__device__ __forceinline__ void store_any(void *p, const V &v) {
+    __builtin_memcpy(p, &v, sizeof(V));
+}
+
 // ---- dispatch of up to kSortMax routes in one launch.  Workgroup (t + 1, c) has its piece of
 // token t's row in flight, counts for each of the token's routes the routes that sort before
 // it (16 compares a thread and route at most) and stores the piece at each position;
 // workgroup 0 counts the experts' offsets.
 template <class U>
-__global__ __launch_bounds__(256) void dispatch_rows_kernel(const int32_t *__restrict__ ids, const U *__restrict__ x,
-                                                            int R, int top_k, int units, int n_experts,
-                                                            int32_t *__restrict__ offsets,
+__global__ __launch_bounds__(256) void dispatch_rows_kernel(const int32_t *__restrict__ ids,
+                                                            const uint16_t *__restrict__ x, int R, int top_k,
+                                                            int row_len, int n_experts, int32_t *__restrict__ offsets,
                                                             int32_t *__restrict__ src_route,
-                                                            int32_t *__restrict__ dst_of_route, U *__restrict__ rows) {
-    constexpr int kIds = kSortMax / 256, kUnits = 4;
+                                                            int32_t *__restrict__ dst_of_route,
+                                                            uint16_t *__restrict__ rows) {
+    constexpr int kIds = kSortMax / 256, kUnits = 4, kLen = sizeof(U) / 2;  // row_len: in 2-byte units
     __shared__ int s_cnt[1024];
     __shared__ int s_part[4][32];
     __shared__ int s_pos[32];
@@ -84,12 +100,12 @@ __global__ __launch_bounds__(256) void dispatch_rows_kernel(const int32_t *__res
         return;
     }
     const int t = blockIdx.x - 1, u0 = blockIdx.y * (256 * kUnits);
-    const U *row = x + (size_t)t * units;
+    const uint16_t *row = x + (size_t)t * row_len;
     U v[kUnits];
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
-        const int u = u0 + tid + 256 * i;
-        if (u < units) v[i] = row[u];
+        const int u = (u0 + tid + 256 * i) * kLen;
+        if (u < row_len) v[i] = load_any<U>(row + min(u, row_len - kLen));
     }
     int key[kIds];  // expert * kSortMax + route; a dropped route sorts behind all
 #pragma unroll
@@ -123,11 +139,11 @@ __global__ __launch_bounds__(256) void dispatch_rows_kernel(const int32_t *__res
     for (int k = 0; k < top_k; ++k) {
         const int pos = s_pos[k];
         if (pos < 0) continue;
-        U *out = rows + (size_t)pos * units;
+        uint16_t *out = rows + (size_t)pos * row_len;
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
-            const int u = u0 + tid + 256 * i;
-            if (u < units) out[u] = v[i];
+            const int u = (u0 + tid + 256 * i) * kLen;
+            if (u < row_len) store_any(out + min(u, row_len - kLen), v[i]);
         }
     }
 }
@@ -440,18 +456,20 @@ inline int log2_threads(int pieces) {
 
 // rows[dst(t, k)] = x[t], a thread per piece of a token's row.
 template <class U, bool PACKED>
-__global__ __launch_bounds__(256) void scatter_rows_kernel(const U *__restrict__ x,
+__global__ __launch_bounds__(256) void scatter_rows_kernel(const uint16_t *__restrict__ x,
                                                            const int32_t *__restrict__ dst_of_route, int T, int top_k,
-                                                           int units, int log2_row, U *__restrict__ rows) {
+                                                           int row_len, int log2_row, uint16_t *__restrict__ rows) {
+    constexpr int kLen = sizeof(U) / 2;
     const int R = T * top_k;
     // A row a workgroup (the usual case): t is a scalar, and so are the rows' addresses.
     const int t = PACKED ? (blockIdx.x * 256 + threadIdx.x) >> log2_row : blockIdx.x;
-    const int u = PACKED ? threadIdx.x & ((1 << log2_row) - 1) : blockIdx.y * 256 + threadIdx.x;
-    if (t >= T || u >= units) return;
-    const U v = x[(size_t)t * units + u];
+    int u = (PACKED ? threadIdx.x & ((1 << log2_row) - 1) : blockIdx.y * 256 + threadIdx.x) * kLen;
+    if (t >= T || u >= row_len) return;
+    u = min(u, row_len - kLen);
+    const U v = load_any<U>(x + (size_t)t * row_len + u);
     for (int k = 0; k < top_k; ++k) {
         const int pos = dst_of_route[t * top_k + k];
-        if ((unsigned)pos < (unsigned)R) rows[(size_t)pos * units + u] = v;
+        if ((unsigned)pos < (unsigned)R) store_any(rows + (size_t)pos * row_len + u, v);
     }
 }
 
@@ -462,8 +480,9 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const TI *__restrict__ r
                                                         const float *__restrict__ weights, int T, int top_k, int H,
                                                         int log2_row, TO *__restrict__ y) {
     const int t = PACKED ? (blockIdx.x * 256 + threadIdx.x) >> log2_row : blockIdx.x, R = T * top_k;
-    const int h = (PACKED ? threadIdx.x & ((1 << log2_row) - 1) : blockIdx.y * 256 + threadIdx.x) * VEC;
+    int h = (PACKED ? threadIdx.x & ((1 << log2_row) - 1) : blockIdx.y * 256 + threadIdx.x) * VEC;
     if (t >= T || h >= H) return;
+    h = min(h, H - VEC);
     float acc[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
@@ -474,10 +493,9 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const TI *__restrict__ r
         for (int j = 0; j < 4; ++j) {
             pos[j] = k0 + j < top_k ? dst_of_route[t * top_k + k0 + j] : -1;
             if ((unsigned)pos[j] < (unsigned)R)
-                v[j] = *reinterpret_cast<const MxVec<TI, VEC> *>(rows + (size_t)pos[j] * H + h);
+                v[j] = load_any<MxVec<TI, VEC>>(rows + (size_t)pos[j] * H + h);
             if (SLICES == 2 && (unsigned)pos[j] < (unsigned)R)
-                v2[SLICES == 2 ? j : 0] =
-                    *reinterpret_cast<const MxVec<TI, VEC> *>(rows + ((size_t)R + pos[j]) * H + h);
+                v2[SLICES == 2 ? j : 0] = load_any<MxVec<TI, VEC>>(rows + ((size_t)R + pos[j]) * H + h);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -494,7 +512,7 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const TI *__restrict__ r
     MxVec<TO, VEC> o;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) o.v[i] = (TO)acc[i];
-    *reinterpret_cast<MxVec<TO, VEC> *>(y + (size_t)t * H + h) = o;
+    store_any(y + (size_t)t * H + h, o);
 }
 
 // ---- gradients of the combine: a workgroup per token, its gradient row read once per route
@@ -514,16 +532,17 @@ __global__ __launch_bounds__(256) void combine_rows_backward_kernel(
             const float w = weights[t * top_k + k];
             const T *e = rows + (size_t)pos * H;
             T *ge = grad_rows + (size_t)pos * H;
-            for (int h = threadIdx.x * VEC; h < H; h += 256 * VEC) {
-                const MxVec<T, VEC> gv = *reinterpret_cast<const MxVec<T, VEC> *>(g + h);
-                const MxVec<T, VEC> ev = *reinterpret_cast<const MxVec<T, VEC> *>(e + h);
+            for (int h0 = threadIdx.x * VEC; h0 < H; h0 += 256 * VEC) {
+                const int h = min(h0, H - VEC);
+                const MxVec<T, VEC> gv = load_any<MxVec<T, VEC>>(g + h), ev = load_any<MxVec<T, VEC>>(e + h);
                 MxVec<T, VEC> o;
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    dot = fmaf((float)gv.v[i], (float)ev.v[i], dot);
+                    // What the last piece shares with the one before is counted there.
+                    dot = fmaf(h + i >= h0 ? (float)gv.v[i] : 0.0f, h + i >= h0 ? (float)ev.v[i] : 0.0f, dot);
                     o.v[i] = (T)(w * (float)gv.v[i]);
                 }
-                *reinterpret_cast<MxVec<T, VEC> *>(ge + h) = o;
+                store_any(ge + h, o);
             }
         }
 #pragma unroll
@@ -537,16 +556,14 @@ __global__ __launch_bounds__(256) void combine_rows_backward_kernel(
     }
 }
 
-bool aligned_to(const void *a, const void *b, size_t n) { return (((uintptr_t)a | (uintptr_t)b) & (n - 1)) == 0; }
-
 template <class U>
 hipError_t run_dispatch(const int32_t *ids, const void *x, int T, int top_k, size_t row_bytes, int E, int32_t *offsets,
                         int32_t *src_route, int32_t *dst_of_route, void *rows, hipStream_t stream) {
-    const int R = T * top_k, units = (int)(row_bytes / sizeof(U));
+    const int R = T * top_k, row_len = (int)(row_bytes / 2), units = (int)((row_bytes + sizeof(U) - 1) / sizeof(U));
     if (R <= kSortMax) {
         const dim3 grid((unsigned)T + 1, (unsigned)((units + 1023) / 1024));
-        hipLaunchKernelGGL(dispatch_rows_kernel<U>, grid, dim3(256), 0, stream, ids, (const U *)x, R, top_k, units, E,
-                           offsets, src_route, dst_of_route, (U *)rows);
+        hipLaunchKernelGGL(dispatch_rows_kernel<U>, grid, dim3(256), 0, stream, ids, (const uint16_t *)x, R, top_k,
+                           row_len, E, offsets, src_route, dst_of_route, (uint16_t *)rows);
         return hipGetLastError();
     }
     const hipError_t e = launch_moe_sort(ids, R, E, offsets, src_route, dst_of_route, stream);
@@ -554,11 +571,11 @@ hipError_t run_dispatch(const int32_t *ids, const void *x, int T, int top_k, siz
     const int log2_row = log2_threads(units), tokens = 256 >> log2_row;
     const dim3 grid((unsigned)((T + tokens - 1) / tokens), (unsigned)((units + 255) / 256));
     if (log2_row == 8)
-        hipLaunchKernelGGL((scatter_rows_kernel<U, false>), grid, dim3(256), 0, stream, (const U *)x, dst_of_route, T,
-                           top_k, units, log2_row, (U *)rows);
+        hipLaunchKernelGGL((scatter_rows_kernel<U, false>), grid, dim3(256), 0, stream, (const uint16_t *)x,
+                           dst_of_route, T, top_k, row_len, log2_row, (uint16_t *)rows);
     else
-        hipLaunchKernelGGL((scatter_rows_kernel<U, true>), grid, dim3(256), 0, stream, (const U *)x, dst_of_route, T,
-                           top_k, units, log2_row, (U *)rows);
+        hipLaunchKernelGGL((scatter_rows_kernel<U, true>), grid, dim3(256), 0, stream, (const uint16_t *)x,
+                           dst_of_route, T, top_k, row_len, log2_row, (uint16_t *)rows);
     return hipGetLastError();
 }
 
@@ -615,19 +632,17 @@ hipError_t launch_moe_dispatch_rows(const int32_t *ids, const void *x, int elem_
                                     int32_t *offsets, int32_t *src_route, int32_t *dst_of_route, void *rows,
                                     hipStream_t stream) {
     const size_t bytes = (size_t)H * elem_bytes;
-    if (bytes % 16 == 0 && aligned_to(x, rows, 16))
-        return run_dispatch<uint4>(ids, x, T, top_k, bytes, E, offsets, src_route, dst_of_route, rows, stream);
-    if (bytes % 4 == 0 && aligned_to(x, rows, 4))
-        return run_dispatch<uint32_t>(ids, x, T, top_k, bytes, E, offsets, src_route, dst_of_route, rows, stream);
-    return run_dispatch<uint16_t>(ids, x, T, top_k, bytes, E, offsets, src_route, dst_of_route, rows, stream);
+    return bytes >= 16
+               ? run_dispatch<uint4>(ids, x, T, top_k, bytes, E, offsets, src_route, dst_of_route, rows, stream)
+               : run_dispatch<uint16_t>(ids, x, T, top_k, bytes, E, offsets, src_route, dst_of_route, rows, stream);
 }
 
 namespace {
 template <class TI, class TO, int VEC, bool PACKED>
 hipError_t run_join(const void *rows, const int32_t *dst, const float *weights, void *y, int T, int H, int top_k,
                     hipStream_t stream, int slices) {
-    const int log2_row = log2_threads(H / VEC), tokens = 256 >> log2_row;
-    const dim3 grid((unsigned)((T + tokens - 1) / tokens), (unsigned)((H / VEC + 255) / 256));
+    const int pieces = (H + VEC - 1) / VEC, log2_row = log2_threads(pieces), tokens = 256 >> log2_row;
+    const dim3 grid((unsigned)((T + tokens - 1) / tokens), (unsigned)((pieces + 255) / 256));
     auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, (const TI *)rows, dst, weights, T, top_k, H, log2_row,
                            (TO *)y);
@@ -645,7 +660,7 @@ hipError_t run_join(const void *rows, const int32_t *dst, const float *weights, 
 template <class TI, class TO, int VEC>
 hipError_t run_join_rows(const void *rows, const int32_t *dst, const float *weights, void *y, int T, int H, int top_k,
                          hipStream_t stream, int slices) {
-    return H / VEC > 128 ? run_join<TI, TO, VEC, false>(rows, dst, weights, y, T, H, top_k, stream, slices)
+    return H > 128 * VEC ? run_join<TI, TO, VEC, false>(rows, dst, weights, y, T, H, top_k, stream, slices)
                          : run_join<TI, TO, VEC, true>(rows, dst, weights, y, T, H, top_k, stream, slices);
 }
 
@@ -653,11 +668,8 @@ template <class TI, class TO>
 hipError_t run_join_types(const void *rows, const int32_t *dst, const float *weights, void *y, int T, int H, int top_k,
                           hipStream_t stream, int slices) {
     constexpr int kWide = 16 / sizeof(TI);
-    if (H % kWide == 0 && aligned_to(rows, y, 16))
-        return run_join_rows<TI, TO, kWide>(rows, dst, weights, y, T, H, top_k, stream, slices);
-    if (sizeof(TI) == 2 && H % 2 == 0 && aligned_to(rows, y, 4))
-        return run_join_rows<TI, TO, 2>(rows, dst, weights, y, T, H, top_k, stream, slices);
-    return run_join_rows<TI, TO, 1>(rows, dst, weights, y, T, H, top_k, stream, slices);
+    return H >= kWide ? run_join_rows<TI, TO, kWide>(rows, dst, weights, y, T, H, top_k, stream, slices)
+                      : run_join_rows<TI, TO, 1>(rows, dst, weights, y, T, H, top_k, stream, slices);
 }
 }  // namespace
 
@@ -680,8 +692,6 @@ hipError_t launch_moe_combine_rows_backward(const void *grad_y, const void *rows
     return mx_by_dtype(dtype, [&](auto tag) {
         using E = typename decltype(tag)::type;
         constexpr int kWide = 16 / sizeof(E);
-        const bool a16 = aligned_to(grad_y, rows, 16) && aligned_to(grad_rows, grad_rows, 16);
-        const bool a4 = aligned_to(grad_y, rows, 4) && aligned_to(grad_rows, grad_rows, 4);
         auto run = [&](auto vec) {
             constexpr int V = decltype(vec)::value;
             hipLaunchKernelGGL((combine_rows_backward_kernel<E, V>), dim3((unsigned)T), dim3(256), 0, stream,
@@ -689,9 +699,7 @@ hipError_t launch_moe_combine_rows_backward(const void *grad_y, const void *rows
                                (E *)grad_rows, grad_weights);
             return hipGetLastError();
         };
-        if (H % kWide == 0 && a16) return run(std::integral_constant<int, kWide>{});
-        if (sizeof(E) == 2 && H % 2 == 0 && a4) return run(std::integral_constant<int, 2>{});
-        return run(std::integral_constant<int, 1>{});
+        return H >= kWide ? run(std::integral_constant<int, kWide>{}) : run(std::integral_constant<int, 1>{});
     });
 }
 
