@@ -56,7 +56,7 @@ __device__ __forceinline__ void expert_bases(int *s_cnt, int *s_part) {
 // A row of any length in pieces of 16 bytes, whatever its alignment (a load or store of a wave then
 // touches a line more): the last piece ends with the row and overlaps the one before, which is
 // the same values once more.  Rows shorter than a piece go by single elements.  8192 tokens top-2 of
-// 4095 bf16 values: the combine ODD us, 71 by single elements (30 for 4096).
+// 4095 bf16 values: the combine 32 us, 71 by single elements (31 for 4096).
 template <class V>
 __device__ __forceinline__ V load_any(const void *p) {
     V v;
@@ -515,6 +515,23 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const TI *__restrict__ r
     store_any(y + (size_t)t * H + h, o);
 }
 
+// A piece of a route's row: its gradient stored, its part of the dot product added.
+template <class T, int VEC>
+__device__ __forceinline__ float backward_piece(const T *__restrict__ g, const T *__restrict__ e, T *__restrict__ ge,
+                                                float w, int h0, int H, float dot) {
+    const int h = min(h0, H - VEC);
+    const MxVec<T, VEC> gv = load_any<MxVec<T, VEC>>(g + h), ev = load_any<MxVec<T, VEC>>(e + h);
+    MxVec<T, VEC> o;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        // What the last piece shares with the one before is counted there.
+        dot = fmaf(h + i >= h0 ? (float)gv.v[i] : 0.0f, h + i >= h0 ? (float)ev.v[i] : 0.0f, dot);
+        o.v[i] = (T)(w * (float)gv.v[i]);
+    }
+    store_any(ge + h, o);
+    return dot;
+}
+
 // ---- gradients of the combine: a workgroup per token, its gradient row read once per route
 // from the cache, the routes' dot products reduced in a fixed order.
 template <class T, int VEC>
@@ -532,18 +549,8 @@ __global__ __launch_bounds__(256) void combine_rows_backward_kernel(
             const float w = weights[t * top_k + k];
             const T *e = rows + (size_t)pos * H;
             T *ge = grad_rows + (size_t)pos * H;
-            for (int h0 = threadIdx.x * VEC; h0 < H; h0 += 256 * VEC) {
-                const int h = min(h0, H - VEC);
-                const MxVec<T, VEC> gv = load_any<MxVec<T, VEC>>(g + h), ev = load_any<MxVec<T, VEC>>(e + h);
-                MxVec<T, VEC> o;
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    // What the last piece shares with the one before is counted there.
-                    dot = fmaf(h + i >= h0 ? (float)gv.v[i] : 0.0f, h + i >= h0 ? (float)ev.v[i] : 0.0f, dot);
-                    o.v[i] = (T)(w * (float)gv.v[i]);
-                }
-                store_any(ge + h, o);
-            }
+            for (int h0 = threadIdx.x * VEC; h0 < H; h0 += 256 * VEC)
+                dot = backward_piece<T, VEC>(g, e, ge, w, h0, H, dot);
         }
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) dot += __shfl_xor(dot, d);
@@ -554,6 +561,27 @@ __global__ __launch_bounds__(256) void combine_rows_backward_kernel(
         const float *d = s_dot[threadIdx.x];
         grad_weights[t * top_k + threadIdx.x] = (d[0] + d[1]) + (d[2] + d[3]);
     }
+}
+
+// The same for short rows: 2^log2_row lanes of a wave to a route, so that none of a workgroup's waves is idle
+// (8192 tokens top-8 of 300 bf16 values: 21 us, 32 with a workgroup a token).
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void combine_rows_backward_short_kernel(
+    const T *__restrict__ grad_y, const T *__restrict__ rows, const int32_t *__restrict__ dst_of_route,
+    const float *__restrict__ weights, int R, int top_k, int H, int log2_row, T *__restrict__ grad_rows,
+    float *__restrict__ grad_weights) {
+    const int r = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) >> log2_row);
+    const int len = 1 << log2_row, lane = threadIdx.x & (len - 1);
+    const int pos = r < R ? dst_of_route[r] : -1;
+    float dot = 0.0f;
+    if ((unsigned)pos < (unsigned)R) {
+        const float w = weights[r];
+        const T *g = grad_y + (size_t)(r / top_k) * H, *e = rows + (size_t)pos * H;
+        T *ge = grad_rows + (size_t)pos * H;
+        for (int h0 = lane * VEC; h0 < H; h0 += len * VEC) dot = backward_piece<T, VEC>(g, e, ge, w, h0, H, dot);
+    }
+    for (int d = len / 2; d > 0; d >>= 1) dot += __shfl_xor(dot, d);
+    if (r < R && lane == 0) grad_weights[r] = dot;
 }
 
 template <class U>
@@ -694,6 +722,14 @@ hipError_t launch_moe_combine_rows_backward(const void *grad_y, const void *rows
         constexpr int kWide = 16 / sizeof(E);
         auto run = [&](auto vec) {
             constexpr int V = decltype(vec)::value;
+            if (H <= 128 * V) {
+                const int log2_row = std::min(log2_threads((H + V - 1) / V), 6), routes = 256 >> log2_row;
+                hipLaunchKernelGGL((combine_rows_backward_short_kernel<E, V>),
+                                   dim3((unsigned)((T * top_k + routes - 1) / routes)), dim3(256), 0, stream,
+                                   (const E *)grad_y, (const E *)rows, dst_of_route, weights, T * top_k, top_k, H,
+                                   log2_row, (E *)grad_rows, grad_weights);
+                return hipGetLastError();
+            }
             hipLaunchKernelGGL((combine_rows_backward_kernel<E, V>), dim3((unsigned)T), dim3(256), 0, stream,
                                (const E *)grad_y, (const E *)rows, dst_of_route, weights, T * top_k, top_k, H,
                                (E *)grad_rows, grad_weights);
