@@ -54,7 +54,8 @@ struct MxTile {
 
 // A wave's outputs (from weight row n, token t on) through its own 4 KB of LDS, 16 tokens at a time:
 // the matrix instruction leaves 4 consecutive outputs of a token in a lane, 32 bytes of a row in
-// an instruction; read back a row is 16 RT outputs in whole 128-byte lines.  N % 8 == 0.
+// an instruction; read back a row is 16 RT outputs in whole 128-byte lines.  Any N: where rows are not
+// aligned the 16-byte stores are not either (2047 tokens, 14335 x 4096: 83 us, 123 by single outputs).
 template <class T, int RT, int TT>
 __device__ __forceinline__ void store_rows(T *__restrict__ y, const f32x4v (&acc)[RT][TT], uint8_t *stage, int n,
                                            int t, int end, int N, const int32_t *__restrict__ route_dst) {
@@ -76,11 +77,18 @@ __device__ __forceinline__ void store_rows(T *__restrict__ y, const f32x4v (&acc
 #pragma unroll
         for (int k = 0; k < 16 / kRowsAtOnce; ++k) {
             const int r = kRowsAtOnce * k + row, token = t + 16 * tt + r;
-            const u32x4v v =
-                *reinterpret_cast<const u32x4v *>(stage + r * (kChunks * 16) + 16 * (chunk ^ (r % kChunks)));
-            if (token < end && n + chunk * kVec < N) {
-                const size_t to = route_dst != nullptr ? route_dst[token] : token;
-                *reinterpret_cast<u32x4v *>(y + to * N + n + chunk * kVec) = v;
+            const MxVec<T, kVec> v =
+                *reinterpret_cast<const MxVec<T, kVec> *>(stage + r * (kChunks * 16) + 16 * (chunk ^ (r % kChunks)));
+            const int at = n + chunk * kVec;
+            if (token < end && at < N) {
+                T *const to = y + (size_t)(route_dst != nullptr ? route_dst[token] : token) * N + at;
+                if (at + kVec <= N) {
+                    store_any(to, v);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kVec - 1; ++i)
+                        if (at + i < N) to[i] = v.v[i];
+                }
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -310,31 +318,16 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
             mx_swiglu_store(gate, up, codes + row * (p.N / 2) + n / 2, scales + row * (p.N / kQK) + n / kQK, t < end);
         }
     } else {
-        if (p.N % 8 == 0) {
-            if constexpr (KG == 1) __syncthreads();  // no wave reads a stage any more
-            uint8_t *stage = lds + wave * 4096;
-            const int nw = n0 + 16 * RT * wn, tw = first + 16 * TT * wt;
-            const int32_t *route_dst = GROUPED ? p.g.route_dst : nullptr;
-            if (p.dtype == JJO_DTYPE_F32)
-                store_rows<float, RT, TT>((float *)p.y + (size_t)blockIdx.y * p.M * p.N, acc, stage, nw, tw, end, p.N,
-                                          route_dst);
-            else if (p.dtype == JJO_DTYPE_F16)
-                store_rows<_Float16, RT, TT>((_Float16 *)p.y, acc, stage, nw, tw, end, p.N, route_dst);
-            else store_rows<__bf16, RT, TT>((__bf16 *)p.y, acc, stage, nw, tw, end, p.N, route_dst);
-            return;
-        }
-        const bool vec = p.N % 4 == 0;  // y is 16-byte aligned
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-            const int t = first + 16 * (TT * wt + tt) + r16;
-            if (t >= end) continue;
-            const size_t row = GROUPED && p.g.route_dst != nullptr ? p.g.route_dst[t] : t;
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const int n = n0 + 16 * (RT * wn + rt) + 4 * q;
-                if (n < p.N) mx_store4(p.y, p.dtype, row * p.N + n, acc[rt][tt], p.N - n, vec);
-            }
-        }
+        if constexpr (KG == 1) __syncthreads();  // no wave reads a stage any more
+        uint8_t *stage = lds + wave * 4096;
+        const int nw = n0 + 16 * RT * wn, tw = first + 16 * TT * wt;
+        const int32_t *route_dst = GROUPED ? p.g.route_dst : nullptr;
+        if (p.dtype == JJO_DTYPE_F32)
+            store_rows<float, RT, TT>((float *)p.y + (size_t)blockIdx.y * p.M * p.N, acc, stage, nw, tw, end, p.N,
+                                      route_dst);
+        else if (p.dtype == JJO_DTYPE_F16)
+            store_rows<_Float16, RT, TT>((_Float16 *)p.y, acc, stage, nw, tw, end, p.N, route_dst);
+        else store_rows<__bf16, RT, TT>((__bf16 *)p.y, acc, stage, nw, tw, end, p.N, route_dst);
     }
 }
 
@@ -438,7 +431,7 @@ MxTileChoice tile_for(int K, int64_t N, int M, const MxGroups &g, int64_t cus) {
 
 }  // namespace
 
-// Two slices of K (fp32 outputs, N % 8 == 0, added by the reader) for experts whose whole tiles leave
+// Two slices of K (fp32 outputs, added by the reader) for experts whose whole tiles leave
 // CUs without work: the cheapest tile for half the length on twice the workgroups, against the
 // cheapest for all of it (of the difference 0.4 to 0.5 was measured) and the second slice's way
 // through memory, 4 bytes an output at 5 TB/s.  8 experts, K = 14336 to 4096: of 128 rows each 66 us on
@@ -451,7 +444,7 @@ int mxfp4_down_slices(int K, int N, int M, int n_experts) {
     static const int32_t grouped = 0;
     g.offsets = &grouped, g.n_experts = n_experts;
     const MxTileChoice one = tile_for(K, N, M, g, kMxCus);
-    if (one.tokens == 0 || one.split || K < 4096 || N % 8 != 0) return 1;
+    if (one.tokens == 0 || one.split || K < 4096) return 1;
     const MxTileChoice two = tile_for(K, N, M, g, kMxCus / 2);  // tiles as well, and whole ones: fewer CUs
     return 0.4f * (one.cost - 0.5f * two.cost) * (float)K / 4096.f > (float)M * (float)N * 4.f / 5e6f ? 2 : 1;
 }

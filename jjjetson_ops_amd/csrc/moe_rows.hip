@@ -57,16 +57,6 @@ __device__ __forceinline__ void expert_bases(int *s_cnt, int *s_part) {
 // touches a line more): the last piece ends with the row and overlaps the one before, which is
 // the same values once more.  Rows shorter than a piece go by single elements.  8192 tokens top-2 of
 // 4095 bf16 values: the combine 32 us, 71 by single elements (31 for 4096).
-template <class V>
-__device__ __forceinline__ V load_any(const void *p) {
-    V v;
-    __builtin_memcpy(&v, p, sizeof(V));
-    return v;
-}
-template <class V>
-__device__ __forceinline__ void store_any(void *p, const V &v) {
-    __builtin_memcpy(p, &v, sizeof(V));
-}
 
 // ---- dispatch of up to kSortMax routes in one launch.  Workgroup (t + 1, c) has its piece of
 // token t's row in flight, counts for each of the token's routes the routes that sort before

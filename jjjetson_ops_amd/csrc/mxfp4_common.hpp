@@ -56,6 +56,18 @@ struct alignas(sizeof(T) * VEC) MxVec {
     T v[VEC];
 };
 
+// The same at any alignment: one access all the same, over one line more where it crosses one.
+template <class V>
+__device__ __forceinline__ V load_any(const void *p) {
+    V v;
+    __builtin_memcpy(&v, p, sizeof(V));
+    return v;
+}
+template <class V>
+__device__ __forceinline__ void store_any(void *p, const V &v) {
+    __builtin_memcpy(p, &v, sizeof(V));
+}
+
 // ---- quantizer.  The scale byte of a block whose largest |x| has the fp32 bits `amax`:
 // 2^(floor(log2 amax) - 2), the exponent of e2m1's largest power of two, taken from the
 // exponent field (fp32 subnormals and smaller exponents: 2^-127); 255 for a NaN or an infinity.

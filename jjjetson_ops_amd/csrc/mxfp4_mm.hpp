@@ -1,5 +1,5 @@
-// Device pieces that the MXFP4 matrix kernels share: the scaled matrix instruction, output
-// rows in the three types, an expert's tile of sorted rows, and the SwiGLU epilogue.
+// Device pieces that the MXFP4 matrix kernels share: the scaled matrix instruction, an expert's tile
+// of sorted rows, and the SwiGLU epilogue.
 #pragma once
 
 #include "mxfp4_common.hpp"
@@ -14,27 +14,6 @@ __device__ __forceinline__ f32x4v mx_mfma(u32x4v w, u32x4v x, f32x4v acc, uint32
     const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
     const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, BW, (int)sw, BX, (int)sx);
-}
-
-// Four consecutive outputs of one row (the first `live` of them), in y's type.  `vec`: the row
-// and y are aligned for one access.  Every index is a constant: an indexed copy would be moved to
-// LDS, addressed by the workgroup size of the launch packet, which lies in host memory (14 us more
-// for a decode step).
-template <class T>
-__device__ __forceinline__ void mx_store4_as(T *p, f32x4v v, int live, bool vec) {
-    if (vec && live >= 4) {
-        *reinterpret_cast<MxVec<T, 4> *>(p) = MxVec<T, 4>{{(T)v[0], (T)v[1], (T)v[2], (T)v[3]}};
-    } else {
-        p[0] = (T)v[0];
-        if (live > 1) p[1] = (T)v[1];
-        if (live > 2) p[2] = (T)v[2];
-        if (live > 3) p[3] = (T)v[3];
-    }
-}
-__device__ __forceinline__ void mx_store4(void *y, int dtype, size_t at, f32x4v v, int live, bool vec) {
-    if (dtype == JJO_DTYPE_F32) mx_store4_as((float *)y + at, v, live, vec);
-    else if (dtype == JJO_DTYPE_F16) mx_store4_as((_Float16 *)y + at, v, live, vec);
-    else mx_store4_as((__bf16 *)y + at, v, live, vec);
 }
 
 // Inclusive sums over the wave's lanes: row shifts inside the rows of 16, then row_bcast15 and

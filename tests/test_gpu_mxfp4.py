@@ -358,7 +358,8 @@ def _close_dev(got, exp, bound):
 # last pair of stages and row and token tiles that are not full.
 @pytest.mark.parametrize("K,N,M", [(2080, 8264, 50), (2336, 16424, 33), (2080, 16424, 70), (2048, 16420, 100),
                                    (544, 16424, 16), (1056, 16424, 50), (608, 16420, 90), (768, 16424, 127),
-                                   (544, 14344, 625), (544, 14344, 700), (800, 14340, 1000)])
+                                   (544, 14344, 625), (544, 14341, 700), (800, 14339, 1000), (2080, 16423, 70),
+                                   (1056, 16417, 50)])
 def test_mat_mul_tiles(K, N, M, dev):
     note(f"mat_mul tiles K={K} N={N} M={M}")
     gen = torch.Generator(device=dev).manual_seed(K + N + M)
