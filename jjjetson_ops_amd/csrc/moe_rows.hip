@@ -8,8 +8,8 @@
 //   its gradients         grows[dst(t, k)] = w(t, k) gy[t],  gw(t, k) = <gy[t], rows[dst(t, k)]>
 //
 // All of it is bound by HBM once there are some hundred rows and by latency below: a row is
-// moved in 16-byte pieces where its length allows, sums are fp32 in k order (one rounding, at
-// the store), and nothing is added with atomics, so a result does not depend on timing.
+// moved in 16-byte pieces, sums are fp32 in k order (one rounding, at the store), and only counts
+// are added with atomics, so a result does not depend on timing.
 #include <hip/hip_runtime.h>
 
 #include "moe_top_k.hpp"

@@ -267,7 +267,8 @@ def _ffn_case(rng, T, H, I, E, dev, dtype):
 
 FFN = [(1, 64, 32, 4, 1, "f32"), (1, 512, 256, 8, 2, "bf16"), (4, 1024, 512, 8, 2, "bf16"), (16, 160, 96, 64, 8, "f32"),
        (33, 512, 224, 8, 2, "f16"), (100, 256, 128, 64, 8, "bf16"), (300, 512, 416, 8, 2, "f32"),
-       (700, 256, 256, 4, 2, "bf16"), (3, 128, 64, 300, 32, "f32")]
+       (700, 256, 256, 4, 2, "bf16"), (3, 128, 64, 300, 32, "f32"), (2100, 256, 128, 8, 2, "bf16"),
+       (600, 128, 64, 300, 8, "f32")]
 
 
 @pytest.mark.parametrize("T,H,I,E,k,dtype", FFN)
