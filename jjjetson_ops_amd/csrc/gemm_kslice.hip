@@ -106,7 +106,8 @@ __device__ __forceinline__ void kslice_loop(f32x16 (&acc)[RT][CT], uint8_t *stag
     const uint32_t stage_lds = (uint32_t)(uintptr_t)stage;
     float *wde = reinterpret_cast<float *>(stage + L::kOffScale);
     // Inline asm: the compiler would order every later LDS access behind these; their
-    // completion is waited for at the top of a stage.
+    // completion is waited for at the top of a stage.  It does not count the wait state that a DMA
+    // needs after a write of M0 either: s_nop 0.
     constexpr int kPieces = 3 * RT + L::kXRuns;
     // One DMA instruction of a stage.  The spread form takes them in this order: the weights,
     // which come from further away, first.
@@ -115,7 +116,7 @@ __device__ __forceinline__ void kslice_loop(f32x16 (&acc)[RT][CT], uint8_t *stag
             const int i = k - 3 * RT;
             const uint32_t m0v = __builtin_amdgcn_readfirstlane(stage_lds + i * 1024);
             if ((i + 1) * 1024 <= L::kXBytes || lane < 32)
-                asm volatile("global_load_lds_dwordx4 %0, %1"
+                asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                              :
                              : "v"(min((uint32_t)(i * 1024 + lane * 16), xlim)), "s"(xb + (size_t)s * x_stride),
                                "{m0}"(m0v)
@@ -125,17 +126,17 @@ __device__ __forceinline__ void kslice_loop(f32x16 (&acc)[RT][CT], uint8_t *stag
         const int rt = k / 3, i = k % 3;
         const uint32_t m0v = __builtin_amdgcn_readfirstlane(stage_lds + L::kOffW + rt * L::kWTile + i * 1024);
         if constexpr (!SPLIT)
-            asm volatile("global_load_lds_dwordx3 %0, %1"
+            asm volatile("s_nop 0\n\tglobal_load_lds_dwordx3 %0, %1"
                          :
                          : "v"(woff[rt][i]), "s"(wq[rt] + (size_t)s * (4 * kQ4BlockBytes)), "{m0}"(m0v)
                          : "memory");
         else if (i < 2)
-            asm volatile("global_load_lds_dwordx4 %0, %1"
+            asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                          :
                          : "v"(woff[rt][i]), "s"(wq[rt] + (size_t)s * 64), "{m0}"(m0v)
                          : "memory");
         else
-            asm volatile("global_load_lds_dword %0, %1"
+            asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1"
                          :
                          : "v"(woff[rt][i]), "s"(wd[rt] + (size_t)s * 8), "{m0}"(m0v)
                          : "memory");

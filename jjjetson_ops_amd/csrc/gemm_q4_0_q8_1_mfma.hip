@@ -249,7 +249,8 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_q4_0_q8_1_mfma_kernel(
     // same iteration writes and reads, and would wait for every load in flight
     // (vmcnt(0)) before the next LDS access, collapsing the weight prefetch.  Their
     // completion is waited for explicitly (the vmcnt(3) before each unpack and the
-    // vmcnt(0) after the K loop); the hardware counter counts them like any load.
+    // vmcnt(0) after the K loop); the hardware counter counts them like any load.  s_nop 0: the
+    // wait state between a write of M0 and the DMA, which the compiler does not count for asm.
     auto load_x = [&](int c) {
         const uint32_t xs = (uint32_t)(uintptr_t)(smem + (c & 1) * kXsBytes);
         const uint8_t *src = x_base + (size_t)c * x_stride;
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_q4_0_q8_1_mfma_kernel(
             // (grouped tails): skipped.  Wave-uniform.
             if (run * 64 >= x_valid_units) continue;
             const uint32_t m0v = __builtin_amdgcn_readfirstlane(xs + run * 1024);
-            asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(src + x_off[i]), "{m0}"(m0v) : "memory");
+            asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src + x_off[i]), "{m0}"(m0v) : "memory");
         }
     };
 

@@ -152,7 +152,8 @@ __global__ __launch_bounds__(kSThreads) void gemm_q4_0_q8_1_mfma64_kernel(const 
     }
     // Inline-asm DMA, as in the 128 x 128 kernel: the compiler's wait insertion would
     // otherwise wait for every load in flight before the next LDS access.  Waited for
-    // explicitly below; the hardware counter counts them like any load.
+    // explicitly below; the hardware counter counts them like any load.  s_nop 0: the wait
+    // state after a write of M0.
     auto load_x = [&](int c) {
         const uint32_t xs = (uint32_t)(uintptr_t)(smem + (c & 1) * kSXsBytes);
         const uint8_t *src = x_base + (size_t)c * x_stride;
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(kSThreads) void gemm_q4_0_q8_1_mfma64_kernel(const 
             const int run = wave + 4 * i;
             if (run >= kSXRuns || run * 64 >= x_valid_units) continue;  // uniform per wave
             const uint32_t m0v = __builtin_amdgcn_readfirstlane(xs + run * 1024);
-            asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(src + x_off[i]), "{m0}"(m0v) : "memory");
+            asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src + x_off[i]), "{m0}"(m0v) : "memory");
         }
     };
     auto zero_tail_headers = [&](int buf) {

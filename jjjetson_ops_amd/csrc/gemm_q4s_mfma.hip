@@ -105,6 +105,8 @@ __global__ __launch_bounds__(g2::kThreads, 2) void gemm_q4s_mfma_kernel(const ui
         const int unit = min(wave + 4 * i, kXRuns - 1) * 64 + lane;
         x_off[i] = unit < x_valid_units ? unit * 16 : 0;
     }
+    // s_nop 0 in front of every DMA: the wait state that it needs after a write of M0, which the
+    // compiler does not count for asm.
     auto dma_x = [&](int c, int buf, int i0, int i1) {  // 1 KB runs wave + 4i, i0 <= i < i1
         const uint32_t xs = (uint32_t)(uintptr_t)(smem + buf * kBufBytes);
         const uint8_t *src = x_base + (size_t)c * x_stride;
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(g2::kThreads, 2) void gemm_q4s_mfma_kernel(const ui
             if (i < i0 || i >= i1) continue;
             const int run = min(wave + 4 * i, kXRuns - 1);
             const uint32_t m0v = __builtin_amdgcn_readfirstlane(xs + run * 1024);
-            asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(x_off[i]), "s"(src), "{m0}"(m0v) : "memory");
+            asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(x_off[i]), "s"(src), "{m0}"(m0v) : "memory");
         }
     };
 
@@ -139,8 +141,8 @@ __global__ __launch_bounds__(g2::kThreads, 2) void gemm_q4s_mfma_kernel(const ui
             const uint32_t m0a = __builtin_amdgcn_readfirstlane(wqs);
             const uint32_t m0b = __builtin_amdgcn_readfirstlane(wqs + 64 * 16);
             const uint8_t *src = wq_base + (size_t)c * (KB * 16);
-            asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(wq_off0), "s"(src), "{m0}"(m0a) : "memory");
-            asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(wq_off1), "s"(src), "{m0}"(m0b) : "memory");
+            asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(wq_off0), "s"(src), "{m0}"(m0a) : "memory");
+            asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(wq_off1), "s"(src), "{m0}"(m0b) : "memory");
             wst[0] = *reinterpret_cast<const uint32_t *>(wd_base + (size_t)c * (KB * 2) + wd_off);
         } else {
             const uint8_t *p = wr_base + (size_t)c * (KB * kQ4BlockBytes) + wr_off;

@@ -80,9 +80,10 @@ __device__ __forceinline__ void p_vm_wait_items(int pre) {  // pre wave-uniform,
 // 16 bytes per lane, global -> LDS at m0 + 16*lane.  Inline asm so that the
 // compiler's wait insertion does not treat the ring writes as aliasing every other
 // LDS access (it would wait for all loads in flight); completion is waited for
-// explicitly.
+// explicitly.  s_nop 0: the wait state between a write of M0 and the DMA, which it does
+// not count for asm.
 __device__ __forceinline__ void dma16(const void *src, uint32_t lds_base) {
-    asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(src), "{m0}"(__builtin_amdgcn_readfirstlane(lds_base))
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "{m0}"(__builtin_amdgcn_readfirstlane(lds_base))
                  : "memory");
 }
 
