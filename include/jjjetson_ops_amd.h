@@ -553,8 +553,8 @@ int moe_mxfp4_gate_up_swiglu_device(void *stream, const void *w_gate, const void
 /*
  * The whole MoE FFN with MXFP4 experts, beside moe_q4_0_ffn_forward_device: x, y of `dtype`
  * [T][H], logits fp32 [T][E]; w_gate, w_up [E*I][H], w_down [E*H][I].  top_k <= min(32, E), E <= 1024,
- * H and I multiples of 32, T * top_k <= 2^26.  `workspace` (256-byte aligned) holds every intermediate; it may be
- * used again by the next call on the same stream.
+ * H and I multiples of 32, H <= 2^23, I <= 2^28, T <= 2^23, T * top_k <= 2^26.  `workspace` (256-byte aligned) holds
+ * every intermediate; it may be used again by the next call on the same stream.
  */
 int64_t moe_mxfp4_ffn_workspace_bytes(int num_tokens, int hidden_size, int intermediate_size, int num_experts,
                                       int top_k);
@@ -568,7 +568,8 @@ int moe_mxfp4_ffn_forward_device(void *stream, const void *x, const float *logit
  * siblings of moe_dispatch_q8_1_device and moe_combine_device.  R = num_tokens * top_k routes
  * r = t*top_k + k.  A route whose expert id is outside [0, num_experts) is dropped (a padded
  * token, an expert of another process): dst_of_route is -1, it has no sorted row.
- * num_experts <= 1024, top_k <= 32, at most 2^26 routes; hidden_size is any positive number.
+ * num_experts <= 1024, top_k <= 32, at most 2^26 routes; num_tokens and hidden_size are any positive
+ * numbers up to 2^23.
  */
 
 /*

@@ -712,12 +712,13 @@ hipError_t launch_moe_combine_rows_backward(const void *grad_y, const void *rows
         constexpr int kWide = 16 / sizeof(E);
         auto run = [&](auto vec) {
             constexpr int V = decltype(vec)::value;
-            if (H <= 128 * V) {
-                const int log2_row = std::min(log2_threads((H + V - 1) / V), 6), routes = 256 >> log2_row;
-                hipLaunchKernelGGL((combine_rows_backward_short_kernel<E, V>),
-                                   dim3((unsigned)((T * top_k + routes - 1) / routes)), dim3(256), 0, stream,
-                                   (const E *)grad_y, (const E *)rows, dst_of_route, weights, T * top_k, top_k, H,
-                                   log2_row, (E *)grad_rows, grad_weights);
+            const int log2_row = std::min(log2_threads((H + V - 1) / V), 6), routes = 256 >> log2_row;
+            const int64_t groups = ((int64_t)T * top_k + routes - 1) / routes;
+            // (A grid has fewer than 2^32 threads: 2^26 routes of 64 lanes go by tokens.)
+            if (H <= 128 * V && groups * 256 < 1LL << 32) {
+                hipLaunchKernelGGL((combine_rows_backward_short_kernel<E, V>), dim3((unsigned)groups), dim3(256), 0,
+                                   stream, (const E *)grad_y, (const E *)rows, dst_of_route, weights, T * top_k, top_k,
+                                   H, log2_row, (E *)grad_rows, grad_weights);
                 return hipGetLastError();
             }
             hipLaunchKernelGGL((combine_rows_backward_kernel<E, V>), dim3((unsigned)T), dim3(256), 0, stream,
