@@ -487,7 +487,9 @@ int safetensors_quantize_q4_0(const char *in_path, const char *out_path, const c
  * 2^-127; x / s rounded to nearest even, at most 6 in magnitude.  A block that holds a NaN or
  * an infinity gets s = 255 and zero codes.
  * Activations and outputs are fp32, fp16 or bf16 (JJO_DTYPE_*), 16-byte aligned and contiguous
- * unless a row stride is given; all sums are fp32, outputs rounded once.
+ * unless a row stride is given; all sums are fp32, outputs rounded once.  Sizes of the products (K, N,
+ * rows) are at most 2^28 each; a call of the quantizer or its inverse takes at most 2^35 - 2^23
+ * values.
  */
 #define JJO_DTYPE_F32 0
 #define JJO_DTYPE_F16 1

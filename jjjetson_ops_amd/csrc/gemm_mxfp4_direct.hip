@@ -29,7 +29,8 @@ struct MxProblem {
     void *y;                    // outputs, or the MXFP4 rows of the SwiGLU form
     int dtype;
     int K, N, M;
-    int tiles_n;  // row tiles of the launch
+    int tiles_n;           // row tiles of the launch
+    int first_t, first_n;  // its first token tile and row tile
     MxGroups g;
 };
 
@@ -75,7 +76,8 @@ __global__ __launch_bounds__(64 * KW * RW) void mxfp4_direct_kernel(MxProblem p)
     const int la = lane >> 2 & 3, lb = lane & 3, lj = lane >> 4, blk0 = 4 * lj + lb;
     // Row tiles vary fastest: the eight XCDs, which take workgroups in turn, then have the same
     // share of the token tiles that exist.
-    const int tile_t = (int)(blockIdx.x / (unsigned)p.tiles_n), tile_n = (int)(blockIdx.x % (unsigned)p.tiles_n);
+    const int tile_t = p.first_t + (int)(blockIdx.x / (unsigned)p.tiles_n);
+    const int tile_n = p.first_n + (int)(blockIdx.x % (unsigned)p.tiles_n);
     int expert = 0, first = tile_t * kTokens, end = p.M;
     if constexpr (GROUPED) {
         if (!mx_expert_tile(p.g.offsets, p.g.n_experts, p.M, kTokens, tile_t, expert, first, end)) return;
@@ -256,19 +258,27 @@ hipError_t run_direct(MxProblem p, hipStream_t stream) {
     // token tiles of M rows, and one more for each expert that can have a rest
     const int64_t rests = p.g.offsets != nullptr ? std::min(p.g.n_experts, p.M) : 0;
     const int64_t token_tiles = (p.M + 4 * TG - 1) / (4 * TG) + rests;
-    p.tiles_n = (p.N + rows - 1) / rows;
-    const int64_t wgs = token_tiles * p.tiles_n;
-    if (wgs * threads >= 1LL << 32) return hipErrorInvalidConfiguration;
-    const dim3 grid((unsigned)wgs), block(threads);
-    if constexpr (!std::is_void_v<XT>)
-        hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, false, false, XT>), grid, block, 0, stream, p);
-    else if (p.g.offsets != nullptr)
-        hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, true, SWIGLU, void>), grid, block, 0, stream, p);
-    else if constexpr (!SWIGLU)
-        hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, false, false, void>), grid, block, 0, stream, p);
-    else
-        return hipErrorInvalidValue;
-    return hipGetLastError();
+    const int64_t row_tiles = (p.N + rows - 1) / rows;
+    // A grid has fewer than 2^32 threads: more (2^33 outputs of short rows, 2^28 weight rows) are several launches.
+    constexpr int64_t kMost = ((1LL << 32) - 1) / threads;
+    for (int64_t n = 0; n < row_tiles; n += kMost) {
+        p.first_n = (int)n, p.tiles_n = (int)std::min(kMost, row_tiles - n);
+        const int64_t at_once = kMost / p.tiles_n;
+        for (int64_t t = 0; t < token_tiles; t += at_once) {
+            p.first_t = (int)t;
+            const dim3 grid((unsigned)(p.tiles_n * std::min(at_once, token_tiles - t))), block(threads);
+            if constexpr (!std::is_void_v<XT>)
+                hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, false, false, XT>), grid, block, 0, stream, p);
+            else if (p.g.offsets != nullptr)
+                hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, true, SWIGLU, void>), grid, block, 0, stream, p);
+            else if constexpr (!SWIGLU)
+                hipLaunchKernelGGL((mxfp4_direct_kernel<TG, KW, RW, false, false, void>), grid, block, 0, stream, p);
+            else
+                return hipErrorInvalidValue;
+            if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        }
+    }
+    return hipSuccess;
 }
 
 }  // namespace
@@ -279,7 +289,7 @@ hipError_t run_direct(MxProblem p, hipStream_t stream) {
 // and 32 took longer at every size (4096 x 4096, 32 tokens: 7.6 against 5.9 us).
 hipError_t launch_mxfp4_direct(const void *w, const void *xq, void *y, int dtype, int K, int N, int M,
                                const MxGroups &groups, hipStream_t stream) {
-    const MxProblem p{(const uint8_t *)w, nullptr, (const uint8_t *)xq, y, dtype, K, N, M, 0, groups};
+    const MxProblem p{(const uint8_t *)w, nullptr, (const uint8_t *)xq, y, dtype, K, N, M, 0, 0, 0, groups};
     const bool grouped = groups.offsets != nullptr;
     const int64_t experts = mx_experts(M, groups), rows = mx_rows(M, groups), mean = (M + experts - 1) / experts;
     if (mean <= (grouped ? 3 : 4)) return run_direct<1, 4, 1, false>(p, stream);
@@ -294,7 +304,7 @@ hipError_t launch_mxfp4_direct(const void *w, const void *xq, void *y, int dtype
 hipError_t launch_mxfp4_direct_swiglu(const void *w_gate, const void *w_up, const void *xq, void *mid, int K, int I,
                                       int M, const MxGroups &groups, hipStream_t stream) {
     const MxProblem p{(const uint8_t *)w_gate, (const uint8_t *)w_up, (const uint8_t *)xq, mid, JJO_DTYPE_F32, K, I, M,
-                      0, groups};
+                      0, 0, 0, groups};
     const int experts = mx_experts(M, groups), mean = (M + experts - 1) / experts;
     if (mean <= 3) return run_direct<1, 1, 4, true>(p, stream);
     return run_direct<4, 1, 4, true>(p, stream);
@@ -302,7 +312,7 @@ hipError_t launch_mxfp4_direct_swiglu(const void *w_gate, const void *w_up, cons
 
 hipError_t launch_mxfp4_gemv(const void *w, const void *x, int x_dtype, void *y, int y_dtype, int K, int N,
                              hipStream_t stream) {
-    const MxProblem p{(const uint8_t *)w, nullptr, (const uint8_t *)x, y, y_dtype, K, N, 1, 0, MxGroups{}};
+    const MxProblem p{(const uint8_t *)w, nullptr, (const uint8_t *)x, y, y_dtype, K, N, 1, 0, 0, 0, MxGroups{}};
     return mx_by_dtype(x_dtype, [&](auto tag) {
         using T = typename decltype(tag)::type;
         return run_direct<1, 4, 1, false, T>(p, stream);

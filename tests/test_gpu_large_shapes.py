@@ -50,3 +50,81 @@ def test_combine_backward_of_all_routes(dev):
         want = w[t:t + step].double()[..., None] * g
         bad = ~((got.double() - want).abs() <= mx.HALF_STEP["f32"] * want.abs() + mx.TINY["f32"])
         assert not bad.any(), (t, bad.nonzero()[:4].tolist())
+
+
+def _codes(gen, rows, cols, dev):
+    """Random codes under one scale, 1: a product is a whole number of quarters, 144 at most, so a sum of
+    up to 2^16 of them is exact in fp32 in any order."""
+    half = rows * cols // 2
+    q = torch.randint(0, 256, (rows * cols // 32 * 17,), dtype=torch.uint8, device=dev, generator=gen)
+    q[half:] = 127
+    return q
+
+
+def _rows_of(q, rows, cols, first, n):
+    """The values (fp64) of rows first.. of a matrix under one scale."""
+    table = torch.from_numpy(mx.values(torch.arange(16, dtype=torch.uint8).numpy())).to(q.device)
+    b = q[first * cols // 2:(first + n) * cols // 2].view(n, cols // 2).int()
+    return torch.stack([table[b & 15], table[b >> 4]], 2).view(n, cols)
+
+
+def test_mat_mul_of_short_rows_and_many_outputs(dev):
+    """2^33 outputs of K = 32: 16 tokens x 32 rows a workgroup would be a grid of 2^32 threads.  The sums
+    are exact, so the outputs are the fp64 products rounded once."""
+    K, N, M = 32, 8200, (1 << 20) + 5
+    note(f"mat_mul K={K} N={N} M={M}")
+    gen = torch.Generator(device=dev).manual_seed(2)
+    w, x = _codes(gen, N, K, dev), _codes(gen, M, K, dev)
+    y = torch.full((M, N), float("nan"), dtype=torch.bfloat16, device=dev)
+    capi.mat_mul_mxfp4(w, x, y, K, N, M)
+    wv = _rows_of(w, N, K, 0, N).float().t().contiguous()
+    step = 1 << 15
+    for t in range(0, M, step):
+        n = min(step, M - t)
+        assert torch.equal(y[t:t + n], (_rows_of(x, M, K, t, n).float() @ wv).bfloat16()), t
+
+
+def test_mat_mul_of_most_weight_rows(dev):
+    """2^28 weight rows, 16 a workgroup: as many workgroups of 256 threads would be 2^32."""
+    K, N = 32, 1 << 28
+    note(f"mat_mul K={K} N={N} M=1")
+    gen = torch.Generator(device=dev).manual_seed(4)
+    w, x = _codes(gen, N, K, dev), _codes(gen, 1, K, dev)
+    xv = _rows_of(x, 1, K, 0, 1)
+    for call in ("mat_mul", "linear"):
+        y = torch.full((1, N), float("nan"), device=dev)
+        if call == "mat_mul":
+            capi.mat_mul_mxfp4(w, x, y, K, N, 1)
+        else:  # the row's largest code is 6 or 4, so its quantized form is the row itself
+            assert xv.abs().max() >= 4
+            capi.linear_mxfp4(xv.float(), w, y, K, N, 1)
+        step = 1 << 22
+        for n in range(0, N, step):
+            assert torch.equal(y[0, n:n + step].double(), (_rows_of(w, N, K, n, step) * xv).sum(1)), (call, n)
+
+
+def test_gate_up_of_short_rows_and_many_outputs(dev):
+    """The same for gate|up: equal rows give equal bytes, whichever launch they are in."""
+    K, I, E, base_rows = 32, 8224, 2, 1 << 11
+    R = 1 << 20
+    note(f"gate_up K={K} I={I} R={R}")
+    gen = torch.Generator(device=dev).manual_seed(3)
+    wg, wu = _codes(gen, E * I, K, dev), _codes(gen, E * I, K, dev)
+    few = _codes(gen, base_rows, K, dev)
+    half = base_rows * K // 2
+    x = torch.cat([few[:half].repeat(R // base_rows), few[half:].repeat(R // base_rows)])
+
+    def run(q, rows):
+        mid = torch.full((capi.mxfp4_bytes(rows, I),), 0x5A, dtype=torch.uint8, device=dev)
+        off = torch.tensor([0, rows // 2, rows], dtype=torch.int32, device=dev)
+        capi.moe_gate_up_swiglu_mxfp4(wg, wu, q, off, E, mid, K, I, rows)
+        n = rows * I // 2
+        return mid[:n].view(rows, I // 2), mid[n:].view(rows, I // 32)
+
+    two = torch.cat([few[:half], few[:half], few[half:], few[half:]])  # each expert has every row once
+    small = run(two, 2 * base_rows)
+    for got, want in zip(run(x, R), small):
+        for e in range(E):
+            g = got[e * R // 2:(e + 1) * R // 2].view(-1, base_rows, got.shape[1])
+            for part in g:
+                assert torch.equal(part, want[e * base_rows:(e + 1) * base_rows])
