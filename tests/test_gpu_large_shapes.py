@@ -9,7 +9,7 @@ import torch
 
 import _mxfp4 as mx
 from jjjetson_ops_amd import capi
-from test_gpu_mxfp4 import note
+from test_gpu_mxfp4 import _close_dev, _product, _values, note
 
 pytestmark = pytest.mark.gpu
 
@@ -128,3 +128,52 @@ def test_gate_up_of_short_rows_and_many_outputs(dev):
             g = got[e * R // 2:(e + 1) * R // 2].view(-1, base_rows, got.shape[1])
             for part in g:
                 assert torch.equal(part, want[e * base_rows:(e + 1) * base_rows])
+
+
+def test_ffn_of_tokens_beyond_4_gib(dev):
+    """More than 4 GiB of MXFP4 tokens, whose rows gate|up gathers: tokens of the first rows, around the
+    middle and of the last rows against the public stages on these tokens alone.  One scale for
+    tokens and for gate and up: their sums are exact, so the intermediate bytes do not depend on
+    the tile."""
+    T, H, I, E, k = (1 << 20) + 3, 8192, 4096, 4, 2
+    note(f"ffn T={T} H={H} I={I} E={E} k={k}")
+    gen = torch.Generator(device=dev).manual_seed(5)
+    wg, wu = _codes(gen, E * I, H, dev), _codes(gen, E * I, H, dev)
+    for w in (wg, wu):
+        w[E * I * H // 2:] = 119  # sums of some 2^14 quarters, times 2^-8
+    wd = _codes(gen, E * H, I, dev)
+    wd[E * H * I // 2:] = 110
+    few = 1 << 10
+    values = _rows_of(_codes(gen, few, H, dev), few, H, 0, few).bfloat16()
+    values.view(few, -1, 32)[..., 5] = 6.0  # every block's scale is 1
+    x = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
+    for t in range(0, T, few):
+        x[t:t + few] = values[:min(few, T - t)]
+    logits = torch.randn(T, E, device=dev, generator=gen)
+    y = torch.full((T, H), float("nan"), dtype=torch.bfloat16, device=dev)
+    ws = torch.empty(capi.moe_ffn_mxfp4_workspace_bytes(T, H, I, E, k), dtype=torch.uint8, device=dev)
+    capi.moe_ffn_mxfp4(x, logits, wg, wu, wd, y, T, H, I, E, k, ws)
+    del ws
+    for part in y.split(1 << 16):
+        assert not part.isnan().any()
+
+    at = torch.cat([torch.arange(64), torch.arange(T // 2 - 64, T // 2 + 64), torch.arange(T - 64, T)]).to(dev)
+    n, i32 = len(at), dict(dtype=torch.int32, device=dev)
+    R = n * k
+    share, ids, off = torch.empty(n, k, device=dev), torch.empty(n, k, **i32), torch.empty(E + 1, **i32)
+    src, dst = torch.empty(R, **i32), torch.empty(R, **i32)
+    rows = torch.empty(R, H, dtype=torch.bfloat16, device=dev)
+    xq, mid = (torch.empty(capi.mxfp4_bytes(R, c), dtype=torch.uint8, device=dev) for c in (H, I))
+    capi.moe_top_k(logits[at].contiguous(), share, ids, n, E, k)
+    capi.moe_dispatch_rows(ids, x[at].contiguous(), rows, off, src, dst, n, k, H, E)
+    capi.quantize_mxfp4(rows, xq, R, H)
+    capi.moe_gate_up_swiglu_mxfp4(wg, wu, xq, off, E, mid, H, I, R)
+    o, midv, wdv = off.tolist(), _values(mid, R, I), _values(wd, E * H, I)
+    eo, eb = (torch.zeros(R, H, dtype=torch.float64, device=dev) for _ in range(2))
+    for e in range(E):
+        q = slice(o[e], o[e + 1])
+        eo[q], eb[q] = _product(midv[q], wdv[e * H:(e + 1) * H])
+    d, w = dst.long().view(n, k), share.double()[..., None]
+    exp = (w * eo[d]).sum(1)
+    bound = (w * (eb[d] + k * 2.0 ** -23 * eo[d].abs())).sum(1)
+    _close_dev(y[at], exp, bound + mx.HALF_STEP["bf16"] * (exp.abs() + bound) + mx.TINY["bf16"])
