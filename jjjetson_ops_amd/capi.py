@@ -692,8 +692,11 @@ def _typed(name: str, t, dtype, n: int) -> None:
 
 def _rows_of(t, name: str, rows: int, cols: int):
     """(argument, row stride) of rows x cols values: a contiguous tensor, or a 2-D one whose
-    rows are contiguous."""
+    rows are contiguous.  The first cols values of the tensor's rows where it has that many rows of
+    more, as of a slice of it; else its values in order."""
     if t.is_contiguous():
+        if t.dim() > 1 and (width := t.shape[-1]) > cols and t.numel() >= rows * width:
+            return t, width
         _room(name, t, rows * cols)
         return t, cols
     if t.dim() != 2 or t.stride(1) != 1 or t.shape[0] < rows or t.shape[1] < cols or (rows > 1 and t.stride(0) < cols):
@@ -711,7 +714,7 @@ def mxfp4_bytes(rows: int, cols: int) -> int:
 
 
 def quantize_mxfp4(x, out, rows: int, cols: int, stream=None) -> None:
-    """out = MXFP4 of x [rows, cols] (float32, float16 or bfloat16; rows may be strided)."""
+    """out = MXFP4 of x [rows, cols] (float32, float16 or bfloat16; rows may be strided or longer)."""
     d = _dtype(x, "x")
     p, row_stride = _rows_of(x, "x", rows, cols)
     _mx_room("out", out, rows, cols)
@@ -719,7 +722,7 @@ def quantize_mxfp4(x, out, rows: int, cols: int, stream=None) -> None:
 
 
 def dequantize_mxfp4(q, y, rows: int, cols: int, stream=None) -> None:
-    """y [rows, cols] (float32, float16 or bfloat16; rows may be strided) = the values of q."""
+    """y [rows, cols] (float32, float16 or bfloat16; rows may be strided or longer) = the values of q."""
     d = _dtype(y, "y")
     p, row_stride = _rows_of(y, "y", rows, cols)
     _mx_room("q", q, rows, cols)
