@@ -756,14 +756,14 @@ def linear_mxfp4(x, w, y, in_features: int, out_features: int, num_tokens: int, 
 
 def grouped_mat_mul_mxfp4(w, xq, expert_offsets, y, K: int, N: int, n_routes: int, route_dst=None,
                           stream=None) -> None:
-    """mat_mul_mxfp4_grouped_device: rows sorted by expert times their experts' weights."""
+    """mat_mul_mxfp4_grouped_device: rows sorted by expert times their experts' weights.  route_dst, where
+    given, names rows of y; they are the caller's to keep inside it."""
     d = _dtype(y, "y")
     n_experts = expert_offsets.numel() - 1
     _typed("expert_offsets", expert_offsets, _torch.int32, 2)
     if route_dst is not None:
         _typed("route_dst", route_dst, _torch.int32, n_routes)
-    else:
-        _room("y", y, n_routes * N)
+    _room("y", y, N if route_dst is not None else n_routes * N)
     _mx_room("w", w, n_experts * N, K)
     _mx_room("xq", xq, n_routes, K)
     _entry(_GROUPED, "mat_mul_mxfp4_grouped_device", stream, w, xq, expert_offsets, n_experts, route_dst, y, d, K, N,

@@ -163,6 +163,14 @@ def test_wrapper_refuses_sizes(on_device_0):
     assert e.value.code == BAD and "ncols_k=48" in str(e.value)
 
 
+def test_scattered_outputs_need_a_row(on_device_0):
+    """With route_dst the rows of y are the table's to name, but there is at least one."""
+    u, i = Fake(U8), Fake(I32, n=9)
+    for n in (0, 3):
+        with pytest.raises(ValueError, match="y is too small"):
+            capi.grouped_mat_mul_mxfp4(u, u, i, Fake(n=n), 32, 4, 2, route_dst=i, stream=0)
+
+
 def test_oracle_of_the_format():
     """The oracle's rounding against the nearest of all e2m1 values, ties to the even code."""
     v = np.concatenate([np.linspace(-8, 8, 4097), np.array(mx.BOUNDS), np.nextafter(mx.BOUNDS, 0)])
