@@ -221,9 +221,10 @@ int moe_mxfp4_ffn_forward_device(void *stream, const void *x, const float *logit
                                  int hidden_size, int intermediate_size, int num_experts, int top_k, void *workspace,
                                  int64_t workspace_bytes) {
     clear_error();
-    const int T = num_tokens, H = hidden_size, I = intermediate_size, E = num_experts, R = T * top_k;
+    const int T = num_tokens, H = hidden_size, I = intermediate_size, E = num_experts;
     int rc = check_ffn(T, H, I, E, top_k);
     if (rc != JJO_OK) return rc;
+    const int R = T * top_k;
     if (!dtype_ok(dtype)) return set_error(JJO_ERR_INVALID_ARG, "moe_mxfp4_ffn: unknown dtype %d", dtype);
     for (const void *p : {x, (const void *)logits, w_gate, w_up, w_down, (const void *)y, (const void *)workspace})
         if (p == nullptr) return set_error(JJO_ERR_INVALID_ARG, "moe_mxfp4_ffn: null pointer argument");
