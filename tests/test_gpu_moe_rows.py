@@ -133,6 +133,28 @@ def test_combine_backward(T, k, H, E, dtype, dropped, dev):
     _close(_host(gw), terms.sum(2), (H // 256 + 17) * 2.0 ** -24 * np.abs(terms).sum(2))
 
 
+@pytest.mark.parametrize("T,k,H,dtype", [(300, 4, 1024, "bf16"), (300, 4, 1024, "f16"), (200, 3, 512, "f32"),
+                                         (64, 2, 1000, "bf16"), (40, 3, 514, "bf16"), (50, 2, 4096, "f32"),
+                                         (50, 2, 1032, "f16"), (30, 2, 33, "f32"), (9, 8, 7, "f16")])
+def test_combine_backward_weights(T, k, H, dtype, dev):
+    """grad_weights within the roundings of either kernel, 2^-24 of the magnitudes each, V values a
+    piece (8, or 4 of fp32).  Up to 128 pieces a wave or part of one has the row: at most two pieces a
+    lane, 2 V products added in turn, then at most six steps of lanes.  Longer, a workgroup: a thread
+    has every 256th piece, then six steps and two for the waves."""
+    note(f"join grad weights T={T} k={k} H={H} {dtype}")
+    rng = np.random.default_rng(T + H + 3)
+    V, R = (4 if dtype == "f32" else 8), T * k
+    dst = rng.permutation(R).astype(np.int32).reshape(T, k)
+    rows, g = (torch.from_numpy(rng.standard_normal((n, H))).to(DT[dtype]) for n in (R, T))
+    ge = torch.empty(R, H, dtype=DT[dtype], device=dev)
+    gw = torch.full((T, k), float("nan"), device=dev)
+    capi.moe_combine_rows_backward(g.to(dev), rows.to(dev), torch.from_numpy(dst).to(dev), torch.rand(T, k, device=dev),
+                                   ge, gw, T, H, k)
+    terms = g.double().numpy()[:, None, :] * rows.double().numpy()[dst]
+    roundings = 2 * V + 6 if H <= 128 * V else -(-H // (256 * V)) * V + 8
+    _close(_host(gw), terms.sum(2), roundings * 2.0 ** -24 * np.abs(terms).sum(2))
+
+
 def test_gradients_against_differences(dev):
     """The combine is linear in the rows and in the weights, the dispatch in x: a difference of the
     forward pass along a direction is the gradient's product with it, up to the fp32 rounding
