@@ -31,15 +31,12 @@ typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
 // to nearest even on the way out.
 struct MxF32 {
     typedef float type;
-    static constexpr int kDtype = JJO_DTYPE_F32;
 };
 struct MxF16 {
     typedef _Float16 type;
-    static constexpr int kDtype = JJO_DTYPE_F16;
 };
 struct MxBF16 {
     typedef __bf16 type;
-    static constexpr int kDtype = JJO_DTYPE_BF16;
 };
 
 // Calls F(tag) with the type tag of a JJO_DTYPE_* value (checked by the entries).
