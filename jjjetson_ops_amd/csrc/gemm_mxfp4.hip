@@ -49,7 +49,7 @@ struct MxTile {
     static constexpr int kLds = KG * kGroupLds + kRows * 4;
     static_assert(kLds <= 160 * 1024, "LDS of a CU");
     static_assert(KG == 1 || kThreads * RT * TT * 16 <= kGroupLds, "a group's sums fit its stages");
-    static_assert(NW == 2 || (NW == 3 && KG == 1), "weights one stage ahead or two");
+    static_assert(NW == 2 || (NW == 3 && KG == 1), "weights one stage ahead, or two in every other stage");
 };
 
 // A wave's outputs (from weight row n, token t on) through its own 4 KB of LDS, 16 tokens at a time:
@@ -139,8 +139,8 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
     const size_t x_all = p.g.src_route != nullptr ? p.g.x_rows : p.M;
 
     // ---- the DMA: instruction i of a wave takes run kDma * wave + i of 8 rows, a lane piece
-    // (lane % 8) ^ (row / 2 % 8) of row lane / 8.  The rows' offsets stand in LDS: kept in registers
-    // they would spill, and a reload from scratch waits for every DMA before it.
+    // (lane % 8) ^ (row / 2 % 8) of row lane / 8.  The rows' offsets stand in LDS (in registers
+    // they would take up to eight of the 60 and more that every tile leaves).
     const int t0 = GROUPED && p.g.src_route != nullptr ? 0 : first;
     for (int row = threadIdx.x; row < Tile::kRows; row += KG * Tile::kThreads)
         lds_rows[row] = row < Tile::kRowsN ? (uint32_t)(weight_row(row) - n0) * half
@@ -240,7 +240,9 @@ __global__ __launch_bounds__(Tile::KG *Tile::kThreads) void mxfp4_tiled_kernel(M
     const uint32_t sw0 = 16u * ((2 * q) ^ (r16 >> 1)), sw1 = 16u * ((2 * q + 1) ^ (r16 >> 1));
     for (int round = 0; round < rounds; ++round) {
         const int st = s_beg + round;  // s_beg is even
-        // Stage st has landed: loads return in order, the last ones are the next stage's weights (NW == 3).
+        // Stage st has landed: loads return in order, the last ones are the next stage's weights (NW == 3).  In even
+        // stages the compiler waits for the scales' registers below, and not counting the asm's loads it waits for all
+        // of them: there the next stage's weights have landed too.
         asm volatile("s_waitcnt vmcnt(%0)" ::"i"(Tile::NW == 3 ? Tile::kDmaN : 0) : "memory");
         if ((st & 1) == 0 && (KG == 1 || st < s_end)) store_scales(st >> 1);
         if (round == cut) {  // the row ends inside the last stage: zero weights behind it
@@ -357,8 +359,9 @@ struct MxTileChoice {
 };
 
 // 128 weight rows on four waves up to 128 tokens, 256 on eight above; there the weights come two stages
-// ahead where LDS has room (8 experts of 28672 rows, 128 tokens each: 152 us on tiles of 160, 159
-// with one stage ahead; no difference where several token tiles read the same weights).
+// ahead where LDS has room, in every other stage (the wait for the scales drains them in the rest; 8
+// experts of 28672 rows, 128 tokens each: 152 us on tiles of 160, 159 with one stage ahead; no difference
+// where several token tiles read the same weights).
 template <bool SWIGLU>
 hipError_t run_tile(const MxTiled &p, const MxTileChoice &tile, hipStream_t stream) {
     if (tile.split) {
