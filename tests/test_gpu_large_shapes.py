@@ -177,3 +177,71 @@ def test_ffn_of_tokens_beyond_4_gib(dev):
     exp = (w * eo[d]).sum(1)
     bound = (w * (eb[d] + k * 2.0 ** -23 * eo[d].abs())).sum(1)
     _close_dev(y[at], exp, bound + mx.HALF_STEP["bf16"] * (exp.abs() + bound) + mx.TINY["bf16"])
+
+
+@pytest.mark.parametrize("T,k,E,H", [(1 << 21, 32, 1000, 8), (1 << 23, 8, 3, 1), (1 << 23, 1, 64, 40)])
+def test_rows_of_most_routes(T, k, E, H, dev):
+    """The most tokens and the most routes, there and back: the sort against torch's stable one, whole
+    numbers as rows, so that their sums are exact."""
+    R = T * k
+    note(f"rows T={T} k={k} E={E} H={H}")
+    gen = torch.Generator(device=dev).manual_seed(6)
+    ids = torch.randint(-1, E, (T, k), dtype=torch.int32, device=dev, generator=gen)  # -1: dropped
+    x = torch.randint(-4, 5, (T, H), device=dev, generator=gen).bfloat16()
+    rows = torch.full((R, H), 7.0, dtype=torch.bfloat16, device=dev)
+    off, src, dst = (torch.full((n,), -5, dtype=torch.int32, device=dev) for n in (E + 1, R, R))
+    capi.moe_dispatch_rows(ids, x, rows, off, src, dst, T, k, H, E)
+    key, order = torch.where(ids < 0, E, ids).view(-1).sort(stable=True)
+    live = int((key < E).sum())
+    assert torch.equal(off.long(), torch.searchsorted(key[:live], torch.arange(E + 1, device=dev, dtype=torch.int32)))
+    assert torch.equal(src[:live].long(), order[:live]) and (src[live:] == -5).all()
+    want = torch.full((R,), -1, dtype=torch.int32, device=dev)
+    want[order[:live]] = torch.arange(live, dtype=torch.int32, device=dev)
+    assert torch.equal(dst, want)
+    del key, want
+    step = 1 << 22
+    for p in range(0, live, step):
+        n = min(step, live - p)
+        assert torch.equal(rows[p:p + n], x[order[p:p + n] // k])
+    assert (rows[live:] == 7.0).all()
+    del order, src
+    counts = (ids >= 0).sum(1, keepdim=True)
+    back, y = torch.full_like(x, float("nan")), torch.full_like(x, float("nan"))
+    capi.moe_dispatch_rows_backward(rows, dst, back, T, H, k)
+    assert torch.equal(back.float(), (x.float() * counts).bfloat16().float())
+    w = torch.full((T, k), 0.5, device=dev)
+    capi.moe_combine_rows(rows, dst, w, y, T, H, k)
+    assert torch.equal(y.float(), (x.float() * counts * 0.5).bfloat16().float())
+    gw = torch.full((T, k), float("nan"), device=dev)
+    ge = torch.full_like(rows, 7.0)
+    capi.moe_combine_rows_backward(x, rows, dst, w, ge, gw, T, H, k)
+    assert torch.equal(gw, (x.float() ** 2).sum(1, keepdim=True) * (ids >= 0))
+    assert torch.equal(ge[:live], rows[:live] * 0.5) and (ge[live:] == 7.0).all()
+
+
+def test_quantize_of_most_values(dev):
+    """2^35 - 2^23 values in one call and back: rows that repeat give bytes that repeat, and one more row
+    of blocks is refused."""
+    rows, cols, few = (1 << 20) - (1 << 8), 1 << 15, 1 << 8
+    note(f"quantize {rows}x{cols}")
+    gen = torch.Generator(device=dev).manual_seed(7)
+    some = torch.randn(few, cols, device=dev, generator=gen).bfloat16()
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=dev)
+    x.view(-1, few, cols)[:] = some
+    q = torch.empty(capi.mxfp4_bytes(rows, cols), dtype=torch.uint8, device=dev)
+    capi.quantize_mxfp4(x, q, rows, cols)
+    q0 = torch.empty(capi.mxfp4_bytes(few, cols), dtype=torch.uint8, device=dev)
+    capi.quantize_mxfp4(some, q0, few, cols)
+    half, half0 = rows * cols // 2, few * cols // 2
+    for got, want in ((q[:half], q0[:half0]), (q[half:], q0[half0:])):
+        for part in got.view(-1, want.numel()).split(256):
+            assert (part == want).all()
+    back0 = torch.empty_like(some)
+    capi.dequantize_mxfp4(q0, back0, few, cols)
+    x.fill_(float("nan"))
+    capi.dequantize_mxfp4(q, x, rows, cols)
+    for part in x.view(-1, few * cols).split(256):
+        assert (part == back0.view(-1)).all()
+    with pytest.raises(capi.JJOError, match="exceeds one launch"):
+        capi._check(capi.lib().quantize_mxfp4_device(None, x.data_ptr(), capi.DTYPE_BF16, cols, q.data_ptr(), rows + 1,
+                                                     cols), "quantize_mxfp4_device")
