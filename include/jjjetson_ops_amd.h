@@ -603,6 +603,98 @@ int moe_combine_rows_backward_device(void *stream, const void *grad_y, const voi
                                      const int32_t *dst_of_route, const float *route_weights, void *grad_expert_out,
                                      float *grad_route_weights, int num_tokens, int hidden_size, int top_k);
 
+/* ------------------------------------------------------------------ products of float matrices
+ * Weights in fp32, fp16 or bf16 beside the quantized ones: a linear layer (the reference's engine
+ * multiplies fp32 weights, src/cuda/linear.cu), the experts' products of rows sorted by expert
+ * (moe_dispatch_rows_device and moe_combine_rows_device above move the rows) and gate|up with SwiGLU, each
+ * with its gradients.
+ * All operands of a call are of `dtype` unless it says otherwise; sums are fp32, each result is rounded
+ * once, and the gradient through an activation is rounded to `dtype` before it is multiplied.
+ * Sums are added in an order that depends on the sizes alone.  Buffers are aligned to
+ * their elements; where rows are 16-byte aligned as well the products are faster.  Sizes (in, out, rows) are
+ * positive, any other number up to 2^28, a matrix has at most 2^40 elements.  Row strides are in
+ * elements, at least the row's length.
+ * Outputs may not overlap inputs, except where said.  Workspaces are 256-byte aligned, may be NULL where
+ * their size is 0, and may be used again by the next call on the same stream; the sizes do not depend
+ * on the device.  The *_bytes functions return -1 for sizes that the call refuses.
+ */
+#define JJO_ACT_NONE 0
+#define JJO_ACT_RELU 1      /* max(z, 0) */
+#define JJO_ACT_GELU 2      /* z/2 (1 + erf(z / sqrt 2)) */
+#define JJO_ACT_GELU_TANH 3 /* z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+#define JJO_ACT_SILU 4      /* z / (1 + e^-z) */
+
+/*
+ * y = act(x . weight^T + bias) + residual: x [T][in], weight [out][in] contiguous, bias [out] or NULL,
+ * residual [T][out] or NULL, y [T][out].  pre (or NULL) receives x . weight^T + bias, [T][out]
+ * contiguous, for the backward pass.  residual may be y itself (with its stride).
+ */
+int64_t linear_rows_workspace_bytes(int dtype, int in_features, int out_features, int num_tokens);
+int linear_rows_forward_device(void *stream, const void *x, int64_t x_stride, const void *weight, const void *bias,
+                               const void *residual, int64_t residual_stride, void *y, int64_t y_stride, void *pre,
+                               int dtype, int activation, int in_features, int out_features, int num_tokens,
+                               void *workspace, int64_t workspace_bytes);
+/*
+ * Its gradients, gz = grad_y * act'(pre): grad_x = gz . weight, grad_weight = gz^T . x, grad_bias = the
+ * columns' sums of gz; each may be NULL, and with it what only it needs (weight; x; pre where
+ * activation is none).  The residual's gradient is grad_y.  grad_weight and grad_bias are of
+ * grad_weight_dtype: `dtype` or fp32.
+ */
+int64_t linear_rows_backward_workspace_bytes(int dtype, int in_features, int out_features, int num_tokens);
+int linear_rows_backward_device(void *stream, const void *grad_y, int64_t grad_y_stride, const void *x,
+                                int64_t x_stride, const void *weight, const void *pre, void *grad_x,
+                                int64_t grad_x_stride, void *grad_weight, void *grad_bias, int dtype,
+                                int grad_weight_dtype, int activation, int in_features, int out_features,
+                                int num_tokens, void *workspace, int64_t workspace_bytes);
+
+/*
+ * Experts' products: y[p] = weights[e] . x_sorted[p] for the rows expert_offsets[e] <= p <
+ * expert_offsets[e+1] of each expert; x_sorted [n_routes][ncols_k], weights [E][nrows_out][ncols_k], y
+ * [n_routes][nrows_out].  expert_offsets (device, E + 1 entries, non-decreasing, first 0) may end below
+ * n_routes: the rows behind the last expert's are not read and their outputs not written.  Ranges are
+ * clamped to [0, n_routes].  E <= 4096.
+ */
+int64_t mat_mul_rows_grouped_workspace_bytes(int dtype, int ncols_k, int nrows_out, int n_routes, int n_experts);
+int mat_mul_rows_grouped_device(void *stream, const void *x_sorted, const void *weights, const int32_t *expert_offsets,
+                                int n_experts, void *y, int dtype, int ncols_k, int nrows_out, int n_routes,
+                                void *workspace, int64_t workspace_bytes);
+/*
+ * Their gradients: grad_x_sorted[p] = grad_y[p] . weights[e], grad_weights[e] = the sum over e's rows of
+ * grad_y[p]^T . x_sorted[p] (zero for an expert without rows), of grad_weights_dtype: `dtype` or fp32.
+ * Either may be NULL, and with it what only it needs (weights; x_sorted).
+ */
+int64_t mat_mul_rows_grouped_backward_workspace_bytes(int dtype, int ncols_k, int nrows_out, int n_routes,
+                                                      int n_experts);
+int mat_mul_rows_grouped_backward_device(void *stream, const void *grad_y, const void *x_sorted, const void *weights,
+                                         const int32_t *expert_offsets, int n_experts, void *grad_x_sorted,
+                                         void *grad_weights, int dtype, int grad_weights_dtype, int ncols_k,
+                                         int nrows_out, int n_routes, void *workspace, int64_t workspace_bytes);
+
+/*
+ * gate|up projection with SwiGLU of rows sorted by expert, beside moe_mxfp4_gate_up_swiglu_device:
+ * mid[p] = silu(w_gate[e] . x_sorted[p]) * (w_up[e] . x_sorted[p]), [n_routes][intermediate_size].
+ * gate_up (or NULL) receives both products for the backward pass, [n_routes][2 * intermediate_size], gate
+ * first.
+ */
+int64_t moe_rows_gate_up_swiglu_workspace_bytes(int dtype, int hidden_size, int intermediate_size, int n_routes,
+                                                int num_experts);
+int moe_rows_gate_up_swiglu_device(void *stream, const void *x_sorted, const void *w_gate, const void *w_up,
+                                   const int32_t *expert_offsets, int num_experts, void *gate_up, void *mid, int dtype,
+                                   int hidden_size, int intermediate_size, int n_routes, void *workspace,
+                                   int64_t workspace_bytes);
+/*
+ * Its gradients from that of mid and the saved gate|up.  grad_x_sorted may be NULL, and so may both
+ * grad_w_gate and grad_w_up (of grad_weights_dtype: `dtype` or fp32), each with what only it needs.
+ */
+int64_t moe_rows_gate_up_swiglu_backward_workspace_bytes(int dtype, int hidden_size, int intermediate_size,
+                                                         int n_routes, int num_experts);
+int moe_rows_gate_up_swiglu_backward_device(void *stream, const void *grad_mid, const void *gate_up,
+                                            const void *x_sorted, const void *w_gate, const void *w_up,
+                                            const int32_t *expert_offsets, int num_experts, void *grad_x_sorted,
+                                            void *grad_w_gate, void *grad_w_up, int dtype, int grad_weights_dtype,
+                                            int hidden_size, int intermediate_size, int n_routes, void *workspace,
+                                            int64_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

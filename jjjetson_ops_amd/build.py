@@ -26,7 +26,9 @@ LIB = PKG / "libjjjetson_ops_amd.so"
 
 HIP_SOURCES = ["quantize_q8_1.hip", "gemv_q4_0_q8_1.hip", "gemm_skinny_q4_0_q8_1.hip", "gemm_skinny_persist.hip", "gemm_q4_0_q8_1_mfma.hip", "gemm_q4_0_q8_1_mfma64.hip", "moe_route.hip",
                "quantize_q4_0.hip", "q4_0_split.hip", "gemm_q4s_mfma.hip", "gemm_kslice.hip",
-               "mxfp4_quant.hip", "gemm_mxfp4_direct.hip", "gemm_mxfp4.hip", "moe_rows.hip", "weights_q4_0.cpp", "capi.hip", "capi_mxfp4.hip"]
+               "mxfp4_quant.hip", "gemm_mxfp4_direct.hip", "gemm_mxfp4.hip", "moe_rows.hip",
+               "gemm_rows_f32.hip", "gemm_rows_f16.hip", "gemm_rows_bf16.hip", "rows_parts.hip",
+               "weights_q4_0.cpp", "capi.hip", "capi_mxfp4.hip", "capi_rows.hip"]
 HIP_FLAGS = [
     "--offload-arch=gfx950",
     "-O3",
@@ -55,7 +57,7 @@ def _run(cmd: list[str]) -> None:
         sys.stderr.write("\n".join(noise) + "\n")
 
 
-def build_lib(jobs: int = 4) -> Path:
+def build_lib(jobs: int = 8) -> Path:
     BUILD.mkdir(exist_ok=True)
     objs = []
     cmds = []

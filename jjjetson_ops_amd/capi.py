@@ -96,11 +96,30 @@ EXPORTED_SYMBOLS = (
     "moe_dispatch_rows_backward_device",
     "moe_combine_rows_device",
     "moe_combine_rows_backward_device",
+    "linear_rows_workspace_bytes",
+    "linear_rows_forward_device",
+    "linear_rows_backward_workspace_bytes",
+    "linear_rows_backward_device",
+    "mat_mul_rows_grouped_workspace_bytes",
+    "mat_mul_rows_grouped_device",
+    "mat_mul_rows_grouped_backward_workspace_bytes",
+    "mat_mul_rows_grouped_backward_device",
+    "moe_rows_gate_up_swiglu_workspace_bytes",
+    "moe_rows_gate_up_swiglu_device",
+    "moe_rows_gate_up_swiglu_backward_workspace_bytes",
+    "moe_rows_gate_up_swiglu_backward_device",
 )
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
 DTYPE_BF16 = 2
+
+ACT_NONE = 0
+ACT_RELU = 1
+ACT_GELU = 2
+ACT_GELU_TANH = 3
+ACT_SILU = 4
+
 MX_BLOCK_BYTES = 17
 
 WEIGHT_DTYPE_F32 = 0
@@ -263,6 +282,29 @@ def lib() -> ctypes.CDLL:
         L.moe_combine_rows_device.argtypes = [vp, vp, i32, vp, vp, vp, i32, i32, i32]
         L.moe_combine_rows_backward_device.restype = i32
         L.moe_combine_rows_backward_device.argtypes = [vp, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32]
+        for name in ("linear_rows", "linear_rows_backward"):
+            f = getattr(L, name + "_workspace_bytes")
+            f.restype, f.argtypes = i64, [i32, i32, i32, i32]
+        for name in ("mat_mul_rows_grouped", "mat_mul_rows_grouped_backward", "moe_rows_gate_up_swiglu",
+                     "moe_rows_gate_up_swiglu_backward"):
+            f = getattr(L, name + "_workspace_bytes")
+            f.restype, f.argtypes = i64, [i32, i32, i32, i32, i32]
+        L.linear_rows_forward_device.restype = i32
+        L.linear_rows_forward_device.argtypes = [vp, vp, i64, vp, vp, vp, i64, vp, i64, vp, i32, i32, i32, i32, i32,
+                                                 vp, i64]
+        L.linear_rows_backward_device.restype = i32
+        L.linear_rows_backward_device.argtypes = [vp, vp, i64, vp, i64, vp, vp, vp, i64, vp, vp, i32, i32, i32, i32,
+                                                  i32, i32, vp, i64]
+        L.mat_mul_rows_grouped_device.restype = i32
+        L.mat_mul_rows_grouped_device.argtypes = [vp, vp, vp, vp, i32, vp, i32, i32, i32, i32, vp, i64]
+        L.mat_mul_rows_grouped_backward_device.restype = i32
+        L.mat_mul_rows_grouped_backward_device.argtypes = [vp, vp, vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32,
+                                                           vp, i64]
+        L.moe_rows_gate_up_swiglu_device.restype = i32
+        L.moe_rows_gate_up_swiglu_device.argtypes = [vp, vp, vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, i64]
+        L.moe_rows_gate_up_swiglu_backward_device.restype = i32
+        L.moe_rows_gate_up_swiglu_backward_device.argtypes = [vp, vp, vp, vp, vp, vp, vp, i32, vp, vp, vp, i32, i32,
+                                                              i32, i32, i32, vp, i64]
         _lib = L
     return _lib
 
@@ -626,7 +668,8 @@ def moe_ffn(x, logits, w_gate, w_up, w_down, y, num_tokens: int, hidden: int, in
 # ---------------------------------------------------------------- MXFP4 and sorted rows
 # The entries of csrc/bind_linear.cpp by their places in its table.
 (_QUANTIZE, _DEQUANTIZE, _MAT_MUL, _LINEAR, _GROUPED, _GATE_UP, _FFN, _DISPATCH, _DISPATCH_BACKWARD, _COMBINE,
- _COMBINE_BACKWARD) = range(11)
+ _COMBINE_BACKWARD, _LINEAR_ROWS, _LINEAR_ROWS_BACKWARD, _ROWS_GROUPED, _ROWS_GROUPED_BACKWARD, _ROWS_GATE_UP,
+ _ROWS_GATE_UP_BACKWARD) = range(17)
 _entry_native = None
 _dtypes = None
 
@@ -861,3 +904,154 @@ def moe_combine_rows_backward(grad_y, expert_out, dst_of_route, weights, grad_ex
     _room("grad_expert_out", grad_expert_out, r * hidden)
     _entry(_COMBINE_BACKWARD, "moe_combine_rows_backward_device", stream, grad_y, expert_out, d, dst_of_route, weights,
            grad_expert_out, grad_weights, num_tokens, hidden, top_k)
+
+
+# ---------------------------------------------------------------- products of float matrices
+def _optional(t, name: str, d: int, n: int) -> None:
+    """None, or a tensor of the dtype d with at least n elements."""
+    if t is not None:
+        _same_dtype(name, d, t)
+        _room(name, t, n)
+
+
+def _strided(t, name: str, rows: int, cols: int):
+    """(argument, row stride) of rows x cols values, (None, 0) of None."""
+    return (None, 0) if t is None else _rows_of(t, name, rows, cols)
+
+
+def _grad_dtype(d: int, *grads) -> int:
+    """The dtype of the weights' gradients that are given: d or float32."""
+    found = {_dtype(g, "a weight's gradient") for g in grads if g is not None} or {d}
+    if len(found) != 1 or not found <= {d, DTYPE_F32}:
+        raise ValueError("gradients of weights must have one dtype, the weights' or float32")
+    return found.pop()
+
+
+def _bytes_of(ws) -> int:
+    return 0 if ws is None else ws.numel() * ws.element_size()
+
+
+def linear_rows_workspace_bytes(dtype: int, in_features: int, out_features: int, num_tokens: int) -> int:
+    return int(lib().linear_rows_workspace_bytes(dtype, in_features, out_features, num_tokens))
+
+
+def linear_rows(x, w, y, in_features: int, out_features: int, num_tokens: int, bias=None, residual=None,
+                activation: int = ACT_NONE, pre=None, ws=None, stream=None) -> None:
+    """y [T, out] = act(x [T, in] . w [out, in]^T + bias) + residual, all of one dtype (float32, float16 or
+    bfloat16).  Rows of x, residual and y may be strided; residual may be y.  pre [T, out], where given,
+    receives x . w^T + bias for the backward pass; ws of linear_rows_workspace_bytes (None where that is 0)."""
+    d = _dtype(x, "x")
+    for name, t in (("w", w), ("y", y)):
+        _same_dtype(name, d, t)
+    _room("w", w, out_features * in_features)
+    _optional(bias, "bias", d, out_features)
+    _optional(residual, "residual", d, 0)
+    _optional(pre, "pre", d, num_tokens * out_features)
+    px, x_stride = _rows_of(x, "x", num_tokens, in_features)
+    pr, r_stride = _strided(residual, "residual", num_tokens, out_features)
+    py, y_stride = _rows_of(y, "y", num_tokens, out_features)
+    _entry(_LINEAR_ROWS, "linear_rows_forward_device", stream, px, x_stride, w, bias, pr, r_stride, py, y_stride, pre, d,
+           activation, in_features, out_features, num_tokens, ws, _bytes_of(ws))
+
+
+def linear_rows_backward_workspace_bytes(dtype: int, in_features: int, out_features: int, num_tokens: int) -> int:
+    return int(lib().linear_rows_backward_workspace_bytes(dtype, in_features, out_features, num_tokens))
+
+
+def linear_rows_backward(grad_y, x, w, grad_x, grad_w, grad_b, in_features: int, out_features: int, num_tokens: int,
+                         activation: int = ACT_NONE, pre=None, ws=None, stream=None) -> None:
+    """The gradients of linear_rows (None: not wanted) from that of y: grad_x of x's dtype, grad_w and grad_b
+    of x's or float32.  pre is what the forward pass kept (needed with an activation).  The residual's
+    gradient is grad_y."""
+    d = _dtype(grad_y, "grad_y")
+    gd = _grad_dtype(d, grad_w, grad_b)
+    _optional(x, "x", d, 0)
+    _optional(w, "w", d, out_features * in_features)
+    _optional(pre, "pre", d, num_tokens * out_features)
+    _optional(grad_x, "grad_x", d, 0)
+    _optional(grad_w, "grad_w", gd, out_features * in_features)
+    _optional(grad_b, "grad_b", gd, out_features)
+    pg, g_stride = _rows_of(grad_y, "grad_y", num_tokens, out_features)
+    px, x_stride = _strided(x, "x", num_tokens, in_features)
+    pgx, gx_stride = _strided(grad_x, "grad_x", num_tokens, in_features)
+    _entry(_LINEAR_ROWS_BACKWARD, "linear_rows_backward_device", stream, pg, g_stride, px, x_stride, w, pre, pgx,
+           gx_stride, grad_w, grad_b, d, gd, activation, in_features, out_features, num_tokens, ws, _bytes_of(ws))
+
+
+def grouped_mat_mul_rows_workspace_bytes(dtype: int, K: int, N: int, n_routes: int, num_experts: int) -> int:
+    return int(lib().mat_mul_rows_grouped_workspace_bytes(dtype, K, N, n_routes, num_experts))
+
+
+def grouped_mat_mul_rows(x, w, expert_offsets, y, K: int, N: int, n_routes: int, ws=None, stream=None) -> None:
+    """mat_mul_rows_grouped_device: rows of x [n_routes, K] sorted by expert times their experts' weights w
+    [E, N, K]; E is one less than expert_offsets' (int32) length."""
+    d = _dtype(x, "x")
+    n_experts = expert_offsets.numel() - 1
+    for name, t, n in (("x", x, n_routes * K), ("w", w, n_experts * N * K), ("y", y, n_routes * N)):
+        _optional(t, name, d, n)
+    _typed("expert_offsets", expert_offsets, _torch.int32, 2)
+    _entry(_ROWS_GROUPED, "mat_mul_rows_grouped_device", stream, x, w, expert_offsets, n_experts, y, d, K, N, n_routes,
+           ws, _bytes_of(ws))
+
+
+def grouped_mat_mul_rows_backward_workspace_bytes(dtype: int, K: int, N: int, n_routes: int, num_experts: int) -> int:
+    return int(lib().mat_mul_rows_grouped_backward_workspace_bytes(dtype, K, N, n_routes, num_experts))
+
+
+def grouped_mat_mul_rows_backward(grad_y, x, w, expert_offsets, grad_x, grad_w, K: int, N: int, n_routes: int,
+                                  ws=None, stream=None) -> None:
+    """The gradients of grouped_mat_mul_rows (None: not wanted): grad_x [n_routes, K] of grad_y's dtype, grad_w
+    [E, N, K] of that or float32."""
+    d = _dtype(grad_y, "grad_y")
+    gd = _grad_dtype(d, grad_w)
+    n_experts = expert_offsets.numel() - 1
+    for name, t, n in (("grad_y", grad_y, n_routes * N), ("x", x, n_routes * K), ("w", w, n_experts * N * K),
+                       ("grad_x", grad_x, n_routes * K)):
+        _optional(t, name, d, n)
+    _optional(grad_w, "grad_w", gd, n_experts * N * K)
+    _typed("expert_offsets", expert_offsets, _torch.int32, 2)
+    _entry(_ROWS_GROUPED_BACKWARD, "mat_mul_rows_grouped_backward_device", stream, grad_y, x, w, expert_offsets,
+           n_experts, grad_x, grad_w, d, gd, K, N, n_routes, ws, _bytes_of(ws))
+
+
+def moe_gate_up_swiglu_rows_workspace_bytes(dtype: int, hidden: int, inter: int, n_routes: int, num_experts: int) -> int:
+    return int(lib().moe_rows_gate_up_swiglu_workspace_bytes(dtype, hidden, inter, n_routes, num_experts))
+
+
+def moe_gate_up_swiglu_rows(x, w_gate, w_up, expert_offsets, num_experts: int, mid, hidden: int, inter: int,
+                            n_routes: int, gate_up=None, ws=None, stream=None) -> None:
+    """mid [n_routes, inter] = silu(x . w_gate^T) * (x . w_up^T) of rows sorted by expert, w_gate and w_up
+    [E, inter, hidden]; gate_up [n_routes, 2 * inter], where given, receives both products."""
+    d = _dtype(x, "x")
+    for name, t, n in (("x", x, n_routes * hidden), ("w_gate", w_gate, num_experts * inter * hidden),
+                       ("w_up", w_up, num_experts * inter * hidden), ("mid", mid, n_routes * inter),
+                       ("gate_up", gate_up, n_routes * 2 * inter)):
+        _optional(t, name, d, n)
+    _typed("expert_offsets", expert_offsets, _torch.int32, num_experts + 1)
+    _entry(_ROWS_GATE_UP, "moe_rows_gate_up_swiglu_device", stream, x, w_gate, w_up, expert_offsets, num_experts,
+           gate_up, mid, d, hidden, inter, n_routes, ws, _bytes_of(ws))
+
+
+def moe_gate_up_swiglu_rows_backward_workspace_bytes(dtype: int, hidden: int, inter: int, n_routes: int,
+                                                     num_experts: int) -> int:
+    return int(lib().moe_rows_gate_up_swiglu_backward_workspace_bytes(dtype, hidden, inter, n_routes, num_experts))
+
+
+def moe_gate_up_swiglu_rows_backward(grad_mid, gate_up, x, w_gate, w_up, expert_offsets, num_experts: int, grad_x,
+                                     grad_w_gate, grad_w_up, hidden: int, inter: int, n_routes: int, ws=None,
+                                     stream=None) -> None:
+    """The gradients of moe_gate_up_swiglu_rows (None: not wanted) from that of mid and the saved gate_up:
+    grad_x of their dtype, grad_w_gate and grad_w_up of that or float32."""
+    d = _dtype(grad_mid, "grad_mid")
+    gd = _grad_dtype(d, grad_w_gate, grad_w_up)
+    weights = num_experts * inter * hidden
+    for name, t, n in (("grad_mid", grad_mid, n_routes * inter), ("gate_up", gate_up, n_routes * 2 * inter),
+                       ("x", x, n_routes * hidden), ("w_gate", w_gate, weights), ("w_up", w_up, weights),
+                       ("grad_x", grad_x, n_routes * hidden)):
+        _optional(t, name, d, n)
+    _optional(grad_w_gate, "grad_w_gate", gd, weights)
+    _optional(grad_w_up, "grad_w_up", gd, weights)
+    _typed("expert_offsets", expert_offsets, _torch.int32, num_experts + 1)
+    _entry(_ROWS_GATE_UP_BACKWARD, "moe_rows_gate_up_swiglu_backward_device", stream, grad_mid, gate_up, x, w_gate,
+           w_up, expert_offsets, num_experts, grad_x, grad_w_gate, grad_w_up, d, gd, hidden, inter, n_routes, ws,
+           _bytes_of(ws))

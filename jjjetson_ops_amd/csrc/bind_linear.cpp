@@ -1,5 +1,5 @@
-// CPython binding of the two Q4_0 linear-layer entries and of the MXFP4 and sorted-row entries
-// for device tensors.
+// CPython binding of the two Q4_0 linear-layer entries and of the MXFP4, sorted-row and float-product
+// entries for device tensors.
 //
 // A decode step's kernel takes 3 to 6 us, less than Python needs to pass four tensors
 // through ctypes (7.1 us a call at K=4096, N=4096, whose kernel takes 3.5 us).  Here the
@@ -153,10 +153,34 @@ int run_combine_backward(void *s, const Arg *a) {
     return moe_combine_rows_backward_device(s, P(0), P(1), I(2), (const int32_t *)P(3), (const float *)P(4), P(5),
                                             (float *)P(6), I(7), I(8), I(9));
 }
+int run_linear_rows(void *s, const Arg *a) {
+    return linear_rows_forward_device(s, P(0), a[1].i, P(2), P(3), P(4), a[5].i, P(6), a[7].i, P(8), I(9), I(10), I(11),
+                                      I(12), I(13), P(14), a[15].i);
+}
+int run_linear_rows_backward(void *s, const Arg *a) {
+    return linear_rows_backward_device(s, P(0), a[1].i, P(2), a[3].i, P(4), P(5), P(6), a[7].i, P(8), P(9), I(10), I(11),
+                                       I(12), I(13), I(14), I(15), P(16), a[17].i);
+}
+int run_rows_grouped(void *s, const Arg *a) {
+    return mat_mul_rows_grouped_device(s, P(0), P(1), (const int32_t *)P(2), I(3), P(4), I(5), I(6), I(7), I(8), P(9),
+                                       a[10].i);
+}
+int run_rows_grouped_backward(void *s, const Arg *a) {
+    return mat_mul_rows_grouped_backward_device(s, P(0), P(1), P(2), (const int32_t *)P(3), I(4), P(5), P(6), I(7), I(8),
+                                                I(9), I(10), I(11), P(12), a[13].i);
+}
+int run_rows_gate_up(void *s, const Arg *a) {
+    return moe_rows_gate_up_swiglu_device(s, P(0), P(1), P(2), (const int32_t *)P(3), I(4), P(5), P(6), I(7), I(8), I(9),
+                                          I(10), P(11), a[12].i);
+}
+int run_rows_gate_up_backward(void *s, const Arg *a) {
+    return moe_rows_gate_up_swiglu_backward_device(s, P(0), P(1), P(2), P(3), P(4), (const int32_t *)P(5), I(6), P(7),
+                                                   P(8), P(9), I(10), I(11), I(12), I(13), I(14), P(15), a[16].i);
+}
 #undef P
 #undef I
 
-constexpr int kMaxArgs = 14;
+constexpr int kMaxArgs = 18;
 // The argument kinds: t a tensor or an address, o one that may be None, i a C int, l an int64_t.  The names
 // stand in the messages of the arguments that are refused.
 struct Entry {
@@ -186,7 +210,25 @@ const Entry kEntries[] = {
     {run_combine_backward, "ttittttiii",
      {"grad_y", "expert_out", "dtype", "dst_of_route", "weights", "grad_expert_out", "grad_weights", "num_tokens",
       "hidden", "top_k"}},
+    {run_linear_rows, "tltooltloiiiiiol",
+     {"x", "x_stride", "w", "bias", "residual", "residual_stride", "y", "y_stride", "pre", "dtype", "activation",
+      "in_features", "out_features", "num_tokens", "ws", "ws_bytes"}},
+    {run_linear_rows_backward, "tlolooolooiiiiiiol",
+     {"grad_y", "grad_y_stride", "x", "x_stride", "w", "pre", "grad_x", "grad_x_stride", "grad_w", "grad_b", "dtype",
+      "grad_dtype", "activation", "in_features", "out_features", "num_tokens", "ws", "ws_bytes"}},
+    {run_rows_grouped, "tttitiiiiol",
+     {"x", "w", "expert_offsets", "num_experts", "y", "dtype", "K", "N", "n_routes", "ws", "ws_bytes"}},
+    {run_rows_grouped_backward, "tootiooiiiiiol",
+     {"grad_y", "x", "w", "expert_offsets", "num_experts", "grad_x", "grad_w", "dtype", "grad_dtype", "K", "N",
+      "n_routes", "ws", "ws_bytes"}},
+    {run_rows_gate_up, "ttttiotiiiiol",
+     {"x", "w_gate", "w_up", "expert_offsets", "num_experts", "gate_up", "mid", "dtype", "hidden", "inter", "n_routes",
+      "ws", "ws_bytes"}},
+    {run_rows_gate_up_backward, "ttoootioooiiiiiol",
+     {"grad_mid", "gate_up", "x", "w_gate", "w_up", "expert_offsets", "num_experts", "grad_x", "grad_w_gate",
+      "grad_w_up", "dtype", "grad_dtype", "hidden", "inter", "n_routes", "ws", "ws_bytes"}},
 };
+static_assert(sizeof kEntries / sizeof kEntries[0] == 17, "the places that capi.py names");
 
 // A tensor's or an int's address; false with an exception set.
 bool entry_ptr(PyObject *t, const char *name, long device, void **out) {
@@ -279,7 +321,7 @@ PyObject *entry(PyObject *, PyObject *const *a, Py_ssize_t n) {
 }
 
 PyMethodDef methods[] = {
-    {"entry", (PyCFunction)(void (*)(void))entry, METH_FASTCALL, "One MXFP4 or sorted-row entry on device tensors."},
+    {"entry", (PyCFunction)(void (*)(void))entry, METH_FASTCALL, "One MXFP4, sorted-row or float-product entry on device tensors."},
     {"linear", (PyCFunction)(void (*)(void))linear, METH_FASTCALL, "One linear layer on device tensors."},
     {nullptr, nullptr, 0, nullptr},
 };

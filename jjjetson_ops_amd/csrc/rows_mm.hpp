@@ -1,0 +1,165 @@
+// Products of float matrices (fp32, fp16, bf16) with fp32 sums: what the kernels and the entries share.
+//
+//     forward   y[t][n]  = act(sum_k x[t][k] w[n][k] + b[n]) + r[t][n]
+//     SwiGLU    mid[t][i] = silu(x[t] . w_gate[i]) * (x[t] . w_up[i])
+//     input     gx[t][k] = sum_n gz[t][n] w[n][k]
+//     weight    gw[n][k] = sum_t gz[t][n] x[t][k]
+//
+// of one matrix, or of stacked experts' matrices and rows sorted by expert.
+#pragma once
+
+#include "mxfp4_common.hpp"
+
+namespace jjo {
+
+enum RowsMode { kRowsForward, kRowsSwiglu, kRowsInput, kRowsWeight };
+
+// What follows a sum: bias, the sum kept, activation, residual.  SwiGLU: pre is gate|up.
+struct RowsEpilogue {
+    const void *bias = nullptr, *residual = nullptr;
+    int64_t residual_stride = 0;
+    void *pre = nullptr;
+    int act = JJO_ACT_NONE;
+};
+
+// out[Q rows][P columns] = Qmat . Pmat^T over K: of either operand either the sums' elements of a row
+// are contiguous (forward), or the rows' of an element are (weight; input: of P).
+struct RowsMm {
+    const void *p, *p2;  // p2: the up matrix (SwiGLU), or the operand of the sums' second half (input)
+    const void *q;
+    int64_t ldp, ldq;  // elements from one memory row to the next
+    void *y, *y2;      // y2: of the second half's output rows (weight)
+    int64_t ldy;
+    int P, Q, K;
+    int halves;              // 2: input sums over p, then over p2; weight has rows of y, then of y2
+    const int32_t *offsets;  // [n_experts + 1], or nullptr
+    int n_experts, M;        // M: sorted rows
+    int64_t expert_stride;   // elements of a matrix (of an expert's part of y: weight)
+    bool wide;               // y is fp32
+    int slices;              // of the sums, each in its own part[Q][P] (SwiGLU: [Q][2P])
+    float *part;
+    RowsEpilogue epi;
+    int tiles_p, tiles_q;  // of the launch
+};
+
+// ---- activations.  sigmoid and tanh through the hardware's exp2 and reciprocal (1 ulp each):
+// 0.5 (1 + tanh u) = sigmoid(2u).  The normal distribution by erfc, so that its lower tail keeps its
+// relative precision.
+__device__ __forceinline__ float rows_sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896f * z));
+}
+constexpr float kGeluC = 0.797884560802865f, kGeluA = 0.044715f;  // sqrt(2 / pi)
+
+__device__ __forceinline__ float rows_act(float z, int act) {
+    switch (act) {
+        case JJO_ACT_RELU: return z > 0.0f ? z : z != z ? z : 0.0f;
+        case JJO_ACT_GELU: return 0.5f * z * erfcf(-0.707106781186548f * z);
+        case JJO_ACT_GELU_TANH: return z * rows_sigmoid(2.0f * kGeluC * (z + kGeluA * z * z * z));
+        case JJO_ACT_SILU: return z * rows_sigmoid(z);
+    }
+    return z;
+}
+
+// The activation's derivative at z.
+__device__ __forceinline__ float rows_slope(float z, int act) {
+    switch (act) {
+        case JJO_ACT_RELU: return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
+        case JJO_ACT_GELU:
+            return 0.5f * erfcf(-0.707106781186548f * z) +
+                   z * 0.398942280401433f * __builtin_amdgcn_exp2f(-0.721347520444482f * z * z);
+        case JJO_ACT_GELU_TANH: {
+            const float s = rows_sigmoid(2.0f * kGeluC * (z + kGeluA * z * z * z));
+            return s + z * 2.0f * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * kGeluA * z * z);
+        }
+        case JJO_ACT_SILU: {
+            const float s = rows_sigmoid(z);
+            return s * (1.0f + z * (1.0f - s));
+        }
+    }
+    return 1.0f;
+}
+
+// ---- eight consecutive values of a row, n of them inside it, at any alignment
+template <class T>
+__device__ __forceinline__ void rows_load8(const T *p, int n, float *v) {
+    if (n >= 8) {
+        const MxVec<T, 8> a = load_any<MxVec<T, 8>>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)a.v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.0f;
+    }
+}
+template <class T>
+__device__ __forceinline__ void rows_store8(T *p, int n, const float *v) {
+    if (n >= 8) {
+        MxVec<T, 8> a;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a.v[i] = (T)v[i];
+        store_any(p, a);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (i < n) p[i] = (T)v[i];
+    }
+}
+
+// Sums of columns col.. of a row (n of them) to the output.
+template <class T>
+__device__ __forceinline__ void rows_finish(const RowsEpilogue &e, float *v, int64_t row, int col, int n, int cols,
+                                            void *y, int64_t ldy, bool wide) {
+    if (e.bias != nullptr) {
+        float b[8];
+        rows_load8((const T *)e.bias + col, n, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += b[i];
+    }
+    if (e.pre != nullptr) rows_store8((T *)e.pre + row * cols + col, n, v);
+    if (e.act != JJO_ACT_NONE) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = rows_act(v[i], e.act);
+    }
+    if (e.residual != nullptr) {
+        float r[8];
+        rows_load8((const T *)e.residual + row * e.residual_stride + col, n, r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += r[i];
+    }
+    if (wide) rows_store8((float *)y + row * ldy + col, n, v);
+    else rows_store8((T *)y + row * ldy + col, n, v);
+}
+
+template <class T>
+__device__ __forceinline__ void rows_finish_swiglu(const RowsEpilogue &e, float *gate, const float *up, int64_t row,
+                                                   int col, int n, int cols, void *y) {
+    if (e.pre != nullptr) {
+        T *const at = (T *)e.pre + row * 2 * cols + col;
+        rows_store8(at, n, gate);
+        rows_store8(at + cols, n, up);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) gate[i] = gate[i] * rows_sigmoid(gate[i]) * up[i];
+    rows_store8((T *)y + row * cols + col, n, gate);
+}
+
+// ---- launchers (asynchronous; arguments validated by the entries)
+hipError_t launch_rows_mm(RowsMode mode, int dtype, const RowsMm &p, hipStream_t stream);
+// Slices that launch_rows_mm is best given for a product, and the bytes of their sums.
+int rows_mm_slices(RowsMode mode, int dtype, int P, int Q, int K, int halves, int n_experts, int M);
+int64_t rows_part_bytes(RowsMode mode, const RowsMm &p);
+
+template <class E>
+hipError_t rows_mm_tiles(RowsMode mode, const RowsMm &p, int tile, hipStream_t stream);
+
+// gz[t] = grad_y[t] * act'(pre[t]) (act none: not written) and the columns' sums of gz (sums nullable;
+// column_part: rows_column_chunks(T, N) * N floats).
+int rows_column_chunks(int T, int N);
+hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, const void *pre, void *gz, int dtype,
+                                    int act, void *sums, bool sums_wide, float *column_part, int T, int N,
+                                    hipStream_t stream);
+// grad_gate_up [R][2I] from grad_mid and the saved gate|up, rows below offsets[n_experts].
+hipError_t launch_rows_swiglu_backward(const void *grad_mid, const void *gate_up, void *grad_gate_up, int dtype,
+                                       const int32_t *offsets, int n_experts, int I, int R, hipStream_t stream);
+
+}  // namespace jjo

@@ -1,0 +1,399 @@
+// Products of float matrices on LDS tiles: see rows_mm.hpp for the four forms.
+//
+// out[Q][P] += Qmat[Q][K] . Pmat[P][K]^T.  A stage is 128 bytes of the sums' direction (64 elements of 16
+// bits, 32 of 32) of every row of the tile's two operands, two steps of the matrix instruction.  Where
+// a row's elements are contiguous, its 128 bytes are a row of LDS, 16-byte pieces permuted by the row
+// (piece ^ row / 2 % 8); where the rows of an element are, an LDS row is one element of all the tile's
+// rows, and the transposing LDS read puts four elements of a row into a lane; pieces are permuted by
+// the element's number so that the lanes served together fall into different banks.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "mxfp4_mm.hpp"
+#include "rows_mm.hpp"
+
+namespace jjo {
+namespace {
+
+typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8v __attribute__((ext_vector_type(8)));
+typedef short s16x4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+
+// acc[16 of P][16 of Q] += 16 bytes of a row in each lane (row lane % 16, piece lane / 16 of four).  A lane's
+// acc holds P rows 4 * (lane / 16) + 0..3 of Q row lane % 16.
+template <class T>
+__device__ __forceinline__ f32x4v rows_mfma(u32x4v p, u32x4v q, f32x4v acc) {
+    if constexpr (std::is_same_v<T, __bf16>) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8v, p), __builtin_bit_cast(bf16x8v, q),
+                                                       acc, 0, 0, 0);
+    } else if constexpr (std::is_same_v<T, _Float16>) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8v, p), __builtin_bit_cast(f16x8v, q),
+                                                      acc, 0, 0, 0);
+    } else {
+        const f32x4v a = __builtin_bit_cast(f32x4v, p), b = __builtin_bit_cast(f32x4v, q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
+        return acc;
+    }
+}
+
+// WP x WQ waves of RT tiles of 16 output columns x TT tiles of 16 output rows each.
+template <int RT_, int TT_, int WP_, int WQ_>
+struct RowsTile {
+    static constexpr int RT = RT_, TT = TT_, WP = WP_, WQ = WQ_;
+    static constexpr int kWaves = WP * WQ, kThreads = 64 * kWaves;
+    static constexpr int kP = 16 * RT * WP, kQ = 16 * TT * WQ;
+    static constexpr int kStageP = kP * 128, kStageQ = kQ * 128, kStage = kStageP + kStageQ;
+    static constexpr int kOutPitch = 16 * RT * 4 + 16;  // a row of outputs in LDS: + 4 banks
+    static constexpr int kLds = std::max(2 * kStage, kWaves * 16 * kOutPitch);
+    static_assert(kLds <= 160 * 1024, "LDS of a CU");
+};
+
+// One operand's part of a stage: ROWS rows of the tile, TRANS: the rows of an element contiguous.
+template <class T, bool TRANS, int ROWS, int THREADS>
+struct RowsOperand {
+    static constexpr int kPiece = 16 / sizeof(T), kStep = 128 / sizeof(T);
+    static constexpr int kPitch = TRANS ? ROWS * (int)sizeof(T) : 128;  // bytes of an LDS row
+    static constexpr int kRowPieces = kPitch / 16;
+    static constexpr int kMine = ROWS * 8 / THREADS;
+    static_assert(ROWS * 8 % THREADS == 0, "whole pieces a thread");
+    static_assert(!TRANS || ROWS % 128 == 0 || ROWS == 64, "the permutations below");
+
+    // The permutation of element k's pieces (of 16 bits: pairs, 16 rows each; of 32: fours).
+    static __device__ __forceinline__ int swizzle(int k) {
+        if constexpr (sizeof(T) == 4) return 4 * ((k >> 2) & 3);
+        else if constexpr (ROWS == 64) return 2 * (((k >> 1) & 1) + 2 * ((k >> 3) & 1));
+        else return 2 * ((k & 3) + 4 * ((k >> 3) & 1));
+    }
+    // What stands in the piece at place `at` of LDS: row i and element k of the stage (the first ones).
+    static __device__ __forceinline__ void piece(int at, int &i, int &k) {
+        const int line = at / kRowPieces, place = at % kRowPieces;
+        if constexpr (TRANS) k = line, i = (place ^ swizzle(line)) * kPiece;
+        else i = line, k = (place ^ ((line >> 1) & 7)) * kPiece;
+    }
+    static __device__ __forceinline__ int64_t offset(int i, int k, int64_t ld) {
+        return TRANS ? k * ld + i : i * ld + k;
+    }
+
+    // ---- through registers: any address.  `from`(i, k, have) is the address of a piece, `have` the elements
+    // from it on that exist (zeros behind them).
+    template <class F>
+    static __device__ __forceinline__ void copy(F from, uint8_t *lds) {
+        u32x4v v[kMine];
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) {
+            int i, k, have;
+            piece(n * THREADS + threadIdx.x, i, k);
+            const T *const at = from(i, k, have);
+            v[n] = u32x4v{0u, 0u, 0u, 0u};
+            if (have >= kPiece) {
+                v[n] = load_any<u32x4v>(at);
+            } else if (have > 0) {
+                MxVec<T, kPiece> e;
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j) e.v[j] = j < have ? at[j] : (T)0.0f;
+                v[n] = __builtin_bit_cast(u32x4v, e);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) *reinterpret_cast<u32x4v *>(lds + 16 * (n * THREADS + threadIdx.x)) = v[n];
+    }
+
+    // ---- by DMA, 64 pieces an instruction: a lane's offsets; rows behind the last are the last again.
+    template <class F>
+    static __device__ __forceinline__ void dma_offsets(uint32_t (&off)[kMine], int wave, int64_t ld, F row) {
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) {
+            int i, k;
+            piece((wave * kMine + n) * 64 + (threadIdx.x & 63), i, k);
+            off[n] = (uint32_t)(offset(row(i), k, ld) * sizeof(T));
+        }
+    }
+
+    // ---- a lane's 16 bytes of a step's operand, rows base + 16 * t + lane % 16
+    template <int TILES>
+    struct Reader {
+        static constexpr int kAddresses = TRANS ? TILES : 2;
+        uint32_t at[kAddresses];
+        __device__ __forceinline__ explicit Reader(int base) {
+            const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
+            if constexpr (!TRANS) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) at[u] = (base + r16) * 128 + 16 * ((4 * u + q) ^ (r16 >> 1));
+            } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) at[t] = 4 * q * kPitch + 64 * ((base / 16 + t) ^ q) + 4 * r16;
+            } else {
+#pragma unroll
+                for (int t = 0; t < TILES; ++t)
+                    at[t] = (8 * q + (r16 >> 2)) * kPitch +
+                            32 * ((base / 16 + t) ^ (swizzle(8 * q + (r16 >> 2)) / 2)) + 8 * (r16 & 3);
+            }
+        }
+        template <int U>
+        __device__ __forceinline__ u32x4v read(const uint8_t *lds, int t) const {
+            if constexpr (!TRANS) {
+                return *reinterpret_cast<const u32x4v *>(lds + at[U] + t * 2048);
+            } else if constexpr (sizeof(T) == 4) {
+                u32x4v v;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint32_t *>(lds + at[t] + (16 * U + j) * kPitch);
+                return v;
+            } else {
+                typedef __attribute__((address_space(3))) s16x4v Lds;
+                const u32x2v a = __builtin_bit_cast(
+                    u32x2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds *)(lds + at[t] + 32 * U * kPitch)));
+                const u32x2v b = __builtin_bit_cast(
+                    u32x2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds *)(lds + at[t] + (32 * U + 4) * kPitch)));
+                return u32x4v{a[0], a[1], b[0], b[1]};
+            }
+        }
+    };
+};
+
+// 64 pieces of 16 bytes to LDS.
+__device__ __forceinline__ void rows_dma(uint32_t off, uint64_t from, uint32_t lds) {
+    const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds);
+    // Five wait states: an SGPR that a VALU instruction wrote is not read by a load before, nor M0 in the
+    // next cycle, and the compiler does not count them for an asm statement.
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(from), "{m0}"(m0v) : "memory");
+}
+
+// DMA: the operands' memory rows are 16-byte aligned and a tile's offsets fit 32 bits; stages that end
+// inside themselves and every stage of other operands go through registers.
+template <class E, RowsMode MODE, class Tile, bool DMA>
+__global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
+    typedef typename E::type T;
+    constexpr int RT = Tile::RT, TT = Tile::TT, kStep = 128 / sizeof(T);
+    constexpr bool PT = MODE == kRowsInput || MODE == kRowsWeight, QT = MODE == kRowsWeight;
+    using OpP = RowsOperand<T, PT, Tile::kP, Tile::kThreads>;
+    using OpQ = RowsOperand<T, QT, Tile::kQ, Tile::kThreads>;
+    // SwiGLU: a wave's first columns are gate's, the other half up's of the same.
+    constexpr int kOutP = MODE == kRowsSwiglu ? Tile::kP / 2 : Tile::kP;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r16 = lane & 15, q4 = lane >> 4;
+    const int wp = wave % Tile::WP, wq = wave / Tile::WP;
+
+    // Workgroups go to the eight XCDs in turn: each takes a contiguous run of tiles, row tiles
+    // fastest, so that a tile of the matrix is read into one L2.
+    const int total = gridDim.x, per = total / 8, rest = total % 8;
+    const int xcd = blockIdx.x % 8;
+    int tile = xcd * per + min(xcd, rest) + (int)(blockIdx.x / 8);
+    int expert = 0, first = 0, end = p.Q, half = 0, q0, length = p.K;
+    if constexpr (MODE == kRowsWeight) {
+        const int each = p.tiles_p * p.tiles_q;
+        int first_row = 0;
+        if (p.offsets != nullptr) {
+            expert = tile / each, tile %= each;
+            first_row = min(max(p.offsets[expert], 0), p.M);
+            length = min(max(p.offsets[expert + 1], first_row), p.M) - first_row;
+        }
+        const int tiles_half = p.tiles_q / p.halves;
+        const int tile_q = tile % p.tiles_q;
+        half = tile_q / tiles_half;
+        q0 = tile_q % tiles_half * Tile::kQ;
+        first = first_row;
+    } else {
+        const int tile_q = tile % p.tiles_q;
+        q0 = tile_q * Tile::kQ;
+        if (p.offsets != nullptr && !mx_expert_tile(p.offsets, p.n_experts, p.M, Tile::kQ, tile_q, expert, q0, end))
+            return;
+    }
+    const int p0 = tile / p.tiles_q * kOutP;
+    const int rows_p = min(p.P - p0, kOutP), rows_q = min(end - q0, Tile::kQ);
+
+    // The operands from the tile's first row and the sums' first element on.
+    const T *const pm = (const T *)p.p + (MODE == kRowsWeight ? first * p.ldp + p0
+                                                              : expert * p.expert_stride + (PT ? p0 : p0 * p.ldp));
+    const T *const pm2 = MODE == kRowsWeight ? pm : (const T *)p.p2 + (pm - (const T *)p.p);
+    const T *const qm = (const T *)p.q + (QT ? first * p.ldq + (int64_t)half * p.Q + q0 : q0 * p.ldq);
+
+    const int stages_half = (length + kStep - 1) / kStep;
+    const int stages = MODE == kRowsInput ? p.halves * stages_half : stages_half;
+    const int s_beg = (int)((int64_t)stages * blockIdx.y / p.slices);
+    const int s_end = (int)((int64_t)stages * (blockIdx.y + 1) / p.slices);
+
+    // Row i of the P operand's part of a stage: of SwiGLU a wave's first 8 * RT are gate's, the others up's.
+    auto is_up = [&](int i) { return MODE == kRowsSwiglu && i % (16 * RT) >= 8 * RT; };
+    auto row_p = [&](int i) { return MODE == kRowsSwiglu ? i / (16 * RT) * (8 * RT) + i % (8 * RT) : i; };
+    uint32_t off_p[OpP::kMine], off_q[OpQ::kMine];
+    if constexpr (DMA) {
+        OpP::dma_offsets(off_p, wave, p.ldp, [&](int i) { return min(row_p(i), PT ? rows_p - OpP::kPiece : rows_p - 1); });
+        OpQ::dma_offsets(off_q, wave, p.ldq, [&](int i) { return min(i, QT ? rows_q - OpQ::kPiece : rows_q - 1); });
+    }
+    auto bring = [&](int st, int buffer) {
+        const bool second = MODE == kRowsInput && st >= stages_half;
+        const int k0 = (second ? st - stages_half : st) * kStep, left = length - k0;
+        uint8_t *const to = lds + buffer * Tile::kStage;
+        const T *const from_p = (second ? pm2 : pm) + (PT ? k0 * p.ldp : k0);
+        const T *const from_up = MODE == kRowsSwiglu ? pm2 + k0 : from_p;
+        const T *const from_q = qm + (QT ? k0 * p.ldq : (second ? p.K : 0) + (int64_t)k0);
+        if (DMA && left >= kStep) {
+            const uint32_t at = (uint32_t)(uintptr_t)to;
+#pragma unroll
+            for (int n = 0; n < OpP::kMine; ++n) {
+                const int run = wave * OpP::kMine + n;  // of SwiGLU 8 rows of one matrix
+                rows_dma(off_p[n], (uint64_t)(is_up(8 * run) ? from_up : from_p), at + 1024 * run);
+            }
+#pragma unroll
+            for (int n = 0; n < OpQ::kMine; ++n) {
+                const int run = wave * OpQ::kMine + n;
+                rows_dma(off_q[n], (uint64_t)from_q, at + Tile::kStageP + 1024 * run);
+            }
+        } else {
+            OpP::copy([&](int i, int k, int &have) {
+                const int row = row_p(i);
+                have = PT ? (k < left ? rows_p - row : 0) : (row < rows_p ? left - k : 0);
+                return (is_up(i) ? from_up : from_p) + OpP::offset(row, k, p.ldp);
+            }, to);
+            OpQ::copy([&](int i, int k, int &have) {
+                have = QT ? (k < left ? rows_q - i : 0) : (i < rows_q ? left - k : 0);
+                return from_q + OpQ::offset(i, k, p.ldq);
+            }, to + Tile::kStageP);
+        }
+    };
+
+    f32x4v acc[RT][TT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = f32x4v{0.f, 0.f, 0.f, 0.f};
+
+    const typename OpP::template Reader<RT> read_p(16 * RT * wp);
+    const typename OpQ::template Reader<TT> read_q(16 * TT * wq);
+    if (s_beg < s_end) bring(s_beg, 0);
+    for (int st = s_beg; st < s_end; ++st) {
+        const int buffer = (st - s_beg) & 1;
+        // Stage st has landed, and no wave reads the other buffer any more.
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (st + 1 < s_end) bring(st + 1, buffer ^ 1);
+        const uint8_t *const in_p = lds + buffer * Tile::kStage, *const in_q = in_p + Tile::kStageP;
+        auto step = [&](auto u_tag) {
+            constexpr int U = decltype(u_tag)::value;
+            u32x4v a[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) a[rt] = read_p.template read<U>(in_p, rt);
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) {
+                const u32x4v b = read_q.template read<U>(in_q, tt);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) acc[rt][tt] = rows_mfma<T>(a[rt], b, acc[rt][tt]);
+            }
+        };
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+    }
+    __syncthreads();  // no wave reads a stage any more
+
+    // ---- outputs: 16 rows at a time through the wave's own LDS, read back 8 columns a lane
+    uint8_t *const stage = lds + wave * (16 * Tile::kOutPitch);
+    constexpr int kChunks = (MODE == kRowsSwiglu ? RT : 2 * RT), kAtOnce = 64 / kChunks;
+    const int chunk = lane % kChunks;
+    const int col = p0 + wp * 8 * kChunks + 8 * chunk, n = min(8, p.P - col);
+    const bool parts = p.slices > 1;
+    void *const y = MODE == kRowsWeight ? (void *)((uint8_t *)(half == 0 ? p.y : p.y2) +
+                                                   expert * p.expert_stride * (p.wide ? 4 : sizeof(T)))
+                                        : p.y;
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+            *reinterpret_cast<f32x4v *>(stage + r16 * Tile::kOutPitch + 64 * rt + 16 * q4) = acc[rt][tt];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < (16 + kAtOnce - 1) / kAtOnce; ++k) {
+            const int r = kAtOnce * k + lane / kChunks, in_tile = 16 * (TT * wq + tt) + r;
+            if (r < 16 && in_tile < rows_q && n > 0) {
+                float v[8], up[8];
+                auto take = [&](float *to, int at) {
+                    const f32x4v *const from = reinterpret_cast<const f32x4v *>(stage + r * Tile::kOutPitch + 32 * at);
+                    const f32x4v a = from[0], b = from[1];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) to[i] = a[i], to[4 + i] = b[i];
+                };
+                take(v, chunk);
+                if constexpr (MODE == kRowsSwiglu) take(up, RT + chunk);
+                const int64_t row = q0 + in_tile;
+                if (parts) {
+                    const int64_t cols = MODE == kRowsSwiglu ? 2 * (int64_t)p.P : p.P;
+                    // A slice's rows: of weight those of all matrices.
+                    const int64_t all = MODE == kRowsWeight ? (int64_t)p.Q * p.halves * max(p.n_experts, 1) : p.Q;
+                    const int64_t mine = MODE == kRowsWeight ? ((int64_t)half * max(p.n_experts, 1) + expert) * p.Q + row
+                                                             : row;
+                    float *const to = p.part + (blockIdx.y * all + mine) * cols + col;
+                    rows_store8(to, n, v);
+                    if constexpr (MODE == kRowsSwiglu) rows_store8(to + p.P, n, up);
+                } else if constexpr (MODE == kRowsSwiglu) {
+                    rows_finish_swiglu<T>(p.epi, v, up, row, col, n, p.P, y);
+                } else {
+                    rows_finish<T>(p.epi, v, row, col, n, p.P, y, p.ldy, p.wide);
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <class E, RowsMode MODE, class Tile, bool DMA>
+hipError_t run_rows(RowsMm p, hipStream_t stream) {
+    constexpr int kOutP = MODE == kRowsSwiglu ? Tile::kP / 2 : Tile::kP;
+    p.tiles_p = (p.P + kOutP - 1) / kOutP;
+    p.tiles_q = (p.Q + Tile::kQ - 1) / Tile::kQ;
+    int64_t wgs;
+    if (MODE == kRowsWeight) {
+        p.tiles_q *= p.halves;
+        wgs = (int64_t)p.tiles_p * p.tiles_q * (p.offsets != nullptr ? p.n_experts : 1);
+        if ((int64_t)p.tiles_p * p.tiles_q > INT32_MAX) return hipErrorInvalidConfiguration;
+    } else {
+        if (p.offsets != nullptr) p.tiles_q += std::min(p.n_experts, p.M);
+        wgs = (int64_t)p.tiles_p * p.tiles_q;
+    }
+    if (wgs * Tile::kThreads >= 1LL << 32) return hipErrorInvalidConfiguration;
+    const auto kernel = rows_mm_kernel<E, MODE, Tile, DMA>;
+    const hipError_t e = ensure_dynamic_lds((const void *)kernel, Tile::kLds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)wgs, (unsigned)p.slices), dim3(Tile::kThreads), Tile::kLds, stream, p);
+    return hipGetLastError();
+}
+
+// DMA where every memory row of both operands is 16-byte aligned, a tile's rows and a stage's elements
+// are within 4 GiB of its first, and (where rows of an element are contiguous) rows come in whole pieces.
+inline bool rows_dma_accepts(RowsMode mode, int es, const RowsMm &p) {
+    const int piece = 16 / es;
+    auto fits = [&](const void *m, int64_t ld) {
+        return (uintptr_t)m % 16 == 0 && ld % piece == 0 && ld * es < (1LL << 32) / 512;
+    };
+    if (!fits(p.p, p.ldp) || !fits(p.q, p.ldq)) return false;
+    if (p.p2 != nullptr && !fits(p.p2, p.ldp)) return false;
+    if (mode == kRowsInput) return p.P % piece == 0 && (p.halves == 1 || p.K % piece == 0);
+    if (mode == kRowsWeight) return p.P % piece == 0 && p.Q % piece == 0;
+    return true;
+}
+
+template <class E, RowsMode MODE>
+hipError_t rows_by_tile(const RowsMm &p, int tile, hipStream_t stream) {
+    if (!rows_dma_accepts(MODE, (int)sizeof(typename E::type), p)) return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, false>(p, stream);
+    switch (tile) {
+        case 0: return run_rows<E, MODE, RowsTile<2, 2, 2, 2>, true>(p, stream);
+        case 1: return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, true>(p, stream);
+    }
+    return run_rows<E, MODE, RowsTile<8, 4, 2, 4>, true>(p, stream);
+}
+
+}  // namespace
+
+template <class E>
+hipError_t rows_mm_tiles(RowsMode mode, const RowsMm &p, int tile, hipStream_t stream) {
+    switch (mode) {
+        case kRowsForward: return rows_by_tile<E, kRowsForward>(p, tile, stream);
+        case kRowsSwiglu: return rows_by_tile<E, kRowsSwiglu>(p, tile, stream);
+        case kRowsInput: return rows_by_tile<E, kRowsInput>(p, tile, stream);
+        case kRowsWeight: return rows_by_tile<E, kRowsWeight>(p, tile, stream);
+    }
+    return hipErrorInvalidValue;
+}
+
+}  // namespace jjo
