@@ -609,7 +609,8 @@ int moe_combine_rows_backward_device(void *stream, const void *grad_y, const voi
  * (moe_dispatch_rows_device and moe_combine_rows_device above move the rows) and gate|up with SwiGLU, each
  * with its gradients.
  * All operands of a call are of `dtype` unless it says otherwise; sums are fp32, each result is rounded
- * once, and the gradient through an activation is rounded to `dtype` before it is multiplied.
+ * once.  The gradient through an activation is rounded to `dtype` before it is multiplied; for weights'
+ * gradients in fp32 what that rounding left is multiplied as well (twice the work).
  * Sums are added in an order that depends on the sizes alone.  Buffers are aligned to
  * their elements; where rows are 16-byte aligned as well the products are faster.  Sizes (in, out, rows) are
  * positive, any other number up to 2^28, a matrix has at most 2^40 elements.  Row strides are in
@@ -694,6 +695,19 @@ int moe_rows_gate_up_swiglu_backward_device(void *stream, const void *grad_mid, 
                                             void *grad_w_gate, void *grad_w_up, int dtype, int grad_weights_dtype,
                                             int hidden_size, int intermediate_size, int n_routes, void *workspace,
                                             int64_t workspace_bytes);
+
+/*
+ * One product on a given kernel (measurements and tests), no epilogue, contiguous operands of `dtype`.
+ * form 0: y [rows][cols] = q [rows][sums] . p [cols][sums]^T; 1: SwiGLU, p gate and p2 up; 2: y = q
+ * [rows][sums] . p [sums][cols] (p2 not NULL: q [rows][2 sums], its second half times p2 is added); 3: y
+ * [rows][cols] = q [sums][rows]^T . p [sums][cols] (y2 not NULL: q [sums][2 rows], the second half's
+ * rows go to y2).  expert_offsets NULL, or of sorted rows (forms 0 to 2) or of the sums (3).  kernel: 0 to 2
+ * the LDS tiles, 64 + w and 80 + w (forms 0 and 1) the direct kernel on w <= 8 waves with one or two
+ * tiles of 16 rows.  slices of the sums, each 4 bytes an output of the workspace where more than one.
+ */
+int jjo_rows_kernel_device(void *stream, int form, int kernel, int slices, int dtype, const void *p, const void *p2,
+                           const void *q, const int32_t *expert_offsets, int n_experts, void *y, void *y2, int cols,
+                           int rows, int sums, void *workspace, int64_t workspace_bytes);
 
 #ifdef __cplusplus
 }

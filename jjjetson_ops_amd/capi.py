@@ -108,6 +108,7 @@ EXPORTED_SYMBOLS = (
     "moe_rows_gate_up_swiglu_device",
     "moe_rows_gate_up_swiglu_backward_workspace_bytes",
     "moe_rows_gate_up_swiglu_backward_device",
+    "jjo_rows_kernel_device",
 )
 
 DTYPE_F32 = 0
@@ -282,6 +283,8 @@ def lib() -> ctypes.CDLL:
         L.moe_combine_rows_device.argtypes = [vp, vp, i32, vp, vp, vp, i32, i32, i32]
         L.moe_combine_rows_backward_device.restype = i32
         L.moe_combine_rows_backward_device.argtypes = [vp, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32]
+        L.jjo_rows_kernel_device.restype = i32
+        L.jjo_rows_kernel_device.argtypes = [vp, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp, vp, i32, i32, i32, vp, i64]
         for name in ("linear_rows", "linear_rows_backward"):
             f = getattr(L, name + "_workspace_bytes")
             f.restype, f.argtypes = i64, [i32, i32, i32, i32]
@@ -1055,3 +1058,24 @@ def moe_gate_up_swiglu_rows_backward(grad_mid, gate_up, x, w_gate, w_up, expert_
     _entry(_ROWS_GATE_UP_BACKWARD, "moe_rows_gate_up_swiglu_backward_device", stream, grad_mid, gate_up, x, w_gate,
            w_up, expert_offsets, num_experts, grad_x, grad_w_gate, grad_w_up, d, gd, hidden, inter, n_routes, ws,
            _bytes_of(ws))
+
+
+ROWS_FORWARD, ROWS_SWIGLU, ROWS_INPUT, ROWS_WEIGHT = range(4)
+ROWS_DIRECT = 64  # + 16 * (tiles of 16 rows - 1) + waves
+
+
+def rows_kernel(form: int, kernel: int, p, q, y, cols: int, rows: int, sums: int, p2=None, y2=None, offsets=None,
+                slices: int = 1, ws=None, stream=None) -> None:
+    """jjo_rows_kernel_device: one product of float matrices on a given kernel (measurements and tests)."""
+    d = _dtype(p, "p")
+    halves = 2 if (p2 if form == ROWS_INPUT else y2) is not None else 1
+    E = 1 if offsets is None else offsets.numel() - 1
+    weights = 1 if form == ROWS_WEIGHT else E
+    for name, t, n in (("p", p, weights * cols * sums), ("p2", p2, weights * cols * sums), ("q", q, halves * rows * sums),
+                       ("y", y, (E if form == ROWS_WEIGHT else 1) * rows * cols),
+                       ("y2", y2, (E if form == ROWS_WEIGHT else 1) * rows * cols)):
+        _optional(t, name, d, n)
+    _check(lib().jjo_rows_kernel_device(
+        _stream(stream), form, kernel, slices, d, *(None if t is None else _dev(t, "an operand") for t in (p, p2, q, offsets)),
+        E, *(None if t is None else _dev(t, "an output") for t in (y, y2)), cols, rows, sums,
+        None if ws is None else _dev(ws, "ws"), _bytes_of(ws)), "jjo_rows_kernel_device")

@@ -78,7 +78,7 @@ int64_t stride_of(int64_t stride, int cols, int rows) { return rows > 1 ? stride
 // ---- the products, without pointers to the operands
 RowsMm product(RowsMode mode, int dtype, int P, int Q, int K, int halves, int n_experts) {
     RowsMm m{};
-    m.P = P, m.Q = Q, m.K = K, m.halves = halves;
+    m.P = P, m.Q = Q, m.K = K, m.halves = halves, m.terms = 1;
     m.n_experts = n_experts;
     m.M = mode == kRowsWeight ? K : Q;
     m.slices = rows_mm_slices(mode, dtype, P, Q, K, halves, n_experts, m.M);
@@ -109,12 +109,18 @@ RowsMm weight(int dtype, int K, int N, int rows, int n_experts, int halves, bool
     return m;
 }
 
+// The gradient through an activation in 16 bits, and where the weights' gradients are fp32 what that rounding
+// left, in 16 bits again: the sums of both are those of a gradient of 16 (bf16) or 22 bits (fp16).
+int64_t gz_bytes(int dtype, int64_t values) { return up256(elem_bytes(dtype) * values); }
+int64_t gz_planes(int dtype) { return dtype == JJO_DTYPE_F32 ? 1 : 2; }
+
 struct LinearBackwardWs {
-    int64_t gz, columns, parts, bytes;  // offsets
+    int64_t gz, rest, columns, parts, bytes;  // offsets
 };
 LinearBackwardWs linear_backward_ws(int dtype, int K, int N, int T) {
     LinearBackwardWs w{};
-    w.columns = up256((int64_t)elem_bytes(dtype) * T * N);
+    w.rest = gz_bytes(dtype, (int64_t)T * N);
+    w.columns = gz_planes(dtype) * w.rest;
     w.parts = w.columns + up256(4LL * rows_column_chunks(T, N) * N);
     w.bytes = w.parts + up256(std::max(rows_part_bytes(kRowsInput, input(dtype, K, N, T, 0, 1)),
                                        rows_part_bytes(kRowsWeight, weight(dtype, K, N, T, 0, 1, false))));
@@ -206,9 +212,10 @@ int linear_rows_backward_device(void *stream, const void *grad_y, int64_t grad_y
     uint8_t *const base = (uint8_t *)workspace;
     const void *gz = grad_y;
     int64_t gz_stride = stride_of(grad_y_stride, N, T);
+    void *const rest = act && wide && dtype != JJO_DTYPE_F32 && grad_weight != nullptr ? base + ws.rest : nullptr;
     if (act || grad_bias != nullptr) {
-        const hipError_t e = launch_rows_act_backward(grad_y, gz_stride, pre, base + ws.gz, dtype, activation, grad_bias,
-                                                      wide, (float *)(base + ws.columns), T, N, s);
+        const hipError_t e = launch_rows_act_backward(grad_y, gz_stride, pre, base + ws.gz, rest, dtype, activation,
+                                                      grad_bias, wide, (float *)(base + ws.columns), T, N, s);
         if (e != hipSuccess) return launched(e, "linear_rows_backward activation");
         if (act) gz = base + ws.gz, gz_stride = N;
     }
@@ -222,6 +229,7 @@ int linear_rows_backward_device(void *stream, const void *grad_y, int64_t grad_y
     if (grad_weight != nullptr) {
         RowsMm m = weight(dtype, K, N, T, 0, 1, wide);
         m.p = x, m.ldp = stride_of(x_stride, K, T), m.q = gz, m.ldq = gz_stride, m.y = grad_weight;
+        if (rest != nullptr) m.q2 = rest, m.terms = 2;
         m.part = (float *)(base + ws.parts);
         const hipError_t e = launch_rows_mm(kRowsWeight, dtype, m, s);
         if (e != hipSuccess) return launched(e, "linear_rows_backward weight");
@@ -333,7 +341,7 @@ int64_t moe_rows_gate_up_swiglu_backward_workspace_bytes(int dtype, int hidden_s
     if (check_sizes("moe_rows_gate_up_swiglu_backward", dtype, hidden_size, intermediate_size, n_routes, num_experts) !=
         JJO_OK)
         return -1;
-    return up256(2LL * elem_bytes(dtype) * n_routes * intermediate_size) +
+    return gz_planes(dtype) * gz_bytes(dtype, 2LL * n_routes * intermediate_size) +
            grouped_backward_bytes(dtype, hidden_size, intermediate_size, n_routes, num_experts, 2);
 }
 
@@ -366,9 +374,11 @@ int moe_rows_gate_up_swiglu_backward_device(void *stream, const void *grad_mid, 
                             moe_rows_gate_up_swiglu_backward_workspace_bytes(dtype, H, I, R, E)));
     JJO_TRY(require_device());
     hipStream_t s = (hipStream_t)stream;
-    void *const gz = workspace;
-    float *const part = (float *)((uint8_t *)workspace + up256(2LL * es * R * I));
-    hipError_t e = launch_rows_swiglu_backward(grad_mid, gate_up, gz, dtype, expert_offsets, E, I, R, s);
+    uint8_t *const gz = (uint8_t *)workspace;
+    const int64_t plane = gz_bytes(dtype, 2LL * R * I);
+    void *const rest = grad_weights_dtype != dtype && grad_w_gate != nullptr ? gz + plane : nullptr;
+    float *const part = (float *)(gz + gz_planes(dtype) * plane);
+    hipError_t e = launch_rows_swiglu_backward(grad_mid, gate_up, gz, rest, dtype, expert_offsets, E, I, R, s);
     if (e != hipSuccess) return launched(e, "moe_rows_gate_up_swiglu_backward activation");
     if (grad_x_sorted != nullptr) {
         RowsMm m = input(dtype, H, I, R, E, 2);
@@ -379,10 +389,42 @@ int moe_rows_gate_up_swiglu_backward_device(void *stream, const void *grad_mid, 
     if (grad_w_gate != nullptr) {
         RowsMm m = weight(dtype, H, I, R, E, 2, grad_weights_dtype == JJO_DTYPE_F32);
         m.p = x_sorted, m.q = gz, m.y = grad_w_gate, m.y2 = grad_w_up, m.offsets = expert_offsets, m.part = part;
+        if (rest != nullptr) m.q2 = rest, m.terms = 2;
         if ((e = launch_rows_mm(kRowsWeight, dtype, m, s)) != hipSuccess)
             return launched(e, "moe_rows_gate_up_swiglu_backward weights");
     }
     return JJO_OK;
+}
+
+int jjo_rows_kernel_device(void *stream, int form, int kernel, int slices, int dtype, const void *p, const void *p2,
+                           const void *q, const int32_t *expert_offsets, int n_experts, void *y, void *y2, int cols,
+                           int rows, int sums, void *workspace, int64_t workspace_bytes) {
+    clear_error();
+    const char *who = "jjo_rows_kernel";
+    JJO_TRY(check_sizes(who, dtype, cols, sums, rows, expert_offsets != nullptr ? n_experts : 1));
+    const int es = elem_bytes(dtype), halves = (form == kRowsInput ? (const void *)p2 : y2) != nullptr ? 2 : 1;
+    const int waves = kernel >= 64 ? kernel % 16 : 0, tiles16 = kernel >= 64 ? kernel / 16 - 3 : 0;
+    const bool direct = kernel >= 64;
+    if (form < kRowsForward || form > kRowsWeight || slices < 1 || slices > 64 || kernel < 0 ||
+        (direct ? form > kRowsSwiglu || slices != 1 || tiles16 > 2 || waves < 1 || waves > 8 : kernel >= kRowsTiles))
+        return set_error(JJO_ERR_INVALID_ARG, "%s: form %d has no kernel %d in %d slices", who, form, kernel, slices);
+    JJO_TRY(check_ptr(who, "p", p, es));
+    JJO_TRY(check_ptr(who, "p2", p2, es, form != kRowsSwiglu));
+    JJO_TRY(check_ptr(who, "q", q, es));
+    JJO_TRY(check_ptr(who, "expert_offsets", expert_offsets, 4, true));
+    JJO_TRY(check_ptr(who, "y", y, es));
+    JJO_TRY(check_ptr(who, "y2", y2, es, true));
+    const int E = expert_offsets != nullptr ? n_experts : 0;
+    RowsMm m = form == kRowsForward  ? forward(dtype, sums, cols, rows, E)
+               : form == kRowsSwiglu ? swiglu(dtype, sums, cols, rows, E)
+               : form == kRowsInput  ? input(dtype, cols, sums, rows, E, halves)
+                                     : weight(dtype, cols, rows, sums, E, halves, false);
+    m.slices = slices;
+    JJO_TRY(check_workspace(who, workspace, workspace_bytes, rows_part_bytes((RowsMode)form, m)));
+    JJO_TRY(require_device());
+    m.p = p, m.p2 = p2, m.q = q, m.y = y, m.y2 = y2, m.offsets = expert_offsets, m.part = (float *)workspace;
+    const RowsChoice choice{direct ? -tiles16 : kernel, waves};
+    return launched(launch_rows_mm((RowsMode)form, dtype, m, (hipStream_t)stream, &choice), "jjo_rows_kernel launch");
 }
 
 }  // extern "C"

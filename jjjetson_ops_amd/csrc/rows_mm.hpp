@@ -26,12 +26,13 @@ struct RowsEpilogue {
 // are contiguous (forward), or the rows' of an element are (weight; input: of P).
 struct RowsMm {
     const void *p, *p2;  // p2: the up matrix (SwiGLU), or the operand of the sums' second half (input)
-    const void *q;
+    const void *q, *q2;  // q2: what is left of q's values behind their rounding (weight, terms 2)
     int64_t ldp, ldq;  // elements from one memory row to the next
     void *y, *y2;      // y2: of the second half's output rows (weight)
     int64_t ldy;
     int P, Q, K;
     int halves;              // 2: input sums over p, then over p2; weight has rows of y, then of y2
+    int terms;               // of q in a weight's sums: 1, or 2 (q, then q2)
     const int32_t *offsets;  // [n_experts + 1], or nullptr
     int n_experts, M;        // M: sorted rows
     int64_t expert_stride;   // elements of a matrix (of an expert's part of y: weight)
@@ -144,22 +145,31 @@ __device__ __forceinline__ void rows_finish_swiglu(const RowsEpilogue &e, float 
 }
 
 // ---- launchers (asynchronous; arguments validated by the entries)
-hipError_t launch_rows_mm(RowsMode mode, int dtype, const RowsMm &p, hipStream_t stream);
+struct RowsChoice;
+hipError_t launch_rows_mm(RowsMode mode, int dtype, const RowsMm &p, hipStream_t stream,
+                          const RowsChoice *pinned = nullptr);
 // Slices that launch_rows_mm is best given for a product, and the bytes of their sums.
 int rows_mm_slices(RowsMode mode, int dtype, int P, int Q, int K, int halves, int n_experts, int M);
 int64_t rows_part_bytes(RowsMode mode, const RowsMm &p);
 
-template <class E>
-hipError_t rows_mm_tiles(RowsMode mode, const RowsMm &p, int tile, hipStream_t stream);
 
-// gz[t] = grad_y[t] * act'(pre[t]) (act none: not written) and the columns' sums of gz (sums nullable;
+// The kernel for a product: an LDS tile (>= 0), or the direct kernel with one (-1) or two (-2) tiles of 16
+// rows and so many waves that cut K between them.
+struct RowsChoice {
+    int tile, waves;
+};
+constexpr int kRowsTiles = 10;
+template <class E>
+hipError_t rows_mm_run(RowsMode mode, const RowsMm &p, const RowsChoice &c, hipStream_t stream);
+
+// gz[t] = grad_y[t] * act'(pre[t]) (act none: not written; rest, where not null: what its rounding left) and the columns' sums of gz (sums nullable;
 // column_part: rows_column_chunks(T, N) * N floats).
 int rows_column_chunks(int T, int N);
-hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, const void *pre, void *gz, int dtype,
-                                    int act, void *sums, bool sums_wide, float *column_part, int T, int N,
+hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, const void *pre, void *gz, void *rest,
+                                    int dtype, int act, void *sums, bool sums_wide, float *column_part, int T, int N,
                                     hipStream_t stream);
 // grad_gate_up [R][2I] from grad_mid and the saved gate|up, rows below offsets[n_experts].
-hipError_t launch_rows_swiglu_backward(const void *grad_mid, const void *gate_up, void *grad_gate_up, int dtype,
+hipError_t launch_rows_swiglu_backward(const void *grad_mid, const void *gate_up, void *grad_gate_up, void *rest, int dtype,
                                        const int32_t *offsets, int n_experts, int I, int R, hipStream_t stream);
 
 }  // namespace jjo

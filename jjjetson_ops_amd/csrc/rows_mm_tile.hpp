@@ -39,15 +39,15 @@ __device__ __forceinline__ f32x4v rows_mfma(u32x4v p, u32x4v q, f32x4v acc) {
     }
 }
 
-// WP x WQ waves of RT tiles of 16 output columns x TT tiles of 16 output rows each.
-template <int RT_, int TT_, int WP_, int WQ_>
+// WP x WQ waves of RT tiles of 16 output columns x TT tiles of 16 output rows each, NB stages in LDS.
+template <int RT_, int TT_, int WP_, int WQ_, int NB_ = 2>
 struct RowsTile {
-    static constexpr int RT = RT_, TT = TT_, WP = WP_, WQ = WQ_;
+    static constexpr int RT = RT_, TT = TT_, WP = WP_, WQ = WQ_, NB = NB_;
     static constexpr int kWaves = WP * WQ, kThreads = 64 * kWaves;
     static constexpr int kP = 16 * RT * WP, kQ = 16 * TT * WQ;
     static constexpr int kStageP = kP * 128, kStageQ = kQ * 128, kStage = kStageP + kStageQ;
     static constexpr int kOutPitch = 16 * RT * 4 + 16;  // a row of outputs in LDS: + 4 banks
-    static constexpr int kLds = std::max(2 * kStage, kWaves * 16 * kOutPitch);
+    static constexpr int kLds = std::max(NB * kStage, kWaves * 16 * kOutPitch);
     static_assert(kLds <= 160 * 1024, "LDS of a CU");
 };
 
@@ -57,8 +57,8 @@ struct RowsOperand {
     static constexpr int kPiece = 16 / sizeof(T), kStep = 128 / sizeof(T);
     static constexpr int kPitch = TRANS ? ROWS * (int)sizeof(T) : 128;  // bytes of an LDS row
     static constexpr int kRowPieces = kPitch / 16;
-    static constexpr int kMine = ROWS * 8 / THREADS;
-    static_assert(ROWS * 8 % THREADS == 0, "whole pieces a thread");
+    static constexpr int kRuns = ROWS / 8, kWaves = THREADS / 64;  // of 64 pieces: a DMA instruction's
+    static constexpr int kMine = (kRuns + kWaves - 1) / kWaves;    // of a wave
     static_assert(!TRANS || ROWS % 128 == 0 || ROWS == 64, "the permutations below");
 
     // The permutation of element k's pieces (of 16 bits: pairs, 16 rows each; of 32: fours).
@@ -73,6 +73,10 @@ struct RowsOperand {
         if constexpr (TRANS) k = line, i = (place ^ swizzle(line)) * kPiece;
         else i = line, k = (place ^ ((line >> 1) & 7)) * kPiece;
     }
+    // A wave's n-th run; the last one again where they do not divide.
+    static __device__ __forceinline__ int run(int wave, int n) {
+        return kRuns % kWaves == 0 ? wave * kMine + n : min(wave * kMine + n, kRuns - 1);
+    }
     static __device__ __forceinline__ int64_t offset(int i, int k, int64_t ld) {
         return TRANS ? k * ld + i : i * ld + k;
     }
@@ -82,10 +86,12 @@ struct RowsOperand {
     template <class F>
     static __device__ __forceinline__ void copy(F from, uint8_t *lds) {
         u32x4v v[kMine];
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));  // one stage of many comes this way: no addresses kept in registers for it
 #pragma unroll
         for (int n = 0; n < kMine; ++n) {
             int i, k, have;
-            piece(n * THREADS + threadIdx.x, i, k);
+            piece(64 * run(tid >> 6, n) + (tid & 63), i, k);
             const T *const at = from(i, k, have);
             v[n] = u32x4v{0u, 0u, 0u, 0u};
             if (have >= kPiece) {
@@ -98,7 +104,8 @@ struct RowsOperand {
             }
         }
 #pragma unroll
-        for (int n = 0; n < kMine; ++n) *reinterpret_cast<u32x4v *>(lds + 16 * (n * THREADS + threadIdx.x)) = v[n];
+        for (int n = 0; n < kMine; ++n)
+            *reinterpret_cast<u32x4v *>(lds + 16 * (64 * run(tid >> 6, n) + (tid & 63))) = v[n];
     }
 
     // ---- by DMA, 64 pieces an instruction: a lane's offsets; rows behind the last are the last again.
@@ -107,29 +114,25 @@ struct RowsOperand {
 #pragma unroll
         for (int n = 0; n < kMine; ++n) {
             int i, k;
-            piece((wave * kMine + n) * 64 + (threadIdx.x & 63), i, k);
+            piece(64 * run(wave, n) + (threadIdx.x & 63), i, k);
             off[n] = (uint32_t)(offset(row(i), k, ld) * sizeof(T));
         }
     }
 
     // ---- a lane's 16 bytes of a step's operand, rows base + 16 * t + lane % 16
-    template <int TILES>
+    // (base a multiple of 16 times the tiles that are read from it; those are a power of two where TRANS).
     struct Reader {
-        static constexpr int kAddresses = TRANS ? TILES : 2;
-        uint32_t at[kAddresses];
+        uint32_t at[TRANS ? 1 : 2];
         __device__ __forceinline__ explicit Reader(int base) {
             const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
             if constexpr (!TRANS) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) at[u] = (base + r16) * 128 + 16 * ((4 * u + q) ^ (r16 >> 1));
             } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                for (int t = 0; t < TILES; ++t) at[t] = 4 * q * kPitch + 64 * ((base / 16 + t) ^ q) + 4 * r16;
+                at[0] = 4 * q * kPitch + 64 * ((base / 16) ^ q) + 4 * r16;
             } else {
-#pragma unroll
-                for (int t = 0; t < TILES; ++t)
-                    at[t] = (8 * q + (r16 >> 2)) * kPitch +
-                            32 * ((base / 16 + t) ^ (swizzle(8 * q + (r16 >> 2)) / 2)) + 8 * (r16 & 3);
+                at[0] = (8 * q + (r16 >> 2)) * kPitch + 32 * ((base / 16) ^ (swizzle(8 * q + (r16 >> 2)) / 2)) +
+                        8 * (r16 & 3);
             }
         }
         template <int U>
@@ -137,16 +140,17 @@ struct RowsOperand {
             if constexpr (!TRANS) {
                 return *reinterpret_cast<const u32x4v *>(lds + at[U] + t * 2048);
             } else if constexpr (sizeof(T) == 4) {
+                const uint8_t *const from = lds + (at[0] ^ (64 * t));
                 u32x4v v;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint32_t *>(lds + at[t] + (16 * U + j) * kPitch);
+                for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint32_t *>(from + (16 * U + j) * kPitch);
                 return v;
             } else {
                 typedef __attribute__((address_space(3))) s16x4v Lds;
-                const u32x2v a = __builtin_bit_cast(
-                    u32x2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds *)(lds + at[t] + 32 * U * kPitch)));
-                const u32x2v b = __builtin_bit_cast(
-                    u32x2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds *)(lds + at[t] + (32 * U + 4) * kPitch)));
+                const uint8_t *const from = lds + (at[0] ^ (32 * t)) + 32 * U * kPitch;
+                const u32x2v a = __builtin_bit_cast(u32x2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds *)from));
+                const u32x2v b =
+                    __builtin_bit_cast(u32x2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds *)(from + 4 * kPitch)));
                 return u32x4v{a[0], a[1], b[0], b[1]};
             }
         }
@@ -156,9 +160,63 @@ struct RowsOperand {
 // 64 pieces of 16 bytes to LDS.
 __device__ __forceinline__ void rows_dma(uint32_t off, uint64_t from, uint32_t lds) {
     const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds);
+    from = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(from >> 32)) << 32 |
+           (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)from);
     // Five wait states: an SGPR that a VALU instruction wrote is not read by a load before, nor M0 in the
     // next cycle, and the compiler does not count them for an asm statement.
     asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(from), "{m0}"(m0v) : "memory");
+}
+
+// Workgroups go to the eight XCDs in turn: each takes a contiguous run of `total` tiles, so that tiles
+// that read the same rows follow each other in one L2.  -1 behind the last.
+__device__ __forceinline__ int rows_xcd_run(int block, int total) {
+    const int per = total / 8, rest = total % 8, xcd = block % 8, at = block / 8;
+    return at < per + (xcd < rest) ? xcd * per + min(xcd, rest) + at : -1;
+}
+
+// The workgroup's tile of `rows` sorted rows x one of tiles_p of their expert's columns: expert by expert, its
+// row tiles fastest; false behind the last.  Ranges are clamped to [0, M], so a malformed table
+// drops rows instead of leaving the buffers.  All lanes of a wave call it together.
+__device__ __forceinline__ bool rows_expert_tile(const int32_t *__restrict__ offsets, int n_experts, int M, int rows,
+                                                 int tiles_p, int &expert, int &first, int &end, int &tile_p) {
+    const int lane = threadIdx.x & 63;
+    int beg = 0, fin = 0, incl = 0, mine = 0, total = 0;
+    auto count = [&](int e0) {
+        const int e = e0 + lane;
+        beg = fin = 0;
+        if (e < n_experts) {
+            beg = min(max(offsets[e], 0), M);
+            fin = min(max(offsets[e + 1], beg), M);
+        }
+        mine = (fin - beg + rows - 1) / rows;
+        incl = mx_scan(mine);
+    };
+    for (int e0 = 0; e0 < n_experts; e0 += 64) {
+        count(e0);
+        total += __builtin_amdgcn_readlane(incl, 63);
+    }
+    const int64_t all = (int64_t)total * tiles_p;
+    if (all > gridDim.x) return false;  // only the sums of a malformed table
+    const int tile = rows_xcd_run(blockIdx.x, (int)all);
+    if (tile < 0) return false;
+    int base = 0;
+    for (int e0 = 0; e0 < n_experts; e0 += 64) {
+        if (n_experts > 64) count(e0);
+        const uint64_t past = __ballot((int64_t)(base + incl) * tiles_p > tile);
+        if (past != 0) {
+            const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
+            const int tiles = __builtin_amdgcn_readlane(mine, l);
+            const int local = tile - (base + __builtin_amdgcn_readlane(incl, l) - tiles) * tiles_p;
+            if (tiles <= 0 || local < 0) return false;
+            expert = e0 + l;
+            first = __builtin_amdgcn_readlane(beg, l) + local % tiles * rows;
+            end = __builtin_amdgcn_readlane(fin, l);
+            tile_p = local / tiles;
+            return first < end && tile_p < tiles_p;
+        }
+        base += __builtin_amdgcn_readlane(incl, 63);
+    }
+    return false;
 }
 
 // DMA: the operands' memory rows are 16-byte aligned and a tile's offsets fit 32 bits; stages that end
@@ -177,32 +235,27 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
     const int r16 = lane & 15, q4 = lane >> 4;
     const int wp = wave % Tile::WP, wq = wave / Tile::WP;
 
-    // Workgroups go to the eight XCDs in turn: each takes a contiguous run of tiles, row tiles
-    // fastest, so that a tile of the matrix is read into one L2.
-    const int total = gridDim.x, per = total / 8, rest = total % 8;
-    const int xcd = blockIdx.x % 8;
-    int tile = xcd * per + min(xcd, rest) + (int)(blockIdx.x / 8);
-    int expert = 0, first = 0, end = p.Q, half = 0, q0, length = p.K;
+    int expert = 0, first = 0, end = p.Q, half = 0, q0, tile_p, length = p.K;
     if constexpr (MODE == kRowsWeight) {
         const int each = p.tiles_p * p.tiles_q;
-        int first_row = 0;
+        int tile = rows_xcd_run(blockIdx.x, gridDim.x);
         if (p.offsets != nullptr) {
             expert = tile / each, tile %= each;
-            first_row = min(max(p.offsets[expert], 0), p.M);
-            length = min(max(p.offsets[expert + 1], first_row), p.M) - first_row;
+            first = min(max(p.offsets[expert], 0), p.M);
+            length = min(max(p.offsets[expert + 1], first), p.M) - first;
         }
-        const int tiles_half = p.tiles_q / p.halves;
-        const int tile_q = tile % p.tiles_q;
+        const int tiles_half = p.tiles_q / p.halves, tile_q = tile % p.tiles_q;
         half = tile_q / tiles_half;
         q0 = tile_q % tiles_half * Tile::kQ;
-        first = first_row;
-    } else {
-        const int tile_q = tile % p.tiles_q;
-        q0 = tile_q * Tile::kQ;
-        if (p.offsets != nullptr && !mx_expert_tile(p.offsets, p.n_experts, p.M, Tile::kQ, tile_q, expert, q0, end))
-            return;
+        tile_p = tile / p.tiles_q;
+    } else if (p.offsets == nullptr) {
+        const int tile = rows_xcd_run(blockIdx.x, gridDim.x);
+        q0 = tile % p.tiles_q * Tile::kQ;
+        tile_p = tile / p.tiles_q;
+    } else if (!rows_expert_tile(p.offsets, p.n_experts, p.M, Tile::kQ, p.tiles_p, expert, q0, end, tile_p)) {
+        return;
     }
-    const int p0 = tile / p.tiles_q * kOutP;
+    const int p0 = tile_p * kOutP;
     const int rows_p = min(p.P - p0, kOutP), rows_q = min(end - q0, Tile::kQ);
 
     // The operands from the tile's first row and the sums' first element on.
@@ -210,9 +263,10 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
                                                               : expert * p.expert_stride + (PT ? p0 : p0 * p.ldp));
     const T *const pm2 = MODE == kRowsWeight ? pm : (const T *)p.p2 + (pm - (const T *)p.p);
     const T *const qm = (const T *)p.q + (QT ? first * p.ldq + (int64_t)half * p.Q + q0 : q0 * p.ldq);
+    const T *const qm2 = MODE == kRowsWeight ? (const T *)p.q2 + (qm - (const T *)p.q) : qm;
 
     const int stages_half = (length + kStep - 1) / kStep;
-    const int stages = MODE == kRowsInput ? p.halves * stages_half : stages_half;
+    const int stages = MODE == kRowsInput ? p.halves * stages_half : MODE == kRowsWeight ? p.terms * stages_half : stages_half;
     const int s_beg = (int)((int64_t)stages * blockIdx.y / p.slices);
     const int s_end = (int)((int64_t)stages * (blockIdx.y + 1) / p.slices);
 
@@ -225,22 +279,23 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
         OpQ::dma_offsets(off_q, wave, p.ldq, [&](int i) { return min(i, QT ? rows_q - OpQ::kPiece : rows_q - 1); });
     }
     auto bring = [&](int st, int buffer) {
-        const bool second = MODE == kRowsInput && st >= stages_half;
+        const bool second = (MODE == kRowsInput || MODE == kRowsWeight) && st >= stages_half;
         const int k0 = (second ? st - stages_half : st) * kStep, left = length - k0;
         uint8_t *const to = lds + buffer * Tile::kStage;
         const T *const from_p = (second ? pm2 : pm) + (PT ? k0 * p.ldp : k0);
         const T *const from_up = MODE == kRowsSwiglu ? pm2 + k0 : from_p;
-        const T *const from_q = qm + (QT ? k0 * p.ldq : (second ? p.K : 0) + (int64_t)k0);
+        const T *const from_q = (MODE == kRowsWeight && second ? qm2 : qm) +
+                                (QT ? k0 * p.ldq : (second ? p.K : 0) + (int64_t)k0);
         if (DMA && left >= kStep) {
             const uint32_t at = (uint32_t)(uintptr_t)to;
 #pragma unroll
             for (int n = 0; n < OpP::kMine; ++n) {
-                const int run = wave * OpP::kMine + n;  // of SwiGLU 8 rows of one matrix
+                const int run = OpP::run(wave, n);  // of SwiGLU 8 rows of one matrix
                 rows_dma(off_p[n], (uint64_t)(is_up(8 * run) ? from_up : from_p), at + 1024 * run);
             }
 #pragma unroll
             for (int n = 0; n < OpQ::kMine; ++n) {
-                const int run = wave * OpQ::kMine + n;
+                const int run = OpQ::run(wave, n);
                 rows_dma(off_q[n], (uint64_t)from_q, at + Tile::kStageP + 1024 * run);
             }
         } else {
@@ -262,31 +317,84 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = f32x4v{0.f, 0.f, 0.f, 0.f};
 
-    const typename OpP::template Reader<RT> read_p(16 * RT * wp);
-    const typename OpQ::template Reader<TT> read_q(16 * TT * wq);
-    if (s_beg < s_end) bring(s_beg, 0);
-    for (int st = s_beg; st < s_end; ++st) {
-        const int buffer = (st - s_beg) & 1;
-        // Stage st has landed, and no wave reads the other buffer any more.
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (st + 1 < s_end) bring(st + 1, buffer ^ 1);
+    const typename OpP::Reader read_p(16 * RT * wp);
+    const typename OpQ::Reader read_q(16 * TT * wq);
+    constexpr int kDma = OpP::kMine + OpQ::kMine;  // of a wave and stage
+    constexpr int kAhead = Tile::NB - 1;           // stages on their way while one is multiplied
+    u32x4v a[RT], b[TT];
+    auto read = [&](auto u_tag, int buffer) {
+        constexpr int U = decltype(u_tag)::value;
         const uint8_t *const in_p = lds + buffer * Tile::kStage, *const in_q = in_p + Tile::kStageP;
-        auto step = [&](auto u_tag) {
-            constexpr int U = decltype(u_tag)::value;
-            u32x4v a[RT];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) a[rt] = read_p.template read<U>(in_p, rt);
+        for (int rt = 0; rt < RT; ++rt) a[rt] = read_p.template read<U>(in_p, rt);
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt) {
-                const u32x4v b = read_q.template read<U>(in_q, tt);
+        for (int tt = 0; tt < TT; ++tt) b[tt] = read_q.template read<U>(in_q, tt);
+    };
+    auto multiply = [&]() {
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) acc[rt][tt] = rows_mfma<T>(a[rt], b, acc[rt][tt]);
-            }
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) acc[rt][tt] = rows_mfma<T>(a[rt], b[tt], acc[rt][tt]);
+    };
+    constexpr std::integral_constant<int, 0> kU0{};
+    constexpr std::integral_constant<int, 1> kU1{};
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (s_beg + i < s_end) bring(s_beg + i, i);
+    int buffer = 0;
+    if constexpr (Tile::kWaves == 8) {
+        // Two waves a SIMD, one half of the waves a slot behind the other: while one reads its operands of a step,
+        // the other multiplies.  A barrier ends each slot.
+        auto slot_end = [&]() {
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
         };
-        step(std::integral_constant<int, 0>{});
-        step(std::integral_constant<int, 1>{});
+        // The next stage has landed (stages behind it may be on their way).
+        auto landed = [&](int next) {
+            if (next + kAhead - 1 < s_end) asm volatile("s_waitcnt vmcnt(%0)" ::"i"((kAhead - 1) * kDma) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        };
+        auto products = [&]() {
+            __builtin_amdgcn_s_setprio(1);
+            multiply();
+            __builtin_amdgcn_s_setprio(0);
+        };
+        if (s_beg < s_end) landed(s_beg);
+        slot_end();
+        if (wave >= 4) slot_end();
+        for (int st = s_beg; st < s_end; ++st) {
+            // Into the buffer of stage st - 1, whose last readers ended before this slot.
+            if (st + kAhead < s_end) bring(st + kAhead, buffer == 0 ? Tile::NB - 1 : buffer - 1);
+            read(kU0, buffer);
+            slot_end();
+            products();
+            slot_end();
+            read(kU1, buffer);
+            if (wave >= 4 && st + 1 < s_end) landed(st + 1);
+            slot_end();
+            products();
+            if (wave < 4 && st + 1 < s_end) landed(st + 1);
+            slot_end();
+            buffer = buffer == Tile::NB - 1 ? 0 : buffer + 1;
+        }
+        if (wave < 4) slot_end();
+    } else {
+        for (int st = s_beg; st < s_end; ++st) {
+            // Stage st has landed, and no wave reads the buffer of stage st - 1 any more.
+            if (st + kAhead - 1 < s_end)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((kAhead - 1) * kDma) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (st + kAhead < s_end) bring(st + kAhead, buffer == 0 ? Tile::NB - 1 : buffer - 1);
+            read(kU0, buffer);
+            multiply();
+            read(kU1, buffer);
+            multiply();
+            buffer = buffer == Tile::NB - 1 ? 0 : buffer + 1;
+        }
+        __syncthreads();  // no wave reads a stage any more
     }
-    __syncthreads();  // no wave reads a stage any more
 
     // ---- outputs: 16 rows at a time through the wave's own LDS, read back 8 columns a lane
     uint8_t *const stage = lds + wave * (16 * Tile::kOutPitch);
@@ -368,6 +476,7 @@ inline bool rows_dma_accepts(RowsMode mode, int es, const RowsMm &p) {
     };
     if (!fits(p.p, p.ldp) || !fits(p.q, p.ldq)) return false;
     if (p.p2 != nullptr && !fits(p.p2, p.ldp)) return false;
+    if (p.q2 != nullptr && !fits(p.q2, p.ldq)) return false;
     if (mode == kRowsInput) return p.P % piece == 0 && (p.halves == 1 || p.K % piece == 0);
     if (mode == kRowsWeight) return p.P % piece == 0 && p.Q % piece == 0;
     return true;
@@ -379,21 +488,19 @@ hipError_t rows_by_tile(const RowsMm &p, int tile, hipStream_t stream) {
     switch (tile) {
         case 0: return run_rows<E, MODE, RowsTile<2, 2, 2, 2>, true>(p, stream);
         case 1: return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, true>(p, stream);
+        case 2: return run_rows<E, MODE, RowsTile<8, 4, 2, 4>, true>(p, stream);
+        case 3: return run_rows<E, MODE, RowsTile<4, 8, 4, 2>, true>(p, stream);
+        case 4: return run_rows<E, MODE, RowsTile<4, 4, 4, 2, 3>, true>(p, stream);
+        case 5: return run_rows<E, MODE, RowsTile<2, 2, 2, 2, 4>, true>(p, stream);
+        case 6: return run_rows<E, MODE, RowsTile<4, 4, 2, 2, 3>, true>(p, stream);
     }
-    return run_rows<E, MODE, RowsTile<8, 4, 2, 4>, true>(p, stream);
-}
-
-}  // namespace
-
-template <class E>
-hipError_t rows_mm_tiles(RowsMode mode, const RowsMm &p, int tile, hipStream_t stream) {
-    switch (mode) {
-        case kRowsForward: return rows_by_tile<E, kRowsForward>(p, tile, stream);
-        case kRowsSwiglu: return rows_by_tile<E, kRowsSwiglu>(p, tile, stream);
-        case kRowsInput: return rows_by_tile<E, kRowsInput>(p, tile, stream);
-        case kRowsWeight: return rows_by_tile<E, kRowsWeight>(p, tile, stream);
+    if constexpr (MODE != kRowsWeight) {
+        if (tile == 7) return run_rows<E, MODE, RowsTile<4, 5, 4, 2, 3>, true>(p, stream);
+        if (tile == 8) return run_rows<E, MODE, RowsTile<4, 6, 4, 2>, true>(p, stream);
+        if (tile == 9) return run_rows<E, MODE, RowsTile<4, 3, 4, 2, 3>, true>(p, stream);
     }
     return hipErrorInvalidValue;
 }
 
+}  // namespace
 }  // namespace jjo

@@ -44,12 +44,23 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsMm p, int chunks, in
     }
 }
 
+// Eight values rounded to T and, where it is wanted, what the rounding left of them.
+template <class T>
+__device__ __forceinline__ void store_split(void *to, void *rest, int64_t at, int n, const float *v) {
+    rows_store8((T *)to + at, n, v);
+    if (rest == nullptr) return;
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = v[i] - (float)(T)v[i];
+    rows_store8((T *)rest + at, n, r);
+}
+
 constexpr int kColumnsAtOnce = 512;  // of a workgroup: 64 lanes x 8; its four waves take every fourth row
 
 template <class E>
 __global__ __launch_bounds__(256) void rows_act_backward_kernel(const void *grad_y, int64_t grad_y_stride,
-                                                                const void *pre, void *gz, int act, float *part,
-                                                                int T_, int N) {
+                                                                const void *pre, void *gz, void *rest, int act,
+                                                                float *part, int T_, int N) {
     typedef typename E::type T;
     __shared__ float sums[4][kColumnsAtOnce];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -64,7 +75,7 @@ __global__ __launch_bounds__(256) void rows_act_backward_kernel(const void *grad
                 rows_load8((const T *)pre + (int64_t)t * N + col, n, z);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) g[i] *= rows_slope(z[i], act);
-                rows_store8((T *)gz + (int64_t)t * N + col, n, g);
+                store_split<T>(gz, rest, (int64_t)t * N + col, n, g);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) total[i] += g[i];
@@ -90,8 +101,9 @@ __global__ __launch_bounds__(256) void rows_column_join_kernel(const float *part
 
 template <class E>
 __global__ __launch_bounds__(256) void rows_swiglu_backward_kernel(const void *grad_mid, const void *gate_up,
-                                                                   void *grad_gate_up, const int32_t *offsets,
-                                                                   int n_experts, int chunks, int I, int R) {
+                                                                   void *grad_gate_up, void *rest,
+                                                                   const int32_t *offsets, int n_experts, int chunks,
+                                                                   int I, int R) {
     typedef typename E::type T;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / chunks;
     if (row >= rows_limit(offsets, n_experts, R)) return;
@@ -107,8 +119,8 @@ __global__ __launch_bounds__(256) void rows_swiglu_backward_kernel(const void *g
         g[i] = gm * up[i] * s * (1.0f + gate[i] * (1.0f - s));
         up[i] = gm * gate[i] * s;
     }
-    rows_store8((T *)grad_gate_up + at, n, g);
-    rows_store8((T *)grad_gate_up + at + I, n, up);
+    store_split<T>(grad_gate_up, rest, at, n, g);
+    store_split<T>(grad_gate_up, rest, at + I, n, up);
 }
 
 bool grid_of(int64_t threads, dim3 *grid) {
@@ -129,9 +141,23 @@ int64_t rows_part_bytes(RowsMode mode, const RowsMm &p) {
 
 int rows_mm_slices(RowsMode, int, int, int, int, int, int, int) { return 1; }
 
-hipError_t launch_rows_mm(RowsMode mode, int dtype, const RowsMm &p, hipStream_t stream) {
+namespace {
+RowsChoice rows_mm_choose(RowsMode mode, int dtype, const RowsMm &p) {
+    const int64_t experts = p.offsets != nullptr ? std::min(p.n_experts, p.M) : 1;
+    const int64_t mean = (p.Q + experts - 1) / experts;
+    if ((mode == kRowsForward || mode == kRowsSwiglu) && mean <= 32) {
+        const int tile = mean <= (p.offsets != nullptr ? 10 : 16) ? -1 : -2;
+        const int64_t wgs = experts * ((p.P + 15) / 16) / (mode == kRowsForward && tile == -2 ? 2 : 1);
+        return {tile, wgs >= 2048 ? 2 : wgs >= 640 ? 4 : 8};
+    }
+    return {1, 0};
+}
+}  // namespace
+
+hipError_t launch_rows_mm(RowsMode mode, int dtype, const RowsMm &p, hipStream_t stream, const RowsChoice *pinned) {
+    const RowsChoice c = pinned != nullptr ? *pinned : rows_mm_choose(mode, dtype, p);
     const hipError_t e = mx_by_dtype(dtype, [&](auto tag) {
-        return rows_mm_tiles<decltype(tag)>(mode, p, 1, stream);
+        return rows_mm_run<decltype(tag)>(mode, p, c, stream);
     });
     if (e != hipSuccess || p.slices == 1) return e;
     const int chunks = (p.P + 7) / 8;
@@ -158,8 +184,8 @@ int rows_column_chunks(int T, int N) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(1024 / across, ((int64_t)T + 15) / 16));
 }
 
-hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, const void *pre, void *gz, int dtype,
-                                    int act, void *sums, bool sums_wide, float *column_part, int T, int N,
+hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, const void *pre, void *gz, void *rest,
+                                    int dtype, int act, void *sums, bool sums_wide, float *column_part, int T, int N,
                                     hipStream_t stream) {
     const int chunks = rows_column_chunks(T, N);
     const dim3 grid((unsigned)((N + (int64_t)kColumnsAtOnce - 1) / kColumnsAtOnce), (unsigned)chunks);
@@ -167,8 +193,8 @@ hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, c
     return mx_by_dtype(dtype, [&](auto tag) {
         using E = decltype(tag);
         typedef typename E::type V;
-        hipLaunchKernelGGL(rows_act_backward_kernel<E>, grid, dim3(256), 0, stream, grad_y, grad_y_stride, pre, gz, act,
-                           part, T, N);
+        hipLaunchKernelGGL(rows_act_backward_kernel<E>, grid, dim3(256), 0, stream, grad_y, grad_y_stride, pre, gz, rest,
+                           act, part, T, N);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess || sums == nullptr) return e;
         const dim3 join((unsigned)((N + 255LL) / 256));
@@ -180,14 +206,14 @@ hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, c
     });
 }
 
-hipError_t launch_rows_swiglu_backward(const void *grad_mid, const void *gate_up, void *grad_gate_up, int dtype,
+hipError_t launch_rows_swiglu_backward(const void *grad_mid, const void *gate_up, void *grad_gate_up, void *rest, int dtype,
                                        const int32_t *offsets, int n_experts, int I, int R, hipStream_t stream) {
     const int chunks = (I + 7) / 8;
     dim3 grid;
     if (!grid_of((int64_t)R * chunks, &grid)) return hipErrorInvalidConfiguration;
     return mx_by_dtype(dtype, [&](auto tag) {
         hipLaunchKernelGGL(rows_swiglu_backward_kernel<decltype(tag)>, grid, dim3(256), 0, stream, grad_mid, gate_up,
-                           grad_gate_up, offsets, n_experts, chunks, I, R);
+                           grad_gate_up, rest, offsets, n_experts, chunks, I, R);
         return hipGetLastError();
     });
 }

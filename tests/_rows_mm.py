@@ -59,14 +59,20 @@ def linear(x, w, bias, residual, name):
     return y, ey, z, e
 
 
-def gz_of(g, pre, name, dtype):
-    """The gradient through an activation, and its error once it is rounded to dtype."""
+def kept(x, dtype, wide):
+    """The error of a gradient x that is rounded to dtype; wide: and of what that left, rounded again."""
+    once = rounding(x, dtype)
+    return rounding(once, dtype) if wide and dtype != torch.float32 else once
+
+
+def gz_of(g, pre, name, dtype, wide=False):
+    """The gradient through an activation, its error in fp32, and that once it is rounded to dtype."""
     g = g.double()
     if name == "none":
         return g, torch.zeros_like(g), torch.zeros_like(g)
     gz = g * slope(pre.double(), name)
     fp32 = g.abs() * 2.0 ** -19 * pre.double().abs().clamp(min=1.0)
-    return gz, fp32, fp32 + rounding(gz.abs() + fp32, dtype)
+    return gz, fp32, fp32 + kept(gz.abs() + fp32, dtype, wide)
 
 
 def mm_of(a, ea, b):
@@ -75,13 +81,13 @@ def mm_of(a, ea, b):
     return ref, 1.01 * e + ea @ b.double().abs().t()
 
 
-def swiglu_back(g, gate, up, dtype):
+def swiglu_back(g, gate, up, dtype, wide=False):
     """Gradients of gate and up, each with its error once rounded."""
     g, gate, up = g.double(), gate.double(), up.double()
     gg, gu = g * up * slope(gate, "silu"), g * act(gate, "silu")
     big = gate.abs().clamp(min=1.0)
     eg, eu = (g * up).abs() * 2.0 ** -19 * big, g.abs() * 2.0 ** -19 * big
-    return gg, eg + rounding(gg.abs() + eg, dtype), gu, eu + rounding(gu.abs() + eu, dtype)
+    return gg, eg + kept(gg.abs() + eg, dtype, wide), gu, eu + kept(gu.abs() + eu, dtype, wide)
 
 
 def workspace(n):

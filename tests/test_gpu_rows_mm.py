@@ -86,7 +86,10 @@ def _linear_back(name, K, N, T, act, wide, want="xwb"):
     if gx is not None:
         R.check(gx, *R.mm_of(gz, e, w.t()), "grad_x")
     if gw is not None:
-        R.check(gw, *R.mm_of(gz.t(), e.t(), x.t()), "grad_w")
+        # a sum over both parts of a split gradient has twice the additions
+        _, _, ew = R.gz_of(g, pre, act, d, wide)
+        ref, bound = R.mm_of(gz.t(), ew.t(), x.t())
+        R.check(gw, ref, 2 * bound if wide else bound, "grad_w")
     if gb is not None:
         R.check(gb, gz.sum(0), 1.01 * (e32.sum(0) + (T + 2) * 2.0 ** -23 * gz.abs().sum(0)), "grad_b")
 
@@ -96,6 +99,7 @@ def _linear_back(name, K, N, T, act, wide, want="xwb"):
 def test_linear_backward(dev, name, K, N, T):
     _linear_back(name, K, N, T, "none", True)
     _linear_back(name, K, N, T, "gelu_tanh", False)
+    _linear_back(name, K, N, T, "gelu", True)
 
 
 @pytest.mark.parametrize("act", list(R.ACTS))
@@ -166,5 +170,7 @@ def test_grouped(dev, name, K, N, counts):
         rb, eb = R.mm_of(gu, egu, w2[e].t())
         # one sum of 2 N products: twice the additions
         R.check(sx[a:b], ra + rb, 2 * (ea + eb), f"swiglu grad_x {e}")
-        R.check(sg[e], *R.mm_of(gg.t(), eg.t(), xs.t()), f"grad_w_gate {e}")
-        R.check(su[e], *R.mm_of(gu.t(), egu.t(), xs.t()), f"grad_w_up {e}")
+        _, eg, _, egu = R.swiglu_back(gs, saved[a:b, :N], saved[a:b, N:], d, True)
+        for got, gz, ez in ((sg[e], gg, eg), (su[e], gu, egu)):  # fp32: sums over both parts of the gradient
+            ref, bound = R.mm_of(gz.t(), ez.t(), xs.t())
+            R.check(got, ref, 2 * bound, f"grad_w_gate, grad_w_up {e}")
