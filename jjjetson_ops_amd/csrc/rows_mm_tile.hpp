@@ -46,8 +46,7 @@ struct RowsTile {
     static constexpr int kWaves = WP * WQ, kThreads = 64 * kWaves;
     static constexpr int kP = 16 * RT * WP, kQ = 16 * TT * WQ;
     static constexpr int kStageP = kP * 128, kStageQ = kQ * 128, kStage = kStageP + kStageQ;
-    static constexpr int kOutPitch = 16 * RT * 4 + 16;  // a row of outputs in LDS: + 4 banks
-    static constexpr int kLds = std::max(NB * kStage, kWaves * 16 * kOutPitch);
+    static constexpr int kLds = NB * kStage;
     static_assert(kLds <= 160 * 1024, "LDS of a CU");
 };
 
@@ -86,8 +85,7 @@ struct RowsOperand {
     template <class F>
     static __device__ __forceinline__ void copy(F from, uint8_t *lds) {
         u32x4v v[kMine];
-        int tid = threadIdx.x;
-        asm volatile("" : "+v"(tid));  // one stage of many comes this way: no addresses kept in registers for it
+        const int tid = threadIdx.x;
 #pragma unroll
         for (int n = 0; n < kMine; ++n) {
             int i, k, have;
@@ -157,6 +155,16 @@ struct RowsOperand {
     };
 };
 
+// Of tiles a and b (a lane holds columns 4 * (lane / 16) + 0..3 of both) eight columns of one: lanes 0..15
+// columns 0..7 of a, the next 16 those of b, then columns 8..15 of a and of b.
+__device__ __forceinline__ void rows_exchange(f32x4v a, f32x4v b, float *v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[i]), __float_as_uint(b[i]), false, false);
+        v[i] = __uint_as_float(s[0]), v[4 + i] = __uint_as_float(s[1]);
+    }
+}
+
 // 64 pieces of 16 bytes to LDS.
 __device__ __forceinline__ void rows_dma(uint32_t off, uint64_t from, uint32_t lds) {
     const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds);
@@ -219,8 +227,16 @@ __device__ __forceinline__ bool rows_expert_tile(const int32_t *__restrict__ off
     return false;
 }
 
-// DMA: the operands' memory rows are 16-byte aligned and a tile's offsets fit 32 bits; stages that end
-// inside themselves and every stage of other operands go through registers.
+// The same from an address of each lane's own.
+__device__ __forceinline__ void rows_dma(const void *from, uint32_t lds) {
+    const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds);
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(m0v) : "memory");
+}
+
+__device__ const uint32_t rows_zeros[4] = {0u, 0u, 0u, 0u};  // the pieces behind the sums' end
+
+// DMA: the operands' memory rows are 16-byte aligned, the sums' elements whole pieces, and a tile's offsets
+// fit 32 bits; other operands go through registers.
 template <class E, RowsMode MODE, class Tile, bool DMA>
 __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
     typedef typename E::type T;
@@ -286,17 +302,38 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
         const T *const from_up = MODE == kRowsSwiglu ? pm2 + k0 : from_p;
         const T *const from_q = (MODE == kRowsWeight && second ? qm2 : qm) +
                                 (QT ? k0 * p.ldq : (second ? p.K : 0) + (int64_t)k0);
-        if (DMA && left >= kStep) {
+        if constexpr (DMA) {
             const uint32_t at = (uint32_t)(uintptr_t)to;
+            if (left >= kStep) {
 #pragma unroll
-            for (int n = 0; n < OpP::kMine; ++n) {
-                const int run = OpP::run(wave, n);  // of SwiGLU 8 rows of one matrix
-                rows_dma(off_p[n], (uint64_t)(is_up(8 * run) ? from_up : from_p), at + 1024 * run);
-            }
+                for (int n = 0; n < OpP::kMine; ++n) {
+                    const int run = OpP::run(wave, n);  // of SwiGLU 8 rows of one matrix
+                    rows_dma(off_p[n], (uint64_t)(is_up(8 * run) ? from_up : from_p), at + 1024 * run);
+                }
 #pragma unroll
-            for (int n = 0; n < OpQ::kMine; ++n) {
-                const int run = OpQ::run(wave, n);
-                rows_dma(off_q[n], (uint64_t)from_q, at + Tile::kStageP + 1024 * run);
+                for (int n = 0; n < OpQ::kMine; ++n) {
+                    const int run = OpQ::run(wave, n);
+                    rows_dma(off_q[n], (uint64_t)from_q, at + Tile::kStageP + 1024 * run);
+                }
+            } else {  // the sums end inside the stage
+                int in_run = lane;
+                asm volatile("" : "+v"(in_run));  // one stage of many: nothing kept in registers for it
+#pragma unroll
+                for (int n = 0; n < OpP::kMine; ++n) {
+                    int i, k;
+                    const int run = OpP::run(wave, n);
+                    OpP::piece(64 * run + in_run, i, k);
+                    const T *const from = (is_up(8 * run) ? from_up : from_p) + off_p[n] / sizeof(T);
+                    rows_dma(k < left ? (const void *)from : rows_zeros, at + 1024 * run);
+                }
+#pragma unroll
+                for (int n = 0; n < OpQ::kMine; ++n) {
+                    int i, k;
+                    const int run = OpQ::run(wave, n);
+                    OpQ::piece(64 * run + in_run, i, k);
+                    rows_dma(k < left ? (const void *)(from_q + off_q[n] / sizeof(T)) : rows_zeros,
+                             at + Tile::kStageP + 1024 * run);
+                }
             }
         } else {
             OpP::copy([&](int i, int k, int &have) {
@@ -364,7 +401,7 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
         slot_end();
         if (wave >= 4) slot_end();
         for (int st = s_beg; st < s_end; ++st) {
-            // Into the buffer of stage st - 1, whose last readers ended before this slot.
+            // Into the buffer of stage st - 1, whose last readers' slot has ended.
             if (st + kAhead < s_end) bring(st + kAhead, buffer == 0 ? Tile::NB - 1 : buffer - 1);
             read(kU0, buffer);
             slot_end();
@@ -393,55 +430,53 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
             multiply();
             buffer = buffer == Tile::NB - 1 ? 0 : buffer + 1;
         }
-        __syncthreads();  // no wave reads a stage any more
     }
 
-    // ---- outputs: 16 rows at a time through the wave's own LDS, read back 8 columns a lane
-    uint8_t *const stage = lds + wave * (16 * Tile::kOutPitch);
-    constexpr int kChunks = (MODE == kRowsSwiglu ? RT : 2 * RT), kAtOnce = 64 / kChunks;
-    const int chunk = lane % kChunks;
-    const int col = p0 + wp * 8 * kChunks + 8 * chunk, n = min(8, p.P - col);
+    // ---- outputs straight from the registers: of two tiles side by side lanes exchange halves, so that each
+    // holds eight columns of a row and a row's four lanes 64 contiguous bytes (of 16 bits).
     const bool parts = p.slices > 1;
     void *const y = MODE == kRowsWeight ? (void *)((uint8_t *)(half == 0 ? p.y : p.y2) +
                                                    expert * p.expert_stride * (p.wide ? 4 : sizeof(T)))
                                         : p.y;
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-            *reinterpret_cast<f32x4v *>(stage + r16 * Tile::kOutPitch + 64 * rt + 16 * q4) = acc[rt][tt];
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int k = 0; k < (16 + kAtOnce - 1) / kAtOnce; ++k) {
-            const int r = kAtOnce * k + lane / kChunks, in_tile = 16 * (TT * wq + tt) + r;
-            if (r < 16 && in_tile < rows_q && n > 0) {
-                float v[8], up[8];
-                auto take = [&](float *to, int at) {
-                    const f32x4v *const from = reinterpret_cast<const f32x4v *>(stage + r * Tile::kOutPitch + 32 * at);
-                    const f32x4v a = from[0], b = from[1];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) to[i] = a[i], to[4 + i] = b[i];
-                };
-                take(v, chunk);
-                if constexpr (MODE == kRowsSwiglu) take(up, RT + chunk);
-                const int64_t row = q0 + in_tile;
-                if (parts) {
-                    const int64_t cols = MODE == kRowsSwiglu ? 2 * (int64_t)p.P : p.P;
-                    // A slice's rows: of weight those of all matrices.
-                    const int64_t all = MODE == kRowsWeight ? (int64_t)p.Q * p.halves * max(p.n_experts, 1) : p.Q;
-                    const int64_t mine = MODE == kRowsWeight ? ((int64_t)half * max(p.n_experts, 1) + expert) * p.Q + row
-                                                             : row;
-                    float *const to = p.part + (blockIdx.y * all + mine) * cols + col;
-                    rows_store8(to, n, v);
-                    if constexpr (MODE == kRowsSwiglu) rows_store8(to + p.P, n, up);
-                } else if constexpr (MODE == kRowsSwiglu) {
-                    rows_finish_swiglu<T>(p.epi, v, up, row, col, n, p.P, y);
-                } else {
-                    rows_finish<T>(p.epi, v, row, col, n, p.P, y, p.ldy, p.wide);
-                }
-            }
+    auto finish = [&](int in_tile, int column, float *v, float *up) {
+        const int col = p0 + column, n = min(8, p.P - col);
+        if (in_tile >= rows_q || n <= 0) return;
+        const int64_t row = q0 + in_tile;
+        if (parts) {
+            const int64_t cols = MODE == kRowsSwiglu ? 2 * (int64_t)p.P : p.P;
+            // A slice's rows: of weight those of all matrices.
+            const int64_t matrices = max(p.n_experts, 1);
+            const int64_t all = MODE == kRowsWeight ? p.Q * p.halves * matrices : p.Q;
+            const int64_t mine = MODE == kRowsWeight ? (half * matrices + expert) * p.Q + row : row;
+            float *const to = p.part + (blockIdx.y * all + mine) * cols + col;
+            rows_store8(to, n, v);
+            if constexpr (MODE == kRowsSwiglu) rows_store8(to + p.P, n, up);
+        } else if constexpr (MODE == kRowsSwiglu) {
+            rows_finish_swiglu<T>(p.epi, v, up, row, col, n, p.P, y);
+        } else {
+            rows_finish<T>(p.epi, v, row, col, n, p.P, y, p.ldy, p.wide);
         }
-        __builtin_amdgcn_wave_barrier();
+    };
+    constexpr int kWaveP = MODE == kRowsSwiglu ? 8 * RT : 16 * RT;  // columns of a wave
+    if constexpr (kWaveP % 32 == 0) {
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+            for (int rt = 0; rt < kWaveP / 16; rt += 2) {
+                float v[8], up[8];
+                rows_exchange(acc[rt][tt], acc[rt + 1][tt], v);
+                if constexpr (MODE == kRowsSwiglu) rows_exchange(acc[RT / 2 + rt][tt], acc[RT / 2 + rt + 1][tt], up);
+                finish(16 * (TT * wq + tt) + r16, kWaveP * wp + 16 * (rt + (q4 & 1)) + 8 * (q4 >> 1), v, up);
+            }
+    } else {  // one tile of columns: of two tiles of rows
+        static_assert(TT % 2 == 0 && RT == 2 && MODE == kRowsSwiglu, "the small tile's gate and up");
+#pragma unroll
+        for (int tt = 0; tt < TT; tt += 2) {
+            float v[8], up[8];
+            rows_exchange(acc[0][tt], acc[0][tt + 1], v);
+            rows_exchange(acc[1][tt], acc[1][tt + 1], up);
+            finish(16 * (TT * wq + tt + (q4 & 1)) + r16, 16 * wp + 8 * (q4 >> 1), v, up);
+        }
     }
 }
 
@@ -477,9 +512,8 @@ inline bool rows_dma_accepts(RowsMode mode, int es, const RowsMm &p) {
     if (!fits(p.p, p.ldp) || !fits(p.q, p.ldq)) return false;
     if (p.p2 != nullptr && !fits(p.p2, p.ldp)) return false;
     if (p.q2 != nullptr && !fits(p.q2, p.ldq)) return false;
-    if (mode == kRowsInput) return p.P % piece == 0 && (p.halves == 1 || p.K % piece == 0);
     if (mode == kRowsWeight) return p.P % piece == 0 && p.Q % piece == 0;
-    return true;
+    return p.K % piece == 0 && (mode != kRowsInput || p.P % piece == 0);
 }
 
 template <class E, RowsMode MODE>
