@@ -51,10 +51,22 @@ __device__ __forceinline__ float rows_sigmoid(float z) {
 }
 constexpr float kGeluC = 0.797884560802865f, kGeluA = 0.044715f;  // sqrt(2 / pi)
 
+// erfc(x).  For results of 16 bits the rational approximation 7.1.26 of Abramowitz and Stegun (error at
+// most 1.5e-7, a fifth of their instructions of a result of fp32).
+template <class T>
+__device__ __forceinline__ float rows_erfc(float x) {
+    if constexpr (sizeof(T) == 4) return erfcf(x);
+    const float a = fabsf(x), t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * a);
+    const float poly = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float tail = poly * __builtin_amdgcn_exp2f(-1.44269504088896f * a * a);
+    return x < 0.0f ? 2.0f - tail : tail;
+}
+
+template <class T>
 __device__ __forceinline__ float rows_act(float z, int act) {
     switch (act) {
         case JJO_ACT_RELU: return z > 0.0f ? z : z != z ? z : 0.0f;
-        case JJO_ACT_GELU: return 0.5f * z * erfcf(-0.707106781186548f * z);
+        case JJO_ACT_GELU: return 0.5f * z * rows_erfc<T>(-0.707106781186548f * z);
         case JJO_ACT_GELU_TANH: return z * rows_sigmoid(2.0f * kGeluC * (z + kGeluA * z * z * z));
         case JJO_ACT_SILU: return z * rows_sigmoid(z);
     }
@@ -62,11 +74,12 @@ __device__ __forceinline__ float rows_act(float z, int act) {
 }
 
 // The activation's derivative at z.
+template <class T>
 __device__ __forceinline__ float rows_slope(float z, int act) {
     switch (act) {
         case JJO_ACT_RELU: return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
         case JJO_ACT_GELU:
-            return 0.5f * erfcf(-0.707106781186548f * z) +
+            return 0.5f * rows_erfc<T>(-0.707106781186548f * z) +
                    z * 0.398942280401433f * __builtin_amdgcn_exp2f(-0.721347520444482f * z * z);
         case JJO_ACT_GELU_TANH: {
             const float s = rows_sigmoid(2.0f * kGeluC * (z + kGeluA * z * z * z));
@@ -92,17 +105,24 @@ __device__ __forceinline__ void rows_load8(const T *p, int n, float *v) {
         for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.0f;
     }
 }
+// A value is rounded to fp32 before it is to T, on every path alike (the compiler would give some paths
+// an instruction that multiplies and rounds to fp16 at once, and so results that depend on the path).
+template <class T>
+__device__ __forceinline__ T rows_round(float v) {
+    asm("" : "+v"(v));
+    return (T)v;
+}
 template <class T>
 __device__ __forceinline__ void rows_store8(T *p, int n, const float *v) {
     if (n >= 8) {
         MxVec<T, 8> a;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a.v[i] = (T)v[i];
+        for (int i = 0; i < 8; ++i) a.v[i] = rows_round<T>(v[i]);
         store_any(p, a);
     } else {
 #pragma unroll
         for (int i = 0; i < 7; ++i)
-            if (i < n) p[i] = (T)v[i];
+            if (i < n) p[i] = rows_round<T>(v[i]);
     }
 }
 
@@ -119,7 +139,7 @@ __device__ __forceinline__ void rows_finish(const RowsEpilogue &e, float *v, int
     if (e.pre != nullptr) rows_store8((T *)e.pre + row * cols + col, n, v);
     if (e.act != JJO_ACT_NONE) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = rows_act(v[i], e.act);
+        for (int i = 0; i < 8; ++i) v[i] = rows_act<T>(v[i], e.act);
     }
     if (e.residual != nullptr) {
         float r[8];
@@ -131,6 +151,11 @@ __device__ __forceinline__ void rows_finish(const RowsEpilogue &e, float *v, int
     else rows_store8((T *)y + row * ldy + col, n, v);
 }
 
+__device__ __forceinline__ void rows_swiglu(float *gate, const float *up) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) gate[i] = gate[i] * rows_sigmoid(gate[i]) * up[i];
+}
+
 template <class T>
 __device__ __forceinline__ void rows_finish_swiglu(const RowsEpilogue &e, float *gate, const float *up, int64_t row,
                                                    int col, int n, int cols, void *y) {
@@ -139,8 +164,7 @@ __device__ __forceinline__ void rows_finish_swiglu(const RowsEpilogue &e, float 
         rows_store8(at, n, gate);
         rows_store8(at + cols, n, up);
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) gate[i] = gate[i] * rows_sigmoid(gate[i]) * up[i];
+    rows_swiglu(gate, up);
     rows_store8((T *)y + row * cols + col, n, gate);
 }
 
@@ -158,7 +182,7 @@ int64_t rows_part_bytes(RowsMode mode, const RowsMm &p);
 struct RowsChoice {
     int tile, waves;
 };
-constexpr int kRowsTiles = 10;
+constexpr int kRowsTiles = 7;
 template <class E>
 hipError_t rows_mm_run(RowsMode mode, const RowsMm &p, const RowsChoice &c, hipStream_t stream);
 

@@ -175,57 +175,117 @@ __device__ __forceinline__ void rows_dma(uint32_t off, uint64_t from, uint32_t l
     asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(from), "{m0}"(m0v) : "memory");
 }
 
-// Workgroups go to the eight XCDs in turn: each takes a contiguous run of `total` tiles, so that tiles
-// that read the same rows follow each other in one L2.  -1 behind the last.
-__device__ __forceinline__ int rows_xcd_run(int block, int total) {
-    const int per = total / 8, rest = total % 8, xcd = block % 8, at = block / 8;
-    return at < per + (xcd < rest) ? xcd * per + min(xcd, rest) + at : -1;
-}
+// Workgroups go to the eight XCDs in turn: each XCD takes a contiguous run of the tiles, its workgroups
+// neighbours of it, so that tiles that read the same rows are read into one L2.  A workgroup's tiles
+// are at, at + step, ... below end.
+struct RowsRun {
+    int at, step, end;
+    __device__ __forceinline__ explicit RowsRun(int total) {
+        const int per = total / 8, rest = total % 8, xcd = blockIdx.x % 8, beg = xcd * per + min(xcd, rest);
+        at = beg + (int)(blockIdx.x / 8);
+        step = ((int)gridDim.x - xcd + 7) / 8;
+        end = beg + per + (xcd < rest);
+    }
+};
 
-// The workgroup's tile of `rows` sorted rows x one of tiles_p of their expert's columns: expert by expert, its
-// row tiles fastest; false behind the last.  Ranges are clamped to [0, M], so a malformed table
-// drops rows instead of leaving the buffers.  All lanes of a wave call it together.
-__device__ __forceinline__ bool rows_expert_tile(const int32_t *__restrict__ offsets, int n_experts, int M, int rows,
-                                                 int tiles_p, int &expert, int &first, int &end, int &tile_p) {
-    const int lane = threadIdx.x & 63;
-    int beg = 0, fin = 0, incl = 0, mine = 0, total = 0;
-    auto count = [&](int e0) {
-        const int e = e0 + lane;
+// A tile of the output: columns p0.., rows q0.. (rows_q of them; of weight in half `half` of expert's matrix),
+// its sums over stages s_beg..s_end of `length` elements from row `first` on (weight).
+struct RowsPlace {
+    int p0, q0, rows_q, expert, half, first, length, slice, s_beg, s_end;
+};
+
+// The tiles of a launch, of Tile::kQ rows and kOutP columns.  Lane l of a wave holds the range of expert
+// l's rows and its row tiles added to those before; of more than 64 experts they are read again for
+// every tile.  Ranges are clamped to [0, M], so a malformed table drops rows instead of leaving the
+// buffers.  All lanes of a wave call these together.
+template <RowsMode MODE, class Tile, int STEP>
+struct RowsTiles {
+    static constexpr int kOutP = MODE == kRowsSwiglu ? Tile::kP / 2 : Tile::kP;
+    int beg = 0, fin = 0, incl = 0;
+    int per_slice;
+
+    __device__ __forceinline__ void count(const RowsMm &p, int e0) {
+        const int e = e0 + (threadIdx.x & 63);
         beg = fin = 0;
-        if (e < n_experts) {
-            beg = min(max(offsets[e], 0), M);
-            fin = min(max(offsets[e + 1], beg), M);
+        if (e < p.n_experts) {
+            beg = min(max(p.offsets[e], 0), p.M);
+            fin = min(max(p.offsets[e + 1], beg), p.M);
         }
-        mine = (fin - beg + rows - 1) / rows;
-        incl = mx_scan(mine);
-    };
-    for (int e0 = 0; e0 < n_experts; e0 += 64) {
-        count(e0);
-        total += __builtin_amdgcn_readlane(incl, 63);
+        incl = mx_scan((fin - beg + Tile::kQ - 1) / Tile::kQ);
     }
-    const int64_t all = (int64_t)total * tiles_p;
-    if (all > gridDim.x) return false;  // only the sums of a malformed table
-    const int tile = rows_xcd_run(blockIdx.x, (int)all);
-    if (tile < 0) return false;
-    int base = 0;
-    for (int e0 = 0; e0 < n_experts; e0 += 64) {
-        if (n_experts > 64) count(e0);
-        const uint64_t past = __ballot((int64_t)(base + incl) * tiles_p > tile);
-        if (past != 0) {
-            const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
-            const int tiles = __builtin_amdgcn_readlane(mine, l);
-            const int local = tile - (base + __builtin_amdgcn_readlane(incl, l) - tiles) * tiles_p;
-            if (tiles <= 0 || local < 0) return false;
-            expert = e0 + l;
-            first = __builtin_amdgcn_readlane(beg, l) + local % tiles * rows;
-            end = __builtin_amdgcn_readlane(fin, l);
-            tile_p = local / tiles;
-            return first < end && tile_p < tiles_p;
+    // The tiles in all; `most`: those the launch was made for (more only by a malformed table: none then).
+    __device__ __forceinline__ int total(const RowsMm &p, int64_t most) {
+        int64_t tiles = (int64_t)p.tiles_p * p.tiles_q;
+        if (p.offsets != nullptr) {
+            int rows = 0;
+            for (int e0 = 0; e0 < p.n_experts; e0 += 64) {
+                count(p, e0);
+                rows += __builtin_amdgcn_readlane(incl, 63);
+            }
+            tiles = MODE == kRowsWeight ? tiles * p.n_experts : (int64_t)p.tiles_p * rows;
         }
-        base += __builtin_amdgcn_readlane(incl, 63);
+        per_slice = tiles * p.slices > most || tiles < 0 ? 0 : (int)tiles;
+        return per_slice * p.slices;
     }
-    return false;
-}
+    __device__ __forceinline__ RowsPlace place(const RowsMm &p, int id) {
+        RowsPlace c{};
+        c.slice = p.slices == 1 ? 0 : id / per_slice;
+        int tile = id - c.slice * per_slice, tile_p;
+        c.length = p.K;
+        if constexpr (MODE == kRowsWeight) {
+            const int each = p.tiles_p * p.tiles_q;
+            if (p.offsets != nullptr) {
+                c.expert = tile / each, tile %= each;
+                int end;
+                if (p.n_experts <= 64) {
+                    c.first = __builtin_amdgcn_readlane(beg, c.expert);
+                    end = __builtin_amdgcn_readlane(fin, c.expert);
+                } else {
+                    c.first = __builtin_amdgcn_readfirstlane(min(max(p.offsets[c.expert], 0), p.M));
+                    end = __builtin_amdgcn_readfirstlane(min(max(p.offsets[c.expert + 1], c.first), p.M));
+                }
+                c.length = end - c.first;
+            }
+            const int tile_q = tile % p.tiles_q, tiles_half = p.tiles_q / p.halves;
+            tile_p = tile / p.tiles_q;
+            c.half = tile_q / tiles_half;
+            c.q0 = tile_q % tiles_half * Tile::kQ;
+            c.rows_q = min(p.Q - c.q0, Tile::kQ);
+        } else if (p.offsets == nullptr) {
+            // Rows fastest: a tile of the matrix is read for all of them.
+            c.q0 = tile % p.tiles_q * Tile::kQ;
+            c.rows_q = min(p.Q - c.q0, Tile::kQ);
+            tile_p = tile / p.tiles_q;
+        } else {  // expert by expert, its row tiles fastest
+            int base = 0, tiles = 1, row = 0, end = 0;
+            tile_p = 0;
+            for (int e0 = 0; e0 < p.n_experts; e0 += 64) {
+                if (p.n_experts > 64) count(p, e0);
+                const uint64_t past = __ballot((int64_t)(base + incl) * p.tiles_p > tile);
+                if (past != 0) {
+                    const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
+                    row = __builtin_amdgcn_readlane(beg, l);
+                    end = __builtin_amdgcn_readlane(fin, l);
+                    tiles = max((end - row + Tile::kQ - 1) / Tile::kQ, 1);
+                    const int local = tile - (base + __builtin_amdgcn_readlane(incl, l) - tiles) * p.tiles_p;
+                    c.expert = e0 + l;
+                    row += local % tiles * Tile::kQ;
+                    tile_p = local / tiles;
+                    break;
+                }
+                base += __builtin_amdgcn_readlane(incl, 63);
+            }
+            c.q0 = row;
+            c.rows_q = min(end - row, Tile::kQ);
+        }
+        c.p0 = tile_p * kOutP;
+        const int half_stages = (c.length + STEP - 1) / STEP;
+        const int stages = MODE == kRowsInput ? p.halves * half_stages : MODE == kRowsWeight ? p.terms * half_stages : half_stages;
+        c.s_beg = p.slices == 1 ? 0 : (int)((int64_t)stages * c.slice / p.slices);
+        c.s_end = p.slices == 1 ? stages : (int)((int64_t)stages * (c.slice + 1) / p.slices);
+        return c;
+    }
+};
 
 // The same from an address of each lane's own.
 __device__ __forceinline__ void rows_dma(const void *from, uint32_t lds) {
@@ -235,69 +295,51 @@ __device__ __forceinline__ void rows_dma(const void *from, uint32_t lds) {
 
 __device__ const uint32_t rows_zeros[4] = {0u, 0u, 0u, 0u};  // the pieces behind the sums' end
 
+// The operands of a tile and the way of their stages into LDS.
+//
 // DMA: the operands' memory rows are 16-byte aligned, the sums' elements whole pieces, and a tile's offsets
 // fit 32 bits; other operands go through registers.
-template <class E, RowsMode MODE, class Tile, bool DMA>
-__global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
-    typedef typename E::type T;
-    constexpr int RT = Tile::RT, TT = Tile::TT, kStep = 128 / sizeof(T);
-    constexpr bool PT = MODE == kRowsInput || MODE == kRowsWeight, QT = MODE == kRowsWeight;
+template <class T, RowsMode MODE, class Tile, bool DMA>
+struct RowsSource {
+    static constexpr int kStep = 128 / sizeof(T);
+    static constexpr bool PT = MODE == kRowsInput || MODE == kRowsWeight, QT = MODE == kRowsWeight;
     using OpP = RowsOperand<T, PT, Tile::kP, Tile::kThreads>;
     using OpQ = RowsOperand<T, QT, Tile::kQ, Tile::kThreads>;
-    // SwiGLU: a wave's first columns are gate's, the other half up's of the same.
-    constexpr int kOutP = MODE == kRowsSwiglu ? Tile::kP / 2 : Tile::kP;
-    extern __shared__ __align__(16) uint8_t lds[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r16 = lane & 15, q4 = lane >> 4;
-    const int wp = wave % Tile::WP, wq = wave / Tile::WP;
+    static constexpr int kDma = OpP::kMine + OpQ::kMine;  // of a wave and stage
 
-    int expert = 0, first = 0, end = p.Q, half = 0, q0, tile_p, length = p.K;
-    if constexpr (MODE == kRowsWeight) {
-        const int each = p.tiles_p * p.tiles_q;
-        int tile = rows_xcd_run(blockIdx.x, gridDim.x);
-        if (p.offsets != nullptr) {
-            expert = tile / each, tile %= each;
-            first = min(max(p.offsets[expert], 0), p.M);
-            length = min(max(p.offsets[expert + 1], first), p.M) - first;
-        }
-        const int tiles_half = p.tiles_q / p.halves, tile_q = tile % p.tiles_q;
-        half = tile_q / tiles_half;
-        q0 = tile_q % tiles_half * Tile::kQ;
-        tile_p = tile / p.tiles_q;
-    } else if (p.offsets == nullptr) {
-        const int tile = rows_xcd_run(blockIdx.x, gridDim.x);
-        q0 = tile % p.tiles_q * Tile::kQ;
-        tile_p = tile / p.tiles_q;
-    } else if (!rows_expert_tile(p.offsets, p.n_experts, p.M, Tile::kQ, p.tiles_p, expert, q0, end, tile_p)) {
-        return;
-    }
-    const int p0 = tile_p * kOutP;
-    const int rows_p = min(p.P - p0, kOutP), rows_q = min(end - q0, Tile::kQ);
-
-    // The operands from the tile's first row and the sums' first element on.
-    const T *const pm = (const T *)p.p + (MODE == kRowsWeight ? first * p.ldp + p0
-                                                              : expert * p.expert_stride + (PT ? p0 : p0 * p.ldp));
-    const T *const pm2 = MODE == kRowsWeight ? pm : (const T *)p.p2 + (pm - (const T *)p.p);
-    const T *const qm = (const T *)p.q + (QT ? first * p.ldq + (int64_t)half * p.Q + q0 : q0 * p.ldq);
-    const T *const qm2 = MODE == kRowsWeight ? (const T *)p.q2 + (qm - (const T *)p.q) : qm;
-
-    const int stages_half = (length + kStep - 1) / kStep;
-    const int stages = MODE == kRowsInput ? p.halves * stages_half : MODE == kRowsWeight ? p.terms * stages_half : stages_half;
-    const int s_beg = (int)((int64_t)stages * blockIdx.y / p.slices);
-    const int s_end = (int)((int64_t)stages * (blockIdx.y + 1) / p.slices);
+    // From the tile's first row and the sums' first element on; the second ones: up's rows (SwiGLU), the sums'
+    // second half (input, and weight with two terms).
+    const T *pm, *pm2, *qm, *qm2;
+    int rows_p, rows_q, length, stages_half;
+    uint32_t off_p[DMA ? OpP::kMine : 1], off_q[DMA ? OpQ::kMine : 1];
 
     // Row i of the P operand's part of a stage: of SwiGLU a wave's first 8 * RT are gate's, the others up's.
-    auto is_up = [&](int i) { return MODE == kRowsSwiglu && i % (16 * RT) >= 8 * RT; };
-    auto row_p = [&](int i) { return MODE == kRowsSwiglu ? i / (16 * RT) * (8 * RT) + i % (8 * RT) : i; };
-    uint32_t off_p[OpP::kMine], off_q[OpQ::kMine];
-    if constexpr (DMA) {
-        OpP::dma_offsets(off_p, wave, p.ldp, [&](int i) { return min(row_p(i), PT ? rows_p - OpP::kPiece : rows_p - 1); });
-        OpQ::dma_offsets(off_q, wave, p.ldq, [&](int i) { return min(i, QT ? rows_q - OpQ::kPiece : rows_q - 1); });
+    static __device__ __forceinline__ bool is_up(int i) {
+        return MODE == kRowsSwiglu && i % (16 * Tile::RT) >= 8 * Tile::RT;
     }
-    auto bring = [&](int st, int buffer) {
+    static __device__ __forceinline__ int row_p(int i) {
+        return MODE == kRowsSwiglu ? i / (16 * Tile::RT) * (8 * Tile::RT) + i % (8 * Tile::RT) : i;
+    }
+
+    __device__ __forceinline__ void open(const RowsMm &p, const RowsPlace &c, int wave) {
+        rows_p = min(p.P - c.p0, MODE == kRowsSwiglu ? Tile::kP / 2 : Tile::kP);
+        rows_q = c.rows_q, length = c.length;
+        stages_half = (length + kStep - 1) / kStep;
+        const int64_t at_p = MODE == kRowsWeight ? c.first * p.ldp + c.p0
+                                                 : c.expert * p.expert_stride + (PT ? c.p0 : c.p0 * p.ldp);
+        const int64_t at_q = QT ? c.first * p.ldq + (int64_t)c.half * p.Q + c.q0 : c.q0 * p.ldq;
+        pm = (const T *)p.p + at_p, pm2 = MODE == kRowsWeight ? pm : (const T *)p.p2 + at_p;
+        qm = (const T *)p.q + at_q, qm2 = MODE == kRowsWeight ? (const T *)p.q2 + at_q : qm;
+        if constexpr (DMA) {
+            OpP::dma_offsets(off_p, wave, p.ldp, [&](int i) { return min(row_p(i), PT ? rows_p - OpP::kPiece : rows_p - 1); });
+            OpQ::dma_offsets(off_q, wave, p.ldq, [&](int i) { return min(i, QT ? rows_q - OpQ::kPiece : rows_q - 1); });
+        }
+    }
+
+    // Stage st to `to`; a stage without elements is zeros.
+    __device__ __forceinline__ void bring(const RowsMm &p, int st, uint8_t *to, int wave) const {
         const bool second = (MODE == kRowsInput || MODE == kRowsWeight) && st >= stages_half;
         const int k0 = (second ? st - stages_half : st) * kStep, left = length - k0;
-        uint8_t *const to = lds + buffer * Tile::kStage;
         const T *const from_p = (second ? pm2 : pm) + (PT ? k0 * p.ldp : k0);
         const T *const from_up = MODE == kRowsSwiglu ? pm2 + k0 : from_p;
         const T *const from_q = (MODE == kRowsWeight && second ? qm2 : qm) +
@@ -316,7 +358,7 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
                     rows_dma(off_q[n], (uint64_t)from_q, at + Tile::kStageP + 1024 * run);
                 }
             } else {  // the sums end inside the stage
-                int in_run = lane;
+                int in_run = threadIdx.x & 63;
                 asm volatile("" : "+v"(in_run));  // one stage of many: nothing kept in registers for it
 #pragma unroll
                 for (int n = 0; n < OpP::kMine; ++n) {
@@ -346,18 +388,251 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
                 return from_q + OpQ::offset(i, k, p.ldq);
             }, to + Tile::kStageP);
         }
+    }
+};
+
+// A tile's sums to the output, straight from the registers: of two tiles side by side lanes exchange halves, so
+// that each holds eight columns of a row and a row's four lanes 64 contiguous bytes (of 16 bits).
+//
+// The code of every epilogue unrolled over a wave's sums would be 150 KB, more than the instruction cache, and
+// cost a tile of 256 x 256 some 8 us.  So plain outputs (whole groups of eight columns) have a path of
+// their own.  kRowsFull has one for each activation, for whole groups too; kRowsAny takes one row of tiles at a time, in a loop that moves the next one's sums into the same
+// registers (which costs registers that the large tiles do not have).
+enum RowsOutput { kRowsPlain, kRowsFull, kRowsAny };
+
+template <class T, RowsMode MODE, RowsOutput KIND, class Tile>
+__device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c, f32x4v (&acc)[Tile::RT][Tile::TT], int wp,
+                                            int wq) {
+    constexpr int RT = Tile::RT, TT = Tile::TT;
+    constexpr int kWaveP = MODE == kRowsSwiglu ? 8 * RT : 16 * RT;  // columns of a wave
+    // Pairs of tiles side by side, or (the small tile's gate and up) of two rows of tiles.
+    constexpr bool kBeside = kWaveP % 32 == 0;
+    static_assert(kBeside || (TT % 2 == 0 && RT == 2 && MODE == kRowsSwiglu), "pairs of tiles");
+    constexpr int kRows = kBeside ? 1 : 2, kPairs = kBeside ? kWaveP / 32 : 1;
+    const int lane = threadIdx.x & 63, r16 = lane & 15, odd = (lane >> 4) & 1, upper = lane >> 5;
+    const bool parts = p.slices > 1, to32 = parts || p.wide;
+    // The output's (or the slice's sums') matrix, and its rows' length.
+    const int64_t cols = MODE == kRowsSwiglu ? 2 * (int64_t)p.P : p.P, matrices = max(p.n_experts, 1);
+    int64_t ld = p.ldy;
+    uint8_t *y;
+    if (parts) {
+        ld = cols;
+        const int64_t all = MODE == kRowsWeight ? p.Q * p.halves * matrices : p.Q;
+        const int64_t mine = MODE == kRowsWeight ? (c.half * matrices + c.expert) * p.Q : 0;
+        y = (uint8_t *)(p.part + (c.slice * all + mine) * cols);
+    } else {
+        y = (uint8_t *)(MODE == kRowsWeight && c.half != 0 ? p.y2 : p.y);
+        if constexpr (MODE == kRowsWeight) y += c.expert * p.expert_stride * (p.wide ? 4 : sizeof(T));
+    }
+    // Row and column of the lane's eight of pair `pair` in row tt of tiles.
+    auto row_of = [&](int tt) { return 16 * (TT * wq + tt + (kBeside ? 0 : odd)) + r16; };
+    auto col_of = [&](int pair) { return c.p0 + kWaveP * wp + (kBeside ? 32 * pair + 16 * odd : 0) + 8 * upper; };
+    auto take = [&](int tt, int pair, float *v, float *up) {
+        if constexpr (kBeside) {
+            rows_exchange(acc[2 * pair][tt], acc[2 * pair + 1][tt], v);
+            if constexpr (MODE == kRowsSwiglu) rows_exchange(acc[RT / 2 + 2 * pair][tt], acc[RT / 2 + 2 * pair + 1][tt], up);
+        } else {
+            rows_exchange(acc[0][tt], acc[0][tt + 1], v);
+            rows_exchange(acc[1][tt], acc[1][tt + 1], up);
+        }
     };
+    const RowsEpilogue &e = p.epi;
+    if constexpr (KIND == kRowsFull && MODE == kRowsForward) {
+        auto all = [&](auto act) {
+#pragma unroll
+            for (int pair = 0; pair < kPairs; ++pair) {
+                const int col = col_of(pair);
+                float bias[8];
+                rows_load8((const T *)e.bias + col, e.bias != nullptr && col < p.P ? 8 : 0, bias);
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt) {
+                    float v[8];
+                    take(tt, pair, v, v);
+                    const int in_tile = row_of(tt);
+                    if (in_tile < c.rows_q && col < p.P) {
+                        const int64_t row = c.q0 + in_tile;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] += bias[i];
+                        if (e.pre != nullptr) rows_store8((T *)e.pre + row * p.P + col, 8, v);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = rows_act<T>(v[i], decltype(act)::value);
+                        if (e.residual != nullptr) {
+                            float r[8];
+                            rows_load8((const T *)e.residual + row * e.residual_stride + col, 8, r);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) v[i] += r[i];
+                        }
+                        rows_store8((T *)y + row * ld + col, 8, v);
+                    }
+                }
+            }
+        };
+        switch (e.act) {
+            case JJO_ACT_RELU: return all(std::integral_constant<int, JJO_ACT_RELU>{});
+            case JJO_ACT_GELU: return all(std::integral_constant<int, JJO_ACT_GELU>{});
+            case JJO_ACT_GELU_TANH: return all(std::integral_constant<int, JJO_ACT_GELU_TANH>{});
+            case JJO_ACT_SILU: return all(std::integral_constant<int, JJO_ACT_SILU>{});
+        }
+        return all(std::integral_constant<int, JJO_ACT_NONE>{});
+    }
+    if (KIND != kRowsAny || (p.P % 8 == 0 && (parts || (e.bias == nullptr && e.residual == nullptr && e.pre == nullptr && e.act == JJO_ACT_NONE)))) {
+        auto all = [&](auto wide_tag) {
+            constexpr bool WIDE = decltype(wide_tag)::value;
+            using Out = std::conditional_t<WIDE, float, T>;
+#pragma unroll
+            for (int tt = 0; tt < TT; tt += kRows)
+#pragma unroll
+                for (int pair = 0; pair < kPairs; ++pair) {
+                    float v[8], up[8];
+                    take(tt, pair, v, up);
+                    const int in_tile = row_of(tt), col = col_of(pair);
+                    if (in_tile < c.rows_q && col < p.P) {
+                        Out *const to = (Out *)y + (c.q0 + in_tile) * ld + col;
+                        if constexpr (MODE == kRowsSwiglu && WIDE) {
+                            rows_store8(to, 8, v);
+                            rows_store8(to + p.P, 8, up);
+                        } else {
+                            if constexpr (MODE == kRowsSwiglu) {
+                                if (KIND == kRowsFull) {
+                                    T *const pre = (T *)e.pre + (int64_t)(c.q0 + in_tile) * 2 * p.P + col;
+                                    rows_store8(pre, 8, v);
+                                    rows_store8(pre + p.P, 8, up);
+                                }
+                                rows_swiglu(v, up);
+                            }
+                            rows_store8(to, 8, v);
+                        }
+                    }
+                }
+        };
+        if (to32) all(std::true_type{});
+        else all(std::false_type{});
+        return;
+    }
+    if constexpr (KIND == kRowsAny)
+#pragma unroll 1
+    for (int tt = 0; tt < TT; tt += kRows) {
+#pragma unroll
+        for (int pair = 0; pair < kPairs; ++pair) {
+            float v[8], up[8];
+            take(0, pair, v, up);
+            const int in_tile = row_of(tt), col = col_of(pair), n = min(8, p.P - col);
+            const int64_t row = c.q0 + in_tile;
+            if (in_tile < c.rows_q && n > 0) {
+                if (parts) {
+                    rows_store8((float *)y + row * ld + col, n, v);
+                    if constexpr (MODE == kRowsSwiglu) rows_store8((float *)y + row * ld + p.P + col, n, up);
+                } else if constexpr (MODE == kRowsSwiglu) {
+                    rows_finish_swiglu<T>(e, v, up, row, col, n, p.P, y);
+                } else {
+                    rows_finish<T>(e, v, row, col, n, p.P, y, ld, p.wide);
+                }
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int t = 0; t + kRows < TT; ++t) acc[rt][t] = acc[rt][t + kRows];
+    }
+}
+
+// ---- four waves, a tile a workgroup, two or more workgroups a CU: one stages while another multiplies.
+template <class E, RowsMode MODE, class Tile, bool DMA>
+__global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
+    typedef typename E::type T;
+    constexpr int RT = Tile::RT, TT = Tile::TT;
+    using Source = RowsSource<T, MODE, Tile, DMA>;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wp = wave % Tile::WP, wq = wave / Tile::WP;
+    RowsTiles<MODE, Tile, Source::kStep> tiles;
+    const RowsRun run(tiles.total(p, gridDim.x));
+    if (run.at >= run.end) return;
+    const RowsPlace c = tiles.place(p, run.at);
+    Source source;
+    source.open(p, c, wave);
 
     f32x4v acc[RT][TT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    const typename Source::OpP::Reader read_p(16 * RT * wp);
+    const typename Source::OpQ::Reader read_q(16 * TT * wq);
+    constexpr int kAhead = Tile::NB - 1;  // stages on their way while one is multiplied
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (c.s_beg + i < c.s_end) source.bring(p, c.s_beg + i, lds + i * Tile::kStage, wave);
+    int buffer = 0;
+    for (int st = c.s_beg; st < c.s_end; ++st) {
+        // Stage st has landed, and no wave reads the buffer of stage st - 1 any more.
+        if (st + kAhead - 1 < c.s_end)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((kAhead - 1) * Source::kDma) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (st + kAhead < c.s_end)
+            source.bring(p, st + kAhead, lds + (buffer == 0 ? Tile::NB - 1 : buffer - 1) * Tile::kStage, wave);
+        const uint8_t *const in_p = lds + buffer * Tile::kStage, *const in_q = in_p + Tile::kStageP;
+        auto step = [&](auto u_tag) {
+            constexpr int U = decltype(u_tag)::value;
+            u32x4v a[RT], b[TT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) a[rt] = read_p.template read<U>(in_p, rt);
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) b[tt] = read_q.template read<U>(in_q, tt);
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) acc[rt][tt] = rows_mfma<T>(a[rt], b[tt], acc[rt][tt]);
+        };
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+        buffer = buffer == Tile::NB - 1 ? 0 : buffer + 1;
+    }
+    rows_output<T, MODE, kRowsAny, Tile>(p, c, acc, wp, wq);
+}
 
-    const typename OpP::Reader read_p(16 * RT * wp);
-    const typename OpQ::Reader read_q(16 * TT * wq);
-    constexpr int kDma = OpP::kMine + OpQ::kMine;  // of a wave and stage
-    constexpr int kAhead = Tile::NB - 1;           // stages on their way while one is multiplied
+// ---- eight waves, a workgroup a CU that goes from tile to tile.
+//
+// Two waves a SIMD, one half of the waves a slot behind the other: while one reads its operands of a step from
+// LDS, the other multiplies.  A barrier ends each slot, four of them a stage.  The stages of a workgroup's
+// tiles are one stream: the next tile's first ones are on their way during a tile's last, and one half of the
+// waves writes its outputs while the other multiplies.
+template <class E, RowsMode MODE, RowsOutput KIND, class Tile>
+__global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, int most) {
+    typedef typename E::type T;
+    constexpr int RT = Tile::RT, TT = Tile::TT;
+    using Source = RowsSource<T, MODE, Tile, true>;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wp = wave % Tile::WP, wq = wave / Tile::WP;
+    RowsTiles<MODE, Tile, Source::kStep> tiles;
+    RowsRun run(tiles.total(p, most));
+    if (run.at >= run.end) return;
+    constexpr int kAhead = Tile::NB - 1;
+    static_assert(kAhead == 1 || kAhead == 2, "the waits below");
+    // The stream's next stage, of the tile `brought`.  A tile without stages has one of zeros.
+    Source source;
+    int brought = run.at, st, st_end, pending = 0;  // pending: stages brought and not multiplied yet
+    auto open = [&]() {
+        const RowsPlace c = tiles.place(p, brought);
+        source.open(p, c, wave);
+        st = c.s_beg, st_end = max(c.s_end, c.s_beg + 1);
+    };
+    open();
+    auto bring = [&](int buffer) {
+        if (st == st_end) {
+            if (brought + run.step >= run.end) return;
+            brought += run.step;
+            open();
+        }
+        source.bring(p, st++, lds + buffer * Tile::kStage, wave);
+        ++pending;
+    };
+
+    f32x4v acc[RT][TT];
+    const typename Source::OpP::Reader read_p(16 * RT * wp);
+    const typename Source::OpQ::Reader read_q(16 * TT * wq);
     u32x4v a[RT], b[TT];
     auto read = [&](auto u_tag, int buffer) {
         constexpr int U = decltype(u_tag)::value;
@@ -367,117 +642,58 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) b[tt] = read_q.template read<U>(in_q, tt);
     };
-    auto multiply = [&]() {
+    auto products = [&]() {
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) acc[rt][tt] = rows_mfma<T>(a[rt], b[tt], acc[rt][tt]);
+        __builtin_amdgcn_s_setprio(0);
+    };
+    auto slot_end = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // The stage behind the current one has landed; the one behind that may be on its way (loads return in order).
+    auto landed = [&](int behind) {
+        if (kAhead == 2 && pending - behind == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(Source::kDma) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     };
     constexpr std::integral_constant<int, 0> kU0{};
     constexpr std::integral_constant<int, 1> kU1{};
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-        if (s_beg + i < s_end) bring(s_beg + i, i);
-    int buffer = 0;
-    if constexpr (Tile::kWaves == 8) {
-        // Two waves a SIMD, one half of the waves a slot behind the other: while one reads its operands of a step,
-        // the other multiplies.  A barrier ends each slot.
-        auto slot_end = [&]() {
-            __builtin_amdgcn_sched_barrier(0);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        // The next stage has landed (stages behind it may be on their way).
-        auto landed = [&](int next) {
-            if (next + kAhead - 1 < s_end) asm volatile("s_waitcnt vmcnt(%0)" ::"i"((kAhead - 1) * kDma) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        };
-        auto products = [&]() {
-            __builtin_amdgcn_s_setprio(1);
-            multiply();
-            __builtin_amdgcn_s_setprio(0);
-        };
-        if (s_beg < s_end) landed(s_beg);
-        slot_end();
-        if (wave >= 4) slot_end();
-        for (int st = s_beg; st < s_end; ++st) {
-            // Into the buffer of stage st - 1, whose last readers' slot has ended.
-            if (st + kAhead < s_end) bring(st + kAhead, buffer == 0 ? Tile::NB - 1 : buffer - 1);
-            read(kU0, buffer);
-            slot_end();
-            products();
-            slot_end();
-            read(kU1, buffer);
-            if (wave >= 4 && st + 1 < s_end) landed(st + 1);
-            slot_end();
-            products();
-            if (wave < 4 && st + 1 < s_end) landed(st + 1);
-            slot_end();
-            buffer = buffer == Tile::NB - 1 ? 0 : buffer + 1;
-        }
-        if (wave < 4) slot_end();
-    } else {
-        for (int st = s_beg; st < s_end; ++st) {
-            // Stage st has landed, and no wave reads the buffer of stage st - 1 any more.
-            if (st + kAhead - 1 < s_end)
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((kAhead - 1) * kDma) : "memory");
-            else
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (st + kAhead < s_end) bring(st + kAhead, buffer == 0 ? Tile::NB - 1 : buffer - 1);
-            read(kU0, buffer);
-            multiply();
-            read(kU1, buffer);
-            multiply();
-            buffer = buffer == Tile::NB - 1 ? 0 : buffer + 1;
-        }
-    }
 
-    // ---- outputs straight from the registers: of two tiles side by side lanes exchange halves, so that each
-    // holds eight columns of a row and a row's four lanes 64 contiguous bytes (of 16 bits).
-    const bool parts = p.slices > 1;
-    void *const y = MODE == kRowsWeight ? (void *)((uint8_t *)(half == 0 ? p.y : p.y2) +
-                                                   expert * p.expert_stride * (p.wide ? 4 : sizeof(T)))
-                                        : p.y;
-    auto finish = [&](int in_tile, int column, float *v, float *up) {
-        const int col = p0 + column, n = min(8, p.P - col);
-        if (in_tile >= rows_q || n <= 0) return;
-        const int64_t row = q0 + in_tile;
-        if (parts) {
-            const int64_t cols = MODE == kRowsSwiglu ? 2 * (int64_t)p.P : p.P;
-            // A slice's rows: of weight those of all matrices.
-            const int64_t matrices = max(p.n_experts, 1);
-            const int64_t all = MODE == kRowsWeight ? p.Q * p.halves * matrices : p.Q;
-            const int64_t mine = MODE == kRowsWeight ? (half * matrices + expert) * p.Q + row : row;
-            float *const to = p.part + (blockIdx.y * all + mine) * cols + col;
-            rows_store8(to, n, v);
-            if constexpr (MODE == kRowsSwiglu) rows_store8(to + p.P, n, up);
-        } else if constexpr (MODE == kRowsSwiglu) {
-            rows_finish_swiglu<T>(p.epi, v, up, row, col, n, p.P, y);
-        } else {
-            rows_finish<T>(p.epi, v, row, col, n, p.P, y, p.ldy, p.wide);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) bring(i);
+    landed(0);
+    slot_end();
+    if (wave >= 4) slot_end();
+    int buffer = 0;
+    for (; run.at < run.end; run.at += run.step) {
+        const RowsPlace c = tiles.place(p, run.at);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = f32x4v{0.f, 0.f, 0.f, 0.f};
+        for (int left = max(c.s_end - c.s_beg, 1); left > 0; --left) {
+            // Into the buffer of the stage before, whose last readers' slot has ended.
+            bring(buffer == 0 ? Tile::NB - 1 : buffer - 1);
+            read(kU0, buffer);
+            slot_end();
+            products();
+            slot_end();
+            read(kU1, buffer);
+            if (wave >= 4) landed(1);
+            slot_end();
+            products();
+            if (wave < 4) landed(1);
+            slot_end();
+            --pending;
+            buffer = buffer == Tile::NB - 1 ? 0 : buffer + 1;
         }
-    };
-    constexpr int kWaveP = MODE == kRowsSwiglu ? 8 * RT : 16 * RT;  // columns of a wave
-    if constexpr (kWaveP % 32 == 0) {
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-            for (int rt = 0; rt < kWaveP / 16; rt += 2) {
-                float v[8], up[8];
-                rows_exchange(acc[rt][tt], acc[rt + 1][tt], v);
-                if constexpr (MODE == kRowsSwiglu) rows_exchange(acc[RT / 2 + rt][tt], acc[RT / 2 + rt + 1][tt], up);
-                finish(16 * (TT * wq + tt) + r16, kWaveP * wp + 16 * (rt + (q4 & 1)) + 8 * (q4 >> 1), v, up);
-            }
-    } else {  // one tile of columns: of two tiles of rows
-        static_assert(TT % 2 == 0 && RT == 2 && MODE == kRowsSwiglu, "the small tile's gate and up");
-#pragma unroll
-        for (int tt = 0; tt < TT; tt += 2) {
-            float v[8], up[8];
-            rows_exchange(acc[0][tt], acc[0][tt + 1], v);
-            rows_exchange(acc[1][tt], acc[1][tt + 1], up);
-            finish(16 * (TT * wq + tt + (q4 & 1)) + r16, 16 * wp + 8 * (q4 >> 1), v, up);
-        }
+        rows_output<T, MODE, KIND, Tile>(p, c, acc, wp, wq);
     }
+    if (wave < 4) slot_end();
 }
 
 template <class E, RowsMode MODE, class Tile, bool DMA>
@@ -485,21 +701,27 @@ hipError_t run_rows(RowsMm p, hipStream_t stream) {
     constexpr int kOutP = MODE == kRowsSwiglu ? Tile::kP / 2 : Tile::kP;
     p.tiles_p = (p.P + kOutP - 1) / kOutP;
     p.tiles_q = (p.Q + Tile::kQ - 1) / Tile::kQ;
-    int64_t wgs;
-    if (MODE == kRowsWeight) {
-        p.tiles_q *= p.halves;
-        wgs = (int64_t)p.tiles_p * p.tiles_q * (p.offsets != nullptr ? p.n_experts : 1);
-        if ((int64_t)p.tiles_p * p.tiles_q > INT32_MAX) return hipErrorInvalidConfiguration;
-    } else {
-        if (p.offsets != nullptr) p.tiles_q += std::min(p.n_experts, p.M);
-        wgs = (int64_t)p.tiles_p * p.tiles_q;
-    }
-    if (wgs * Tile::kThreads >= 1LL << 32) return hipErrorInvalidConfiguration;
-    const auto kernel = rows_mm_kernel<E, MODE, Tile, DMA>;
-    const hipError_t e = ensure_dynamic_lds((const void *)kernel, Tile::kLds);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)wgs, (unsigned)p.slices), dim3(Tile::kThreads), Tile::kLds, stream, p);
-    return hipGetLastError();
+    if (MODE == kRowsWeight) p.tiles_q *= p.halves;
+    else if (p.offsets != nullptr) p.tiles_q += std::min(p.n_experts, p.M);
+    if ((int64_t)p.tiles_p * p.tiles_q > INT32_MAX / 64) return hipErrorInvalidConfiguration;
+    const int64_t most = (int64_t)p.tiles_p * p.tiles_q * p.slices *
+                         (MODE == kRowsWeight && p.offsets != nullptr ? p.n_experts : 1);
+    if (most >= INT32_MAX / 64 || most * Tile::kThreads >= 1LL << 32) return hipErrorInvalidConfiguration;
+    auto go = [&](auto kernel, int wgs, auto... more) {
+        const hipError_t e = ensure_dynamic_lds((const void *)kernel, Tile::kLds);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(Tile::kThreads), Tile::kLds, stream, p, more...);
+        return hipGetLastError();
+    };
+    if constexpr (Tile::kWaves == 8) {
+        const int wgs = (int)std::min<int64_t>(most, device_cu_count());
+        const RowsEpilogue &e = p.epi;
+        if constexpr (MODE == kRowsForward || MODE == kRowsSwiglu)
+            if (p.slices == 1 && (e.bias != nullptr || e.residual != nullptr || e.pre != nullptr || e.act != JJO_ACT_NONE))
+                return go(rows_stream_kernel<E, MODE, kRowsFull, Tile>, wgs, (int)most);
+        return go(rows_stream_kernel<E, MODE, kRowsPlain, Tile>, wgs, (int)most);
+    } else
+        return go(rows_mm_kernel<E, MODE, Tile, DMA>, (int)most);
 }
 
 // DMA where every memory row of both operands is 16-byte aligned, a tile's rows and a stage's elements
@@ -520,18 +742,18 @@ template <class E, RowsMode MODE>
 hipError_t rows_by_tile(const RowsMm &p, int tile, hipStream_t stream) {
     if (!rows_dma_accepts(MODE, (int)sizeof(typename E::type), p)) return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, false>(p, stream);
     switch (tile) {
-        case 0: return run_rows<E, MODE, RowsTile<2, 2, 2, 2>, true>(p, stream);
+        case 0: return run_rows<E, MODE, RowsTile<2, 2, 2, 2, 4>, true>(p, stream);
         case 1: return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, true>(p, stream);
-        case 2: return run_rows<E, MODE, RowsTile<8, 4, 2, 4>, true>(p, stream);
-        case 3: return run_rows<E, MODE, RowsTile<4, 8, 4, 2>, true>(p, stream);
-        case 4: return run_rows<E, MODE, RowsTile<4, 4, 4, 2, 3>, true>(p, stream);
-        case 5: return run_rows<E, MODE, RowsTile<2, 2, 2, 2, 4>, true>(p, stream);
-        case 6: return run_rows<E, MODE, RowsTile<4, 4, 2, 2, 3>, true>(p, stream);
     }
-    if constexpr (MODE != kRowsWeight) {
-        if (tile == 7) return run_rows<E, MODE, RowsTile<4, 5, 4, 2, 3>, true>(p, stream);
-        if (tile == 8) return run_rows<E, MODE, RowsTile<4, 6, 4, 2>, true>(p, stream);
-        if (tile == 9) return run_rows<E, MODE, RowsTile<4, 3, 4, 2, 3>, true>(p, stream);
+    if constexpr (sizeof(typename E::type) == 2) {
+        if (p.P % 8 != 0) return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, true>(p, stream);
+        if (tile == 2) return run_rows<E, MODE, RowsTile<4, 4, 4, 2, 3>, true>(p, stream);
+        if (tile == 3) return run_rows<E, MODE, RowsTile<4, 8, 4, 2>, true>(p, stream);
+        if constexpr (MODE != kRowsWeight) {
+            if (tile == 4) return run_rows<E, MODE, RowsTile<4, 3, 4, 2, 3>, true>(p, stream);
+            if (tile == 5) return run_rows<E, MODE, RowsTile<4, 5, 4, 2, 3>, true>(p, stream);
+            if (tile == 6) return run_rows<E, MODE, RowsTile<4, 6, 4, 2>, true>(p, stream);
+        }
     }
     return hipErrorInvalidValue;
 }
