@@ -125,17 +125,17 @@ __device__ __forceinline__ void rows_store8(T *p, int n, const float *v) {
             if (i < n) p[i] = rows_round<T>(v[i]);
     }
 }
-// The same past the caches (nothing near reads it).
+// Eight values as 16 bytes of T, and 16 bytes to any address past the caches.
 template <class T>
-__device__ __forceinline__ void rows_store8_past(T *p, const float *v) {
-    typedef uint32_t Any __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ u32x4v rows_pack8(const float *v) {
     MxVec<T, 8> a;
 #pragma unroll
     for (int i = 0; i < 8; ++i) a.v[i] = rows_round<T>(v[i]);
-    u32x4v w[sizeof(a) / 16];
-    __builtin_memcpy(w, &a, sizeof(a));
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(a) / 16); ++i) __builtin_nontemporal_store((Any)w[i], (Any *)p + i);
+    return __builtin_bit_cast(u32x4v, a);
+}
+__device__ __forceinline__ void rows_store_past(void *p, u32x4v v) {
+    typedef uint32_t Any __attribute__((ext_vector_type(4), aligned(2)));
+    __builtin_nontemporal_store((Any)v, (Any *)p);
 }
 
 // Sums of columns col.. of a row (n of them) to the output.

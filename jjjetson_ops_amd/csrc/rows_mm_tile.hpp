@@ -485,6 +485,43 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
         }
         return all(std::integral_constant<int, JJO_ACT_NONE>{});
     }
+    // Weights' gradients go past the caches, in whole lines: nothing near reads them, and they would push out what
+    // the tiles beside read (64 experts of 2048 x 1408, 244 tokens each: %NT%).  Stores of 64 bytes a row
+    // reach 3.0 to 4.0 TB/s that way, of 128 bytes 5.6 to 6.3, as through the caches.  So lanes 8..15 of each 16
+    // exchange with 0..7: an instruction writes 128 bytes of eight rows.
+    if constexpr (MODE == kRowsWeight && RT == 4) {
+        if (p.P % 8 == 0) {
+            const bool high = (lane & 8) != 0;
+            auto lines = [&](u32x4v a, u32x4v b, int tt, int col, auto out) {
+                using Out = decltype(out);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t x = __builtin_amdgcn_update_dpp(0, high ? a[i] : b[i], 0x128, 0xf, 0xf, false);  // row_ror:8
+                    a[i] = high ? x : a[i], b[i] = high ? b[i] : x;
+                }
+                const int in_tile = 16 * (TT * wq + tt) + (r16 & 7);
+                if (col >= p.P) return;
+                Out *const to = (Out *)y + (c.q0 + in_tile) * ld + col;
+                if (in_tile < c.rows_q) rows_store_past(to, a);
+                if (in_tile + 8 < c.rows_q) rows_store_past(to + 8 * ld, b);
+            };
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) {
+                if (sizeof(T) == 4 || to32) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt += 2)
+                        lines(__builtin_bit_cast(u32x4v, acc[rt][tt]), __builtin_bit_cast(u32x4v, acc[rt + 1][tt]), tt,
+                              c.p0 + kWaveP * wp + 16 * (rt + high) + 4 * (lane >> 4), 0.0f);
+                } else if constexpr (sizeof(T) == 2) {
+                    float v[8], w[8];
+                    take(tt, 0, v, v);
+                    take(tt, 1, w, w);
+                    lines(rows_pack8<T>(v), rows_pack8<T>(w), tt, col_of(high), (T)0.0f);
+                }
+            }
+            return;
+        }
+    }
     if (KIND != kRowsAny || (p.P % 8 == 0 && (parts || (e.bias == nullptr && e.residual == nullptr && e.pre == nullptr && e.act == JJO_ACT_NONE)))) {
         auto all = [&](auto wide_tag) {
             constexpr bool WIDE = decltype(wide_tag)::value;
@@ -510,8 +547,7 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
                                 }
                                 rows_swiglu(v, up);
                             }
-                            if constexpr (MODE == kRowsWeight) rows_store8_past(to, v);
-                            else rows_store8(to, 8, v);
+                            rows_store8(to, 8, v);
                         }
                     }
                 }
