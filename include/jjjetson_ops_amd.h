@@ -701,9 +701,11 @@ int moe_rows_gate_up_swiglu_backward_device(void *stream, const void *grad_mid, 
  * form 0: y [rows][cols] = q [rows][sums] . p [cols][sums]^T; 1: SwiGLU, p gate and p2 up; 2: y = q
  * [rows][sums] . p [sums][cols] (p2 not NULL: q [rows][2 sums], its second half times p2 is added); 3: y
  * [rows][cols] = q [sums][rows]^T . p [sums][cols] (y2 not NULL: q [sums][2 rows], the second half's
- * rows go to y2).  expert_offsets NULL, or of sorted rows (forms 0 to 2) or of the sums (3).  kernel: 0 to 2
- * the LDS tiles, 64 + w and 80 + w (forms 0 and 1) the direct kernel on w <= 8 waves with one or two
- * tiles of 16 rows.  slices of the sums, each 4 bytes an output of the workspace where more than one.
+ * rows go to y2).  expert_offsets NULL, or of sorted rows (forms 0 to 2) or of the sums (3).  kernel: LDS tiles
+ * of 64 x 64 (0), 128 x 128 (1), 256 columns x 160 rows (2; not form 3) or 256 x 256 (3; both 16 bits only and
+ * cols % 8 == 0: else tile 1 runs), 64 + w the direct kernel on w <= 8 waves (forms 0 and 1).  Operands whose
+ * rows are not 16-byte aligned take tile 1 through registers.  slices of the sums, each 4 bytes an output
+ * of the workspace where more than one.
  */
 int jjo_rows_kernel_device(void *stream, int form, int kernel, int slices, int dtype, const void *p, const void *p2,
                            const void *q, const int32_t *expert_offsets, int n_experts, void *y, void *y2, int cols,

@@ -1061,7 +1061,8 @@ def moe_gate_up_swiglu_rows_backward(grad_mid, gate_up, x, w_gate, w_up, expert_
 
 
 ROWS_FORWARD, ROWS_SWIGLU, ROWS_INPUT, ROWS_WEIGHT = range(4)
-ROWS_DIRECT = 64  # + 16 * (tiles of 16 rows - 1) + waves
+ROWS_TILE_64, ROWS_TILE_128, ROWS_TILE_160, ROWS_TILE_256 = range(4)
+ROWS_DIRECT = 64  # + waves
 
 
 def rows_kernel(form: int, kernel: int, p, q, y, cols: int, rows: int, sums: int, p2=None, y2=None, offsets=None,

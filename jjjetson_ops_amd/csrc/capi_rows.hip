@@ -81,7 +81,7 @@ RowsMm product(RowsMode mode, int dtype, int P, int Q, int K, int halves, int n_
     m.P = P, m.Q = Q, m.K = K, m.halves = halves, m.terms = 1;
     m.n_experts = n_experts;
     m.M = mode == kRowsWeight ? K : Q;
-    m.slices = rows_mm_slices(mode, dtype, P, Q, K, halves, n_experts, m.M);
+    m.slices = rows_mm_choose(mode, dtype, P, Q, K, halves, n_experts).slices;
     return m;
 }
 
@@ -403,10 +403,10 @@ int jjo_rows_kernel_device(void *stream, int form, int kernel, int slices, int d
     const char *who = "jjo_rows_kernel";
     JJO_TRY(check_sizes(who, dtype, cols, sums, rows, expert_offsets != nullptr ? n_experts : 1));
     const int es = elem_bytes(dtype), halves = (form == kRowsInput ? (const void *)p2 : y2) != nullptr ? 2 : 1;
-    const int waves = kernel >= 64 ? kernel % 16 : 0, tiles16 = kernel >= 64 ? kernel / 16 - 3 : 0;
     const bool direct = kernel >= 64;
+    const int waves = direct ? kernel - 64 : 0;
     if (form < kRowsForward || form > kRowsWeight || slices < 1 || slices > 64 || kernel < 0 ||
-        (direct ? form > kRowsSwiglu || slices != 1 || tiles16 > 2 || waves < 1 || waves > 8 : kernel >= kRowsTiles))
+        (direct ? form > kRowsSwiglu || slices != 1 || waves < 1 || waves > 8 : kernel >= kRowsTileKinds))
         return set_error(JJO_ERR_INVALID_ARG, "%s: form %d has no kernel %d in %d slices", who, form, kernel, slices);
     JJO_TRY(check_ptr(who, "p", p, es));
     JJO_TRY(check_ptr(who, "p2", p2, es, form != kRowsSwiglu));
@@ -423,7 +423,7 @@ int jjo_rows_kernel_device(void *stream, int form, int kernel, int slices, int d
     JJO_TRY(check_workspace(who, workspace, workspace_bytes, rows_part_bytes((RowsMode)form, m)));
     JJO_TRY(require_device());
     m.p = p, m.p2 = p2, m.q = q, m.y = y, m.y2 = y2, m.offsets = expert_offsets, m.part = (float *)workspace;
-    const RowsChoice choice{direct ? -tiles16 : kernel, waves};
+    const RowsChoice choice{direct ? (int)kRowsDirect : kernel, waves, slices};
     return launched(launch_rows_mm((RowsMode)form, dtype, m, (hipStream_t)stream, &choice), "jjo_rows_kernel launch");
 }
 

@@ -181,20 +181,20 @@ __device__ __forceinline__ void rows_finish_swiglu(const RowsEpilogue &e, float 
 }
 
 // ---- launchers (asynchronous; arguments validated by the entries)
-struct RowsChoice;
+// The kernel of a product: LDS tiles of 64 x 64, 128 x 128, 256 columns x 160 rows (not weight) or 256 x 256
+// (the last two 16 bits only), or the direct kernel with `waves` that cut the sums between them (forward and
+// SwiGLU); and the slices of the sums that join their fp32 outputs in a second launch.
+enum RowsTileKind { kRowsDirect = -1, kRowsTile64, kRowsTile128, kRowsTile160, kRowsTile256, kRowsTileKinds };
+struct RowsChoice {
+    int tile, waves, slices;
+};
+// By the sizes alone (the workspace depends on it).  n_experts 0: one matrix.
+RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int halves, int n_experts);
 hipError_t launch_rows_mm(RowsMode mode, int dtype, const RowsMm &p, hipStream_t stream,
                           const RowsChoice *pinned = nullptr);
-// Slices that launch_rows_mm is best given for a product, and the bytes of their sums.
-int rows_mm_slices(RowsMode mode, int dtype, int P, int Q, int K, int halves, int n_experts, int M);
 int64_t rows_part_bytes(RowsMode mode, const RowsMm &p);
 
 
-// The kernel for a product: an LDS tile (>= 0), or the direct kernel with one (-1) or two (-2) tiles of 16
-// rows and so many waves that cut K between them.
-struct RowsChoice {
-    int tile, waves;
-};
-constexpr int kRowsTiles = 7;
 template <class E>
 hipError_t rows_mm_run(RowsMode mode, const RowsMm &p, const RowsChoice &c, hipStream_t stream);
 

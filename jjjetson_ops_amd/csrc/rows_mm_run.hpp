@@ -7,11 +7,10 @@ namespace jjo {
 
 template <class E>
 hipError_t rows_mm_run(RowsMode mode, const RowsMm &p, const RowsChoice &c, hipStream_t stream) {
-    if (c.tile < 0) {
-        const bool two = c.tile == -2;  // tiles of 16 rows
-        if (mode == kRowsSwiglu)
-            return two ? run_rows_direct<E, true, 2, 2>(p, c.waves, stream) : run_rows_direct<E, true, 2, 1>(p, c.waves, stream);
-        return two ? run_rows_direct<E, false, 2, 2>(p, c.waves, stream) : run_rows_direct<E, false, 1, 1>(p, c.waves, stream);
+    if (c.tile == kRowsDirect) {
+        if (mode == kRowsForward) return run_rows_direct<E, false, 1, 1>(p, c.waves, stream);
+        if (mode == kRowsSwiglu) return run_rows_direct<E, true, 2, 1>(p, c.waves, stream);
+        return hipErrorInvalidValue;
     }
     switch (mode) {
         case kRowsForward: return rows_by_tile<E, kRowsForward>(p, c.tile, stream);

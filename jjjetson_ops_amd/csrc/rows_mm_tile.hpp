@@ -787,22 +787,16 @@ inline bool rows_dma_accepts(RowsMode mode, int es, const RowsMm &p) {
 
 template <class E, RowsMode MODE>
 hipError_t rows_by_tile(const RowsMm &p, int tile, hipStream_t stream) {
-    if (!rows_dma_accepts(MODE, (int)sizeof(typename E::type), p)) return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, false>(p, stream);
-    switch (tile) {
-        case 0: return run_rows<E, MODE, RowsTile<2, 2, 2, 2, 4>, true>(p, stream);
-        case 1: return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, true>(p, stream);
-    }
+    if (!rows_dma_accepts(MODE, (int)sizeof(typename E::type), p))
+        return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, false>(p, stream);
+    if (tile == kRowsTile64) return run_rows<E, MODE, RowsTile<2, 2, 2, 2, 4>, true>(p, stream);
     if constexpr (sizeof(typename E::type) == 2) {
-        if (p.P % 8 != 0) return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, true>(p, stream);
-        if (tile == 2) return run_rows<E, MODE, RowsTile<4, 4, 4, 2, 3>, true>(p, stream);
-        if (tile == 3) return run_rows<E, MODE, RowsTile<4, 8, 4, 2>, true>(p, stream);
-        if constexpr (MODE != kRowsWeight) {
-            if (tile == 4) return run_rows<E, MODE, RowsTile<4, 3, 4, 2, 3>, true>(p, stream);
-            if (tile == 5) return run_rows<E, MODE, RowsTile<4, 5, 4, 2, 3>, true>(p, stream);
-            if (tile == 6) return run_rows<E, MODE, RowsTile<4, 6, 4, 2>, true>(p, stream);
-        }
+        // The large tiles write whole groups of eight columns.
+        if (tile == kRowsTile256 && p.P % 8 == 0) return run_rows<E, MODE, RowsTile<4, 8, 4, 2>, true>(p, stream);
+        if constexpr (MODE != kRowsWeight)
+            if (tile == kRowsTile160 && p.P % 8 == 0) return run_rows<E, MODE, RowsTile<4, 5, 4, 2, 3>, true>(p, stream);
     }
-    return hipErrorInvalidValue;
+    return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, true>(p, stream);
 }
 
 }  // namespace
