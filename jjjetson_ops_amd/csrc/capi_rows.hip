@@ -109,18 +109,18 @@ RowsMm weight(int dtype, int K, int N, int rows, int n_experts, int halves, bool
     return m;
 }
 
-// The gradient through an activation in 16 bits, and where the weights' gradients are fp32 what that rounding
-// left, in 16 bits again: the sums of both are those of a gradient of 16 (bf16) or 22 bits (fp16).
-int64_t gz_bytes(int dtype, int64_t values) { return up256(elem_bytes(dtype) * values); }
-int64_t gz_planes(int dtype) { return dtype == JJO_DTYPE_F32 ? 1 : 2; }
+// The gradient through an activation, rounded to `dtype`.  Where the weights' gradients are fp32 and it is not, what
+// the rounding left is kept as well, rounded again: two terms of fp16 are 22 bits, three of bf16 24.
+int64_t gz_plane_bytes(int dtype, int64_t values) { return up256(elem_bytes(dtype) * values); }
+int gz_planes(int dtype) { return dtype == JJO_DTYPE_F32 ? 1 : dtype == JJO_DTYPE_F16 ? 2 : 3; }
 
 struct LinearBackwardWs {
-    int64_t gz, rest, columns, parts, bytes;  // offsets
+    int64_t gz, plane, columns, parts, bytes;  // offsets; bytes of a plane of gz
 };
 LinearBackwardWs linear_backward_ws(int dtype, int K, int N, int T) {
     LinearBackwardWs w{};
-    w.rest = gz_bytes(dtype, (int64_t)T * N);
-    w.columns = gz_planes(dtype) * w.rest;
+    w.plane = gz_plane_bytes(dtype, (int64_t)T * N);
+    w.columns = gz_planes(dtype) * w.plane;
     w.parts = w.columns + up256(4LL * rows_column_chunks(T, N) * N);
     w.bytes = w.parts + up256(std::max(rows_part_bytes(kRowsInput, input(dtype, K, N, T, 0, 1)),
                                        rows_part_bytes(kRowsWeight, weight(dtype, K, N, T, 0, 1, false))));
@@ -212,9 +212,9 @@ int linear_rows_backward_device(void *stream, const void *grad_y, int64_t grad_y
     uint8_t *const base = (uint8_t *)workspace;
     const void *gz = grad_y;
     int64_t gz_stride = stride_of(grad_y_stride, N, T);
-    void *const rest = act && wide && dtype != JJO_DTYPE_F32 && grad_weight != nullptr ? base + ws.rest : nullptr;
+    const int planes = act && wide && grad_weight != nullptr ? gz_planes(dtype) : 1;
     if (act || grad_bias != nullptr) {
-        const hipError_t e = launch_rows_act_backward(grad_y, gz_stride, pre, base + ws.gz, rest, dtype, activation,
+        const hipError_t e = launch_rows_act_backward(grad_y, gz_stride, pre, base + ws.gz, planes, ws.plane / es, dtype, activation,
                                                       grad_bias, wide, (float *)(base + ws.columns), T, N, s);
         if (e != hipSuccess) return launched(e, "linear_rows_backward activation");
         if (act) gz = base + ws.gz, gz_stride = N;
@@ -229,7 +229,7 @@ int linear_rows_backward_device(void *stream, const void *grad_y, int64_t grad_y
     if (grad_weight != nullptr) {
         RowsMm m = weight(dtype, K, N, T, 0, 1, wide);
         m.p = x, m.ldp = stride_of(x_stride, K, T), m.q = gz, m.ldq = gz_stride, m.y = grad_weight;
-        if (rest != nullptr) m.q2 = rest, m.terms = 2;
+        if (planes > 1) m.rest = base + ws.gz + ws.plane, m.rest_plane = ws.plane / es, m.terms = planes;
         m.part = (float *)(base + ws.parts);
         const hipError_t e = launch_rows_mm(kRowsWeight, dtype, m, s);
         if (e != hipSuccess) return launched(e, "linear_rows_backward weight");
@@ -341,7 +341,7 @@ int64_t moe_rows_gate_up_swiglu_backward_workspace_bytes(int dtype, int hidden_s
     if (check_sizes("moe_rows_gate_up_swiglu_backward", dtype, hidden_size, intermediate_size, n_routes, num_experts) !=
         JJO_OK)
         return -1;
-    return gz_planes(dtype) * gz_bytes(dtype, 2LL * n_routes * intermediate_size) +
+    return gz_planes(dtype) * gz_plane_bytes(dtype, 2LL * n_routes * intermediate_size) +
            grouped_backward_bytes(dtype, hidden_size, intermediate_size, n_routes, num_experts, 2);
 }
 
@@ -375,10 +375,10 @@ int moe_rows_gate_up_swiglu_backward_device(void *stream, const void *grad_mid, 
     JJO_TRY(require_device());
     hipStream_t s = (hipStream_t)stream;
     uint8_t *const gz = (uint8_t *)workspace;
-    const int64_t plane = gz_bytes(dtype, 2LL * R * I);
-    void *const rest = grad_weights_dtype != dtype && grad_w_gate != nullptr ? gz + plane : nullptr;
+    const int64_t plane = gz_plane_bytes(dtype, 2LL * R * I);
+    const int planes = grad_weights_dtype != dtype && grad_w_gate != nullptr ? gz_planes(dtype) : 1;
     float *const part = (float *)(gz + gz_planes(dtype) * plane);
-    hipError_t e = launch_rows_swiglu_backward(grad_mid, gate_up, gz, rest, dtype, expert_offsets, E, I, R, s);
+    hipError_t e = launch_rows_swiglu_backward(grad_mid, gate_up, gz, planes, plane / es, dtype, expert_offsets, E, I, R, s);
     if (e != hipSuccess) return launched(e, "moe_rows_gate_up_swiglu_backward activation");
     if (grad_x_sorted != nullptr) {
         RowsMm m = input(dtype, H, I, R, E, 2);
@@ -389,7 +389,7 @@ int moe_rows_gate_up_swiglu_backward_device(void *stream, const void *grad_mid, 
     if (grad_w_gate != nullptr) {
         RowsMm m = weight(dtype, H, I, R, E, 2, grad_weights_dtype == JJO_DTYPE_F32);
         m.p = x_sorted, m.q = gz, m.y = grad_w_gate, m.y2 = grad_w_up, m.offsets = expert_offsets, m.part = part;
-        if (rest != nullptr) m.q2 = rest, m.terms = 2;
+        if (planes > 1) m.rest = gz + plane, m.rest_plane = plane / es, m.terms = planes;
         if ((e = launch_rows_mm(kRowsWeight, dtype, m, s)) != hipSuccess)
             return launched(e, "moe_rows_gate_up_swiglu_backward weights");
     }

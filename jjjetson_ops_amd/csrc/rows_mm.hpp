@@ -26,13 +26,14 @@ struct RowsEpilogue {
 // are contiguous (forward), or the rows' of an element are (weight; input: of P).
 struct RowsMm {
     const void *p, *p2;  // p2: the up matrix (SwiGLU), or the operand of the sums' second half (input)
-    const void *q, *q2;  // q2: what is left of q's values behind their rounding (weight, terms 2)
+    const void *q, *rest;  // rest: what q's rounding left, terms - 1 matrices (weight)
+    int64_t rest_plane;    // elements from one of these to the next
     int64_t ldp, ldq;  // elements from one memory row to the next
     void *y, *y2;      // y2: of the second half's output rows (weight)
     int64_t ldy;
     int P, Q, K;
     int halves;              // 2: input sums over p, then over p2; weight has rows of y, then of y2
-    int terms;               // of q in a weight's sums: 1, or 2 (q, then q2)
+    int terms;               // of q in a weight's sums: q, then those of rest
     const int32_t *offsets;  // [n_experts + 1], or nullptr
     int n_experts, M;        // M: sorted rows
     int64_t expert_stride;   // elements of a matrix (of an expert's part of y: weight)
@@ -198,14 +199,14 @@ int64_t rows_part_bytes(RowsMode mode, const RowsMm &p);
 template <class E>
 hipError_t rows_mm_run(RowsMode mode, const RowsMm &p, const RowsChoice &c, hipStream_t stream);
 
-// gz[t] = grad_y[t] * act'(pre[t]) (act none: not written; rest, where not null: what its rounding left) and the columns' sums of gz (sums nullable;
+// gz[t] = grad_y[t] * act'(pre[t]) (act none: not written; planes - 1 more matrices behind it: what the rounding left, rounded) and the columns' sums of gz (sums nullable;
 // column_part: rows_column_chunks(T, N) * N floats).
 int rows_column_chunks(int T, int N);
-hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, const void *pre, void *gz, void *rest,
-                                    int dtype, int act, void *sums, bool sums_wide, float *column_part, int T, int N,
+hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, const void *pre, void *gz, int planes,
+                                    int64_t plane, int dtype, int act, void *sums, bool sums_wide, float *column_part, int T, int N,
                                     hipStream_t stream);
 // grad_gate_up [R][2I] from grad_mid and the saved gate|up, rows below offsets[n_experts].
-hipError_t launch_rows_swiglu_backward(const void *grad_mid, const void *gate_up, void *grad_gate_up, void *rest, int dtype,
+hipError_t launch_rows_swiglu_backward(const void *grad_mid, const void *gate_up, void *grad_gate_up, int planes, int64_t plane, int dtype,
                                        const int32_t *offsets, int n_experts, int I, int R, hipStream_t stream);
 
 }  // namespace jjo

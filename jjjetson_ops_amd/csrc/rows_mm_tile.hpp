@@ -175,16 +175,30 @@ __device__ __forceinline__ void rows_dma(uint32_t off, uint64_t from, uint32_t l
     asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(from), "{m0}"(m0v) : "memory");
 }
 
-// Workgroups go to the eight XCDs in turn: each XCD takes a contiguous run of the tiles, its workgroups
-// neighbours of it, so that tiles that read the same rows are read into one L2.  A workgroup's tiles
+// Workgroups go to the eight XCDs in turn.  Each XCD takes a contiguous run of the tiles, its workgroups
+// neighbours of it, so that tiles that read the same rows are read into one L2; or (tiles of unequal length) the
+// XCDs take turns at chunks of 32, an XCD's workgroups (gradients of 8 experts' 28672 x 4096 matrices, one
+// expert a run: as long as the one with the most tokens, 444 of 2048, %CHUNK%).  A workgroup's places
 // are at, at + step, ... below end.
 struct RowsRun {
-    int at, step, end;
-    __device__ __forceinline__ explicit RowsRun(int total) {
-        const int per = total / 8, rest = total % 8, xcd = blockIdx.x % 8, beg = xcd * per + min(xcd, rest);
-        at = beg + (int)(blockIdx.x / 8);
+    int at, step, end, beg, xcd;
+    bool chunked;
+    __device__ __forceinline__ RowsRun(int total, bool unequal) {
+        xcd = blockIdx.x % 8;
+        at = blockIdx.x / 8;
         step = ((int)gridDim.x - xcd + 7) / 8;
-        end = beg + per + (xcd < rest);
+        chunked = unequal && total >= 1024;
+        if (chunked) {
+            const int chunks = (total + 31) / 32, mine = (chunks - xcd + 7) / 8;
+            const bool last = (chunks - 1) % 8 == xcd;
+            beg = 0, end = 32 * mine - (last ? 32 * chunks - total : 0);
+        } else {
+            const int per = total / 8, rest = total % 8;
+            beg = xcd * per + min(xcd, rest), end = per + (xcd < rest);
+        }
+    }
+    __device__ __forceinline__ int tile(int place) const {
+        return chunked ? (place / 32 * 8 + xcd) * 32 + place % 32 : beg + place;
     }
 };
 
@@ -318,7 +332,7 @@ struct RowsSource {
     static constexpr int kDma = OpP::kMine + OpQ::kMine;  // of a wave and stage
 
     // From the tile's first row and the sums' first element on; the second ones: up's rows (SwiGLU), the sums'
-    // second half (input, and weight with two terms).
+    // second half (input), and what q's rounding left (weight).
     const T *pm, *pm2, *qm, *qm2;
     int rows_p, rows_q, length, stages_half;
     uint32_t off_p[DMA ? OpP::kMine : 1], off_q[DMA ? OpQ::kMine : 1];
@@ -339,7 +353,7 @@ struct RowsSource {
                                                  : c.expert * p.expert_stride + (PT ? c.p0 : c.p0 * p.ldp);
         const int64_t at_q = QT ? c.first * p.ldq + (int64_t)c.half * p.Q + c.q0 : c.q0 * p.ldq;
         pm = (const T *)p.p + at_p, pm2 = MODE == kRowsWeight ? pm : (const T *)p.p2 + at_p;
-        qm = (const T *)p.q + at_q, qm2 = MODE == kRowsWeight ? (const T *)p.q2 + at_q : qm;
+        qm = (const T *)p.q + at_q, qm2 = MODE == kRowsWeight ? (const T *)p.rest + at_q : qm;
         if constexpr (DMA) {
             OpP::dma_offsets(off_p, wave, p.ldp, [&](int i) { return min(row_p(i), PT ? rows_p - OpP::kPiece : rows_p - 1); });
             OpQ::dma_offsets(off_q, wave, p.ldq, [&](int i) { return min(i, QT ? rows_q - OpQ::kPiece : rows_q - 1); });
@@ -348,11 +362,14 @@ struct RowsSource {
 
     // Stage st to `to`; a stage without elements is zeros.
     __device__ __forceinline__ void bring(const RowsMm &p, int st, uint8_t *to, int wave) const {
-        const bool second = (MODE == kRowsInput || MODE == kRowsWeight) && st >= stages_half;
-        const int k0 = (second ? st - stages_half : st) * kStep, left = length - k0;
+        // The half or term of the sums that stage st belongs to.
+        const int part = MODE == kRowsInput ? st >= stages_half
+                         : MODE == kRowsWeight ? (st >= stages_half) + (st >= 2 * stages_half) : 0;
+        const bool second = part > 0;
+        const int k0 = (st - part * stages_half) * kStep, left = length - k0;
         const T *const from_p = (second ? pm2 : pm) + (PT ? k0 * p.ldp : k0);
         const T *const from_up = MODE == kRowsSwiglu ? pm2 + k0 : from_p;
-        const T *const from_q = (MODE == kRowsWeight && second ? qm2 : qm) +
+        const T *const from_q = (MODE == kRowsWeight && second ? qm2 + (part - 1) * p.rest_plane : qm) +
                                 (QT ? k0 * p.ldq : (second ? p.K : 0) + (int64_t)k0);
         if constexpr (DMA) {
             const uint32_t at = (uint32_t)(uintptr_t)to;
@@ -585,7 +602,7 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
 
 // ---- four waves, a tile a workgroup, two or more workgroups a CU: one stages while another multiplies.
 template <class E, RowsMode MODE, class Tile, bool DMA>
-__global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
+__global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p, int most) {
     typedef typename E::type T;
     constexpr int RT = Tile::RT, TT = Tile::TT;
     using Source = RowsSource<T, MODE, Tile, DMA>;
@@ -593,9 +610,9 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wp = wave % Tile::WP, wq = wave / Tile::WP;
     RowsTiles<MODE, Tile, Source::kStep> tiles;
-    const RowsRun run(tiles.total(p, gridDim.x));
+    const RowsRun run(tiles.total(p, most), MODE == kRowsWeight);
     if (run.at >= run.end) return;
-    const RowsPlace c = tiles.place(p, run.at);
+    const RowsPlace c = tiles.place(p, run.tile(run.at));
     Source source;
     source.open(p, c, wave);
 
@@ -627,10 +644,21 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p) {
             for (int rt = 0; rt < RT; ++rt) a[rt] = read_p.template read<U>(in_p, rt);
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt) b[tt] = read_q.template read<U>(in_q, tt);
+            if constexpr (sizeof(T) == 4) {  // in turn: the next sum of a tile does not wait for its last
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) acc[rt][tt] = rows_mfma<T>(a[rt], b[tt], acc[rt][tt]);
+                    for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+                            acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                __uint_as_float(a[rt][j]), __uint_as_float(b[tt][j]), acc[rt][tt], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) acc[rt][tt] = rows_mfma<T>(a[rt], b[tt], acc[rt][tt]);
+            }
         };
         step(std::integral_constant<int, 0>{});
         step(std::integral_constant<int, 1>{});
@@ -654,7 +682,7 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, i
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wp = wave % Tile::WP, wq = wave / Tile::WP;
     RowsTiles<MODE, Tile, Source::kStep> tiles;
-    RowsRun run(tiles.total(p, most));
+    RowsRun run(tiles.total(p, most), MODE == kRowsWeight);
     if (run.at >= run.end) return;
     constexpr int kAhead = Tile::NB - 1;
     static_assert(kAhead == 1 || kAhead == 2, "the waits below");
@@ -662,7 +690,7 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, i
     Source source;
     int brought = run.at, st, st_end, pending = 0;  // pending: stages brought and not multiplied yet
     auto open = [&]() {
-        const RowsPlace c = tiles.place(p, brought);
+        const RowsPlace c = tiles.place(p, run.tile(brought));
         source.open(p, c, wave);
         st = c.s_beg, st_end = max(c.s_end, c.s_beg + 1);
     };
@@ -717,7 +745,7 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, i
     if (wave >= 4) slot_end();
     int buffer = 0;
     for (; run.at < run.end; run.at += run.step) {
-        const RowsPlace c = tiles.place(p, run.at);
+        const RowsPlace c = tiles.place(p, run.tile(run.at));
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -753,22 +781,24 @@ hipError_t run_rows(RowsMm p, hipStream_t stream) {
     if ((int64_t)p.tiles_p * p.tiles_q > INT32_MAX / 64) return hipErrorInvalidConfiguration;
     const int64_t most = (int64_t)p.tiles_p * p.tiles_q * p.slices *
                          (MODE == kRowsWeight && p.offsets != nullptr ? p.n_experts : 1);
-    if (most >= INT32_MAX / 64 || most * Tile::kThreads >= 1LL << 32) return hipErrorInvalidConfiguration;
-    auto go = [&](auto kernel, int wgs, auto... more) {
+    // Whole chunks of every XCD.
+    const int64_t blocks = MODE == kRowsWeight ? (most + 255) / 256 * 256 : most;
+    if (most >= INT32_MAX / 64 || blocks * Tile::kThreads >= 1LL << 32) return hipErrorInvalidConfiguration;
+    auto go = [&](auto kernel, int wgs) {
         const hipError_t e = ensure_dynamic_lds((const void *)kernel, Tile::kLds);
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(Tile::kThreads), Tile::kLds, stream, p, more...);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(Tile::kThreads), Tile::kLds, stream, p, (int)most);
         return hipGetLastError();
     };
     if constexpr (Tile::kWaves == 8) {
-        const int wgs = (int)std::min<int64_t>(most, device_cu_count());
+        const int wgs = (int)std::min<int64_t>(blocks, device_cu_count());
         const RowsEpilogue &e = p.epi;
         if constexpr (MODE == kRowsForward || MODE == kRowsSwiglu)
             if (p.slices == 1 && (e.bias != nullptr || e.residual != nullptr || e.pre != nullptr || e.act != JJO_ACT_NONE))
-                return go(rows_stream_kernel<E, MODE, kRowsFull, Tile>, wgs, (int)most);
-        return go(rows_stream_kernel<E, MODE, kRowsPlain, Tile>, wgs, (int)most);
+                return go(rows_stream_kernel<E, MODE, kRowsFull, Tile>, wgs);
+        return go(rows_stream_kernel<E, MODE, kRowsPlain, Tile>, wgs);
     } else
-        return go(rows_mm_kernel<E, MODE, Tile, DMA>, (int)most);
+        return go(rows_mm_kernel<E, MODE, Tile, DMA>, (int)blocks);
 }
 
 // DMA where every memory row of both operands is 16-byte aligned, a tile's rows and a stage's elements
@@ -780,7 +810,7 @@ inline bool rows_dma_accepts(RowsMode mode, int es, const RowsMm &p) {
     };
     if (!fits(p.p, p.ldp) || !fits(p.q, p.ldq)) return false;
     if (p.p2 != nullptr && !fits(p.p2, p.ldp)) return false;
-    if (p.q2 != nullptr && !fits(p.q2, p.ldq)) return false;
+    if (p.rest != nullptr && (!fits(p.rest, p.ldq) || p.rest_plane % piece != 0)) return false;
     if (mode == kRowsWeight) return p.P % piece == 0 && p.Q % piece == 0;
     return p.K % piece == 0 && (mode != kRowsInput || p.P % piece == 0);
 }

@@ -44,23 +44,25 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsMm p, int chunks, in
     }
 }
 
-// Eight values rounded to T and, where it is wanted, what the rounding left of them.
+// Eight values rounded to T and, in the planes behind, what the rounding left of them, rounded again.
 template <class T>
-__device__ __forceinline__ void store_split(void *to, void *rest, int64_t at, int n, const float *v) {
-    rows_store8((T *)to + at, n, v);
-    if (rest == nullptr) return;
+__device__ __forceinline__ void store_split(void *to, int planes, int64_t plane, int64_t at, int n, const float *v) {
     float r[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = v[i] - (float)(T)v[i];
-    rows_store8((T *)rest + at, n, r);
+    for (int i = 0; i < 8; ++i) r[i] = v[i];
+    for (int k = 0; k < planes; ++k) {
+        rows_store8((T *)to + k * plane + at, n, r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] -= (float)rows_round<T>(r[i]);
+    }
 }
 
 constexpr int kColumnsAtOnce = 512;  // of a workgroup: 64 lanes x 8; its four waves take every fourth row
 
 template <class E>
 __global__ __launch_bounds__(256) void rows_act_backward_kernel(const void *grad_y, int64_t grad_y_stride,
-                                                                const void *pre, void *gz, void *rest, int act,
-                                                                float *part, int T_, int N) {
+                                                                const void *pre, void *gz, int planes,
+                                                                int64_t plane, int act, float *part, int T_, int N) {
     typedef typename E::type T;
     __shared__ float sums[4][kColumnsAtOnce];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -75,7 +77,7 @@ __global__ __launch_bounds__(256) void rows_act_backward_kernel(const void *grad
                 rows_load8((const T *)pre + (int64_t)t * N + col, n, z);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) g[i] *= rows_slope<T>(z[i], act);
-                store_split<T>(gz, rest, (int64_t)t * N + col, n, g);
+                store_split<T>(gz, planes, plane, (int64_t)t * N + col, n, g);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) total[i] += g[i];
@@ -90,18 +92,25 @@ __global__ __launch_bounds__(256) void rows_act_backward_kernel(const void *grad
     }
 }
 
+// Column sums of the chunks: 64 columns a workgroup, its four waves every fourth chunk, eight loads in flight.
 template <class T>
 __global__ __launch_bounds__(256) void rows_column_join_kernel(const float *part, int chunks, int N, T *out) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= N) return;
+    __shared__ float sums[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
     float v = 0.0f;
-    for (int s = 0; s < chunks; ++s) v += part[(int64_t)s * N + c];
-    out[c] = (T)v;
+    if (c < N) {
+#pragma unroll 8
+        for (int s = wave; s < chunks; s += 4) v += part[(int64_t)s * N + c];
+    }
+    sums[wave][lane] = v;
+    __syncthreads();
+    if (wave == 0 && c < N) out[c] = rows_round<T>(sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane]);
 }
 
 template <class E>
 __global__ __launch_bounds__(256) void rows_swiglu_backward_kernel(const void *grad_mid, const void *gate_up,
-                                                                   void *grad_gate_up, void *rest,
+                                                                   void *grad_gate_up, int planes, int64_t plane,
                                                                    const int32_t *offsets, int n_experts, int chunks,
                                                                    int I, int R) {
     typedef typename E::type T;
@@ -119,8 +128,8 @@ __global__ __launch_bounds__(256) void rows_swiglu_backward_kernel(const void *g
         g[i] = gm * up[i] * s * (1.0f + gate[i] * (1.0f - s));
         up[i] = gm * gate[i] * s;
     }
-    store_split<T>(grad_gate_up, rest, at, n, g);
-    store_split<T>(grad_gate_up, rest, at + I, n, up);
+    store_split<T>(grad_gate_up, planes, plane, at, n, g);
+    store_split<T>(grad_gate_up, planes, plane, at + I, n, up);
 }
 
 bool grid_of(int64_t threads, dim3 *grid) {
@@ -174,13 +183,16 @@ RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int hal
     };
     constexpr Cost k16[] = {{64, 64, 2, 2.2f, 0.35f, 0.5f}, {128, 128, 2, 2.9f, 0.65f, 1.0f},
                             {256, 160, 1, 5.f, 1.13f, 1.13f}, {256, 256, 1, 6.f, 1.4f, 1.4f}};
-    constexpr Cost k32[] = {{64, 64, 2, 2.2f, 0.5f, 0.95f}, {128, 128, 2, 2.9f, 1.9f, 3.6f}};
+    // A stage of experts' rows, where few tiles share a matrix's rows and wait for memory.
+    constexpr float kExperts[] = {0.5f, 1.3f, 1.4f, 1.9f};
+    constexpr Cost k32[] = {{64, 64, 2, 2.2f, 0.62f, 1.05f}, {128, 128, 2, 2.9f, 2.0f, 4.0f}};
     const Cost *const costs = fp32 ? k32 : k16;
     RowsChoice best{kRowsTile128, 0, 1};
     double least = 0;
     for (int tile = 0; tile < (fp32 ? 2 : (int)kRowsTileKinds); ++tile) {
         if (weight && tile == kRowsTile160) continue;
-        const Cost &c = costs[tile];
+        Cost c = costs[tile];
+        if (n_experts > 0 && !weight && !fp32) c.two = kExperts[tile], c.one = std::max(c.one, c.two / c.a_cu);
         // Row tiles in all: of experts the mean over a spread of a third of their rows, as routers have.
         double tiles_q, stages;
         if (weight) {
@@ -194,12 +206,17 @@ RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int hal
             tiles_q *= experts;
         }
         const double tiles = tiles_q * ((cols + c.p - 1) / c.p);
-        for (int slices = 1; slices <= (tile <= kRowsTile128 ? 8 : 1); slices *= 2) {
+        for (int slices : {1, 2, 3, 4, 6, 8}) {
             const double per = std::ceil(stages / slices), n = std::ceil(tiles * slices), slots = (double)kCus * c.a_cu;
-            if (slices > 1 && per < 8) break;
-            const double full = std::floor(n / slots), rest = n - full * slots;
-            double us = full * (c.fixed + c.two * per);
-            if (rest > 0) us += c.fixed + (rest <= kCus ? c.one : c.two) * per;
+            if (slices > 1 && (per < 8 || tile > kRowsTile128)) break;
+            double us;
+            if (n_experts > 0 && n > slots / 2) {  // how full the last round is nobody knows: half of one on average
+                us = std::max(n / slots + 0.5, 1.0) * (c.fixed + c.two * per);
+            } else {
+                const double full = std::floor(n / slots), rest = n - full * slots;
+                us = full * (c.fixed + c.two * per);
+                if (rest > 0) us += c.fixed + (rest <= kCus ? c.one : c.two) * per;
+            }
             if (slices > 1) us += 3 + 8e-6 / 4 * slices * (double)cols * (weight ? (double)Q * halves * experts : Q);
             if (least == 0 || us < least) least = us, best = {tile, 0, slices};
         }
@@ -232,14 +249,14 @@ hipError_t launch_rows_mm(RowsMode mode, int dtype, const RowsMm &p, hipStream_t
     });
 }
 
-// About four workgroups a CU, 16 rows each at least.
+// About two workgroups a CU, two rows a wave at least.
 int rows_column_chunks(int T, int N) {
     const int64_t across = ((int64_t)N + kColumnsAtOnce - 1) / kColumnsAtOnce;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(1024 / across, ((int64_t)T + 15) / 16));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(512 / across, ((int64_t)T + 7) / 8));
 }
 
-hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, const void *pre, void *gz, void *rest,
-                                    int dtype, int act, void *sums, bool sums_wide, float *column_part, int T, int N,
+hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, const void *pre, void *gz, int planes,
+                                    int64_t plane, int dtype, int act, void *sums, bool sums_wide, float *column_part, int T, int N,
                                     hipStream_t stream) {
     const int chunks = rows_column_chunks(T, N);
     const dim3 grid((unsigned)((N + (int64_t)kColumnsAtOnce - 1) / kColumnsAtOnce), (unsigned)chunks);
@@ -247,11 +264,11 @@ hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, c
     return mx_by_dtype(dtype, [&](auto tag) {
         using E = decltype(tag);
         typedef typename E::type V;
-        hipLaunchKernelGGL(rows_act_backward_kernel<E>, grid, dim3(256), 0, stream, grad_y, grad_y_stride, pre, gz, rest,
-                           act, part, T, N);
+        hipLaunchKernelGGL(rows_act_backward_kernel<E>, grid, dim3(256), 0, stream, grad_y, grad_y_stride, pre, gz, planes,
+                           plane, act, part, T, N);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess || sums == nullptr) return e;
-        const dim3 join((unsigned)((N + 255LL) / 256));
+        const dim3 join((unsigned)((N + 63LL) / 64));
         if (sums_wide)
             hipLaunchKernelGGL(rows_column_join_kernel<float>, join, dim3(256), 0, stream, part, chunks, N, (float *)sums);
         else
@@ -260,14 +277,14 @@ hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, c
     });
 }
 
-hipError_t launch_rows_swiglu_backward(const void *grad_mid, const void *gate_up, void *grad_gate_up, void *rest, int dtype,
+hipError_t launch_rows_swiglu_backward(const void *grad_mid, const void *gate_up, void *grad_gate_up, int planes, int64_t plane, int dtype,
                                        const int32_t *offsets, int n_experts, int I, int R, hipStream_t stream) {
     const int chunks = (I + 7) / 8;
     dim3 grid;
     if (!grid_of((int64_t)R * chunks, &grid)) return hipErrorInvalidConfiguration;
     return mx_by_dtype(dtype, [&](auto tag) {
         hipLaunchKernelGGL(rows_swiglu_backward_kernel<decltype(tag)>, grid, dim3(256), 0, stream, grad_mid, gate_up,
-                           grad_gate_up, rest, offsets, n_experts, chunks, I, R);
+                           grad_gate_up, planes, plane, offsets, n_experts, chunks, I, R);
         return hipGetLastError();
     });
 }

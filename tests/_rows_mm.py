@@ -60,9 +60,11 @@ def linear(x, w, bias, residual, name):
 
 
 def kept(x, dtype, wide):
-    """The error of a gradient x that is rounded to dtype; wide: and of what that left, rounded again."""
-    once = rounding(x, dtype)
-    return rounding(once, dtype) if wide and dtype != torch.float32 else once
+    """The error of a gradient x that is rounded to dtype; wide: and of what that left, rounded again (bf16: twice)."""
+    left = rounding(x, dtype)
+    for _ in range(0 if not wide else {torch.float16: 1, torch.bfloat16: 2}.get(dtype, 0)):
+        left = rounding(left, dtype)
+    return left
 
 
 def gz_of(g, pre, name, dtype, wide=False):

@@ -86,10 +86,10 @@ def _linear_back(name, K, N, T, act, wide, want="xwb"):
     if gx is not None:
         R.check(gx, *R.mm_of(gz, e, w.t()), "grad_x")
     if gw is not None:
-        # a sum over both parts of a split gradient has twice the additions
+        # a sum over the parts of a split gradient has up to three times the additions
         _, _, ew = R.gz_of(g, pre, act, d, wide)
         ref, bound = R.mm_of(gz.t(), ew.t(), x.t())
-        R.check(gw, ref, 2 * bound if wide else bound, "grad_w")
+        R.check(gw, ref, 3 * bound if wide else bound, "grad_w")
     if gb is not None:
         R.check(gb, gz.sum(0), 1.01 * (e32.sum(0) + (T + 2) * 2.0 ** -23 * gz.abs().sum(0)), "grad_b")
 
@@ -171,6 +171,6 @@ def test_grouped(dev, name, K, N, counts):
         # one sum of 2 N products: twice the additions
         R.check(sx[a:b], ra + rb, 2 * (ea + eb), f"swiglu grad_x {e}")
         _, eg, _, egu = R.swiglu_back(gs, saved[a:b, :N], saved[a:b, N:], d, True)
-        for got, gz, ez in ((sg[e], gg, eg), (su[e], gu, egu)):  # fp32: sums over both parts of the gradient
+        for got, gz, ez in ((sg[e], gg, eg), (su[e], gu, egu)):  # fp32: sums over all parts of the gradient
             ref, bound = R.mm_of(gz.t(), ez.t(), xs.t())
-            R.check(got, ref, 2 * bound, f"grad_w_gate, grad_w_up {e}")
+            R.check(got, ref, 3 * bound, f"grad_w_gate, grad_w_up {e}")
