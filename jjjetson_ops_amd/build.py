@@ -27,7 +27,7 @@ LIB = PKG / "libjjjetson_ops_amd.so"
 HIP_SOURCES = ["quantize_q8_1.hip", "gemv_q4_0_q8_1.hip", "gemm_skinny_q4_0_q8_1.hip", "gemm_skinny_persist.hip", "gemm_q4_0_q8_1_mfma.hip", "gemm_q4_0_q8_1_mfma64.hip", "moe_route.hip",
                "quantize_q4_0.hip", "q4_0_split.hip", "gemm_q4s_mfma.hip", "gemm_kslice.hip",
                "mxfp4_quant.hip", "gemm_mxfp4_direct.hip", "gemm_mxfp4.hip", "moe_rows.hip",
-               "gemm_rows_f32.hip", "gemm_rows_f16.hip", "gemm_rows_bf16.hip", "rows_parts.hip",
+               "gemm_rows_f32.hip", "gemm_rows_f16.hip", "gemm_rows_bf16.hip", "rows_parts.hip", "rows_choose.hip",
                "weights_q4_0.cpp", "capi.hip", "capi_mxfp4.hip", "capi_rows.hip"]
 HIP_FLAGS = [
     "--offload-arch=gfx950",

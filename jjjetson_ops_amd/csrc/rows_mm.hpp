@@ -193,6 +193,8 @@ struct RowsChoice {
 RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int halves, int n_experts);
 hipError_t launch_rows_mm(RowsMode mode, int dtype, const RowsMm &p, hipStream_t stream,
                           const RowsChoice *pinned = nullptr);
+// Rows of a product's output (weight: of all matrices), and the bytes of its slices' sums.
+int64_t rows_output_rows(RowsMode mode, const RowsMm &p);
 int64_t rows_part_bytes(RowsMode mode, const RowsMm &p);
 
 
@@ -201,6 +203,7 @@ hipError_t rows_mm_run(RowsMode mode, const RowsMm &p, const RowsChoice &c, hipS
 
 // gz[t] = grad_y[t] * act'(pre[t]) (act none: not written; planes - 1 more matrices behind it: what the rounding left, rounded) and the columns' sums of gz (sums nullable;
 // column_part: rows_column_chunks(T, N) * N floats).
+constexpr int kRowsColumns = 512;  // of a workgroup
 int rows_column_chunks(int T, int N);
 hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, const void *pre, void *gz, int planes,
                                     int64_t plane, int dtype, int act, void *sums, bool sums_wide, float *column_part, int T, int N,

@@ -307,6 +307,7 @@ struct RowsTiles {
         const int stages = MODE == kRowsInput ? p.halves * half_stages : MODE == kRowsWeight ? p.terms * half_stages : half_stages;
         c.s_beg = p.slices == 1 ? 0 : (int)((int64_t)stages * c.slice / p.slices);
         c.s_end = p.slices == 1 ? stages : (int)((int64_t)stages * (c.slice + 1) / p.slices);
+        if (c.s_beg == c.s_end) c.s_beg = c.s_end = stages;  // a slice without stages: behind the sums' end
         return c;
     }
 };
@@ -362,9 +363,9 @@ struct RowsSource {
 
     // Stage st to `to`; a stage without elements is zeros.
     __device__ __forceinline__ void bring(const RowsMm &p, int st, uint8_t *to, int wave) const {
-        // The half or term of the sums that stage st belongs to.
-        const int part = MODE == kRowsInput ? st >= stages_half
-                         : MODE == kRowsWeight ? (st >= stages_half) + (st >= 2 * stages_half) : 0;
+        // The half or term of the sums that stage st belongs to: the last one's, past its end, behind them.
+        const int parts = MODE == kRowsInput ? p.halves : MODE == kRowsWeight ? p.terms : 1;
+        const int part = min((st >= stages_half) + (st >= 2 * stages_half), parts - 1);
         const bool second = part > 0;
         const int k0 = (st - part * stages_half) * kStep, left = length - k0;
         const T *const from_p = (second ? pm2 : pm) + (PT ? k0 * p.ldp : k0);
