@@ -6,6 +6,13 @@
 // (piece ^ row / 2 % 8); where the rows of an element are, an LDS row is one element of all the tile's
 // rows, and the transposing LDS read puts four elements of a row into a lane; pieces are permuted by
 // the element's number so that the lanes served together fall into different banks.
+//
+// What bounds it (bf16, us and Tflop/s): dense products the matrix cores with LDS behind them, 8192 cubed 833 to 857
+// (1280 to 1320; a library product 839), 2047 x 14336 over 4096 195 to 230 with the card's clock (448 tiles are 1.75
+// rounds; the library 182), gradients of the weights 4096 x 4096 over 2048 59 (1165; the library 75).  Experts with
+// few rows: reading their matrices (64 x 1408 x 2048, 25 rows each, 72 us, 5.3 TB/s on tiles of 64 x 64).  Short sums
+// of large outputs: writing them (8 x 28672 x 4096 over 256 tokens each 733: 1.9 GB, which a fill writes in 273; a
+// tile's output, 128 KB a CU at 5.8 TB/s, and its stages do not overlap, see rows_stream_kernel).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -178,7 +185,7 @@ __device__ __forceinline__ void rows_dma(uint32_t off, uint64_t from, uint32_t l
 // Workgroups go to the eight XCDs in turn.  Each XCD takes a contiguous run of the tiles, its workgroups
 // neighbours of it, so that tiles that read the same rows are read into one L2; or (tiles of unequal length) the
 // XCDs take turns at chunks of 32, an XCD's workgroups (gradients of 8 experts' 28672 x 4096 matrices, one
-// expert a run: as long as the one with the most tokens, 444 of 2048, %CHUNK%).  A workgroup's places
+// expert a run: as long as the one with the most tokens, 444 of 2048, 1036 us, 800 to 880 in turn).  A workgroup's places
 // are at, at + step, ... below end.
 struct RowsRun {
     int at, step, end, beg, xcd;
@@ -243,7 +250,7 @@ struct RowsTiles {
     }
     // The order of an output's tiles: eight rows of tiles at a time, these fastest, so that the 32 that an XCD
     // works on at once read few rows of either operand (gradients of 8 experts' 28672 x 4096 matrices, 256 tokens
-    // each: %ORDER%).
+    // each: 795 us, 990 with all row tiles fastest; 8192 cubed 853 and 943).
     static __device__ __forceinline__ void blocked(int tile, int tiles_q, int tiles_p, int &tile_q, int &tile_p) {
         const int group = tile / (8 * tiles_p), rows = min(tiles_q - 8 * group, 8), at = tile - group * 8 * tiles_p;
         tile_q = 8 * group + at % rows;
@@ -318,7 +325,7 @@ __device__ __forceinline__ void rows_dma(const void *from, uint32_t lds) {
     asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(m0v) : "memory");
 }
 
-__device__ const uint32_t rows_zeros[4] = {0u, 0u, 0u, 0u};  // the pieces behind the sums' end
+__device__ const __align__(16) uint32_t rows_zeros[4] = {0u, 0u, 0u, 0u};  // the pieces behind the sums' end
 
 // The operands of a tile and the way of their stages into LDS.
 //
@@ -504,7 +511,7 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
         return all(std::integral_constant<int, JJO_ACT_NONE>{});
     }
     // Weights' gradients go past the caches, in whole lines: nothing near reads them, and they would push out what
-    // the tiles beside read (64 experts of 2048 x 1408, 244 tokens each: %NT%).  Stores of 64 bytes a row
+    // the tiles beside read (64 experts of 2048 x 1408, 244 tokens each: 160 us, 195 through the caches).  Stores of 64 bytes a row
     // reach 3.0 to 4.0 TB/s that way, of 128 bytes 5.6 to 6.3, as through the caches.  So lanes 8..15 of each 16
     // exchange with 0..7: an instruction writes 128 bytes of eight rows.
     if constexpr (MODE == kRowsWeight && RT == 4) {
@@ -673,7 +680,10 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p, int m
 // Two waves a SIMD, one half of the waves a slot behind the other: while one reads its operands of a step from
 // LDS, the other multiplies.  A barrier ends each slot, four of them a stage.  The stages of a workgroup's
 // tiles are one stream: the next tile's first ones are on their way during a tile's last, and one half of the
-// waves writes its outputs while the other multiplies.
+// waves writes its outputs while the other multiplies.  Against a tile a workgroup: sums of 64 tokens for 8 experts'
+// 28672 x 4096 482 us, 644 before.  Slower, and not kept: both steps of a stage in one slot (2047 x 14336 over 4096
+// 260 against 246 us on 128 rows; no registers for it on 256), stages of 64 bytes five deep (235 against 196), the
+// next stage requested before the outputs and these left in flight (806 against 795 for 256 tokens).
 template <class E, RowsMode MODE, RowsOutput KIND, class Tile>
 __global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, int most) {
     typedef typename E::type T;

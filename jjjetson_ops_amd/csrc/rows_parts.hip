@@ -44,7 +44,8 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsMm p, int chunks, in
     }
 }
 
-// Eight values rounded to T and, in the planes behind, what the rounding left of them, rounded again.
+// Eight values rounded to T and, in the planes behind, what the rounding left of them, rounded again (nothing of an
+// infinity or a NaN, also where the rounding made it).
 template <class T>
 __device__ __forceinline__ void store_split(void *to, int planes, int64_t plane, int64_t at, int n, const float *v) {
     float r[8];
@@ -53,7 +54,10 @@ __device__ __forceinline__ void store_split(void *to, int planes, int64_t plane,
     for (int k = 0; k < planes; ++k) {
         rows_store8((T *)to + k * plane + at, n, r);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] -= (float)rows_round<T>(r[i]);
+        for (int i = 0; i < 8; ++i) {
+            const float kept = (float)rows_round<T>(r[i]);
+            r[i] = fabsf(kept) <= 3.402823466e38f ? r[i] - kept : 0.0f;
+        }
     }
 }
 

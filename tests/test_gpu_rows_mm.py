@@ -108,6 +108,39 @@ def test_linear_backward_parts(dev, act, want):
     _linear_back("bf16", 96, 136, 70, act, False, want)
 
 
+@pytest.mark.parametrize("K,N,T", [(64, 8, 9), (200, 136, 70), (61, 33, 40)])
+@pytest.mark.parametrize("name", DTYPE_NAMES)
+def test_linear_backward_strides(dev, name, K, N, T):
+    """Slices of wider gradients and inputs; the columns beside grad_x stay as they were."""
+    d = R.DTYPES[name]
+    w = R.randn(2, N, K, dtype=d, scale=K ** -0.5)
+    for at, more in ((0, 8), (8, 24), (3, 13)):
+        x, g = _activations(1, T, K + more, d)[:, at:at + K], R.randn(3, T, N + more, dtype=d, scale=0.1)[:, at:at + N]
+        wide = torch.full((T, K + more), 7.0, dtype=d, device="cuda")
+        gx, gw, gb = wide[:, at:at + K], torch.empty_like(w), torch.empty(N, dtype=d, device="cuda")
+        ws = R.workspace(capi.linear_rows_backward_workspace_bytes(CODES[name], K, N, T))
+        for act in ("none", "relu"):
+            pre = None if act == "none" else R.randn(4, T, N, dtype=d)
+            capi.linear_rows_backward(g, x, w, gx, gw, gb, K, N, T, activation=R.ACTS[act], pre=pre, ws=ws)
+            gz, e32, e = R.gz_of(g, pre, act, d)
+            R.check(gx, *R.mm_of(gz, e, w.t()), "grad_x")
+            R.check(gw, *R.mm_of(gz.t(), e.t(), x.t()), "grad_w")
+            R.check(gb, gz.sum(0), 1.01 * (e32.sum(0) + (T + 2) * 2.0 ** -23 * gz.abs().sum(0)), "grad_b")
+            assert (wide[:, :at] == 7.0).all() and (wide[:, at + K:] == 7.0).all()
+
+
+def test_gradients_beyond_fp16(dev):
+    """A gradient that fp16 cannot hold is infinite in the fp32 gradients of the weights, and nothing beside it is lost."""
+    T, K, N = 40, 64, 72
+    x, g, pre = R.randn(1, T, K, dtype=torch.float16), R.randn(2, T, N, dtype=torch.float16), R.randn(3, T, N, dtype=torch.float16)
+    g[5, 7], pre[5, 7] = 60000.0, 1.6  # times gelu'(1.6) = 1.12
+    x[5] = x[5].abs() + 1
+    gw = torch.empty(N, K, dtype=torch.float32, device="cuda")
+    ws = R.workspace(capi.linear_rows_backward_workspace_bytes(CODES["f16"], K, N, T))
+    capi.linear_rows_backward(g, x, None, None, gw, None, K, N, T, activation=capi.ACT_GELU, pre=pre, ws=ws)
+    assert torch.isinf(gw[7]).all() and torch.isfinite(gw[:7]).all() and torch.isfinite(gw[8:]).all()
+
+
 COUNTS = [[1], [0, 3, 0], [5, 0, 1, 64, 0, 65, 2, 0], [128, 129, 0, 7], [0] * 63 + [2], [3] * 70, [300, 1, 0, 20]]
 # K, N of the experts
 GROUPED = [(64, 64), (72, 40), (33, 17), (200, 136), (512, 264)]
