@@ -319,6 +319,27 @@ struct RowsTiles {
     }
 };
 
+// Four of them, to places 1 KB apart.  What a stage's requests cost a wave in instructions is a slot of
+// rows_stream_kernel that is longer than the other's products: 8192 cubed 849 us for 861 to 874 with the addresses computed
+// anew for each, gradients of the weights and rows 820 and 842 for 890.
+__device__ __forceinline__ void rows_dma4(const uint32_t *off, uint64_t from, uint32_t lds) {
+    uint32_t m0v = __builtin_amdgcn_readfirstlane(lds);
+    from = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(from >> 32)) << 32 |
+           (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)from);
+    asm volatile(
+        "s_nop 4\n\t"
+        "global_load_lds_dwordx4 %1, %5\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %2, %5\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %3, %5\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %4, %5"
+        : "+{m0}"(m0v)
+        : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(from)
+        : "memory", "scc");
+}
+
 // The same from an address of each lane's own.
 __device__ __forceinline__ void rows_dma(const void *from, uint32_t lds) {
     const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds);
@@ -366,6 +387,38 @@ struct RowsSource {
             OpP::dma_offsets(off_p, wave, p.ldp, [&](int i) { return min(row_p(i), PT ? rows_p - OpP::kPiece : rows_p - 1); });
             OpQ::dma_offsets(off_q, wave, p.ldq, [&](int i) { return min(i, QT ? rows_q - OpQ::kPiece : rows_q - 1); });
         }
+    }
+
+    // ---- whole stages one after the other: aim at stage st (of those below end), then `whole` of them.
+    uint64_t at_p, at_q;
+    int whole;
+    __device__ __forceinline__ void aim(const RowsMm &p, int st, int end, int wave) {
+        const int parts = MODE == kRowsInput ? p.halves : MODE == kRowsWeight ? p.terms : 1;
+        const int part = min((st >= stages_half) + (st >= 2 * stages_half), parts - 1);
+        const int k0 = (st - part * stages_half) * kStep;
+        // Of SwiGLU a wave's runs are all of one matrix.
+        static_assert(MODE != kRowsSwiglu || Tile::kWaves != 8 || OpP::kMine * 8 == 8 * Tile::RT, "32 rows a wave");
+        at_p = (uint64_t)((part > 0 || is_up(8 * OpP::run(wave, 0)) ? pm2 : pm) + (PT ? k0 * p.ldp : k0));
+        at_q = (uint64_t)((MODE == kRowsWeight && part > 0 ? qm2 + (part - 1) * p.rest_plane : qm) +
+                          (QT ? k0 * p.ldq : (part > 0 ? p.K : 0) + (int64_t)k0));
+        whole = min(max(length - k0, 0) / kStep, end - st);
+    }
+    __device__ __forceinline__ void bring_whole(const RowsMm &p, uint8_t *to, int wave) {
+        const uint32_t at = (uint32_t)(uintptr_t)to;
+        if constexpr (OpP::kMine == 4) {
+            rows_dma4(off_p, at_p, at + 1024 * OpP::run(wave, 0));
+        } else {
+#pragma unroll
+            for (int n = 0; n < OpP::kMine; ++n) rows_dma(off_p[n], at_p, at + 1024 * OpP::run(wave, n));
+        }
+        if constexpr (OpQ::kMine == 4 && OpQ::kRuns % OpQ::kWaves == 0) {
+            rows_dma4(off_q, at_q, at + Tile::kStageP + 1024 * OpQ::run(wave, 0));
+        } else {
+#pragma unroll
+            for (int n = 0; n < OpQ::kMine; ++n) rows_dma(off_q[n], at_q, at + Tile::kStageP + 1024 * OpQ::run(wave, n));
+        }
+        at_p += PT ? 128 * p.ldp : 128, at_q += QT ? 128 * p.ldq : 128;
+        --whole;
     }
 
     // Stage st to `to`; a stage without elements is zeros.
@@ -704,6 +757,7 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, i
         const RowsPlace c = tiles.place(p, run.tile(brought));
         source.open(p, c, wave);
         st = c.s_beg, st_end = max(c.s_end, c.s_beg + 1);
+        source.aim(p, st, c.s_end, wave);
     };
     open();
     auto bring = [&](int buffer) {
@@ -712,7 +766,14 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, i
             brought += run.step;
             open();
         }
-        source.bring(p, st++, lds + buffer * Tile::kStage, wave);
+        uint8_t *const to = lds + buffer * Tile::kStage;
+        if (source.whole > 0) {
+            source.bring_whole(p, to, wave);
+        } else {  // the sums, or their half, end inside the stage (or begin anew with the next)
+            source.bring(p, st, to, wave);
+            source.aim(p, st + 1, st_end, wave);
+        }
+        ++st;
         ++pending;
     };
 
