@@ -7,12 +7,13 @@
 // rows, and the transposing LDS read puts four elements of a row into a lane; pieces are permuted by
 // the element's number so that the lanes served together fall into different banks.
 //
-// What bounds it (bf16, us and Tflop/s): dense products the matrix cores with LDS behind them, 8192 cubed 833 to 857
-// (1280 to 1320; a library product 839), 2047 x 14336 over 4096 195 to 230 with the card's clock (448 tiles are 1.75
-// rounds; the library 182), gradients of the weights 4096 x 4096 over 2048 59 (1165; the library 75).  Experts with
-// few rows: reading their matrices (64 x 1408 x 2048, 25 rows each, 72 us, 5.3 TB/s on tiles of 64 x 64).  Short sums
-// of large outputs: writing them (8 x 28672 x 4096 over 256 tokens each 733: 1.9 GB, which a fill writes in 273; a
-// tile's output, 128 KB a CU at 5.8 TB/s, and its stages do not overlap, see rows_stream_kernel).
+// What bounds it (bf16, us and Tflop/s): dense products the matrix cores with LDS behind them, 8192 cubed 816 to 845
+// (1300 to 1347; a library product 700 to 840 with the card's clock, its input gradient 825, its weights' 960 to 990),
+// 2047 x 14336 over 4096 197 to 210 (448 tiles are 1.75 rounds; the library 170 to 182), gradients of the weights
+// 4096 x 4096 over 2048 60 (1150; the library 66).  Experts with few rows: reading their matrices (64 x 1408 x 2048,
+// 25 rows each, 72 us, 5.3 TB/s on tiles of 64 x 64).  Short sums of large outputs: writing them (8 x 28672 x 4096
+// over 256 tokens each 733: 1.9 GB, which a fill writes in 273; a tile's output, 128 KB a CU at 5.8 TB/s, and its
+// stages do not overlap, see rows_stream_kernel).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -403,7 +404,7 @@ struct RowsSource {
                           (QT ? k0 * p.ldq : (part > 0 ? p.K : 0) + (int64_t)k0));
         whole = min(max(length - k0, 0) / kStep, end - st);
     }
-    __device__ __forceinline__ void bring_whole(const RowsMm &p, uint8_t *to, int wave) {
+    __device__ __forceinline__ void bring_whole_p(const RowsMm &p, uint8_t *to, int wave) {
         const uint32_t at = (uint32_t)(uintptr_t)to;
         if constexpr (OpP::kMine == 4) {
             rows_dma4(off_p, at_p, at + 1024 * OpP::run(wave, 0));
@@ -411,14 +412,18 @@ struct RowsSource {
 #pragma unroll
             for (int n = 0; n < OpP::kMine; ++n) rows_dma(off_p[n], at_p, at + 1024 * OpP::run(wave, n));
         }
+        at_p += PT ? 128 * p.ldp : 128;
+        --whole;
+    }
+    __device__ __forceinline__ void bring_whole_q(const RowsMm &p, uint8_t *to, int wave) {
+        const uint32_t at = (uint32_t)(uintptr_t)to;
         if constexpr (OpQ::kMine == 4 && OpQ::kRuns % OpQ::kWaves == 0) {
             rows_dma4(off_q, at_q, at + Tile::kStageP + 1024 * OpQ::run(wave, 0));
         } else {
 #pragma unroll
             for (int n = 0; n < OpQ::kMine; ++n) rows_dma(off_q[n], at_q, at + Tile::kStageP + 1024 * OpQ::run(wave, n));
         }
-        at_p += PT ? 128 * p.ldp : 128, at_q += QT ? 128 * p.ldq : 128;
-        --whole;
+        at_q += QT ? 128 * p.ldq : 128;
     }
 
     // Stage st to `to`; a stage without elements is zeros.
@@ -760,6 +765,11 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, i
         source.aim(p, st, c.s_end, wave);
     };
     open();
+    // Forward: a stage's rows are asked for between the products of the slot behind the columns' requests, and these
+    // behind the reads (2047 x 14336 over 4096 198 us, 213 otherwise; the other forms lose, SwiGLU of 8 experts 733
+    // against 703, as less of the stage's way to memory is hidden).
+    constexpr bool kBetween = MODE == kRowsForward;
+    uint8_t *rows_due = nullptr;
     auto bring = [&](int buffer) {
         if (st == st_end) {
             if (brought + run.step >= run.end) return;
@@ -768,7 +778,9 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, i
         }
         uint8_t *const to = lds + buffer * Tile::kStage;
         if (source.whole > 0) {
-            source.bring_whole(p, to, wave);
+            source.bring_whole_p(p, to, wave);
+            if (kBetween) rows_due = to;
+            else source.bring_whole_q(p, to, wave);
         } else {  // the sums, or their half, end inside the stage (or begin anew with the next)
             source.bring(p, st, to, wave);
             source.aim(p, st + 1, st_end, wave);
@@ -789,12 +801,18 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, i
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) b[tt] = read_q.template read<U>(in_q, tt);
     };
-    auto products = [&]() {
+    auto products = [&](bool between) {
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
+        for (int tt = 0; tt < TT; ++tt) {
+            if (kBetween && tt == 1 && between) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (rows_due != nullptr) source.bring_whole_q(p, rows_due, wave), rows_due = nullptr;
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) acc[rt][tt] = rows_mfma<T>(a[rt], b[tt], acc[rt][tt]);
+        }
         __builtin_amdgcn_s_setprio(0);
     };
     auto slot_end = [&]() {
@@ -811,7 +829,10 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, i
     constexpr std::integral_constant<int, 1> kU1{};
 
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) bring(i);
+    for (int i = 0; i < kAhead; ++i) {
+        bring(i);
+        if (rows_due != nullptr) source.bring_whole_q(p, rows_due, wave), rows_due = nullptr;
+    }
     landed(0);
     slot_end();
     if (wave >= 4) slot_end();
@@ -824,15 +845,17 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, i
             for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = f32x4v{0.f, 0.f, 0.f, 0.f};
         for (int left = max(c.s_end - c.s_beg, 1); left > 0; --left) {
             // Into the buffer of the stage before, whose last readers' slot has ended.
-            bring(buffer == 0 ? Tile::NB - 1 : buffer - 1);
+            const int before = buffer == 0 ? Tile::NB - 1 : buffer - 1;
+            if (!kBetween) bring(before);
             read(kU0, buffer);
+            if (kBetween) bring(before);
             slot_end();
-            products();
+            products(true);
             slot_end();
             read(kU1, buffer);
             if (wave >= 4) landed(1);
             slot_end();
-            products();
+            products(false);
             if (wave < 4) landed(1);
             slot_end();
             --pending;
