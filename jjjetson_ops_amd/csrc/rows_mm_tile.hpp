@@ -186,8 +186,8 @@ __device__ __forceinline__ void rows_dma(uint32_t off, uint64_t from, uint32_t l
 // Workgroups go to the eight XCDs in turn.  Each XCD takes a contiguous run of the tiles, its workgroups
 // neighbours of it, so that tiles that read the same rows are read into one L2; or (tiles of unequal length) the
 // XCDs take turns at chunks of 32, an XCD's workgroups (gradients of 8 experts' 28672 x 4096 matrices, one
-// expert a run: as long as the one with the most tokens, 444 of 2048, 1036 us, 800 to 880 in turn).  A workgroup's places
-// are at, at + step, ... below end.
+// expert a run: as long as the one with the most tokens, 444 of 2048, 1036 us, 800 to 880 in turn), first to last and last to first, as
+// the experts with the most rows may come first.  A workgroup's places are at, at + step, ... below end.
 struct RowsRun {
     int at, step, end, beg, xcd;
     bool chunked;
@@ -197,8 +197,8 @@ struct RowsRun {
         step = ((int)gridDim.x - xcd + 7) / 8;
         chunked = unequal && total >= 1024;
         if (chunked) {
-            const int chunks = (total + 31) / 32, mine = (chunks - xcd + 7) / 8;
-            const bool last = (chunks - 1) % 8 == xcd;
+            const int chunks = (total + 31) / 32, mine = chunks / 8 + (turn(chunks / 8) < chunks % 8);
+            const bool last = turn((chunks - 1) / 8) == (chunks - 1) % 8;
             beg = 0, end = 32 * mine - (last ? 32 * chunks - total : 0);
         } else {
             const int per = total / 8, rest = total % 8;
@@ -206,8 +206,9 @@ struct RowsRun {
         }
     }
     __device__ __forceinline__ int tile(int place) const {
-        return chunked ? (place / 32 * 8 + xcd) * 32 + place % 32 : beg + place;
+        return chunked ? (place / 32 * 8 + turn(place / 32)) * 32 + place % 32 : beg + place;
     }
+    __device__ __forceinline__ int turn(int round) const { return round % 2 == 0 ? xcd : 7 - xcd; }
 };
 
 // A tile of the output: columns p0.., rows q0.. (rows_q of them; of weight in half `half` of expert's matrix),
@@ -235,6 +236,22 @@ struct RowsTiles {
         }
         incl = mx_scan((fin - beg + Tile::kQ - 1) / Tile::kQ);
     }
+    // Weights' gradients: the experts with the most rows first, lane l the l-th of them.  Its number is in the three
+    // bits above the 2^28 of each end, a register less.  Sorted where an expert has less than a tile for each CU, whose
+    // sums differ then (64 experts' 2048 x 1408, 3 to 730 rows each, rows' gradients included, 342 us, 371 unsorted);
+    // CUs that work on one expert at a time are even, and experts of few rows, bound by their outputs, are better
+    // spread (8 of 28672 x 4096, 256 rows on average: 1540 to 1570 sorted, 1524 not).
+    __device__ __forceinline__ void sort(bool by_rows) {
+        const int lane = threadIdx.x & 63, rows = fin - beg;
+        int at = by_rows ? 0 : lane;
+#pragma unroll 8
+        for (int j = 0; by_rows && j < 64; ++j) {
+            const int other = __builtin_amdgcn_readlane(rows, j);
+            at += other > rows || (other == rows && j < lane);
+        }
+        beg = __builtin_amdgcn_ds_permute(4 * at, beg | lane << 29);
+        fin = __builtin_amdgcn_ds_permute(4 * at, fin | lane >> 3 << 29);
+    }
     // The tiles in all; `most`: those the launch was made for (more only by a malformed table: none then).
     __device__ __forceinline__ int total(const RowsMm &p, int64_t most) {
         int64_t tiles = (int64_t)p.tiles_p * p.tiles_q;
@@ -244,6 +261,7 @@ struct RowsTiles {
                 count(p, e0);
                 rows += __builtin_amdgcn_readlane(incl, 63);
             }
+            if (MODE == kRowsWeight && p.n_experts <= 64) sort(tiles < 256);
             tiles = MODE == kRowsWeight ? tiles * p.n_experts : (int64_t)p.tiles_p * rows;
         }
         per_slice = tiles * p.slices > most || tiles < 0 ? 0 : (int)tiles;
@@ -268,8 +286,10 @@ struct RowsTiles {
                 c.expert = tile / each, tile %= each;
                 int end;
                 if (p.n_experts <= 64) {
-                    c.first = __builtin_amdgcn_readlane(beg, c.expert);
-                    end = __builtin_amdgcn_readlane(fin, c.expert);
+                    const uint32_t a = __builtin_amdgcn_readlane(beg, c.expert);
+                    const uint32_t b = __builtin_amdgcn_readlane(fin, c.expert);
+                    c.expert = a >> 29 | b >> 29 << 3;
+                    c.first = a & 0x1fffffff, end = b & 0x1fffffff;
                 } else {
                     c.first = __builtin_amdgcn_readfirstlane(min(max(p.offsets[c.expert], 0), p.M));
                     end = __builtin_amdgcn_readfirstlane(min(max(p.offsets[c.expert + 1], c.first), p.M));

@@ -98,6 +98,12 @@ def test_many_tiles(dev, kernel):
     _backward("bf16", kernel, 1, 256, 2400, 72, 1, [1] * 100 + [0] * 3 + [70])
 
 
+@pytest.mark.parametrize("kernel,cols,rows", [(capi.ROWS_TILE_64, 520, 500), (capi.ROWS_TILE_256, 1800, 1700)])
+def test_many_experts_of_unlike_rows(dev, kernel, cols, rows):
+    """Weights' gradients of experts taken by their rows, some of them alike, the first and last without."""
+    _backward("bf16", kernel, 1, cols, rows, 72, 1, [0, 5, 130, 64, 5, 300, 0, 1] + [33, 7, 64] * 5 + [0])
+
+
 @pytest.mark.parametrize("waves", [1, 2, 5, 8])
 @pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
 def test_direct(dev, name, waves):
