@@ -242,12 +242,13 @@ struct RowsTiles {
     // CUs that work on one expert at a time are even, and experts of few rows, bound by their outputs, are better
     // spread (8 of 28672 x 4096, 256 rows on average: 1540 to 1570 sorted, 1524 not).
     __device__ __forceinline__ void sort(bool by_rows) {
-        const int lane = threadIdx.x & 63, rows = fin - beg;
+        const int rows = fin - beg;
+        const uint32_t lane = threadIdx.x & 63;
         int at = by_rows ? 0 : lane;
 #pragma unroll 8
         for (int j = 0; by_rows && j < 64; ++j) {
             const int other = __builtin_amdgcn_readlane(rows, j);
-            at += other > rows || (other == rows && j < lane);
+            at += other > rows || (other == rows && j < (int)lane);
         }
         beg = __builtin_amdgcn_ds_permute(4 * at, beg | lane << 29);
         fin = __builtin_amdgcn_ds_permute(4 * at, fin | lane >> 3 << 29);
