@@ -609,9 +609,9 @@ int moe_combine_rows_backward_device(void *stream, const void *grad_y, const voi
  * (moe_dispatch_rows_device and moe_combine_rows_device above move the rows) and gate|up with SwiGLU, each
  * with its gradients.
  * All operands of a call are of `dtype` unless it says otherwise; sums are fp32, each result is rounded
- * once.  The gradient through an activation is rounded to `dtype` before it is multiplied; for weights'
- * gradients in fp32 what that rounding left is multiplied as well (fp16: 22 bits of it in twice the work, bf16: 24
- * in three times).
+ * once.  The gradient through an activation is rounded to `dtype` before it is multiplied (and so infinite beyond
+ * 65504 in fp16); for weights' gradients in fp32 what that rounding left is multiplied as well (fp16: 22 bits of
+ * it, below 2^-14 within 2^-36, in twice the work; bf16: 24 in three times).
  * Sums are added in an order that depends on the sizes alone.  Buffers are aligned to
  * their elements; where rows are 16-byte aligned as well the products are faster.  Sizes (in, out, rows) are
  * positive, any other number up to 2^28, a matrix has at most 2^40 elements.  Row strides are in

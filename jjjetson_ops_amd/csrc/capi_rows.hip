@@ -110,9 +110,19 @@ RowsMm weight(int dtype, int K, int N, int rows, int n_experts, int halves, bool
 }
 
 // The gradient through an activation, rounded to `dtype`.  Where the weights' gradients are fp32 and it is not, what
-// the rounding left is kept as well, rounded again: two terms of fp16 are 22 bits, three of bf16 24.
+// the rounding left is kept as well, rounded again: two terms of fp16 are 22 bits (below 2^-14, fp16's smallest
+// normal number, the second ends at 2^-36, and the matrix unit's additions are as exact as those of 2^-14), three of
+// bf16 24.
 int64_t gz_plane_bytes(int dtype, int64_t values) { return up256(elem_bytes(dtype) * values); }
 int gz_planes(int dtype) { return dtype == JJO_DTYPE_F32 ? 1 : dtype == JJO_DTYPE_F16 ? 2 : 3; }
+
+// The terms of a weight's gradient, planes of gz, the smallest first.
+void terms_of_gz(RowsMm &m, const uint8_t *gz, int64_t plane, int planes, int es) {
+    m.terms = planes;
+    m.q = gz + (planes - 1) * plane;
+    if (planes > 1) m.rest = gz + (planes - 2) * plane, m.rest_plane = -plane / es;
+    if (planes == 2) m.first_scale = 1.0f / kRowsRestScale;
+}
 
 struct LinearBackwardWs {
     int64_t gz, plane, columns, parts, bytes;  // offsets; bytes of a plane of gz
@@ -229,7 +239,7 @@ int linear_rows_backward_device(void *stream, const void *grad_y, int64_t grad_y
     if (grad_weight != nullptr) {
         RowsMm m = weight(dtype, K, N, T, 0, 1, wide);
         m.p = x, m.ldp = stride_of(x_stride, K, T), m.q = gz, m.ldq = gz_stride, m.y = grad_weight;
-        if (planes > 1) m.rest = base + ws.gz + ws.plane, m.rest_plane = ws.plane / es, m.terms = planes;
+        if (act) terms_of_gz(m, base + ws.gz, ws.plane, planes, es);
         m.part = (float *)(base + ws.parts);
         const hipError_t e = launch_rows_mm(kRowsWeight, dtype, m, s);
         if (e != hipSuccess) return launched(e, "linear_rows_backward weight");
@@ -388,8 +398,8 @@ int moe_rows_gate_up_swiglu_backward_device(void *stream, const void *grad_mid, 
     }
     if (grad_w_gate != nullptr) {
         RowsMm m = weight(dtype, H, I, R, E, 2, grad_weights_dtype == JJO_DTYPE_F32);
-        m.p = x_sorted, m.q = gz, m.y = grad_w_gate, m.y2 = grad_w_up, m.offsets = expert_offsets, m.part = part;
-        if (planes > 1) m.rest = gz + plane, m.rest_plane = plane / es, m.terms = planes;
+        m.p = x_sorted, m.y = grad_w_gate, m.y2 = grad_w_up, m.offsets = expert_offsets, m.part = part;
+        terms_of_gz(m, gz, plane, planes, es);
         if ((e = launch_rows_mm(kRowsWeight, dtype, m, s)) != hipSuccess)
             return launched(e, "moe_rows_gate_up_swiglu_backward weights");
     }

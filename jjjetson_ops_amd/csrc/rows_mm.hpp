@@ -26,14 +26,15 @@ struct RowsEpilogue {
 // are contiguous (forward), or the rows' of an element are (weight; input: of P).
 struct RowsMm {
     const void *p, *p2;  // p2: the up matrix (SwiGLU), or the operand of the sums' second half (input)
-    const void *q, *rest;  // rest: what q's rounding left, terms - 1 matrices (weight)
+    const void *q, *rest;  // rest: q's other terms, terms - 1 matrices (weight)
     int64_t rest_plane;    // elements from one of these to the next
+    float first_scale;     // of the sums over q, before those over rest are added (terms 2)
     int64_t ldp, ldq;  // elements from one memory row to the next
     void *y, *y2;      // y2: of the second half's output rows (weight)
     int64_t ldy;
     int P, Q, K;
     int halves;              // 2: input sums over p, then over p2; weight has rows of y, then of y2
-    int terms;               // of q in a weight's sums: q, then those of rest
+    int terms;               // of q in a weight's sums, the smallest first: q, then those of rest
     const int32_t *offsets;  // [n_experts + 1], or nullptr
     int n_experts, M;        // M: sorted rows
     int64_t expert_stride;   // elements of a matrix (of an expert's part of y: weight)
@@ -201,8 +202,11 @@ int64_t rows_part_bytes(RowsMode mode, const RowsMm &p);
 template <class E>
 hipError_t rows_mm_run(RowsMode mode, const RowsMm &p, const RowsChoice &c, hipStream_t stream);
 
-// gz[t] = grad_y[t] * act'(pre[t]) (act none: not written; planes - 1 more matrices behind it: what the rounding left, rounded) and the columns' sums of gz (sums nullable;
-// column_part: rows_column_chunks(T, N) * N floats).
+// What the rounding of a value to fp16 left is kept times this.  It is below 2^-11 of the value, so that it would be a
+// subnormal of fp16 for all values below 2^-3, and lost below 2^-14; of 65504 it is 16, and so 2^15 at most.
+constexpr float kRowsRestScale = 2048.0f;
+// gz[t] = grad_y[t] * act'(pre[t]) (act none: not written; planes - 1 more matrices behind it: what the rounding
+// left, rounded again) and the columns' sums of gz (sums nullable; column_part: rows_column_chunks(T, N) * N floats).
 constexpr int kRowsColumns = 512;  // of a workgroup
 int rows_column_chunks(int T, int N);
 hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, const void *pre, void *gz, int planes,

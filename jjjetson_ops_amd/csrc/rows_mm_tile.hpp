@@ -215,6 +215,7 @@ struct RowsRun {
 // its sums over stages s_beg..s_end of `length` elements from row `first` on (weight).
 struct RowsPlace {
     int p0, q0, rows_q, expert, half, first, length, slice, s_beg, s_end;
+    int turn;  // the stage behind which the sums are scaled (weight: the last of the first term), -1 for none
 };
 
 // The tiles of a launch, of Tile::kQ rows and kOutP columns.  Lane l of a wave holds the range of expert
@@ -337,6 +338,7 @@ struct RowsTiles {
         c.s_beg = p.slices == 1 ? 0 : (int)((int64_t)stages * c.slice / p.slices);
         c.s_end = p.slices == 1 ? stages : (int)((int64_t)stages * (c.slice + 1) / p.slices);
         if (c.s_beg == c.s_end) c.s_beg = c.s_end = stages;  // a slice without stages: behind the sums' end
+        c.turn = MODE == kRowsWeight && p.terms == 2 && c.s_beg < half_stages ? min(half_stages, c.s_end) - 1 : -1;
         return c;
     }
 };
@@ -383,7 +385,7 @@ struct RowsSource {
     static constexpr int kDma = OpP::kMine + OpQ::kMine;  // of a wave and stage
 
     // From the tile's first row and the sums' first element on; the second ones: up's rows (SwiGLU), the sums'
-    // second half (input), and what q's rounding left (weight).
+    // second half (input), and q's other terms (weight).
     const T *pm, *pm2, *qm, *qm2;
     int rows_p, rows_q, length, stages_half;
     uint32_t off_p[DMA ? OpP::kMine : 1], off_q[DMA ? OpQ::kMine : 1];
@@ -687,6 +689,19 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
     }
 }
 
+// Behind stage st, the last one of fp16's first term: the scale that its values were kept with leaves the sums.
+template <class T, RowsMode MODE, class Tile>
+__device__ __forceinline__ void rows_turn(const RowsMm &p, const RowsPlace &c, int st,
+                                          f32x4v (&acc)[Tile::RT][Tile::TT]) {
+    if constexpr (MODE == kRowsWeight && std::is_same_v<T, _Float16>) {
+        if (st == c.turn)
+#pragma unroll
+            for (int rt = 0; rt < Tile::RT; ++rt)
+#pragma unroll
+                for (int tt = 0; tt < Tile::TT; ++tt) acc[rt][tt] *= p.first_scale;
+    }
+}
+
 // ---- four waves, a tile a workgroup, two or more workgroups a CU: one stages while another multiplies.
 template <class E, RowsMode MODE, class Tile, bool DMA>
 __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p, int most) {
@@ -749,6 +764,7 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p, int m
         };
         step(std::integral_constant<int, 0>{});
         step(std::integral_constant<int, 1>{});
+        rows_turn<T, MODE, Tile>(p, c, st, acc);
         buffer = buffer == Tile::NB - 1 ? 0 : buffer + 1;
     }
     rows_output<T, MODE, kRowsAny, Tile>(p, c, acc, wp, wq);
@@ -887,6 +903,7 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, i
             products(false);
             if (wave < 4) landed(1);
             slot_end();
+            rows_turn<T, MODE, Tile>(p, c, c.s_end - left, acc);
             --pending;
             buffer = buffer == Tile::NB - 1 ? 0 : buffer + 1;
         }

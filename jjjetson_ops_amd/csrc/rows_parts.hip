@@ -44,8 +44,8 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsMm p, int chunks, in
     }
 }
 
-// Eight values rounded to T and, in the planes behind, what the rounding left of them, rounded again (nothing of an
-// infinity or a NaN, also where the rounding made it).
+// Eight values rounded to T and, in the planes behind, what the rounding left of them, rounded again (fp16: times
+// kRowsRestScale; nothing of an infinity or a NaN, also where the rounding made it).
 template <class T>
 __device__ __forceinline__ void store_split(void *to, int planes, int64_t plane, int64_t at, int n, const float *v) {
     float r[8];
@@ -57,6 +57,7 @@ __device__ __forceinline__ void store_split(void *to, int planes, int64_t plane,
         for (int i = 0; i < 8; ++i) {
             const float kept = (float)rows_round<T>(r[i]);
             r[i] = fabsf(kept) <= 3.402823466e38f ? r[i] - kept : 0.0f;
+            if (std::is_same_v<T, _Float16>) r[i] *= kRowsRestScale;
         }
     }
 }

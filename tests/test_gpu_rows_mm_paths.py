@@ -1,0 +1,64 @@
+"""Float products through the public entries where precision or a kernel's way differs: the terms of a gradient that
+is split for fp32 weights' gradients."""
+if __name__ == "__main__":  # `python tests/<file>.py`, as the reference runs its tests
+    import sys as _sys
+
+    import pytest as _pytest
+    _sys.exit(_pytest.main([__file__, "-q"]))
+import pytest
+import torch
+
+import _rows_mm as R
+from jjjetson_ops_amd import capi
+
+pytestmark = pytest.mark.gpu
+CODES = {"f32": capi.DTYPE_F32, "f16": capi.DTYPE_F16, "bf16": capi.DTYPE_BF16}
+
+
+def _kept(gz, dtype):
+    """What two terms of fp16, the second times 2^11, or three of bf16 keep of a gradient: half a step of each term,
+    2^-11 * 2^-11 or 2^-8 * 2^-8 * 2^-8 of the value; fp16's last term has steps of 2^-24 times 2^-11 at the least."""
+    if dtype == torch.float16:
+        return (2.0 ** -22 * gz.abs()).clamp(min=2.0 ** -36)
+    return 2.0 ** -24 * gz.abs()
+
+
+def _added(gz, dtype):
+    """What an addition may be off by, per unit of x: 2^-23 of the product.  The matrix unit does not normalize fp16's
+    subnormals: a product of one is exact, but is aligned for an addition by the exponents that its operands have,
+    and so cut as one of 2^-14 would be, 2^-23 * 2^-14 (g of 1e-5 and of 1e-6 show it with grad_y's own product: one
+    token is exact, two are off by up to 2^-39 |x|, of either size)."""
+    return 2.0 ** -23 * (gz.abs().clamp(min=2.0 ** -14) if dtype == torch.float16 else gz.abs())
+
+
+@pytest.mark.parametrize("scale", [1.0, 1e-2, 1e-3, 1e-4, 1e-5])
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+def test_terms_keep_their_bits(dev, name, scale):
+    """fp32 weights' gradients from gradients of any size: two tokens, so that the error is that of gz, 2^-19 of the
+    derivative at |z| < 2 (its own fp32), and of up to six products.  fp16's grad_y has its own steps below 2^-14 and is
+    taken as it is."""
+    d, T, K, N = R.DTYPES[name], 2, 72, 520
+    x = R.randn(1, T, K, dtype=d)
+    g, pre = R.randn(2, T, N, scale=scale).to(d), R.randn(3, T, N, dtype=d).clamp(-2, 2)
+    gw = torch.empty(N, K, dtype=torch.float32, device="cuda")
+    ws = R.workspace(capi.linear_rows_backward_workspace_bytes(CODES[name], K, N, T))
+    for act in ("gelu", "gelu_tanh", "silu"):
+        capi.linear_rows_backward(g, x, None, None, gw, None, K, N, T, activation=R.ACTS[act], pre=pre, ws=ws)
+        gz, e32, _ = R.gz_of(g, pre, act, d)
+        ref = gz.t() @ x.double()
+        bound = (e32 + _kept(gz, d) + 10 * _added(gz, d)).t() @ x.double().abs()
+        R.check(gw, ref, bound, f"{act} grad_w")
+    # SwiGLU: both halves, one expert with a row of its own
+    rows, E = 3, 3
+    offsets = R.offsets_of([1, 0, 2])
+    xs, gm = R.randn(4, rows, K, dtype=d), R.randn(5, rows, N, scale=scale).to(d)
+    both = R.randn(6, rows, 2 * N, dtype=d).clamp(-2, 2)
+    gg, gu = (torch.empty(E, N, K, dtype=torch.float32, device="cuda") for _ in range(2))
+    ws = R.workspace(capi.moe_gate_up_swiglu_rows_backward_workspace_bytes(CODES[name], K, N, rows, E))
+    capi.moe_gate_up_swiglu_rows_backward(gm, both, xs, None, None, offsets, E, None, gg, gu, K, N, rows, ws=ws)
+    gate, up, g64 = both[:, :N].double(), both[:, N:].double(), gm.double()
+    for got, gz, at_one in ((gg, g64 * up * R.slope(gate, "silu"), g64 * up), (gu, g64 * R.act(gate, "silu"), g64)):
+        e = at_one.abs() * 2.0 ** -19 * gate.abs().clamp(min=1.0) + _kept(gz, d)
+        for k, (a, b) in enumerate(((0, 1), (1, 1), (1, 3))):
+            xe = xs[a:b].double()
+            R.check(got[k], gz[a:b].t() @ xe, (e + 10 * _added(gz, d))[a:b].t() @ xe.abs(), f"expert {k}")
