@@ -75,11 +75,10 @@ __device__ __forceinline__ float rows_act(float z, int act) {
     return z;
 }
 
-// The activation's derivative at z.
+// The activation's derivative at z (not of relu).
 template <class T>
 __device__ __forceinline__ float rows_slope(float z, int act) {
     switch (act) {
-        case JJO_ACT_RELU: return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
         case JJO_ACT_GELU:
             return 0.5f * rows_erfc<T>(-0.707106781186548f * z) +
                    z * 0.398942280401433f * __builtin_amdgcn_exp2f(-0.721347520444482f * z * z);
@@ -93,6 +92,12 @@ __device__ __forceinline__ float rows_slope(float z, int act) {
         }
     }
     return 1.0f;
+}
+// A gradient g through an activation: times its derivative at z; of relu g or 0, also where g is infinite.
+template <class T>
+__device__ __forceinline__ float rows_through(float g, float z, int act) {
+    if (act == JJO_ACT_RELU) return z > 0.0f ? g : z != z ? z : 0.0f;
+    return g * rows_slope<T>(z, act);
 }
 
 // ---- eight consecutive values of a row, n of them inside it, at any alignment

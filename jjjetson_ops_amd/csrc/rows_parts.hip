@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void rows_act_backward_kernel(const void *grad
             if (act != JJO_ACT_NONE) {
                 rows_load8((const T *)pre + (int64_t)t * N + col, n, z);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) g[i] *= rows_slope<T>(z[i], act);
+                for (int i = 0; i < 8; ++i) g[i] = rows_through<T>(g[i], z[i], act);
                 store_split<T>(gz, planes, plane, (int64_t)t * N + col, n, g);
             }
 #pragma unroll

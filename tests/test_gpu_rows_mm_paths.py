@@ -62,3 +62,24 @@ def test_terms_keep_their_bits(dev, name, scale):
         for k, (a, b) in enumerate(((0, 1), (1, 1), (1, 3))):
             xe = xs[a:b].double()
             R.check(got[k], gz[a:b].t() @ xe, (e + 10 * _added(gz, d))[a:b].t() @ xe.abs(), f"expert {k}")
+
+
+@pytest.mark.parametrize("name", list(R.DTYPES))
+def test_relu_lets_nothing_through_where_it_is_zero(dev, name):
+    """Infinite and NaN gradients at z <= 0 are zeros behind relu; at z > 0 they stay, and so does a NaN of z."""
+    d, T, K, N = R.DTYPES[name], 5, 24, 40
+    x, w, g = R.randn(1, T, K, dtype=d), R.randn(2, N, K, dtype=d), R.randn(3, T, N, dtype=d)
+    pre = R.randn(4, T, N, dtype=d)
+    pre[0, :4] = torch.tensor([0.0, -1.0, -0.0, float("-inf")])
+    g[0, :4] = torch.tensor([float("inf"), float("-inf"), float("nan"), float("inf")])
+    pre[1, 7], g[1, 7], pre[2, 8] = 1.0, float("inf"), float("nan")
+    gx, gw, gb = torch.empty_like(x), torch.empty_like(w), torch.empty(N, dtype=d, device="cuda")
+    ws = R.workspace(capi.linear_rows_backward_workspace_bytes(CODES[name], K, N, T))
+    capi.linear_rows_backward(g, x, w, gx, gw, gb, K, N, T, activation=capi.ACT_RELU, pre=pre, ws=ws)
+    assert gb[7] == float("inf") and gb[8].isnan() and not torch.isfinite(gx[1:3]).any()
+    gz = torch.where(pre > 0, g, 0.0).double()
+    zero = torch.zeros_like(gz)
+    rows, cols = [0, 3, 4], [n for n in range(N) if n not in (7, 8)]
+    R.check(gx[rows], *R.mm_of(gz[rows], zero[rows], w.t()), "grad_x")
+    R.check(gw[cols], *R.mm_of(gz.t()[cols], zero.t()[cols], x.t()), "grad_w")
+    R.check(gb[cols], gz.sum(0)[cols], (T + 2) * 2.0 ** -23 * gz.abs().sum(0)[cols], "grad_b")
