@@ -83,3 +83,23 @@ def test_relu_lets_nothing_through_where_it_is_zero(dev, name):
     R.check(gx[rows], *R.mm_of(gz[rows], zero[rows], w.t()), "grad_x")
     R.check(gw[cols], *R.mm_of(gz.t()[cols], zero.t()[cols], x.t()), "grad_w")
     R.check(gb[cols], gz.sum(0)[cols], (T + 2) * 2.0 ** -23 * gz.abs().sum(0)[cols], "grad_b")
+
+
+@pytest.mark.parametrize("name", list(R.DTYPES))
+def test_gelu_keeps_its_lower_tail(dev, name):
+    """gelu and its derivative from z = -12 to 12: relative to the normal distribution's tail, not to 1.  Its error: that of
+    erfc's argument x = z / sqrt 2, 2^-23.6 of itself (constant and product), which erfc's slope makes 2 x^2 = 144 times
+    as much, 2^-16.4; that of e^(-x^2)'s argument, rounded twice, 72 * 2^-23 = 2^-16.8; of the fit 2^-19.8 (erfcf: 16
+    ulp) and a few more steps: 2^-15 in all.  fp16 and its subnormals end at z = -5.5."""
+    d = R.DTYPES[name]
+    z = torch.linspace(-12, 12, 4801, device="cuda").to(d)
+    N, x, y = z.numel(), torch.ones(1, 1, dtype=d, device="cuda"), torch.empty(1, z.numel(), dtype=d, device="cuda")
+    capi.linear_rows(x, z.view(-1, 1).contiguous(), y, 1, N, 1, activation=capi.ACT_GELU)
+    z64 = z.double()
+    tail = 0.5 * torch.special.erfc(-z64 * 0.5 ** 0.5)
+    R.check(y[0], z64 * tail, 2.0 ** -15 * (z64 * tail).abs(), "gelu")
+    gb = torch.empty(N, dtype=torch.float32, device="cuda")
+    ws = R.workspace(capi.linear_rows_backward_workspace_bytes(CODES[name], 1, N, 1))
+    capi.linear_rows_backward(torch.ones_like(y), None, None, None, None, gb, 1, N, 1, activation=capi.ACT_GELU, pre=z, ws=ws)
+    density = z64 * torch.exp(-0.5 * z64 * z64) / (2 * torch.pi) ** 0.5
+    R.check(gb, tail + density, 2.0 ** -15 * (tail + density.abs()), "its derivative")
