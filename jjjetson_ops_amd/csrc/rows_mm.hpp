@@ -89,7 +89,9 @@ __device__ __forceinline__ float rows_slope(float z, int act) {
                    z * 0.398942280401433f * __builtin_amdgcn_exp2f(-0.721347520444482f * z * z);
         case JJO_ACT_GELU_TANH: {
             const float s = rows_sigmoid(2.0f * kGeluC * (z + kGeluA * z * z * z));
-            return s + z * 2.0f * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * kGeluA * z * z);
+            // The second term is nothing beyond |z| = 32, where its z^3 would leave fp32 later on.
+            const float c = fminf(fmaxf(z, -32.0f), 32.0f);
+            return s + c * 2.0f * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * kGeluA * c * c);
         }
         case JJO_ACT_SILU: {
             const float s = rows_sigmoid(z);

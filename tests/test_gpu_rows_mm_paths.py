@@ -103,3 +103,19 @@ def test_gelu_keeps_its_lower_tail(dev, name):
     capi.linear_rows_backward(torch.ones_like(y), None, None, None, None, gb, 1, N, 1, activation=capi.ACT_GELU, pre=z, ws=ws)
     density = z64 * torch.exp(-0.5 * z64 * z64) / (2 * torch.pi) ** 0.5
     R.check(gb, tail + density, 2.0 ** -15 * (tail + density.abs()), "its derivative")
+
+
+@pytest.mark.parametrize("name", list(R.DTYPES))
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_activations_far_out(dev, name, act):
+    """Any finite z: the activation and its derivative end as z and 1 above, 0 and 0 below."""
+    d = R.DTYPES[name]
+    most = torch.finfo(d).max
+    z = torch.tensor([s * v for v in (100.0, 1e4, 6e4, 1e13, 2e19, 1e30, most) if v <= most for s in (1, -1)], device="cuda").to(d)
+    N, x, y = z.numel(), torch.ones(1, 1, dtype=d, device="cuda"), torch.empty(1, z.numel(), dtype=d, device="cuda")
+    capi.linear_rows(x, z.view(-1, 1).contiguous(), y, 1, N, 1, activation=R.ACTS[act])
+    assert torch.equal(y[0], z.clamp(min=0.0))
+    gb = torch.empty(N, dtype=torch.float32, device="cuda")
+    ws = R.workspace(capi.linear_rows_backward_workspace_bytes(CODES[name], 1, N, 1))
+    capi.linear_rows_backward(torch.ones_like(y), None, None, None, None, gb, 1, N, 1, activation=R.ACTS[act], pre=z, ws=ws)
+    assert torch.equal(gb, (z > 0).float())
