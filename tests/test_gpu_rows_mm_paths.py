@@ -1,5 +1,5 @@
 """Float products through the public entries where precision or a kernel's way differs: the terms of a gradient that
-is split for fp32 weights' gradients."""
+is split for fp32 weights' gradients, epilogues and saved sums on every tile, rows that are not 16-byte aligned."""
 if __name__ == "__main__":  # `python tests/<file>.py`, as the reference runs its tests
     import sys as _sys
 
@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import _rows_mm as R
+import _rows_paths as P
 from jjjetson_ops_amd import capi
 
 pytestmark = pytest.mark.gpu
@@ -119,3 +120,203 @@ def test_activations_far_out(dev, name, act):
     ws = R.workspace(capi.linear_rows_backward_workspace_bytes(CODES[name], 1, N, 1))
     capi.linear_rows_backward(torch.ones_like(y), None, None, None, None, gb, 1, N, 1, activation=R.ACTS[act], pre=z, ws=ws)
     assert torch.equal(gb, (z > 0).float())
+
+
+@pytest.mark.parametrize("act", list(R.ACTS))
+@pytest.mark.parametrize("sizes", [s[0] for s in P.LINEAR], ids=lambda s: "-".join(map(str, s)))
+def test_epilogues_of_every_tile(dev, sizes, act):
+    """Bias, activation, residual and the kept sums together, and each alone, on every tile and behind slices."""
+    name, K, N, T = sizes
+    d = R.DTYPES[name]
+    x, w = R.randn(1, T, K, dtype=d), R.randn(2, N, K, dtype=d, scale=K ** -0.5)
+    bias, residual = R.randn(3, N, dtype=d), R.randn(4, T, N, dtype=d)
+    ws = R.workspace(capi.linear_rows_workspace_bytes(CODES[name], K, N, T))
+    for b, r, keep in ((bias, residual, True), (None, None, False), (bias, None, False), (None, residual, False)):
+        y = torch.empty(T, N, dtype=d, device="cuda")
+        pre = torch.empty_like(y) if keep else None
+        capi.linear_rows(x, w, y, K, N, T, bias=b, residual=r, activation=R.ACTS[act], pre=pre, ws=ws)
+        ref, bound, z, ez = R.linear(x, w, b, r, act)
+        R.check(y, ref, bound, "y")
+        if keep:
+            R.check(pre, z, ez, "pre")
+
+
+@pytest.mark.parametrize("sizes", [s[0] for s in P.SWIGLU_FORWARD], ids=lambda s: "-".join(map(str, s[:3])))
+def test_swiglu_of_every_tile(dev, sizes):
+    """mid alone, and with the saved gate|up, the same bits; rows behind the last expert's as they were."""
+    name, H, I, counts = sizes
+    d, E, n = R.DTYPES[name], len(counts), sum(counts)
+    offsets = R.offsets_of(counts)
+    ends = offsets.tolist()
+    x = R.randn(1, n + 5, H, dtype=d)
+    wg, wu = (R.randn(s, E, I, H, dtype=d, scale=H ** -0.5) for s in (2, 3))
+    mid, bare = (torch.full((n + 5, I), 7.0, dtype=d, device="cuda") for _ in range(2))
+    both = torch.full((n + 5, 2 * I), 7.0, dtype=d, device="cuda")
+    ws = R.workspace(capi.moe_gate_up_swiglu_rows_workspace_bytes(CODES[name], H, I, n + 5, E))
+    capi.moe_gate_up_swiglu_rows(x, wg, wu, offsets, E, mid, H, I, n + 5, gate_up=both, ws=ws)
+    capi.moe_gate_up_swiglu_rows(x, wg, wu, offsets, E, bare, H, I, n + 5, ws=ws)
+    assert torch.equal(mid, bare) and (mid[n:] == 7.0).all() and (both[n:] == 7.0).all()
+    for e in range(E):
+        a, b = ends[e], ends[e + 1]
+        z, ez = R.mm(x[a:b], wg[e])
+        up, eu = R.mm(x[a:b], wu[e])
+        R.check(both[a:b, :I], z, ez, f"gate {e}")
+        R.check(both[a:b, I:], up, eu, f"up {e}")
+        s, es = R.act(z, "silu"), 1.13 * ez + 2.0 ** -19 * z.abs().clamp(min=1.0)
+        R.check(mid[a:b], s * up, 1.01 * (es * up.abs() + s.abs() * eu + es * eu + 2.0 ** -23 * (s * up).abs()), f"mid {e}")
+
+
+def _terms(name):
+    return {"f16": 2, "bf16": 3}.get(name, 1)
+
+
+def _split_sum(gz, e, x, terms, d):
+    """gz^T . x of a split gradient that is off by e, and its bound: one sum of `terms` parts of each product."""
+    x = x.double()
+    n = terms * x.shape[0] + 2
+    return gz.t() @ x, (e + _kept(gz, d) + n * _added(gz, d)).t() @ x.abs()
+
+
+@pytest.mark.parametrize("sizes", [s[0] for s in P.WEIGHTS] + [("bf16", 515, 333, 500), ("f16", 515, 333, 500), ("f16", 33, 1407, 70),
+                                                               ("bf16", 1407, 33, 70)],
+                         ids=lambda s: "-".join(map(str, s)))
+def test_terms_on_every_tile(dev, sizes):
+    """fp32 weights' gradients of 16 bits, a term's sums of several stages and a part of one."""
+    name, K, N, T = sizes
+    d = R.DTYPES[name]
+    x, g, pre = R.randn(1, T, K, dtype=d), R.randn(2, T, N, dtype=d, scale=0.1), R.randn(3, T, N, dtype=d).clamp(-2, 2)
+    gw = torch.empty(N, K, dtype=torch.float32, device="cuda")
+    ws = R.workspace(capi.linear_rows_backward_workspace_bytes(CODES[name], K, N, T))
+    capi.linear_rows_backward(g, x, None, None, gw, None, K, N, T, activation=capi.ACT_SILU, pre=pre, ws=ws)
+    gz, e32, _ = R.gz_of(g, pre, "silu", d)
+    R.check(gw, *_split_sum(gz, e32, x, _terms(name), d), "grad_w")
+
+
+@pytest.mark.parametrize("sizes", [s[0] for s in P.SWIGLU_WEIGHTS] + [("f16", 515, 333, (200, 1, 0, 131)),
+                                                                      ("bf16", 333, 515, (1, 0, 70, 261))],
+                         ids=lambda s: "-".join(map(str, s[:3])))
+def test_terms_of_both_halves_on_every_tile(dev, sizes):
+    name, H, I, counts = sizes
+    d, E, n = R.DTYPES[name], len(counts), sum(counts)
+    offsets = R.offsets_of(counts)
+    ends = offsets.tolist()
+    x, gm = R.randn(1, n + 5, H, dtype=d), R.randn(2, n + 5, I, dtype=d, scale=0.1)
+    both = R.randn(3, n + 5, 2 * I, dtype=d).clamp(-2, 2)
+    wg, wu = (R.randn(s, E, I, H, dtype=d, scale=I ** -0.5) for s in (4, 5))
+    gx = torch.full((n + 5, H), 7.0, dtype=d, device="cuda")
+    gg, gu = (torch.empty(E, I, H, dtype=torch.float32, device="cuda") for _ in range(2))
+    ws = R.workspace(capi.moe_gate_up_swiglu_rows_backward_workspace_bytes(CODES[name], H, I, n + 5, E))
+    capi.moe_gate_up_swiglu_rows_backward(gm, both, x, wg, wu, offsets, E, gx, gg, gu, H, I, n + 5, ws=ws)
+    assert (gx[n:] == 7.0).all()
+    for e in range(E):
+        a, b = ends[e], ends[e + 1]
+        gate, up, g64 = both[a:b, :I].double(), both[a:b, I:].double(), gm[a:b].double()
+        big = 2.0 ** -19 * gate.abs().clamp(min=1.0)
+        for got, gz, e32 in ((gg[e], g64 * up * R.slope(gate, "silu"), (g64 * up).abs() * big),
+                             (gu[e], g64 * R.act(gate, "silu"), g64.abs() * big)):
+            R.check(got, *_split_sum(gz, e32, x[a:b], _terms(name), d), f"expert {e}")
+        ga, ea, gb, eb = R.swiglu_back(gm[a:b], both[a:b, :I], both[a:b, I:], d)
+        (ra, ba), (rb, bb) = R.mm_of(ga, ea, wg[e].t()), R.mm_of(gb, eb, wu[e].t())
+        R.check(gx[a:b], ra + rb, 2 * (ba + bb), f"grad_x {e}")
+
+
+# Rows that are not 16-byte aligned: few and many tiles, slices, several stages, edges inside a piece of 16 bytes
+ODD = [(1031, 515, 40), (4095, 129, 70), (2047, 1407, 130), (515, 4095, 33), (1025, 3, 300), (3, 1025, 300), (9, 9, 9), (64, 63, 65)]
+
+
+@pytest.mark.parametrize("K,N,T", ODD)
+@pytest.mark.parametrize("name", list(R.DTYPES))
+def test_odd_rows(dev, name, K, N, T):
+    d = R.DTYPES[name]
+    x, w = R.randn(1, T, K, dtype=d), R.randn(2, N, K, dtype=d, scale=K ** -0.5)
+    g, pre = R.randn(3, T, N, dtype=d, scale=0.1), R.randn(4, T, N, dtype=d).clamp(-2, 2)
+    bias, residual = R.randn(5, N, dtype=d), R.randn(6, T, N, dtype=d)
+    y, z_kept, gx = torch.empty(T, N, dtype=d, device="cuda"), torch.empty(T, N, dtype=d, device="cuda"), torch.empty_like(x)
+    gb, narrow = (torch.empty(N, dtype=torch.float32, device="cuda"), torch.empty(N, K, dtype=d, device="cuda"))
+    wide = torch.empty(N, K, dtype=torch.float32, device="cuda")
+    ws = R.workspace(capi.linear_rows_workspace_bytes(CODES[name], K, N, T))
+    capi.linear_rows(x, w, y, K, N, T, bias=bias, residual=residual, activation=capi.ACT_GELU, pre=z_kept, ws=ws)
+    ref, bound, z, ez = R.linear(x, w, bias, residual, "gelu")
+    R.check(y, ref, bound, "y")
+    R.check(z_kept, z, ez, "pre")
+    ws = R.workspace(capi.linear_rows_backward_workspace_bytes(CODES[name], K, N, T))
+    capi.linear_rows_backward(g, x, w, gx, wide, gb, K, N, T, activation=capi.ACT_SILU, pre=pre, ws=ws)
+    capi.linear_rows_backward(g, x, None, None, narrow, None, K, N, T, ws=ws)
+    gz, e32, e = R.gz_of(g, pre, "silu", d)
+    R.check(gx, *R.mm_of(gz, e, w.t()), "grad_x")
+    if name == "f32":
+        R.check(wide, *R.mm_of(gz.t(), e.t(), x.t()), "grad_w")
+    else:
+        R.check(wide, *_split_sum(gz, e32, x, _terms(name), d), "grad_w")
+    R.check(narrow, *R.mm(g.t(), x.t()), "grad_w of grad_y itself")
+    R.check(gb, gz.sum(0), 1.01 * (e32.sum(0) + (T + 2) * 2.0 ** -23 * gz.abs().sum(0)), "grad_b")
+
+
+@pytest.mark.parametrize("K,N", [(2047, 333), (333, 1407), (65, 9), (1031, 1031)])
+@pytest.mark.parametrize("name", list(R.DTYPES))
+def test_odd_rows_of_experts(dev, name, K, N):
+    """The experts' products, SwiGLU and their gradients, rows of ragged experts that no 16-byte alignment has; what is
+    behind the last row of x and of the gradients is not read (NaN) and not written."""
+    d, counts = R.DTYPES[name], [5, 0, 130, 1, 64, 0, 200, 17]
+    E, n, rows = len(counts), sum(counts), sum(counts) + 3
+    offsets = R.offsets_of(counts)
+    ends = offsets.tolist()
+    x, g, both = R.randn(1, rows, K, dtype=d), R.randn(2, rows, N, dtype=d), R.randn(3, rows, 2 * N, dtype=d).clamp(-2, 2)
+    for t in (x, g, both):
+        t[n:] = float("nan")
+    w, w2 = (R.randn(s, E, N, K, dtype=d, scale=K ** -0.5) for s in (4, 5))
+    y, mid = (torch.full((rows, N), 7.0, dtype=d, device="cuda") for _ in range(2))
+    gx, sx = (torch.full((rows, K), 7.0, dtype=d, device="cuda") for _ in range(2))
+    gw, sg, su = (torch.empty(E, N, K, dtype=d, device="cuda") for _ in range(3))
+    need = max(f(CODES[name], K, N, rows, E) for f in (
+        capi.grouped_mat_mul_rows_workspace_bytes, capi.grouped_mat_mul_rows_backward_workspace_bytes,
+        capi.moe_gate_up_swiglu_rows_workspace_bytes, capi.moe_gate_up_swiglu_rows_backward_workspace_bytes))
+    ws = R.workspace(need)
+    capi.grouped_mat_mul_rows(x, w, offsets, y, K, N, rows, ws=ws)
+    capi.moe_gate_up_swiglu_rows(x, w, w2, offsets, E, mid, K, N, rows, ws=ws)
+    capi.grouped_mat_mul_rows_backward(g, x, w, offsets, gx, gw, K, N, rows, ws=ws)
+    capi.moe_gate_up_swiglu_rows_backward(g, both, x, w, w2, offsets, E, sx, sg, su, K, N, rows, ws=ws)
+    for t in (y, mid, gx, sx):
+        assert (t[n:] == 7.0).all()
+    for e in range(E):
+        a, b = ends[e], ends[e + 1]
+        if a == b:
+            assert (gw[e] == 0).all() and (sg[e] == 0).all() and (su[e] == 0).all()
+            continue
+        z, ez = R.mm(x[a:b], w[e])
+        up, eu = R.mm(x[a:b], w2[e])
+        R.check(y[a:b], z, ez, f"y {e}")
+        s, es = R.act(z, "silu"), 1.13 * ez + 2.0 ** -19 * z.abs().clamp(min=1.0)
+        R.check(mid[a:b], s * up, 1.01 * (es * up.abs() + s.abs() * eu + es * eu + 2.0 ** -23 * (s * up).abs()), f"mid {e}")
+        R.check(gx[a:b], *R.mm(g[a:b], w[e].t()), f"grad_x {e}")
+        R.check(gw[e], *R.mm(g[a:b].t(), x[a:b].t()), f"grad_w {e}")
+        ga, ea, gb, eb = R.swiglu_back(g[a:b], both[a:b, :N], both[a:b, N:], d)
+        (ra, ba), (rb, bb) = R.mm_of(ga, ea, w[e].t()), R.mm_of(gb, eb, w2[e].t())
+        R.check(sx[a:b], ra + rb, 2 * (ba + bb), f"swiglu grad_x {e}")
+        R.check(sg[e], *R.mm_of(ga.t(), ea.t(), x[a:b].t()), f"grad_w_gate {e}")
+        R.check(su[e], *R.mm_of(gb.t(), eb.t(), x[a:b].t()), f"grad_w_up {e}")
+
+
+@pytest.mark.parametrize("name", list(R.DTYPES))
+def test_odd_places(dev, name):
+    """Sizes of whole pieces at odd addresses and strides: slices of wider matrices, on every tile that is chosen by the
+    sizes alone; what is beside the outputs stays as it was."""
+    d = R.DTYPES[name]
+    for K, N, T in ((264, 520, 100), (2056, 264, 77), (136, 5128, 1990)):
+        x = R.randn(1, T, K + 5, dtype=d)[:, 3:3 + K]
+        w = R.randn(2, N * K + 1, dtype=d, scale=K ** -0.5)[1:].view(N, K)
+        wide = torch.full((T, N + 3), 7.0, dtype=d, device="cuda")
+        y = wide[:, 1:1 + N]
+        ws = R.workspace(capi.linear_rows_workspace_bytes(CODES[name], K, N, T))
+        capi.linear_rows(x, w, y, K, N, T, activation=capi.ACT_SILU, ws=ws)
+        ref, bound, _, _ = R.linear(x, w, None, None, "silu")
+        R.check(y, ref, bound, "y")
+        assert (wide[:, :1] == 7.0).all() and (wide[:, 1 + N:] == 7.0).all()
+        g = R.randn(3, T, N + 7, dtype=d, scale=0.1)[:, 1:1 + N]
+        wide = torch.full((T, K + 3), 7.0, dtype=d, device="cuda")
+        gx, gw = wide[:, 1:1 + K], torch.full((N * K + 2,), 7.0, dtype=d, device="cuda")
+        ws = R.workspace(capi.linear_rows_backward_workspace_bytes(CODES[name], K, N, T))
+        capi.linear_rows_backward(g, x, w, gx, gw[1:-1].view(N, K), None, K, N, T, ws=ws)
+        R.check(gx, *R.mm(g, w.t()), "grad_x")
+        R.check(gw[1:-1].view(N, K), *R.mm(g.t(), x.t()), "grad_w")
+        assert (wide[:, :1] == 7.0).all() and (wide[:, 1 + K:] == 7.0).all() and gw[0] == 7.0 and gw[-1] == 7.0

@@ -1,0 +1,57 @@
+"""The kernel that the float products choose, without a GPU: the choice is compiled for the host."""
+if __name__ == "__main__":  # `python tests/<file>.py`, as the reference runs its tests
+    import sys as _sys
+
+    import pytest as _pytest
+    _sys.exit(_pytest.main([__file__, "-q"]))
+import ctypes
+import subprocess
+from pathlib import Path
+
+import pytest
+
+import _rows_paths as P
+from jjjetson_ops_amd import build, capi
+
+CODES = {"f32": capi.DTYPE_F32, "f16": capi.DTYPE_F16, "bf16": capi.DTYPE_BF16}
+CHOICE = """
+#include "rows_mm.hpp"
+extern "C" void choice(int mode, int dtype, int P, int Q, int K, int halves, int n_experts, int *out) {
+    const auto c = jjo::rows_mm_choose((jjo::RowsMode)mode, dtype, P, Q, K, halves, n_experts);
+    out[0] = c.tile == jjo::kRowsDirect ? 0 : c.tile == jjo::kRowsTile64 ? 64 : c.tile == jjo::kRowsTile128 ? 128
+             : c.tile == jjo::kRowsTile160 ? 160 : 256;
+    out[1] = c.slices;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def choose(tmp_path_factory):
+    if not Path(build.HIPCC).exists():
+        pytest.skip("no hipcc")
+    at = tmp_path_factory.mktemp("choice")
+    (at / "choice.hip").write_text(CHOICE)
+    subprocess.run([build.HIPCC, *build.HIP_FLAGS, "--offload-host-only", "-O1", "-shared", str(at / "choice.hip"),
+                    str(build.CSRC / "rows_choose.hip"), "-o", str(at / "choice.so")], check=True, capture_output=True)
+    lib = ctypes.CDLL(str(at / "choice.so"))
+
+    def call(mode, name, cols, rows, sums, halves=1, experts=0):
+        out = (ctypes.c_int * 2)()
+        lib.choice(mode, CODES[name], cols, rows, sums, halves, experts, out)
+        return out[0], out[1]
+    return call
+
+
+def _is(got, tile, slices):
+    assert got[0] == tile and (got[1] > 1 if slices == 0 else got[1] == slices), (got, tile, slices)
+
+
+def test_sizes_reach_their_kernels(choose):
+    for (name, k, n, t), tile, slices in P.LINEAR:
+        _is(choose(P.FORWARD, name, n, t, k), tile, slices)
+    for (name, k, n, t), tile, slices in P.WEIGHTS:
+        _is(choose(P.WEIGHT, name, k, n, t), tile, slices)
+    for (name, h, i, counts), tile, slices in P.SWIGLU_FORWARD:
+        _is(choose(P.SWIGLU, name, i, sum(counts), h, experts=len(counts)), tile, slices)
+    for (name, h, i, counts), tile, slices in P.SWIGLU_WEIGHTS:
+        _is(choose(P.WEIGHT, name, h, i, sum(counts), 2, len(counts)), tile, slices)
