@@ -613,9 +613,9 @@ int moe_combine_rows_backward_device(void *stream, const void *grad_y, const voi
  * 65504 in fp16); for weights' gradients in fp32 what that rounding left is multiplied as well (fp16: 22 bits of
  * it, below 2^-14 within 2^-36, in twice the work; bf16: 24 in three times).
  * Sums are added in an order that depends on the sizes alone.  Buffers are aligned to
- * their elements; where rows are 16-byte aligned as well the products are faster.  Sizes (in, out, rows) are
- * positive, any other number up to 2^28, a matrix has at most 2^40 elements.  Row strides are in
- * elements, at least the row's length.
+ * their elements; where all rows are 16-byte aligned as well the products are faster (fp32 by 1.01 to 1.2 times,
+ * 16 bits by 1.1 to 2.3).  Sizes (in, out, rows) are positive, any other number up to 2^28, a matrix has at most
+ * 2^40 elements.  Row strides are in elements, at least the row's length.
  * Outputs may not overlap inputs, except where said.  Workspaces are 256-byte aligned, may be NULL where
  * their size is 0, and may be used again by the next call on the same stream; the sizes do not depend
  * on the device.  The *_bytes functions return -1 for sizes that the call refuses.
@@ -705,8 +705,8 @@ int moe_rows_gate_up_swiglu_backward_device(void *stream, const void *grad_mid, 
  * rows go to y2).  expert_offsets NULL, or of sorted rows (forms 0 to 2) or of the sums (3).  kernel: LDS tiles
  * of 64 x 64 (0), 128 x 128 (1), 256 columns x 160 rows (2; not form 3) or 256 x 256 (3; both 16 bits only and
  * cols % 8 == 0: else tile 1 runs), 64 + w the direct kernel on w <= 8 waves (forms 0 and 1).  Operands whose
- * rows are not 16-byte aligned take tile 1 through registers.  slices of the sums, each 4 bytes an output
- * of the workspace where more than one.
+ * rows are not 16-byte aligned take tile 0 as it is and tile 1 for the others.  slices of the sums, each 4 bytes an
+ * output of the workspace where more than one.
  */
 int jjo_rows_kernel_device(void *stream, int form, int kernel, int slices, int dtype, const void *p, const void *p2,
                            const void *q, const int32_t *expert_offsets, int n_experts, void *y, void *y2, int cols,

@@ -20,8 +20,12 @@ int64_t rows_part_bytes(RowsMode mode, const RowsMm &p) {
 // (25 / 19 / 14).
 RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int halves, int n_experts) {
     constexpr int64_t kCus = 256;
-    const bool fp32 = dtype == JJO_DTYPE_F32, weight = mode == kRowsWeight;
-    const int step = fp32 ? 32 : 64;
+    const bool fp32 = dtype == JJO_DTYPE_F32, weight = mode == kRowsWeight, input = mode == kRowsInput;
+    const int step = fp32 ? 32 : 64, piece = fp32 ? 4 : 8;
+    // Rows that are not whole pieces of 16 bytes: tiles of 64 and 128 only, at times of their own; of less than a
+    // piece (16 bits) those of 128.
+    const int row_a = input || weight ? P : K, row_b = weight ? Q : K;
+    const bool odd = row_a % piece != 0 || row_b % piece != 0, copied = !fp32 && (row_a < piece || row_b < piece);
     const int64_t cols = mode == kRowsSwiglu ? 2LL * P : P;  // columns of tiles
     // Experts with rows, as far as it is known without reading the offsets, and the rows (sums) of one.
     const int M = weight ? K : Q;
@@ -33,9 +37,11 @@ RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int hal
     // workgroups and rows are long (8 rows of 8 experts, 4096 x 14336: 100 against 122 us; 14336 x 4096: 108
     // against 104; SwiGLU of 64 experts' 1408 x 2048: 19.5 against 16.5).
     const int64_t tiles64 = (cols + 63) / 64;
+    // Not on rows of 16 bits that are not aligned (4096 x 4095, 1 / 16 rows 17.4 / 28 us against 14.7 / 17.5 in four
+    // slices; 11008 x 4095 42 / 75 against 29 / 39; fp32 15.3 / 20.4 against 30 / 31).
     const bool few = n_experts == 0 ? Q <= (tiles64 < kCus / 2 ? 16 : 12)
                                     : mean <= 4 && K >= 4096 && (int64_t)experts * tiles64 < 3 * kCus;
-    if (few && (mode == kRowsForward || mode == kRowsSwiglu)) {
+    if (few && (fp32 || !odd) && (mode == kRowsForward || mode == kRowsSwiglu)) {
         const int64_t wgs = (int64_t)experts * ((cols + 15) / 16);
         return {kRowsDirect, wgs >= 4 * kCus ? 2 : 8, 1};  // as above on 2, 4, 8 waves: 100, 111, 110; 1 row 19.0, 18.8, 18.1
     }
@@ -49,13 +55,25 @@ RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int hal
     // A stage of experts' rows, where few tiles share a matrix's rows and wait for memory.
     constexpr float kExperts[] = {0.5f, 1.3f, 1.4f, 1.9f};
     constexpr Cost k32[] = {{64, 64, 2, 2.2f, 0.62f, 1.05f}, {128, 128, 2, 2.9f, 2.0f, 4.0f}};
-    const Cost *const costs = fp32 ? k32 : k16;
+    // The same of rows that are not aligned.  fp32 by words, 1.01 to 1.2 times the above.  16 bits through registers, of
+    // forward, input and weight (4095 x 4095, aligned 4096 x 4096 in brackets: 256 rows 26.5 (23.5), 2047 rows 99 (63);
+    // rows' gradients 35.5 (29) and 122 (71), weights' 31 (17) and 133 (58).  All rows at addresses of an odd number of
+    // elements cost half as much again as those at multiples of four bytes: 512 rows 70, 44 and, staged but aligned, 37).
+    constexpr Cost k32Odd[] = {{64, 64, 2, 2.2f, 0.8f, 1.12f}, {128, 128, 2, 2.9f, 2.25f, 3.9f}};
+    constexpr Cost k16Odd[][2] = {{{64, 64, 2, 2.2f, 0.4f, 0.74f}, {128, 128, 2, 2.9f, 1.0f, 1.5f}},
+                                  {{64, 64, 2, 2.2f, 0.62f, 0.8f}, {128, 128, 2, 2.9f, 1.33f, 1.87f}},
+                                  {{64, 64, 2, 2.2f, 0.73f, 0.76f}, {128, 128, 2, 2.9f, 1.55f, 2.0f}}};
+    constexpr float kExpertsOdd[] = {0.95f, 1.9f};
+    const Cost *const costs = odd ? fp32 ? k32Odd : k16Odd[input ? 1 : weight ? 2 : 0] : fp32 ? k32 : k16;
     RowsChoice best{kRowsTile128, 0, 1};
     double least = 0;
-    for (int tile = 0; tile < (fp32 ? 2 : (int)kRowsTileKinds); ++tile) {
+    // The large tiles write whole groups of eight columns.
+    const int kinds = fp32 || odd || P % 8 != 0 ? 2 : (int)kRowsTileKinds;
+    for (int tile = copied ? kRowsTile128 : kRowsTile64; tile < kinds; ++tile) {
         if (weight && tile == kRowsTile160) continue;
         Cost c = costs[tile];
-        if (n_experts > 0 && !weight && !fp32) c.two = kExperts[tile], c.one = std::max(c.one, c.two / c.a_cu);
+        if (n_experts > 0 && !weight && !fp32)
+            c.two = odd ? kExpertsOdd[tile] : kExperts[tile], c.one = std::max(c.one, c.two / c.a_cu);
         // Row tiles in all: of experts the mean over a spread of a third of their rows, as routers have.
         double tiles_q, stages;
         if (weight) {

@@ -58,14 +58,24 @@ struct RowsTile {
     static_assert(kLds <= 160 * 1024, "LDS of a CU");
 };
 
-// One operand's part of a stage: ROWS rows of the tile, TRANS: the rows of an element contiguous.
-template <class T, bool TRANS, int ROWS, int THREADS>
+// 16 bytes less their first n of eight elements, zeros behind them.
+__device__ __forceinline__ u32x4v rows_shift(u32x4v v, int n) {
+    if (n & 1) v = u32x4v{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+    if (n & 2) v = u32x4v{v[1], v[2], v[3], 0u};
+    if (n & 4) v = u32x4v{v[2], v[3], 0u, 0u};
+    return v;
+}
+
+// One operand's part of a stage: ROWS rows of the tile, TRANS: the rows of an element contiguous.  A DMA instruction
+// moves UNIT bytes a lane, a piece or a word of one.
+template <class T, bool TRANS, int ROWS, int THREADS, int UNIT = 16>
 struct RowsOperand {
     static constexpr int kPiece = 16 / sizeof(T), kStep = 128 / sizeof(T);
     static constexpr int kPitch = TRANS ? ROWS * (int)sizeof(T) : 128;  // bytes of an LDS row
     static constexpr int kRowPieces = kPitch / 16;
     static constexpr int kRuns = ROWS / 8, kWaves = THREADS / 64;  // of 64 pieces: a DMA instruction's
     static constexpr int kMine = (kRuns + kWaves - 1) / kWaves;    // of a wave
+    static constexpr int kUnits = 16 / UNIT, kDmaMine = kMine * kUnits;
     static_assert(!TRANS || ROWS % 128 == 0 || ROWS == 64, "the permutations below");
 
     // The permutation of element k's pieces (of 16 bits: pairs, 16 rows each; of 32: fours).
@@ -88,7 +98,38 @@ struct RowsOperand {
         return TRANS ? k * ld + i : i * ld + k;
     }
 
-    // ---- through registers: any address.  `from`(i, k, have) is the address of a piece, `have` the elements
+    // ---- through registers, a stage ahead, any alignment.  A piece that the rows' or the sums' end cuts is loaded
+    // as the last whole one and shifted on its way to LDS; rows behind the last are any values, sums behind theirs
+    // zeros.  `lead`: columns that the tile lacks of a piece, by which its first address is moved back (TRANS).
+    static __device__ __forceinline__ void fetch(u32x4v (&v)[kMine], const T *from, const uint32_t (&off)[kMine]) {
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) v[n] = load_any<u32x4v>((const uint8_t *)from + off[n]);
+    }
+    // ... `left` elements of a stage.
+    template <class F>
+    static __device__ __forceinline__ void fetch_last(u32x4v (&v)[kMine], int n, const T *from, int64_t ld, int left,
+                                                      int wave, F row) {
+        int i, k;
+        piece(64 * run(wave, n) + (threadIdx.x & 63), i, k);
+        v[n] = load_any<u32x4v>(from + (TRANS ? min(k, left - 1) * ld + row(i) : row(i) * ld + min(k, left - kPiece)));
+    }
+    static __device__ __forceinline__ void put(u32x4v (&v)[kMine], uint8_t *lds, int left, int rows, int wave) {
+        const int in_run = threadIdx.x & 63;
+        if (left < kStep || (TRANS && rows < ROWS && rows % kPiece != 0)) {
+#pragma unroll
+            for (int n = 0; n < kMine; ++n) {
+                int i, k;
+                piece(64 * run(wave, n) + in_run, i, k);
+                const int cut = TRANS ? max(i - (rows - kPiece), 0) : max(k - (left - kPiece), 0);
+                if (k >= left) v[n] = u32x4v{0u, 0u, 0u, 0u};
+                else v[n] = rows_shift(v[n], cut);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) *reinterpret_cast<u32x4v *>(lds + 16 * (64 * run(wave, n) + in_run)) = v[n];
+    }
+
+    // ---- piece by piece: any address and size.  `from`(i, k, have) is the address of a piece, `have` the elements
     // from it on that exist (zeros behind them).
     template <class F>
     static __device__ __forceinline__ void copy(F from, uint8_t *lds) {
@@ -114,13 +155,22 @@ struct RowsOperand {
             *reinterpret_cast<u32x4v *>(lds + 16 * (64 * run(tid >> 6, n) + (tid & 63))) = v[n];
     }
 
-    // ---- by DMA, 64 pieces an instruction: a lane's offsets; rows behind the last are the last again.
+    // ---- by DMA, 64 units an instruction: what the n-th one of a wave moves into this lane's unit, and where to.
+    static __device__ __forceinline__ void dma_unit(int wave, int n, int in_run, int &i, int &k) {
+        const int at = n % kUnits * 64 + in_run;
+        piece(64 * run(wave, n / kUnits) + at / kUnits, i, k);
+        (TRANS ? i : k) += at % kUnits;
+    }
+    static __device__ __forceinline__ uint32_t dma_to(int wave, int n) {
+        return 1024 * run(wave, n / kUnits) + 64 * UNIT * (n % kUnits);
+    }
+    // A lane's offsets; rows behind the last are the last again.
     template <class F>
-    static __device__ __forceinline__ void dma_offsets(uint32_t (&off)[kMine], int wave, int64_t ld, F row) {
+    static __device__ __forceinline__ void dma_offsets(uint32_t (&off)[kDmaMine], int wave, int64_t ld, F row) {
 #pragma unroll
-        for (int n = 0; n < kMine; ++n) {
+        for (int n = 0; n < kDmaMine; ++n) {
             int i, k;
-            piece(64 * run(wave, n) + (threadIdx.x & 63), i, k);
+            dma_unit(wave, n, threadIdx.x & 63, i, k);
             off[n] = (uint32_t)(offset(row(i), k, ld) * sizeof(T));
         }
     }
@@ -364,10 +414,33 @@ __device__ __forceinline__ void rows_dma4(const uint32_t *off, uint64_t from, ui
         : "memory", "scc");
 }
 
-// The same from an address of each lane's own.
+// ... of words, to places 256 bytes apart.
+__device__ __forceinline__ void rows_dma4_words(const uint32_t *off, uint64_t from, uint32_t lds) {
+    uint32_t m0v = __builtin_amdgcn_readfirstlane(lds);
+    from = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(from >> 32)) << 32 |
+           (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)from);
+    asm volatile(
+        "s_nop 4\n\t"
+        "global_load_lds_dword %1, %5\n\t"
+        "s_add_u32 m0, m0, 0x100\n\ts_nop 0\n\t"
+        "global_load_lds_dword %2, %5\n\t"
+        "s_add_u32 m0, m0, 0x100\n\ts_nop 0\n\t"
+        "global_load_lds_dword %3, %5\n\t"
+        "s_add_u32 m0, m0, 0x100\n\ts_nop 0\n\t"
+        "global_load_lds_dword %4, %5"
+        : "+{m0}"(m0v)
+        : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(from)
+        : "memory", "scc");
+}
+
+// One unit a lane from an address of each lane's own.
+template <int UNIT>
 __device__ __forceinline__ void rows_dma(const void *from, uint32_t lds) {
     const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds);
-    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(m0v) : "memory");
+    if constexpr (UNIT == 16)
+        asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(m0v) : "memory");
+    else
+        asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" : : "v"(from), "{m0}"(m0v) : "memory");
 }
 
 __device__ const __align__(16) uint32_t rows_zeros[4] = {0u, 0u, 0u, 0u};  // the pieces behind the sums' end
@@ -375,20 +448,27 @@ __device__ const __align__(16) uint32_t rows_zeros[4] = {0u, 0u, 0u, 0u};  // th
 // The operands of a tile and the way of their stages into LDS.
 //
 // DMA: the operands' memory rows are 16-byte aligned, the sums' elements whole pieces, and a tile's offsets
-// fit 32 bits; other operands go through registers.
-template <class T, RowsMode MODE, class Tile, bool DMA>
+// fit 32 bits.  Where they are not aligned: fp32 by DMA of words.  16 bits staged, sizes of a piece at least: a stage
+// is loaded to registers some stages ahead, and written to LDS behind the products of the one before.  Copied:
+// anything else, a stage at a time.
+enum RowsWay { kRowsDma, kRowsWords, kRowsStaged, kRowsCopied };
+template <class T, RowsMode MODE, class Tile, RowsWay WAY>
 struct RowsSource {
+    static constexpr bool DMA = WAY == kRowsDma || WAY == kRowsWords;
+    static constexpr int kUnit = WAY == kRowsWords ? 4 : 16;
+    static_assert(WAY == kRowsWords ? sizeof(T) == 4 : WAY != kRowsStaged || sizeof(T) == 2, "the ways");
     static constexpr int kStep = 128 / sizeof(T);
     static constexpr bool PT = MODE == kRowsInput || MODE == kRowsWeight, QT = MODE == kRowsWeight;
-    using OpP = RowsOperand<T, PT, Tile::kP, Tile::kThreads>;
-    using OpQ = RowsOperand<T, QT, Tile::kQ, Tile::kThreads>;
-    static constexpr int kDma = OpP::kMine + OpQ::kMine;  // of a wave and stage
+    using OpP = RowsOperand<T, PT, Tile::kP, Tile::kThreads, kUnit>;
+    using OpQ = RowsOperand<T, QT, Tile::kQ, Tile::kThreads, kUnit>;
+    static constexpr int kDma = OpP::kDmaMine + OpQ::kDmaMine;  // of a wave and stage
 
     // From the tile's first row and the sums' first element on; the second ones: up's rows (SwiGLU), the sums'
     // second half (input), and q's other terms (weight).
     const T *pm, *pm2, *qm, *qm2;
-    int rows_p, rows_q, length, stages_half;
-    uint32_t off_p[DMA ? OpP::kMine : 1], off_q[DMA ? OpQ::kMine : 1];
+    int rows_p, rows_q, length, stages_half, lead_p, lead_q;
+    static constexpr bool kOffsets = WAY != kRowsCopied;
+    uint32_t off_p[kOffsets ? OpP::kDmaMine : 1], off_q[kOffsets ? OpQ::kDmaMine : 1];
 
     // Row i of the P operand's part of a stage: of SwiGLU a wave's first 8 * RT are gate's, the others up's.
     static __device__ __forceinline__ bool is_up(int i) {
@@ -402,15 +482,25 @@ struct RowsSource {
         rows_p = min(p.P - c.p0, MODE == kRowsSwiglu ? Tile::kP / 2 : Tile::kP);
         rows_q = c.rows_q, length = c.length;
         stages_half = (length + kStep - 1) / kStep;
-        const int64_t at_p = MODE == kRowsWeight ? c.first * p.ldp + c.p0
-                                                 : c.expert * p.expert_stride + (PT ? c.p0 : c.p0 * p.ldp);
-        const int64_t at_q = QT ? c.first * p.ldq + (int64_t)c.half * p.Q + c.q0 : c.q0 * p.ldq;
+        lead_p = PT && WAY == kRowsStaged ? max(OpP::kPiece - rows_p, 0) : 0;
+        lead_q = QT && WAY == kRowsStaged ? max(OpQ::kPiece - rows_q, 0) : 0;
+        const int64_t at_p = MODE == kRowsWeight ? c.first * p.ldp + c.p0 - lead_p
+                                                 : c.expert * p.expert_stride + (PT ? c.p0 - lead_p : c.p0 * p.ldp);
+        const int64_t at_q = QT ? c.first * p.ldq + (int64_t)c.half * p.Q + c.q0 - lead_q : c.q0 * p.ldq;
         pm = (const T *)p.p + at_p, pm2 = MODE == kRowsWeight ? pm : (const T *)p.p2 + at_p;
         qm = (const T *)p.q + at_q, qm2 = MODE == kRowsWeight ? (const T *)p.rest + at_q : qm;
-        if constexpr (DMA) {
-            OpP::dma_offsets(off_p, wave, p.ldp, [&](int i) { return min(row_p(i), PT ? rows_p - OpP::kPiece : rows_p - 1); });
-            OpQ::dma_offsets(off_q, wave, p.ldq, [&](int i) { return min(i, QT ? rows_q - OpQ::kPiece : rows_q - 1); });
+        if constexpr (kOffsets) {
+            OpP::dma_offsets(off_p, wave, p.ldp, [&](int i) { return from_row_p(i); });
+            OpQ::dma_offsets(off_q, wave, p.ldq, [&](int i) { return from_row_q(i); });
         }
+    }
+    // The memory row (TRANS: column) that row i is loaded from.
+    static constexpr int kUnitElements = kUnit / sizeof(T);
+    __device__ __forceinline__ int from_row_p(int i) const {
+        return PT ? min(i, rows_p - kUnitElements) + lead_p : min(row_p(i), rows_p - 1);
+    }
+    __device__ __forceinline__ int from_row_q(int i) const {
+        return QT ? min(i, rows_q - kUnitElements) + lead_q : min(i, rows_q - 1);
     }
 
     // ---- whole stages one after the other: aim at stage st (of those below end), then `whole` of them.
@@ -449,48 +539,100 @@ struct RowsSource {
         at_q += QT ? 128 * p.ldq : 128;
     }
 
-    // Stage st to `to`; a stage without elements is zeros.
-    __device__ __forceinline__ void bring(const RowsMm &p, int st, uint8_t *to, int wave) const {
+    // Where stage st begins, and how many of the sums' elements are left there.
+    struct Stage {
+        const T *from_p, *from_up, *from_q;
+        int left;
+    };
+    __device__ __forceinline__ Stage stage(const RowsMm &p, int st) const {
         // The half or term of the sums that stage st belongs to: the last one's, past its end, behind them.
         const int parts = MODE == kRowsInput ? p.halves : MODE == kRowsWeight ? p.terms : 1;
         const int part = min((st >= stages_half) + (st >= 2 * stages_half), parts - 1);
         const bool second = part > 0;
-        const int k0 = (st - part * stages_half) * kStep, left = length - k0;
-        const T *const from_p = (second ? pm2 : pm) + (PT ? k0 * p.ldp : k0);
-        const T *const from_up = MODE == kRowsSwiglu ? pm2 + k0 : from_p;
-        const T *const from_q = (MODE == kRowsWeight && second ? qm2 + (part - 1) * p.rest_plane : qm) +
-                                (QT ? k0 * p.ldq : (second ? p.K : 0) + (int64_t)k0);
+        const int k0 = (st - part * stages_half) * kStep;
+        Stage s;
+        s.left = length - k0;
+        s.from_p = (second ? pm2 : pm) + (PT ? k0 * p.ldp : k0);
+        s.from_up = MODE == kRowsSwiglu ? pm2 + k0 : s.from_p;
+        s.from_q = (MODE == kRowsWeight && second ? qm2 + (part - 1) * p.rest_plane : qm) +
+                   (QT ? k0 * p.ldq : (second ? p.K : 0) + (int64_t)k0);
+        return s;
+    }
+
+    // ---- through registers: stage st (one with elements) to these, and these to LDS.
+    struct Held {
+        u32x4v in_p[OpP::kMine], in_q[OpQ::kMine];
+    };
+    __device__ __forceinline__ void fetch(Held &h, const RowsMm &p, int st, int wave) const {
+        auto &in_p = h.in_p;
+        auto &in_q = h.in_q;
+        const Stage s = stage(p, st);
+        if (s.left >= kStep) {
+            if constexpr (MODE == kRowsSwiglu) {
+#pragma unroll
+                for (int n = 0; n < OpP::kMine; ++n)
+                    in_p[n] = load_any<u32x4v>((const uint8_t *)(is_up(8 * OpP::run(wave, n)) ? s.from_up : s.from_p) + off_p[n]);
+            } else {
+                OpP::fetch(in_p, s.from_p, off_p);
+            }
+            OpQ::fetch(in_q, s.from_q, off_q);
+        } else {
+#pragma unroll
+            for (int n = 0; n < OpP::kMine; ++n)
+                OpP::fetch_last(in_p, n, is_up(8 * OpP::run(wave, n)) ? s.from_up : s.from_p, p.ldp, s.left, wave,
+                                [&](int i) { return from_row_p(i); });
+#pragma unroll
+            for (int n = 0; n < OpQ::kMine; ++n)
+                OpQ::fetch_last(in_q, n, s.from_q, p.ldq, s.left, wave, [&](int i) { return from_row_q(i); });
+        }
+    }
+    __device__ __forceinline__ void put(Held &h, const RowsMm &p, int st, uint8_t *to, int wave) const {
+        const int left = stage(p, st).left;
+        OpP::put(h.in_p, to, left, rows_p, wave);
+        OpQ::put(h.in_q, to + Tile::kStageP, left, rows_q, wave);
+    }
+
+    // ---- by DMA, or piece by piece: stage st to `to`; a stage without elements is zeros.
+    __device__ __forceinline__ void bring(const RowsMm &p, int st, uint8_t *to, int wave) const {
+        const Stage s = stage(p, st);
+        const T *const from_p = s.from_p, *const from_up = s.from_up, *const from_q = s.from_q;
+        const int left = s.left;
         if constexpr (DMA) {
             const uint32_t at = (uint32_t)(uintptr_t)to;
+            // The matrix of a wave's n-th instruction: of SwiGLU a run is 8 rows of one.
+            auto base_p = [&](int n) { return is_up(8 * OpP::run(wave, n / OpP::kUnits)) ? from_up : from_p; };
             if (left >= kStep) {
+                if constexpr (WAY == kRowsWords) {
 #pragma unroll
-                for (int n = 0; n < OpP::kMine; ++n) {
-                    const int run = OpP::run(wave, n);  // of SwiGLU 8 rows of one matrix
-                    rows_dma(off_p[n], (uint64_t)(is_up(8 * run) ? from_up : from_p), at + 1024 * run);
-                }
+                    for (int n = 0; n < OpP::kDmaMine; n += 4)
+                        rows_dma4_words(off_p + n, (uint64_t)base_p(n), at + OpP::dma_to(wave, n));
 #pragma unroll
-                for (int n = 0; n < OpQ::kMine; ++n) {
-                    const int run = OpQ::run(wave, n);
-                    rows_dma(off_q[n], (uint64_t)from_q, at + Tile::kStageP + 1024 * run);
+                    for (int n = 0; n < OpQ::kDmaMine; n += 4)
+                        rows_dma4_words(off_q + n, (uint64_t)from_q, at + Tile::kStageP + OpQ::dma_to(wave, n));
+                } else {
+#pragma unroll
+                    for (int n = 0; n < OpP::kDmaMine; ++n)
+                        rows_dma(off_p[n], (uint64_t)base_p(n), at + OpP::dma_to(wave, n));
+#pragma unroll
+                    for (int n = 0; n < OpQ::kDmaMine; ++n)
+                        rows_dma(off_q[n], (uint64_t)from_q, at + Tile::kStageP + OpQ::dma_to(wave, n));
                 }
             } else {  // the sums end inside the stage
                 int in_run = threadIdx.x & 63;
                 asm volatile("" : "+v"(in_run));  // one stage of many: nothing kept in registers for it
 #pragma unroll
-                for (int n = 0; n < OpP::kMine; ++n) {
+                for (int n = 0; n < OpP::kDmaMine; ++n) {
                     int i, k;
-                    const int run = OpP::run(wave, n);
-                    OpP::piece(64 * run + in_run, i, k);
-                    const T *const from = (is_up(8 * run) ? from_up : from_p) + off_p[n] / sizeof(T);
-                    rows_dma(k < left ? (const void *)from : rows_zeros, at + 1024 * run);
+                    OpP::dma_unit(wave, n, in_run, i, k);
+                    rows_dma<kUnit>(k < left ? (const void *)(base_p(n) + off_p[n] / sizeof(T)) : rows_zeros,
+                                    at + OpP::dma_to(wave, n));
                 }
 #pragma unroll
-                for (int n = 0; n < OpQ::kMine; ++n) {
+                for (int n = 0; n < OpQ::kDmaMine; ++n) {
                     int i, k;
-                    const int run = OpQ::run(wave, n);
-                    OpQ::piece(64 * run + in_run, i, k);
-                    rows_dma(k < left ? (const void *)(from_q + off_q[n] / sizeof(T)) : rows_zeros,
-                             at + Tile::kStageP + 1024 * run);
+                    OpQ::dma_unit(wave, n, in_run, i, k);
+                    rows_dma<kUnit>(k < left ? (const void *)(from_q + off_q[n] / sizeof(T)) : rows_zeros,
+                                    at + Tile::kStageP + OpQ::dma_to(wave, n));
                 }
             }
         } else {
@@ -594,39 +736,71 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
     // Weights' gradients go past the caches, in whole lines: nothing near reads them, and they would push out what
     // the tiles beside read (64 experts of 2048 x 1408, 244 tokens each: 160 us, 195 through the caches).  Stores of 64 bytes a row
     // reach 3.0 to 4.0 TB/s that way, of 128 bytes 5.6 to 6.3, as through the caches.  So lanes 8..15 of each 16
-    // exchange with 0..7: an instruction writes 128 bytes of eight rows.
+    // exchange with 0..7: an instruction writes 128 bytes of eight rows.  Rows that do not begin at multiples of 64 bytes
+    // go through the caches, which join the lines that two stores share (64 experts of 2048 x 1408 with 25 rows each, 4
+    // bytes beside: 128 us, past the caches 188; at a multiple 110).  Rows of 16 bits at odd places are written in
+    // whole words but for their ends, each lane taking the next one's first value (odd sizes: 250 us, 302 otherwise).
     if constexpr (MODE == kRowsWeight && RT == 4) {
-        if (p.P % 8 == 0) {
-            const bool high = (lane & 8) != 0;
-            auto lines = [&](u32x4v a, u32x4v b, int tt, int col, auto out) {
-                using Out = decltype(out);
+        const bool high = (lane & 8) != 0;
+        const bool past = ((uintptr_t)y | (uint64_t)ld * (to32 ? 4 : sizeof(T))) % 64 == 0;
+        auto lines = [&](u32x4v a, u32x4v b, int tt, int col, auto out) {
+            using Out = decltype(out);
+            constexpr int kN = 16 / sizeof(Out);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t x = __builtin_amdgcn_update_dpp(0, high ? a[i] : b[i], 0x128, 0xf, 0xf, false);  // row_ror:8
-                    a[i] = high ? x : a[i], b[i] = high ? b[i] : x;
-                }
-                const int in_tile = 16 * (TT * wq + tt) + (r16 & 7);
-                if (col >= p.P) return;
-                Out *const to = (Out *)y + (c.q0 + in_tile) * ld + col;
-                if (in_tile < c.rows_q) rows_store_past(to, a);
-                if (in_tile + 8 < c.rows_q) rows_store_past(to + 8 * ld, b);
-            };
-#pragma unroll
-            for (int tt = 0; tt < TT; ++tt) {
-                if (sizeof(T) == 4 || to32) {
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt += 2)
-                        lines(__builtin_bit_cast(u32x4v, acc[rt][tt]), __builtin_bit_cast(u32x4v, acc[rt + 1][tt]), tt,
-                              c.p0 + kWaveP * wp + 16 * (rt + high) + 4 * (lane >> 4), 0.0f);
-                } else if constexpr (sizeof(T) == 2) {
-                    float v[8], w[8];
-                    take(tt, 0, v, v);
-                    take(tt, 1, w, w);
-                    lines(rows_pack8<T>(v), rows_pack8<T>(w), tt, col_of(high), (T)0.0f);
-                }
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t x = __builtin_amdgcn_update_dpp(0, high ? a[i] : b[i], 0x128, 0xf, 0xf, false);  // row_ror:8
+                a[i] = high ? x : a[i], b[i] = high ? b[i] : x;
             }
-            return;
+            const int in_tile = 16 * (TT * wq + tt) + (r16 & 7);
+            Out *const to = (Out *)y + (c.q0 + in_tile) * ld + col;
+            auto store = [&](Out *at, u32x4v v, uint32_t next) {
+                if (past) return rows_store_past(at, v);
+                const MxVec<Out, kN> e = __builtin_bit_cast(MxVec<Out, kN>, v);
+                if (col + kN > p.P) {
+#pragma unroll
+                    for (int i = 0; i < kN - 1; ++i)
+                        if (col + i < p.P) at[i] = e.v[i];
+                } else if (sizeof(Out) == 4 || (uintptr_t)at % 4 == 0) {
+                    store_any(at, v);
+                } else {  // whole words: from the second value on, with the next lane's first
+                    const bool whole = lane < 56 && col + kN < p.P;
+                    const uint32_t w[4] = {v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16,
+                                           v[3] >> 16 | next << 16};
+                    typedef uint32_t Words3 __attribute__((ext_vector_type(3), aligned(4)));
+                    typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(4)));
+                    if (whole) {
+                        *(Words4 *)(at + 1) = Words4{w[0], w[1], w[2], w[3]};
+                    } else {
+                        *(Words3 *)(at + 1) = Words3{w[0], w[1], w[2]};
+                        at[kN - 1] = e.v[kN - 1];
+                    }
+                    if (lane < 8) at[0] = e.v[0];
+                }
+            };
+            uint32_t next_a = 0, next_b = 0;
+            if (sizeof(Out) == 2 && !past) {  // of the columns' next eight: lanes + 32, then + 16, then + 8
+                const int next = 4 * (upper == 0 ? lane ^ 32 : odd == 0 ? lane ^ 48 : lane ^ 56);
+                next_a = __builtin_amdgcn_ds_bpermute(next, a[0]), next_b = __builtin_amdgcn_ds_bpermute(next, b[0]);
+            }
+            if (col >= p.P) return;
+            if (in_tile < c.rows_q) store(to, a, next_a);
+            if (in_tile + 8 < c.rows_q) store(to + 8 * ld, b, next_b);
+        };
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+            if (sizeof(T) == 4 || to32) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt += 2)
+                    lines(__builtin_bit_cast(u32x4v, acc[rt][tt]), __builtin_bit_cast(u32x4v, acc[rt + 1][tt]), tt,
+                          c.p0 + kWaveP * wp + 16 * (rt + high) + 4 * (lane >> 4), 0.0f);
+            } else if constexpr (sizeof(T) == 2) {
+                float v[8], w[8];
+                take(tt, 0, v, v);
+                take(tt, 1, w, w);
+                lines(rows_pack8<T>(v), rows_pack8<T>(w), tt, col_of(high), (T)0.0f);
+            }
         }
+        return;
     }
     if (KIND != kRowsAny || (p.P % 8 == 0 && (parts || (e.bias == nullptr && e.residual == nullptr && e.pre == nullptr && e.act == JJO_ACT_NONE)))) {
         auto all = [&](auto wide_tag) {
@@ -703,11 +877,16 @@ __device__ __forceinline__ void rows_turn(const RowsMm &p, const RowsPlace &c, i
 }
 
 // ---- four waves, a tile a workgroup, two or more workgroups a CU: one stages while another multiplies.
-template <class E, RowsMode MODE, class Tile, bool DMA>
+// Stages that the staged way holds in registers.  bf16, odd K and N, us: tiles of 64, 64 x 4095 over 4095 with one 18.0,
+// with three 15.9 (of four waves their loads are most of what a CU waits for); tiles of 128, 2047 rows, forward 98 with
+// one and 109 with two, rows' gradients 128 and 123, weights' 136 and 136.
+template <RowsMode MODE, int RT>
+constexpr int kRowsHeld = RT == 2 ? 3 : MODE == kRowsInput ? 2 : 1;
+template <class E, RowsMode MODE, class Tile, RowsWay WAY>
 __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p, int most) {
     typedef typename E::type T;
     constexpr int RT = Tile::RT, TT = Tile::TT;
-    using Source = RowsSource<T, MODE, Tile, DMA>;
+    using Source = RowsSource<T, MODE, Tile, WAY>;
     extern __shared__ __align__(16) uint8_t lds[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wp = wave % Tile::WP, wq = wave / Tile::WP;
@@ -725,47 +904,80 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p, int m
         for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = f32x4v{0.f, 0.f, 0.f, 0.f};
     const typename Source::OpP::Reader read_p(16 * RT * wp);
     const typename Source::OpQ::Reader read_q(16 * TT * wq);
-    constexpr int kAhead = Tile::NB - 1;  // stages on their way while one is multiplied
+    auto step = [&](auto u_tag, const uint8_t *in_p) {
+        constexpr int U = decltype(u_tag)::value;
+        const uint8_t *const in_q = in_p + Tile::kStageP;
+        u32x4v a[RT], b[TT];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-        if (c.s_beg + i < c.s_end) source.bring(p, c.s_beg + i, lds + i * Tile::kStage, wave);
-    int buffer = 0;
-    for (int st = c.s_beg; st < c.s_end; ++st) {
-        // Stage st has landed, and no wave reads the buffer of stage st - 1 any more.
-        if (st + kAhead - 1 < c.s_end)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((kAhead - 1) * Source::kDma) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (st + kAhead < c.s_end)
-            source.bring(p, st + kAhead, lds + (buffer == 0 ? Tile::NB - 1 : buffer - 1) * Tile::kStage, wave);
-        const uint8_t *const in_p = lds + buffer * Tile::kStage, *const in_q = in_p + Tile::kStageP;
-        auto step = [&](auto u_tag) {
-            constexpr int U = decltype(u_tag)::value;
-            u32x4v a[RT], b[TT];
+        for (int rt = 0; rt < RT; ++rt) a[rt] = read_p.template read<U>(in_p, rt);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) a[rt] = read_p.template read<U>(in_p, rt);
+        for (int tt = 0; tt < TT; ++tt) b[tt] = read_q.template read<U>(in_q, tt);
+        if constexpr (sizeof(T) == 4) {  // in turn: the next sum of a tile does not wait for its last
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt) b[tt] = read_q.template read<U>(in_q, tt);
-            if constexpr (sizeof(T) == 4) {  // in turn: the next sum of a tile does not wait for its last
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-                            acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                __uint_as_float(a[rt][j]), __uint_as_float(b[tt][j]), acc[rt][tt], 0, 0, 0);
-            } else {
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) acc[rt][tt] = rows_mfma<T>(a[rt], b[tt], acc[rt][tt]);
+                    for (int rt = 0; rt < RT; ++rt)
+                        acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                            __uint_as_float(a[rt][j]), __uint_as_float(b[tt][j]), acc[rt][tt], 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) acc[rt][tt] = rows_mfma<T>(a[rt], b[tt], acc[rt][tt]);
+        }
+    };
+    auto multiply = [&](int st, const uint8_t *in) {
+        step(std::integral_constant<int, 0>{}, in);
+        step(std::integral_constant<int, 1>{}, in);
+        rows_turn<T, MODE, Tile>(p, c, st, acc);
+    };
+    if constexpr (WAY == kRowsStaged) {
+        static_assert(Tile::NB == 2, "the buffer of the stage before is the next one's");
+        // kAhead stages on their way to registers while one is multiplied.  Behind the last stage it is loaded again:
+        // every wait then counts the same loads behind those that it is for.
+        constexpr int kAhead = kRowsHeld<MODE, RT>;
+        auto all = [&]() {
+            typename Source::Held held[kAhead];
+            const int last = c.s_end - 1;
+            int st = c.s_beg;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) source.fetch(held[i], p, min(st + i, last), wave);
+            uint8_t *in = lds, *next = lds + Tile::kStage;
+            source.put(held[0], p, st, in, wave);
+            for (;;) {
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    source.fetch(held[i], p, min(st + kAhead, last), wave);
+                    // Stage st is in LDS, and no wave reads the buffer of stage st - 1 any more.
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    multiply(st, in);
+                    if (++st > last) return;
+                    source.put(held[(i + 1) % kAhead], p, st, next, wave);
+                    uint8_t *const was = in;
+                    in = next, next = was;
+                }
             }
         };
-        step(std::integral_constant<int, 0>{});
-        step(std::integral_constant<int, 1>{});
-        rows_turn<T, MODE, Tile>(p, c, st, acc);
-        buffer = buffer == Tile::NB - 1 ? 0 : buffer + 1;
+        if (c.s_beg < c.s_end) all();
+    } else {
+        constexpr int kAhead = Tile::NB - 1;  // stages on their way while one is multiplied
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (c.s_beg + i < c.s_end) source.bring(p, c.s_beg + i, lds + i * Tile::kStage, wave);
+        int buffer = 0;
+        for (int st = c.s_beg; st < c.s_end; ++st) {
+            // Stage st has landed, and no wave reads the buffer of stage st - 1 any more.
+            if (st + kAhead - 1 < c.s_end)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((kAhead - 1) * Source::kDma) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (st + kAhead < c.s_end)
+                source.bring(p, st + kAhead, lds + (buffer == 0 ? Tile::NB - 1 : buffer - 1) * Tile::kStage, wave);
+            multiply(st, lds + buffer * Tile::kStage);
+            buffer = buffer == Tile::NB - 1 ? 0 : buffer + 1;
+        }
     }
     rows_output<T, MODE, kRowsAny, Tile>(p, c, acc, wp, wq);
 }
@@ -783,7 +995,7 @@ template <class E, RowsMode MODE, RowsOutput KIND, class Tile>
 __global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, int most) {
     typedef typename E::type T;
     constexpr int RT = Tile::RT, TT = Tile::TT;
-    using Source = RowsSource<T, MODE, Tile, true>;
+    using Source = RowsSource<T, MODE, Tile, kRowsDma>;
     extern __shared__ __align__(16) uint8_t lds[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wp = wave % Tile::WP, wq = wave / Tile::WP;
@@ -912,7 +1124,7 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_stream_kernel(RowsMm p, i
     if (wave < 4) slot_end();
 }
 
-template <class E, RowsMode MODE, class Tile, bool DMA>
+template <class E, RowsMode MODE, class Tile, RowsWay WAY>
 hipError_t run_rows(RowsMm p, hipStream_t stream) {
     constexpr int kOutP = MODE == kRowsSwiglu ? Tile::kP / 2 : Tile::kP;
     p.tiles_p = (p.P + kOutP - 1) / kOutP;
@@ -939,35 +1151,40 @@ hipError_t run_rows(RowsMm p, hipStream_t stream) {
                 return go(rows_stream_kernel<E, MODE, kRowsFull, Tile>, wgs);
         return go(rows_stream_kernel<E, MODE, kRowsPlain, Tile>, wgs);
     } else
-        return go(rows_mm_kernel<E, MODE, Tile, DMA>, (int)blocks);
+        return go(rows_mm_kernel<E, MODE, Tile, WAY>, (int)blocks);
 }
 
 // DMA where every memory row of both operands is 16-byte aligned, a tile's rows and a stage's elements
-// are within 4 GiB of its first, and (where rows of an element are contiguous) rows come in whole pieces.
-inline bool rows_dma_accepts(RowsMode mode, int es, const RowsMm &p) {
+// are within 4 GiB of its first, and rows come in whole pieces.
+inline RowsWay rows_way(RowsMode mode, int es, const RowsMm &p) {
     const int piece = 16 / es;
-    auto fits = [&](const void *m, int64_t ld) {
-        return (uintptr_t)m % 16 == 0 && ld % piece == 0 && ld * es < (1LL << 32) / 512;
-    };
-    if (!fits(p.p, p.ldp) || !fits(p.q, p.ldq)) return false;
-    if (p.p2 != nullptr && !fits(p.p2, p.ldp)) return false;
-    if (p.rest != nullptr && (!fits(p.rest, p.ldq) || p.rest_plane % piece != 0)) return false;
-    if (mode == kRowsWeight) return p.P % piece == 0 && p.Q % piece == 0;
-    return p.K % piece == 0 && (mode != kRowsInput || p.P % piece == 0);
+    // The contiguous directions: of both operands the sums' (forward), P's and the sums' (input), P's and Q's (weight).
+    const int a = mode == kRowsForward || mode == kRowsSwiglu ? p.K : p.P, b = mode == kRowsWeight ? p.Q : p.K;
+    if (p.ldp * es >= (1LL << 32) / 512 || p.ldq * es >= (1LL << 32) / 512) return kRowsCopied;
+    auto aligned = [&](const void *m, int64_t ld) { return (uintptr_t)m % 16 == 0 && ld % piece == 0; };
+    const bool all = aligned(p.p, p.ldp) && aligned(p.q, p.ldq) && aligned(p.p2, p.ldp) && aligned(p.rest, p.ldq) &&
+                     p.rest_plane % piece == 0 && a % piece == 0 && b % piece == 0;
+    return all ? kRowsDma : es == 4 ? kRowsWords : a < piece || b < piece ? kRowsCopied : kRowsStaged;
 }
 
 template <class E, RowsMode MODE>
 hipError_t rows_by_tile(const RowsMm &p, int tile, hipStream_t stream) {
-    if (!rows_dma_accepts(MODE, (int)sizeof(typename E::type), p))
-        return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, false>(p, stream);
-    if (tile == kRowsTile64) return run_rows<E, MODE, RowsTile<2, 2, 2, 2, 4>, true>(p, stream);
+    const RowsWay way = rows_way(MODE, (int)sizeof(typename E::type), p);
+    if (way == kRowsCopied) return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, kRowsCopied>(p, stream);
+    if (way != kRowsDma) {
+        constexpr bool kWords = sizeof(typename E::type) == 4;
+        constexpr RowsWay kWay = kWords ? kRowsWords : kRowsStaged;
+        if (tile == kRowsTile64) return run_rows<E, MODE, RowsTile<2, 2, 2, 2, kWords ? 4 : 2>, kWay>(p, stream);
+        return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, kWay>(p, stream);
+    }
+    if (tile == kRowsTile64) return run_rows<E, MODE, RowsTile<2, 2, 2, 2, 4>, kRowsDma>(p, stream);
     if constexpr (sizeof(typename E::type) == 2) {
         // The large tiles write whole groups of eight columns.
-        if (tile == kRowsTile256 && p.P % 8 == 0) return run_rows<E, MODE, RowsTile<4, 8, 4, 2>, true>(p, stream);
+        if (tile == kRowsTile256 && p.P % 8 == 0) return run_rows<E, MODE, RowsTile<4, 8, 4, 2>, kRowsDma>(p, stream);
         if constexpr (MODE != kRowsWeight)
-            if (tile == kRowsTile160 && p.P % 8 == 0) return run_rows<E, MODE, RowsTile<4, 5, 4, 2, 3>, true>(p, stream);
+            if (tile == kRowsTile160 && p.P % 8 == 0) return run_rows<E, MODE, RowsTile<4, 5, 4, 2, 3>, kRowsDma>(p, stream);
     }
-    return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, true>(p, stream);
+    return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, kRowsDma>(p, stream);
 }
 
 }  // namespace

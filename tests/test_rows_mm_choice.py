@@ -55,3 +55,29 @@ def test_sizes_reach_their_kernels(choose):
         _is(choose(P.SWIGLU, name, i, sum(counts), h, experts=len(counts)), tile, slices)
     for (name, h, i, counts), tile, slices in P.SWIGLU_WEIGHTS:
         _is(choose(P.WEIGHT, name, h, i, sum(counts), 2, len(counts)), tile, slices)
+
+
+def _workgroups(got, cols, rows):
+    return -(-cols // got[0]) * -(-rows // got[0]) * got[1]
+
+
+@pytest.mark.parametrize("name", list(CODES))
+def test_rows_without_alignment_get_kernels_that_run(choose, name):
+    """Sizes that are no multiples of 16 bytes: tiles of 64 or 128, and slices that fill the CUs with those; never the
+    large tiles, and of 16 bits never the direct kernel."""
+    piece = 4 if name == "f32" else 8
+    for rows in (1, 7, 16, 40, 64, 128, 256, 512, 2047):
+        for cols, sums in ((4096, 4095), (4095, 4095), (1408, 2047), (11008, 4094)):
+            got = choose(P.FORWARD, name, cols, rows, sums)
+            assert got[0] in ((0, 64, 128) if name == "f32" and rows <= 16 else (64, 128)), (rows, cols, sums, got)
+            if got[0] and sums > 32 * piece * 8:
+                assert _workgroups(got, cols, rows) >= 128, (rows, cols, sums, got)
+            got = choose(P.INPUT, name, sums, rows, cols)
+            assert got[0] in (64, 128) and _workgroups(got, sums, rows) >= 64, (rows, cols, sums, got)
+            assert choose(P.WEIGHT, name, sums, cols, rows)[0] in (64, 128)
+            assert choose(P.SWIGLU, name, cols, rows * 8, sums, experts=8)[0] in ((0, 64, 128) if name == "f32" else (64, 128))
+    # K aligned, the output's columns not: the tiles of 160 and 256 rows write whole groups of eight columns
+    assert choose(P.FORWARD, name, 14337, 2047, 4096)[0] in (64, 128)
+    # less than a piece: tiles of 128, which these run on
+    if name != "f32":
+        assert choose(P.FORWARD, name, 4096, 2047, 7)[0] == 128 and choose(P.WEIGHT, name, 4096, 5, 2047)[0] == 128
