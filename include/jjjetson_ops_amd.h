@@ -618,7 +618,10 @@ int moe_combine_rows_backward_device(void *stream, const void *grad_y, const voi
  * 2^40 elements.  Row strides are in elements, at least the row's length.
  * Outputs may not overlap inputs, except where said.  Workspaces are 256-byte aligned, may be NULL where
  * their size is 0, and may be used again by the next call on the same stream; the sizes do not depend
- * on the device.  The *_bytes functions return -1 for sizes that the call refuses.
+ * on the device.  The *_bytes functions return -1 for sizes that the call refuses.  Those of the backward passes are
+ * enough for any call of the sizes; the *_bytes_for functions for those of an activation and of a dtype of the weights'
+ * gradients, which may be much less (the gradient through an activation is kept there, in up to three terms).  A call
+ * refuses less than what it uses itself.
  */
 #define JJO_ACT_NONE 0
 #define JJO_ACT_RELU 1      /* max(z, 0) */
@@ -643,6 +646,8 @@ int linear_rows_forward_device(void *stream, const void *x, int64_t x_stride, co
  * grad_weight_dtype: `dtype` or fp32.
  */
 int64_t linear_rows_backward_workspace_bytes(int dtype, int in_features, int out_features, int num_tokens);
+int64_t linear_rows_backward_workspace_bytes_for(int dtype, int grad_weight_dtype, int activation, int in_features,
+                                                 int out_features, int num_tokens);
 int linear_rows_backward_device(void *stream, const void *grad_y, int64_t grad_y_stride, const void *x,
                                 int64_t x_stride, const void *weight, const void *pre, void *grad_x,
                                 int64_t grad_x_stride, void *grad_weight, void *grad_bias, int dtype,
@@ -690,6 +695,8 @@ int moe_rows_gate_up_swiglu_device(void *stream, const void *x_sorted, const voi
  */
 int64_t moe_rows_gate_up_swiglu_backward_workspace_bytes(int dtype, int hidden_size, int intermediate_size,
                                                          int n_routes, int num_experts);
+int64_t moe_rows_gate_up_swiglu_backward_workspace_bytes_for(int dtype, int grad_weights_dtype, int hidden_size,
+                                                             int intermediate_size, int n_routes, int num_experts);
 int moe_rows_gate_up_swiglu_backward_device(void *stream, const void *grad_mid, const void *gate_up,
                                             const void *x_sorted, const void *w_gate, const void *w_up,
                                             const int32_t *expert_offsets, int num_experts, void *grad_x_sorted,

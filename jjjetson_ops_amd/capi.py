@@ -99,6 +99,7 @@ EXPORTED_SYMBOLS = (
     "linear_rows_workspace_bytes",
     "linear_rows_forward_device",
     "linear_rows_backward_workspace_bytes",
+    "linear_rows_backward_workspace_bytes_for",
     "linear_rows_backward_device",
     "mat_mul_rows_grouped_workspace_bytes",
     "mat_mul_rows_grouped_device",
@@ -107,6 +108,7 @@ EXPORTED_SYMBOLS = (
     "moe_rows_gate_up_swiglu_workspace_bytes",
     "moe_rows_gate_up_swiglu_device",
     "moe_rows_gate_up_swiglu_backward_workspace_bytes",
+    "moe_rows_gate_up_swiglu_backward_workspace_bytes_for",
     "moe_rows_gate_up_swiglu_backward_device",
     "jjo_rows_kernel_device",
 )
@@ -292,6 +294,9 @@ def lib() -> ctypes.CDLL:
                      "moe_rows_gate_up_swiglu_backward"):
             f = getattr(L, name + "_workspace_bytes")
             f.restype, f.argtypes = i64, [i32, i32, i32, i32, i32]
+        for name in ("linear_rows_backward", "moe_rows_gate_up_swiglu_backward"):
+            f = getattr(L, name + "_workspace_bytes_for")
+            f.restype, f.argtypes = i64, [i32, i32, i32, i32, i32, i32]
         L.linear_rows_forward_device.restype = i32
         L.linear_rows_forward_device.argtypes = [vp, vp, i64, vp, vp, vp, i64, vp, i64, vp, i32, i32, i32, i32, i32,
                                                  vp, i64]
@@ -957,8 +962,15 @@ def linear_rows(x, w, y, in_features: int, out_features: int, num_tokens: int, b
            activation, in_features, out_features, num_tokens, ws, _bytes_of(ws))
 
 
-def linear_rows_backward_workspace_bytes(dtype: int, in_features: int, out_features: int, num_tokens: int) -> int:
-    return int(lib().linear_rows_backward_workspace_bytes(dtype, in_features, out_features, num_tokens))
+def linear_rows_backward_workspace_bytes(dtype: int, in_features: int, out_features: int, num_tokens: int,
+                                         activation: int | None = None, grad_dtype: int | None = None) -> int:
+    """Enough for any backward pass of these sizes; with an activation and the dtype of the weights' gradients (the
+    rows' where it is None) for those."""
+    if activation is None and grad_dtype is None:
+        return int(lib().linear_rows_backward_workspace_bytes(dtype, in_features, out_features, num_tokens))
+    return int(lib().linear_rows_backward_workspace_bytes_for(
+        dtype, dtype if grad_dtype is None else grad_dtype, ACT_SILU if activation is None else activation, in_features,
+        out_features, num_tokens))
 
 
 def linear_rows_backward(grad_y, x, w, grad_x, grad_w, grad_b, in_features: int, out_features: int, num_tokens: int,
@@ -1036,8 +1048,12 @@ def moe_gate_up_swiglu_rows(x, w_gate, w_up, expert_offsets, num_experts: int, m
 
 
 def moe_gate_up_swiglu_rows_backward_workspace_bytes(dtype: int, hidden: int, inter: int, n_routes: int,
-                                                     num_experts: int) -> int:
-    return int(lib().moe_rows_gate_up_swiglu_backward_workspace_bytes(dtype, hidden, inter, n_routes, num_experts))
+                                                     num_experts: int, grad_dtype: int | None = None) -> int:
+    """Enough for any backward pass of these sizes; with the dtype of the weights' gradients for those."""
+    if grad_dtype is None:
+        return int(lib().moe_rows_gate_up_swiglu_backward_workspace_bytes(dtype, hidden, inter, n_routes, num_experts))
+    return int(lib().moe_rows_gate_up_swiglu_backward_workspace_bytes_for(dtype, grad_dtype, hidden, inter, n_routes,
+                                                                          num_experts))
 
 
 def moe_gate_up_swiglu_rows_backward(grad_mid, gate_up, x, w_gate, w_up, expert_offsets, num_experts: int, grad_x,

@@ -60,6 +60,12 @@ int check_workspace(const char *who, const void *ws, int64_t have, int64_t need)
     return JJO_OK;
 }
 
+int check_activation(const char *who, int activation) {
+    if (activation < JJO_ACT_NONE || activation > JJO_ACT_SILU)
+        return set_error(JJO_ERR_INVALID_ARG, "%s: unknown activation %d", who, activation);
+    return JJO_OK;
+}
+
 int check_grad_dtype(const char *who, int grad_dtype, int dtype) {
     if (grad_dtype != dtype && grad_dtype != JJO_DTYPE_F32)
         return set_error(JJO_ERR_INVALID_ARG, "%s: gradients of the weights are of the weights' dtype or fp32", who);
@@ -124,22 +130,37 @@ void terms_of_gz(RowsMm &m, const uint8_t *gz, int64_t plane, int planes, int es
     if (planes == 2) m.first_scale = 1.0f / kRowsRestScale;
 }
 
+// What a backward pass is asked for, and with it what its workspace holds.
+struct Wanted {
+    bool rows, weights, bias;
+};
+constexpr Wanted kAll{true, true, true};
+
+// Sums in slices of the products asked for, one after the other in the same place (n_experts 0: one matrix).
+int64_t part_bytes(int dtype, int K, int N, int rows, int n_experts, int halves, Wanted want) {
+    const int64_t a = want.rows ? rows_part_bytes(kRowsInput, input(dtype, K, N, rows, n_experts, halves)) : 0;
+    const int64_t b = want.weights ? rows_part_bytes(kRowsWeight, weight(dtype, K, N, rows, n_experts, halves, false)) : 0;
+    return up256(std::max(a, b));
+}
+
+// Planes of gz: none without an activation.
+int planes_of(int dtype, int grad_weight_dtype, bool act, bool weights) {
+    return !act ? 0 : weights && grad_weight_dtype != dtype ? gz_planes(dtype) : 1;
+}
+
 struct LinearBackwardWs {
     int64_t gz, plane, columns, parts, bytes;  // offsets; bytes of a plane of gz
 };
-LinearBackwardWs linear_backward_ws(int dtype, int K, int N, int T) {
+LinearBackwardWs linear_backward_ws(int dtype, int K, int N, int T, int planes, Wanted want) {
     LinearBackwardWs w{};
     w.plane = gz_plane_bytes(dtype, (int64_t)T * N);
-    w.columns = gz_planes(dtype) * w.plane;
-    w.parts = w.columns + up256(4LL * rows_column_chunks(T, N) * N);
-    w.bytes = w.parts + up256(std::max(rows_part_bytes(kRowsInput, input(dtype, K, N, T, 0, 1)),
-                                       rows_part_bytes(kRowsWeight, weight(dtype, K, N, T, 0, 1, false))));
+    w.columns = planes * w.plane;
+    w.parts = w.columns + (want.bias ? up256(4LL * rows_column_chunks(T, N) * N) : 0);
+    w.bytes = w.parts + part_bytes(dtype, K, N, T, 0, 1, want);
     return w;
 }
-
-int64_t grouped_backward_bytes(int dtype, int K, int N, int rows, int n_experts, int halves) {
-    return up256(std::max(rows_part_bytes(kRowsInput, input(dtype, K, N, rows, n_experts, halves)),
-                          rows_part_bytes(kRowsWeight, weight(dtype, K, N, rows, n_experts, halves, false))));
+int64_t swiglu_backward_bytes(int dtype, int H, int I, int rows, int n_experts, int planes, Wanted want) {
+    return planes * gz_plane_bytes(dtype, 2LL * rows * I) + part_bytes(dtype, H, I, rows, n_experts, 2, want);
 }
 
 }  // namespace
@@ -161,8 +182,7 @@ int linear_rows_forward_device(void *stream, const void *x, int64_t x_stride, co
     const int K = in_features, N = out_features, T = num_tokens;
     JJO_TRY(check_sizes(who, dtype, K, N, T, 1));
     const int es = elem_bytes(dtype);
-    if (activation < JJO_ACT_NONE || activation > JJO_ACT_SILU)
-        return set_error(JJO_ERR_INVALID_ARG, "%s: unknown activation %d", who, activation);
+    JJO_TRY(check_activation(who, activation));
     JJO_TRY(check_ptr(who, "x", x, es));
     JJO_TRY(check_ptr(who, "weight", weight_, es));
     JJO_TRY(check_ptr(who, "bias", bias, es, true));
@@ -186,7 +206,18 @@ int linear_rows_forward_device(void *stream, const void *x, int64_t x_stride, co
 int64_t linear_rows_backward_workspace_bytes(int dtype, int in_features, int out_features, int num_tokens) {
     clear_error();
     if (check_sizes("linear_rows_backward", dtype, in_features, out_features, num_tokens, 1) != JJO_OK) return -1;
-    return linear_backward_ws(dtype, in_features, out_features, num_tokens).bytes;
+    return linear_backward_ws(dtype, in_features, out_features, num_tokens, gz_planes(dtype), kAll).bytes;
+}
+
+int64_t linear_rows_backward_workspace_bytes_for(int dtype, int grad_weight_dtype, int activation, int in_features,
+                                                 int out_features, int num_tokens) {
+    clear_error();
+    const char *who = "linear_rows_backward";
+    if (check_sizes(who, dtype, in_features, out_features, num_tokens, 1) != JJO_OK ||
+        check_grad_dtype(who, grad_weight_dtype, dtype) != JJO_OK || check_activation(who, activation) != JJO_OK)
+        return -1;
+    const int planes = planes_of(dtype, grad_weight_dtype, activation != JJO_ACT_NONE, true);
+    return linear_backward_ws(dtype, in_features, out_features, num_tokens, planes, kAll).bytes;
 }
 
 int linear_rows_backward_device(void *stream, const void *grad_y, int64_t grad_y_stride, const void *x,
@@ -201,8 +232,7 @@ int linear_rows_backward_device(void *stream, const void *grad_y, int64_t grad_y
     JJO_TRY(check_grad_dtype(who, grad_weight_dtype, dtype));
     const int es = elem_bytes(dtype), ges = elem_bytes(grad_weight_dtype);
     const bool wide = grad_weight_dtype == JJO_DTYPE_F32, act = activation != JJO_ACT_NONE;
-    if (activation < JJO_ACT_NONE || activation > JJO_ACT_SILU)
-        return set_error(JJO_ERR_INVALID_ARG, "%s: unknown activation %d", who, activation);
+    JJO_TRY(check_activation(who, activation));
     if (grad_x == nullptr && grad_weight == nullptr && grad_bias == nullptr)
         return set_error(JJO_ERR_INVALID_ARG, "%s: no gradient is asked for", who);
     JJO_TRY(check_ptr(who, "grad_y", grad_y, es));
@@ -215,14 +245,15 @@ int linear_rows_backward_device(void *stream, const void *grad_y, int64_t grad_y
     JJO_TRY(check_stride(who, "grad_y_stride", grad_y_stride, N, T));
     if (grad_weight != nullptr) JJO_TRY(check_stride(who, "x_stride", x_stride, K, T));
     if (grad_x != nullptr) JJO_TRY(check_stride(who, "grad_x_stride", grad_x_stride, K, T));
-    const LinearBackwardWs ws = linear_backward_ws(dtype, K, N, T);
+    const int planes = planes_of(dtype, grad_weight_dtype, act, grad_weight != nullptr);
+    const LinearBackwardWs ws =
+        linear_backward_ws(dtype, K, N, T, planes, {grad_x != nullptr, grad_weight != nullptr, grad_bias != nullptr});
     JJO_TRY(check_workspace(who, workspace, workspace_bytes, ws.bytes));
     JJO_TRY(require_device());
     hipStream_t s = (hipStream_t)stream;
     uint8_t *const base = (uint8_t *)workspace;
     const void *gz = grad_y;
     int64_t gz_stride = stride_of(grad_y_stride, N, T);
-    const int planes = act && wide && grad_weight != nullptr ? gz_planes(dtype) : 1;
     if (act || grad_bias != nullptr) {
         const hipError_t e = launch_rows_act_backward(grad_y, gz_stride, pre, base + ws.gz, planes, ws.plane / es, dtype, activation,
                                                       grad_bias, wide, (float *)(base + ws.columns), T, N, s);
@@ -276,7 +307,7 @@ int64_t mat_mul_rows_grouped_backward_workspace_bytes(int dtype, int ncols_k, in
     clear_error();
     if (check_sizes("mat_mul_rows_grouped_backward", dtype, ncols_k, nrows_out, n_routes, n_experts) != JJO_OK)
         return -1;
-    return grouped_backward_bytes(dtype, ncols_k, nrows_out, n_routes, n_experts, 1);
+    return part_bytes(dtype, ncols_k, nrows_out, n_routes, n_experts, 1, kAll);
 }
 
 int mat_mul_rows_grouped_backward_device(void *stream, const void *grad_y, const void *x_sorted, const void *weights,
@@ -297,7 +328,8 @@ int mat_mul_rows_grouped_backward_device(void *stream, const void *grad_y, const
     JJO_TRY(check_ptr(who, "grad_x_sorted", grad_x_sorted, es, true));
     JJO_TRY(check_ptr(who, "grad_weights", grad_weights, elem_bytes(grad_weights_dtype), true));
     JJO_TRY(check_workspace(who, workspace, workspace_bytes,
-                            grouped_backward_bytes(dtype, ncols_k, nrows_out, n_routes, n_experts, 1)));
+                            part_bytes(dtype, ncols_k, nrows_out, n_routes, n_experts, 1,
+                                       {grad_x_sorted != nullptr, grad_weights != nullptr, false})));
     JJO_TRY(require_device());
     hipStream_t s = (hipStream_t)stream;
     if (grad_x_sorted != nullptr) {
@@ -351,8 +383,18 @@ int64_t moe_rows_gate_up_swiglu_backward_workspace_bytes(int dtype, int hidden_s
     if (check_sizes("moe_rows_gate_up_swiglu_backward", dtype, hidden_size, intermediate_size, n_routes, num_experts) !=
         JJO_OK)
         return -1;
-    return gz_planes(dtype) * gz_plane_bytes(dtype, 2LL * n_routes * intermediate_size) +
-           grouped_backward_bytes(dtype, hidden_size, intermediate_size, n_routes, num_experts, 2);
+    return swiglu_backward_bytes(dtype, hidden_size, intermediate_size, n_routes, num_experts, gz_planes(dtype), kAll);
+}
+
+int64_t moe_rows_gate_up_swiglu_backward_workspace_bytes_for(int dtype, int grad_weights_dtype, int hidden_size,
+                                                             int intermediate_size, int n_routes, int num_experts) {
+    clear_error();
+    const char *who = "moe_rows_gate_up_swiglu_backward";
+    if (check_sizes(who, dtype, hidden_size, intermediate_size, n_routes, num_experts) != JJO_OK ||
+        check_grad_dtype(who, grad_weights_dtype, dtype) != JJO_OK)
+        return -1;
+    return swiglu_backward_bytes(dtype, hidden_size, intermediate_size, n_routes, num_experts,
+                                 planes_of(dtype, grad_weights_dtype, true, true), kAll);
 }
 
 int moe_rows_gate_up_swiglu_backward_device(void *stream, const void *grad_mid, const void *gate_up,
@@ -380,14 +422,15 @@ int moe_rows_gate_up_swiglu_backward_device(void *stream, const void *grad_mid, 
     JJO_TRY(check_ptr(who, "grad_x_sorted", grad_x_sorted, es, true));
     JJO_TRY(check_ptr(who, "grad_w_gate", grad_w_gate, ges, true));
     JJO_TRY(check_ptr(who, "grad_w_up", grad_w_up, ges, true));
+    const int planes = planes_of(dtype, grad_weights_dtype, true, grad_w_gate != nullptr);
     JJO_TRY(check_workspace(who, workspace, workspace_bytes,
-                            moe_rows_gate_up_swiglu_backward_workspace_bytes(dtype, H, I, R, E)));
+                            swiglu_backward_bytes(dtype, H, I, R, E, planes,
+                                                  {grad_x_sorted != nullptr, grad_w_gate != nullptr, false})));
     JJO_TRY(require_device());
     hipStream_t s = (hipStream_t)stream;
     uint8_t *const gz = (uint8_t *)workspace;
     const int64_t plane = gz_plane_bytes(dtype, 2LL * R * I);
-    const int planes = grad_weights_dtype != dtype && grad_w_gate != nullptr ? gz_planes(dtype) : 1;
-    float *const part = (float *)(gz + gz_planes(dtype) * plane);
+    float *const part = (float *)(gz + planes * plane);
     hipError_t e = launch_rows_swiglu_backward(grad_mid, gate_up, gz, planes, plane / es, dtype, expert_offsets, E, I, R, s);
     if (e != hipSuccess) return launched(e, "moe_rows_gate_up_swiglu_backward activation");
     if (grad_x_sorted != nullptr) {

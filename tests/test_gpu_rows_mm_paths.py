@@ -320,3 +320,57 @@ def test_odd_places(dev, name):
         R.check(gx, *R.mm(g, w.t()), "grad_x")
         R.check(gw[1:-1].view(N, K), *R.mm(g.t(), x.t()), "grad_w")
         assert (wide[:, :1] == 7.0).all() and (wide[:, 1 + K:] == 7.0).all() and gw[0] == 7.0 and gw[-1] == 7.0
+
+
+@pytest.mark.parametrize("K,N,T", [(136, 264, 70), (4096, 520, 64), (515, 333, 40)])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("name", list(R.DTYPES))
+def test_workspaces_of_a_call_are_enough(dev, name, wide, K, N, T):
+    """Gradients with the workspace of just their activation and type: the same bits as with the largest, and nothing
+    behind it is written."""
+    d, gd = R.DTYPES[name], torch.float32 if wide else R.DTYPES[name]
+    code, g_code = CODES[name], CODES["f32"] if wide else CODES[name]
+    counts = [T // 2, 0, T - T // 2]
+    offsets, E = R.offsets_of(counts), 3
+    x, g, pre = R.randn(1, T, K, dtype=d), R.randn(2, T, N, dtype=d), R.randn(3, T, N, dtype=d)
+    w, both = R.randn(4, E, N, K, dtype=d), R.randn(5, T, 2 * N, dtype=d)
+
+    def linear(act, ws):
+        out = torch.empty(T, K, dtype=d, device="cuda"), torch.empty(N, K, dtype=gd, device="cuda"), torch.empty(N, dtype=gd, device="cuda")
+        capi.linear_rows_backward(g, x, w[0], *out, K, N, T, activation=act, pre=pre, ws=ws)
+        return out
+
+    def experts(ws):
+        out = torch.empty(T, K, dtype=d, device="cuda"), *(torch.empty(E, N, K, dtype=gd, device="cuda") for _ in range(2))
+        capi.moe_gate_up_swiglu_rows_backward(g, both, x, w, w, offsets, E, *out, K, N, T, ws=ws)
+        return out
+    most = R.workspace(capi.linear_rows_backward_workspace_bytes(code, K, N, T))
+    cases = [(lambda ws, act=act: linear(act, ws), most,
+              capi.linear_rows_backward_workspace_bytes(code, K, N, T, activation=act, grad_dtype=g_code))
+             for act in (capi.ACT_NONE, capi.ACT_GELU)]
+    most = R.workspace(capi.moe_gate_up_swiglu_rows_backward_workspace_bytes(code, K, N, T, E))
+    cases.append((experts, most, capi.moe_gate_up_swiglu_rows_backward_workspace_bytes(code, K, N, T, E, grad_dtype=g_code)))
+    for call, largest, need in cases:
+        guarded = torch.full((need + 1024,), 0x5a, dtype=torch.uint8, device="cuda")
+        for a, b in zip(call(largest), call(guarded[:need])):
+            assert torch.equal(a, b)
+        assert (guarded[need:] == 0x5a).all()
+
+
+@pytest.mark.parametrize("name", list(R.DTYPES))
+def test_rows_far_apart(dev, name):
+    """Strides of 8 MiB and more, at which a tile's offsets leave 32 bits."""
+    d, K, N, T = R.DTYPES[name], 72, 40, 5
+    stride = (1 << 23) // d.itemsize
+    for step in (stride - 8, stride, stride + 8, stride + 3):
+        far = torch.zeros(T, step, dtype=d, device="cuda")
+        x, w = far[:, :K], R.randn(2, N, K, dtype=d)
+        x.copy_(R.randn(1, T, K, dtype=d))
+        y, g = torch.empty(T, N, dtype=d, device="cuda"), R.randn(3, T, N, dtype=d)
+        ws = R.workspace(capi.linear_rows_workspace_bytes(CODES[name], K, N, T))
+        capi.linear_rows(x, w, y, K, N, T, ws=ws)
+        R.check(y, *R.mm(x, w), "y")
+        gw = torch.empty(N, K, dtype=torch.float32, device="cuda")
+        ws = R.workspace(capi.linear_rows_backward_workspace_bytes(CODES[name], K, N, T))
+        capi.linear_rows_backward(g, x, None, None, gw, None, K, N, T, ws=ws)
+        R.check(gw, *R.mm(g.t(), x.t()), "grad_w")
