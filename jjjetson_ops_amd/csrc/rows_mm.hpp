@@ -38,7 +38,7 @@ struct RowsMm {
     const int32_t *offsets;  // [n_experts + 1], or nullptr
     int n_experts, M;        // M: sorted rows
     int64_t expert_stride;   // elements of a matrix (of an expert's part of y: weight)
-    bool wide;               // y is fp32
+    bool wide;               // y is fp32 (weight)
     int slices;              // of the sums, each in its own part[Q][P] (SwiGLU: [Q][2P])
     float *part;
     RowsEpilogue epi;

@@ -1,9 +1,9 @@
 // Products of float matrices with few rows on the right (a decoded token, a small batch, experts with a few
 // rows): the weights go from memory straight to the matrix instruction's operand registers.
 //
-// A wave holds RT x 16 weight rows of a workgroup's and every kWaves-th run of kSteps steps along K; a lane
-// loads 16 bytes of a row a step (four lanes 64 contiguous bytes of each of 16 rows, the next step the other
-// half of the line), and the same of up to 16 * TT rows of x, which the caches hold.  The loads of the next
+// A workgroup has 16 weight rows (SwiGLU: of gate and of up), a wave of it every kWaves-th run of kSteps steps along
+// K; a lane loads 16 bytes of a row a step (four lanes 64 contiguous bytes of each of 16 rows, the next step the other
+// half of the line), and the same of up to 16 rows of x, which the caches hold.  The loads of the next
 // run are in flight while this one is multiplied.  The waves' sums are added through LDS in their
 // order and leave through the epilogue eight columns a thread.  Any K and alignment: a lane's piece that
 // reaches behind the row's end is taken element by element.
@@ -16,52 +16,43 @@
 namespace jjo {
 namespace {
 
-template <class E, bool SWIGLU, int RT, int TT>
+template <class E, bool SWIGLU>
 __global__ __launch_bounds__(512) void rows_direct_kernel(RowsMm p) {
     typedef typename E::type T;
+    constexpr int kMats = SWIGLU ? 2 : 1;  // gate and up
     constexpr int kPiece = 16 / sizeof(T), kStep = 4 * kPiece, kSteps = 4;  // a step: 64 bytes of a row
-    constexpr int kCols = SWIGLU ? 8 * RT : 16 * RT;                        // of the output
-    static_assert(!SWIGLU || RT % 2 == 0, "gate's tiles, then up's");
-    constexpr int kPitch = 16 * RT + 4;
-    extern __shared__ __align__(16) float sums[];  // [waves][16 * TT][kPitch]
+    constexpr int kPitch = 16 * kMats + 4;
+    extern __shared__ __align__(16) float sums[];  // [waves][16][kPitch]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int waves = blockDim.x >> 6, r16 = lane & 15, q4 = lane >> 4;
 
     // Row tiles fastest: the workgroups that read the same weights follow each other on one XCD.
     const int total = gridDim.x, per = total / 8, rest = total % 8, xcd = blockIdx.x % 8;
     const int tile = xcd * per + min(xcd, rest) + (int)(blockIdx.x / 8), tile_q = tile % p.tiles_q;
-    int expert = 0, q0 = tile_q * 16 * TT, end = p.Q;
-    if (p.offsets != nullptr && !mx_expert_tile(p.offsets, p.n_experts, p.M, 16 * TT, tile_q, expert, q0, end)) return;
-    const int p0 = tile / p.tiles_q * kCols;
+    int expert = 0, q0 = tile_q * 16, end = p.Q;
+    if (p.offsets != nullptr && !mx_expert_tile(p.offsets, p.n_experts, p.M, 16, tile_q, expert, q0, end)) return;
+    const int p0 = tile / p.tiles_q * 16;
 
-    const T *wrow[RT], *xrow[TT];
+    const T *wrow[kMats];
+    f32x4v acc[kMats];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const bool up = SWIGLU && rt >= RT / 2;
-        const int row = min(p0 + 16 * (up ? rt - RT / 2 : rt) + r16, p.P - 1);
-        wrow[rt] = (const T *)(up ? p.p2 : p.p) + expert * p.expert_stride + row * p.ldp + q4 * kPiece;
+    for (int m = 0; m < kMats; ++m) {
+        wrow[m] = (const T *)(m == 0 ? p.p : p.p2) + expert * p.expert_stride + min(p0 + r16, p.P - 1) * p.ldp + q4 * kPiece;
+        acc[m] = f32x4v{0.f, 0.f, 0.f, 0.f};
     }
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) xrow[tt] = (const T *)p.q + min(q0 + 16 * tt + r16, end - 1) * p.ldq + q4 * kPiece;
-
-    f32x4v acc[RT][TT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    const T *const xrow = (const T *)p.q + min(q0 + r16, end - 1) * p.ldq + q4 * kPiece;
 
     // Run r of a wave: steps kSteps * (wave + waves * r) on.  Whole steps only, then the rest of the row.
     const int whole = p.K / kStep, runs = whole / kSteps;
-    u32x4v w[2][kSteps][RT], x[2][kSteps][TT];
+    u32x4v w[2][kSteps][kMats], x[2][kSteps];
     auto load = [&](int run, auto buffer) {
         constexpr int B = decltype(buffer)::value;
         const int64_t k = (int64_t)run * kSteps * kStep;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) w[B][s][rt] = load_any<u32x4v>(wrow[rt] + k + s * kStep);
-#pragma unroll
-            for (int tt = 0; tt < TT; ++tt) x[B][s][tt] = load_any<u32x4v>(xrow[tt] + k + s * kStep);
+            for (int m = 0; m < kMats; ++m) w[B][s][m] = load_any<u32x4v>(wrow[m] + k + s * kStep);
+            x[B][s] = load_any<u32x4v>(xrow + k + s * kStep);
         }
     };
     auto multiply = [&](auto buffer) {
@@ -69,9 +60,7 @@ __global__ __launch_bounds__(512) void rows_direct_kernel(RowsMm p) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = rows_mfma<T>(w[B][s][rt], x[B][s][tt], acc[rt][tt]);
+            for (int m = 0; m < kMats; ++m) acc[m] = rows_mfma<T>(w[B][s][m], x[B][s], acc[m]);
     };
     constexpr std::integral_constant<int, 0> kB0{};
     constexpr std::integral_constant<int, 1> kB1{};
@@ -101,32 +90,24 @@ __global__ __launch_bounds__(512) void rows_direct_kernel(RowsMm p) {
             }
             return v;
         };
-        u32x4v a[RT], b[TT];
+        const u32x4v b = piece(xrow);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) a[rt] = piece(wrow[rt]);
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) b[tt] = piece(xrow[tt]);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = rows_mfma<T>(a[rt], b[tt], acc[rt][tt]);
+        for (int m = 0; m < kMats; ++m) acc[m] = rows_mfma<T>(piece(wrow[m]), b, acc[m]);
     }
 
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
-            *reinterpret_cast<f32x4v *>(sums + (wave * 16 * TT + 16 * tt + r16) * kPitch + 16 * rt + 4 * q4) = acc[rt][tt];
+    for (int m = 0; m < kMats; ++m)
+        *reinterpret_cast<f32x4v *>(sums + (wave * 16 + r16) * kPitch + 16 * m + 4 * q4) = acc[m];
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * TT * (kCols / 8); i += blockDim.x) {
-        const int r = i / (kCols / 8), chunk = i % (kCols / 8), col = p0 + 8 * chunk, n = min(8, p.P - col);
+    for (int i = threadIdx.x; i < 32; i += blockDim.x) {  // 16 rows of two chunks of eight columns
+        const int r = i / 2, chunk = i % 2, col = p0 + 8 * chunk, n = min(8, p.P - col);
         if (q0 + r >= end || n <= 0) continue;
         float v[8], up[8];
         auto take = [&](float *to, int at) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) to[j] = 0.0f;
             for (int k = 0; k < waves; ++k) {
-                const f32x4v *const from = reinterpret_cast<const f32x4v *>(sums + (k * 16 * TT + r) * kPitch + at);
+                const f32x4v *const from = reinterpret_cast<const f32x4v *>(sums + (k * 16 + r) * kPitch + at);
                 const f32x4v a = from[0], b = from[1];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) to[j] += a[j], to[4 + j] += b[j];
@@ -134,23 +115,22 @@ __global__ __launch_bounds__(512) void rows_direct_kernel(RowsMm p) {
         };
         take(v, 8 * chunk);
         if constexpr (SWIGLU) {
-            take(up, 8 * RT + 8 * chunk);
+            take(up, 16 + 8 * chunk);
             rows_finish_swiglu<T>(p.epi, v, up, q0 + r, col, n, p.P, p.y);
         } else {
-            rows_finish<T>(p.epi, v, q0 + r, col, n, p.P, p.y, p.ldy, p.wide);
+            rows_finish<T>(p.epi, v, q0 + r, col, n, p.P, p.y, p.ldy, false);
         }
     }
 }
 
-template <class E, bool SWIGLU, int RT, int TT>
+template <class E, bool SWIGLU>
 hipError_t run_rows_direct(RowsMm p, int waves, hipStream_t stream) {
-    constexpr int kCols = SWIGLU ? 8 * RT : 16 * RT;
-    const int tiles_p = (p.P + kCols - 1) / kCols;
-    p.tiles_q = (p.Q + 16 * TT - 1) / (16 * TT) + (p.offsets != nullptr ? std::min(p.n_experts, p.M) : 0);
+    const int tiles_p = (p.P + 15) / 16;
+    p.tiles_q = (p.Q + 15) / 16 + (p.offsets != nullptr ? std::min(p.n_experts, p.M) : 0);
     const int64_t wgs = (int64_t)tiles_p * p.tiles_q;
     if (wgs * waves * 64 >= 1LL << 32) return hipErrorInvalidConfiguration;
-    const auto kernel = rows_direct_kernel<E, SWIGLU, RT, TT>;
-    const size_t lds = (size_t)waves * 16 * TT * (16 * RT + 4) * sizeof(float);
+    const auto kernel = rows_direct_kernel<E, SWIGLU>;
+    const size_t lds = (size_t)waves * 16 * (SWIGLU ? 36 : 20) * sizeof(float);
     const hipError_t e = ensure_dynamic_lds((const void *)kernel, lds);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(waves * 64), lds, stream, p);

@@ -8,8 +8,8 @@ namespace jjo {
 template <class E>
 hipError_t rows_mm_run(RowsMode mode, const RowsMm &p, const RowsChoice &c, hipStream_t stream) {
     if (c.tile == kRowsDirect) {
-        if (mode == kRowsForward) return run_rows_direct<E, false, 1, 1>(p, c.waves, stream);
-        if (mode == kRowsSwiglu) return run_rows_direct<E, true, 2, 1>(p, c.waves, stream);
+        if (mode == kRowsForward) return run_rows_direct<E, false>(p, c.waves, stream);
+        if (mode == kRowsSwiglu) return run_rows_direct<E, true>(p, c.waves, stream);
         return hipErrorInvalidValue;
     }
     switch (mode) {

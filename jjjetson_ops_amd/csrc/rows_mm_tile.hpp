@@ -668,7 +668,7 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
     static_assert(kBeside || (TT % 2 == 0 && RT == 2 && MODE == kRowsSwiglu), "pairs of tiles");
     constexpr int kRows = kBeside ? 1 : 2, kPairs = kBeside ? kWaveP / 32 : 1;
     const int lane = threadIdx.x & 63, r16 = lane & 15, odd = (lane >> 4) & 1, upper = lane >> 5;
-    const bool parts = p.slices > 1, to32 = parts || p.wide;
+    const bool parts = p.slices > 1, wide = MODE == kRowsWeight && p.wide, to32 = parts || wide;
     // The output's (or the slice's sums') matrix, and its rows' length.
     const int64_t cols = MODE == kRowsSwiglu ? 2 * (int64_t)p.P : p.P, matrices = max(p.n_experts, 1);
     int64_t ld = p.ldy;
@@ -680,7 +680,7 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
         y = (uint8_t *)(p.part + (c.slice * all + mine) * cols);
     } else {
         y = (uint8_t *)(MODE == kRowsWeight && c.half != 0 ? p.y2 : p.y);
-        if constexpr (MODE == kRowsWeight) y += c.expert * p.expert_stride * (p.wide ? 4 : sizeof(T));
+        if constexpr (MODE == kRowsWeight) y += c.expert * p.expert_stride * (wide ? 4 : sizeof(T));
     }
     // Row and column of the lane's eight of pair `pair` in row tt of tiles.
     auto row_of = [&](int tt) { return 16 * (TT * wq + tt + (kBeside ? 0 : odd)) + r16; };
@@ -852,7 +852,7 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
                 } else if constexpr (MODE == kRowsSwiglu) {
                     rows_finish_swiglu<T>(e, v, up, row, col, n, p.P, y);
                 } else {
-                    rows_finish<T>(e, v, row, col, n, p.P, y, ld, p.wide);
+                    rows_finish<T>(e, v, row, col, n, p.P, y, ld, wide);
                 }
             }
         }

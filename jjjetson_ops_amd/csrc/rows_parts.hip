@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsMm p, int chunks, in
     } else {
         void *y = p.y;
         if (MODE == kRowsWeight && p.halves == 2 && row >= rows / 2) y = p.y2, row -= rows / 2;
-        rows_finish<T>(p.epi, v, row, col, n, p.P, y, p.ldy, p.wide);
+        rows_finish<T>(p.epi, v, row, col, n, p.P, y, p.ldy, MODE == kRowsWeight && p.wide);
     }
 }
 
