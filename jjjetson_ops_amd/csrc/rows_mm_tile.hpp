@@ -656,7 +656,36 @@ struct RowsSource {
 // cost a tile of 256 x 256 some 8 us.  So plain outputs (whole groups of eight columns) have a path of
 // their own.  kRowsFull has one for each activation, for whole groups too; kRowsAny takes one row of tiles at a time, in a loop that moves the next one's sums into the same
 // registers (which costs registers that the large tiles do not have).
+// Of weights' gradients kRowsPlain has rows at multiples of 64 bytes, kRowsFull others.
 enum RowsOutput { kRowsPlain, kRowsFull, kRowsAny };
+
+// 16 bytes of a row, values col.. of P, through the caches.  Of 16 bits at an odd place whole words, from the second
+// value on: `next` holds the first of the lane with the columns behind, which lanes 56 and up have not.
+template <class Out>
+__device__ __forceinline__ void rows_store_line(Out *to, u32x4v v, uint32_t next, int col, int P) {
+    constexpr int kN = 16 / sizeof(Out);
+    const int lane = threadIdx.x & 63;
+    const MxVec<Out, kN> e = __builtin_bit_cast(MxVec<Out, kN>, v);
+    if (col + kN > P) {
+#pragma unroll
+        for (int i = 0; i < kN - 1; ++i)
+            if (col + i < P) to[i] = e.v[i];
+    } else if (sizeof(Out) == 4 || (uintptr_t)to % 4 == 0) {
+        store_any(to, v);
+    } else {
+        typedef uint32_t Words3 __attribute__((ext_vector_type(3), aligned(4)));
+        typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(4)));
+        const uint32_t w[4] = {v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16,
+                               v[3] >> 16 | next << 16};
+        if (lane < 56 && col + kN < P) {
+            *(Words4 *)(to + 1) = Words4{w[0], w[1], w[2], w[3]};
+        } else {
+            *(Words3 *)(to + 1) = Words3{w[0], w[1], w[2]};
+            to[kN - 1] = e.v[kN - 1];
+        }
+        if (lane < 8) to[0] = e.v[0];
+    }
+}
 
 template <class T, RowsMode MODE, RowsOutput KIND, class Tile>
 __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c, f32x4v (&acc)[Tile::RT][Tile::TT], int wp,
@@ -742,65 +771,50 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
     // whole words but for their ends, each lane taking the next one's first value (odd sizes: 250 us, 302 otherwise).
     if constexpr (MODE == kRowsWeight && RT == 4) {
         const bool high = (lane & 8) != 0;
-        const bool past = ((uintptr_t)y | (uint64_t)ld * (to32 ? 4 : sizeof(T))) % 64 == 0;
-        auto lines = [&](u32x4v a, u32x4v b, int tt, int col, auto out) {
-            using Out = decltype(out);
-            constexpr int kN = 16 / sizeof(Out);
+        auto all = [&](auto past_tag) {
+            constexpr bool PAST = decltype(past_tag)::value;
+            auto lines = [&](u32x4v a, u32x4v b, int tt, int col, auto out) {
+                using Out = decltype(out);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t x = __builtin_amdgcn_update_dpp(0, high ? a[i] : b[i], 0x128, 0xf, 0xf, false);  // row_ror:8
-                a[i] = high ? x : a[i], b[i] = high ? b[i] : x;
-            }
-            const int in_tile = 16 * (TT * wq + tt) + (r16 & 7);
-            Out *const to = (Out *)y + (c.q0 + in_tile) * ld + col;
-            auto store = [&](Out *at, u32x4v v, uint32_t next) {
-                if (past) return rows_store_past(at, v);
-                const MxVec<Out, kN> e = __builtin_bit_cast(MxVec<Out, kN>, v);
-                if (col + kN > p.P) {
-#pragma unroll
-                    for (int i = 0; i < kN - 1; ++i)
-                        if (col + i < p.P) at[i] = e.v[i];
-                } else if (sizeof(Out) == 4 || (uintptr_t)at % 4 == 0) {
-                    store_any(at, v);
-                } else {  // whole words: from the second value on, with the next lane's first
-                    const bool whole = lane < 56 && col + kN < p.P;
-                    const uint32_t w[4] = {v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16,
-                                           v[3] >> 16 | next << 16};
-                    typedef uint32_t Words3 __attribute__((ext_vector_type(3), aligned(4)));
-                    typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(4)));
-                    if (whole) {
-                        *(Words4 *)(at + 1) = Words4{w[0], w[1], w[2], w[3]};
-                    } else {
-                        *(Words3 *)(at + 1) = Words3{w[0], w[1], w[2]};
-                        at[kN - 1] = e.v[kN - 1];
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t x = __builtin_amdgcn_update_dpp(0, high ? a[i] : b[i], 0x128, 0xf, 0xf, false);  // row_ror:8
+                    a[i] = high ? x : a[i], b[i] = high ? b[i] : x;
+                }
+                const int in_tile = 16 * (TT * wq + tt) + (r16 & 7);
+                Out *const to = (Out *)y + (c.q0 + in_tile) * ld + col;
+                if constexpr (PAST) {
+                    if (col >= p.P) return;
+                    if (in_tile < c.rows_q) rows_store_past(to, a);
+                    if (in_tile + 8 < c.rows_q) rows_store_past(to + 8 * ld, b);
+                } else {
+                    uint32_t next_a = 0, next_b = 0;
+                    if constexpr (sizeof(Out) == 2) {  // of the columns' next eight: lanes + 32, then + 16, then + 8
+                        const int next = 4 * (upper == 0 ? lane ^ 32 : odd == 0 ? lane ^ 48 : lane ^ 56);
+                        next_a = __builtin_amdgcn_ds_bpermute(next, a[0]), next_b = __builtin_amdgcn_ds_bpermute(next, b[0]);
                     }
-                    if (lane < 8) at[0] = e.v[0];
+                    if (in_tile < c.rows_q) rows_store_line(to, a, next_a, col, p.P);
+                    if (in_tile + 8 < c.rows_q) rows_store_line(to + 8 * ld, b, next_b, col, p.P);
                 }
             };
-            uint32_t next_a = 0, next_b = 0;
-            if (sizeof(Out) == 2 && !past) {  // of the columns' next eight: lanes + 32, then + 16, then + 8
-                const int next = 4 * (upper == 0 ? lane ^ 32 : odd == 0 ? lane ^ 48 : lane ^ 56);
-                next_a = __builtin_amdgcn_ds_bpermute(next, a[0]), next_b = __builtin_amdgcn_ds_bpermute(next, b[0]);
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) {
+                if (sizeof(T) == 4 || to32) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt += 2)
+                        lines(__builtin_bit_cast(u32x4v, acc[rt][tt]), __builtin_bit_cast(u32x4v, acc[rt + 1][tt]), tt,
+                              c.p0 + kWaveP * wp + 16 * (rt + high) + 4 * (lane >> 4), 0.0f);
+                } else if constexpr (sizeof(T) == 2) {
+                    float v[8], w[8];
+                    take(tt, 0, v, v);
+                    take(tt, 1, w, w);
+                    lines(rows_pack8<T>(v), rows_pack8<T>(w), tt, col_of(high), (T)0.0f);
+                }
             }
-            if (col >= p.P) return;
-            if (in_tile < c.rows_q) store(to, a, next_a);
-            if (in_tile + 8 < c.rows_q) store(to + 8 * ld, b, next_b);
         };
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-            if (sizeof(T) == 4 || to32) {
-#pragma unroll
-                for (int rt = 0; rt < RT; rt += 2)
-                    lines(__builtin_bit_cast(u32x4v, acc[rt][tt]), __builtin_bit_cast(u32x4v, acc[rt + 1][tt]), tt,
-                          c.p0 + kWaveP * wp + 16 * (rt + high) + 4 * (lane >> 4), 0.0f);
-            } else if constexpr (sizeof(T) == 2) {
-                float v[8], w[8];
-                take(tt, 0, v, v);
-                take(tt, 1, w, w);
-                lines(rows_pack8<T>(v), rows_pack8<T>(w), tt, col_of(high), (T)0.0f);
-            }
-        }
-        return;
+        if (KIND == kRowsPlain) return all(std::true_type{});
+        if (KIND == kRowsFull) return all(std::false_type{});
+        if (((uintptr_t)y | (uint64_t)ld * (to32 ? 4 : sizeof(T))) % 64 == 0) return all(std::true_type{});
+        return all(std::false_type{});
     }
     if (KIND != kRowsAny || (p.P % 8 == 0 && (parts || (e.bias == nullptr && e.residual == nullptr && e.pre == nullptr && e.act == JJO_ACT_NONE)))) {
         auto all = [&](auto wide_tag) {
@@ -1149,6 +1163,12 @@ hipError_t run_rows(RowsMm p, hipStream_t stream) {
         if constexpr (MODE == kRowsForward || MODE == kRowsSwiglu)
             if (p.slices == 1 && (e.bias != nullptr || e.residual != nullptr || e.pre != nullptr || e.act != JJO_ACT_NONE))
                 return go(rows_stream_kernel<E, MODE, kRowsFull, Tile>, wgs);
+        if constexpr (MODE == kRowsWeight) {
+            const int es = p.wide ? 4 : (int)sizeof(typename E::type);
+            const bool lines = p.slices > 1 ? (uintptr_t)p.part % 64 == 0 && p.P % 16 == 0
+                                            : ((uintptr_t)p.y | (uintptr_t)p.y2 | (uintptr_t)(p.ldy * es)) % 64 == 0;
+            if (!lines) return go(rows_stream_kernel<E, MODE, kRowsFull, Tile>, wgs);
+        }
         return go(rows_stream_kernel<E, MODE, kRowsPlain, Tile>, wgs);
     } else
         return go(rows_mm_kernel<E, MODE, Tile, WAY>, (int)blocks);
