@@ -710,7 +710,7 @@ int moe_rows_gate_up_swiglu_backward_device(void *stream, const void *grad_mid, 
  * [rows][sums] . p [sums][cols] (p2 not NULL: q [rows][2 sums], its second half times p2 is added); 3: y
  * [rows][cols] = q [sums][rows]^T . p [sums][cols] (y2 not NULL: q [sums][2 rows], the second half's
  * rows go to y2).  expert_offsets NULL, or of sorted rows (forms 0 to 2) or of the sums (3).  kernel: LDS tiles
- * of 64 x 64 (0), 128 x 128 (1), 256 columns x 160 rows (2; not form 3) or 256 x 256 (3; both 16 bits only and
+ * of 64 x 64 (0), 128 x 128 (1), 256 columns x 160 rows (2; forms 0 and 2) or 256 x 256 (3; both 16 bits only and
  * cols % 8 == 0: else tile 1 runs), 64 + w the direct kernel on w <= 8 waves (forms 0 and 1).  Operands whose
  * rows are not 16-byte aligned take tile 0 as it is and tile 1 for the others.  slices of the sums, each 4 bytes an
  * output of the workspace where more than one.

@@ -15,9 +15,9 @@ int64_t rows_part_bytes(RowsMode mode, const RowsMm &p) {
 // (the device's own number would change the workspace): two of the small tiles a CU, one of the large; a round takes
 // `fixed` and one[] or two[] for each stage where a CU has one workgroup or two.  Slices of the sums divide the
 // stages and cost a second launch and 8 bytes an output at 4 TB/s.  Measured (us, bf16; estimates in brackets): 2047
-// x 14336 over 4096 on tiles of 256 / 160 / 128 rows 198 / 225 / 228 (191 / 232 / 267); 2048 x 4096 over 4096
-// 90 / 76 / 64 (96 / 78 / 67); 64 x 4096 over 4096 on tiles of 64 x 64 in 1, 2, 4 slices 22.9 / 17.7 / 13.9
-// (25 / 19 / 14).
+// x 14336 over 4096 on tiles of 256 / 160 / 128 rows 198 / 225 / 228 (191 / 232 / 245); 2048 x 4096 over 4096
+// 90 / 76 / 64 (96 / 77 / 67); 64 x 4096 over 4096 on tiles of 64 x 64 in 1, 2, 4 slices 22.9 / 17.7 / 13.9
+// (24.6 / 17.4 / 12.9).
 RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int halves, int n_experts) {
     constexpr int64_t kCus = 256;
     const bool fp32 = dtype == JJO_DTYPE_F32, weight = mode == kRowsWeight, input = mode == kRowsInput;
@@ -31,19 +31,28 @@ RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int hal
     const int M = weight ? K : Q;
     const double experts = n_experts == 0 ? 1 : std::min(n_experts, M), mean = M / experts;
 
-    // Few rows: a matrix is best read by the direct kernel up to 16 rows, up to 12 where tiles of 64 columns
-    // occupy every other CU (11008 x 4096: 1 / 8 / 16 rows 18.1 / 21.2 / 25.0 us against 23.6 / 23.9 / 23.9 on tiles;
-    // 4096 x 4096 16 rows 10.6 against 12.9 in four slices).  Of experts only where the tiles leave CUs without two
-    // workgroups and rows are long (8 rows of 8 experts, 4096 x 14336: 100 against 122 us; 14336 x 4096: 108
-    // against 104; SwiGLU of 64 experts' 1408 x 2048: 19.5 against 16.5).
-    const int64_t tiles64 = (cols + 63) / 64;
+    // Few rows: a matrix is best read by the direct kernel up to 16 rows, of 16 bits up to 12 where tiles of 64 columns
+    // occupy every other CU (11008 x 4096, 1 / 8 / 16 rows: 18.1 / 21.2 / 25.0 us against 23.6 / 23.9 / 23.9 on tiles,
+    // fp32 35 / 40 / 47 against 62; 4096 x 4096, 16 rows: 10.6 against 12.9 in four slices).
     // Not on rows of 16 bits that are not aligned (4096 x 4095, 1 / 16 rows 17.4 / 28 us against 14.7 / 17.5 in four
     // slices; 11008 x 4095 42 / 75 against 29 / 39; fp32 15.3 / 20.4 against 30 / 31).
-    const bool few = n_experts == 0 ? Q <= (tiles64 < kCus / 2 ? 16 : 12)
-                                    : mean <= 4 && K >= 4096 && (int64_t)experts * tiles64 < 3 * kCus;
+    // Of experts fp32, whose matrix instructions are slow on rows that are not there, up to 8 rows (8 experts' 4096 x
+    // 2048 and 4096 x 4096, 1 row each: 54 and 99 against 75 and 146; 8 rows 65 and 119 against 75 and 145; 16 rows 78
+    // and 141 against 75 and 147).  16 bits up to 4 rows: where the tiles are fewer than the CUs (8 experts of 704 and 1408
+    // columns over 2048: 8.5 and 14.2 against 11.8 and 14.5; over 4096: 13 and 20 against 16 and 25; over 512 all
+    // within 3%), and, about even on average and ahead where few experts have rows, where sums are long and the tiles
+    // leave CUs without a third workgroup (4096 x 14336, 8, 4 and 1 experts of 8 active: 214, 153 and 62 against 219, 144
+    // and 54 to 87; 4096 x 4096: 97, 53 and 22 against 98, 54 and 21 to 28; over 2048 29 against 30, over 2560 32 and 32).
+    const int64_t tiles64 = (cols + 63) / 64;
+    const double in_all = experts * (double)tiles64;
+    const bool few = n_experts == 0 ? Q <= (fp32 || tiles64 < kCus / 2 ? 16 : 12)
+                     : fp32         ? mean <= 8
+                                    : mean <= 4 && (in_all < kCus || (K >= 4096 && in_all < 3 * kCus));
     if (few && (fp32 || !odd) && (mode == kRowsForward || mode == kRowsSwiglu)) {
+        // Eight waves, but two for short sums of many workgroups (8 experts' 4096 x 512, 2 / 4 / 8 waves: 10.4 / 11.3 /
+        // 15.8 us; x 2048 28.6 / 27.6 / 31.6; x 4096 59 / 54 / 51; one row of 11008 x 4096 19.0 / 18.8 / 18.1).
         const int64_t wgs = (int64_t)experts * ((cols + 15) / 16);
-        return {kRowsDirect, wgs >= 4 * kCus ? 2 : 8, 1};  // as above on 2, 4, 8 waves: 100, 111, 110; 1 row 19.0, 18.8, 18.1
+        return {kRowsDirect, K / (16 * piece) < 32 && wgs >= 4 * kCus ? 2 : 8, 1};
     }
 
     struct Cost {
@@ -52,8 +61,12 @@ RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int hal
     };
     constexpr Cost k16[] = {{64, 64, 2, 2.2f, 0.35f, 0.5f}, {128, 128, 2, 2.9f, 0.65f, 1.0f},
                             {256, 160, 1, 5.f, 1.13f, 1.13f}, {256, 256, 1, 6.f, 1.4f, 1.4f}};
-    // A stage of experts' rows, where few tiles share a matrix's rows and wait for memory.
-    constexpr float kExperts[] = {0.5f, 1.3f, 1.4f, 1.9f};
+    // A stage of experts' rows, where few tiles share a matrix's rows and wait for memory: the tile with the least
+    // estimate was within 4% of the best one's time on average, 30% at most (16 experts' 4096 x 4096, 64 rows: 153 us,
+    // 118 on tiles of 256), over 53 products of 8 to 128 experts with 25 to 1024 rows on average, 704 to 14336 columns
+    // and sums.  By the estimate's own rounds a stage took 0.42 to 0.67, 0.98 to 1.48 and 1.1 to 1.9.  Tiles of 160 rows
+    // were the best by 4% at most (4096 x 4096, 1024 rows: 291, 302 otherwise), and are left to one matrix.
+    constexpr float kExperts[] = {0.42f, 0.96f, 0.0f, 1.5f};
     constexpr Cost k32[] = {{64, 64, 2, 2.2f, 0.62f, 1.05f}, {128, 128, 2, 2.9f, 2.0f, 4.0f}};
     // The same of rows that are not aligned.  fp32 by words, 1.01 to 1.2 times the above.  16 bits through registers, of
     // forward, input and weight (4095 x 4095, aligned 4096 x 4096 in brackets: 256 rows 26.5 (23.5), 2047 rows 99 (63);
@@ -70,7 +83,7 @@ RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int hal
     // The large tiles write whole groups of eight columns.
     const int kinds = fp32 || odd || P % 8 != 0 ? 2 : (int)kRowsTileKinds;
     for (int tile = copied ? kRowsTile128 : kRowsTile64; tile < kinds; ++tile) {
-        if (weight && tile == kRowsTile160) continue;
+        if ((weight || n_experts > 0) && tile == kRowsTile160) continue;
         Cost c = costs[tile];
         if (n_experts > 0 && !weight && !fp32)
             c.two = odd ? kExpertsOdd[tile] : kExperts[tile], c.one = std::max(c.one, c.two / c.a_cu);

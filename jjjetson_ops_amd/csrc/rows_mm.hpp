@@ -195,7 +195,7 @@ __device__ __forceinline__ void rows_finish_swiglu(const RowsEpilogue &e, float 
 }
 
 // ---- launchers (asynchronous; arguments validated by the entries)
-// The kernel of a product: LDS tiles of 64 x 64, 128 x 128, 256 columns x 160 rows (not weight) or 256 x 256
+// The kernel of a product: LDS tiles of 64 x 64, 128 x 128, 256 columns x 160 rows (forward and input) or 256 x 256
 // (the last two 16 bits only), or the direct kernel with `waves` that cut the sums between them (forward and
 // SwiGLU); and the slices of the sums that join their fp32 outputs in a second launch.
 enum RowsTileKind { kRowsDirect = -1, kRowsTile64, kRowsTile128, kRowsTile160, kRowsTile256, kRowsTileKinds };

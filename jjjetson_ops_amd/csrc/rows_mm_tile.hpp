@@ -1201,7 +1201,7 @@ hipError_t rows_by_tile(const RowsMm &p, int tile, hipStream_t stream) {
     if constexpr (sizeof(typename E::type) == 2) {
         // The large tiles write whole groups of eight columns.
         if (tile == kRowsTile256 && p.P % 8 == 0) return run_rows<E, MODE, RowsTile<4, 8, 4, 2>, kRowsDma>(p, stream);
-        if constexpr (MODE != kRowsWeight)
+        if constexpr (MODE == kRowsForward || MODE == kRowsInput)
             if (tile == kRowsTile160 && p.P % 8 == 0) return run_rows<E, MODE, RowsTile<4, 5, 4, 2, 3>, kRowsDma>(p, stream);
     }
     return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, kRowsDma>(p, stream);

@@ -11,7 +11,7 @@ WEIGHTS = [(("bf16", 4104, 2056, 333), 256, 1), (("f16", 4104, 2056, 333), 256, 
            (("bf16", 4104, 4104, 201), 128, 1), (("f16", 4104, 4104, 201), 128, 1), (("bf16", 264, 520, 2100), 64, 0),
            (("f16", 264, 520, 2100), 64, 0)]
 # (dtype, hidden, intermediate, rows of each expert): the forward pass, and its weights' gradients
-SWIGLU_FORWARD = [(("bf16", 2056, 2056, (300, 1, 0, 899)), 160, 1),
+SWIGLU_FORWARD = [(("bf16", 2056, 2056, (300, 1, 0, 899)), 128, 1),
                   (("f16", 2056, 4104, (600, 500, 130, 1, 0, 1300, 900, 1069)), 256, 1),
                   (("bf16", 136, 2056, (300, 1, 0, 899)), 128, 1)]
 SWIGLU_WEIGHTS = [(("bf16", 2056, 2056, (300, 1, 0, 899)), 256, 1), (("f16", 2056, 2056, (300, 1, 0, 899)), 256, 1),

@@ -81,3 +81,18 @@ def test_rows_without_alignment_get_kernels_that_run(choose, name):
     # less than a piece: tiles of 128, which these run on
     if name != "f32":
         assert choose(P.FORWARD, name, 4096, 2047, 7)[0] == 128 and choose(P.WEIGHT, name, 4096, 5, 2047)[0] == 128
+
+
+def test_few_rows_of_experts(choose):
+    """fp32 on the direct kernel at any size (a tile's products would cost what 64 rows do); 16 bits where the tiles are
+    fewer than the CUs."""
+    for cols, sums, experts in ((4096, 512, 8), (4096, 2048, 8), (1408, 2048, 64), (704, 4096, 16)):
+        for rows in (1, 8, 32, 8 * experts):
+            if rows <= 8 * min(experts, rows):
+                assert choose(P.FORWARD, "f32", cols, rows, sums, experts=experts)[0] == 0, (cols, sums, rows)
+                assert choose(P.SWIGLU, "f32", cols, rows, sums, experts=experts)[0] == 0, (cols, sums, rows)
+    for name in ("f16", "bf16"):
+        assert choose(P.FORWARD, name, 1408, 8, 2048, experts=64)[0] == 0
+        assert choose(P.FORWARD, name, 4096, 8, 2048, experts=8)[0] == 64
+        assert choose(P.FORWARD, name, 4096, 8, 14336, experts=8)[0] == 0
+        assert choose(P.SWIGLU, name, 1408, 8, 2048, experts=64)[0] == 64
