@@ -17,7 +17,8 @@ int64_t rows_part_bytes(RowsMode mode, const RowsMm &p) {
 // stages and cost a second launch and 8 bytes an output at 4 TB/s.  Measured (us, bf16; estimates in brackets): 2047
 // x 14336 over 4096 on tiles of 256 / 160 / 128 rows 198 / 225 / 228 (191 / 232 / 245); 2048 x 4096 over 4096
 // 90 / 76 / 64 (96 / 77 / 67); 64 x 4096 over 4096 on tiles of 64 x 64 in 1, 2, 4 slices 22.9 / 17.7 / 13.9
-// (24.6 / 17.4 / 12.9).
+// (24.6 / 17.4 / 12.9).  fp32: 77 x 10624 over 6264 on tiles of 128 in 3 and 6 slices 155 and 138 (143 and 131), on
+// tiles of 64 in 3 149 (151); 29 x 12440 over 6744 on tiles of 64 in 5 and 6 slices 113 and 124 (101 and 112).
 RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int halves, int n_experts) {
     constexpr int64_t kCus = 256;
     const bool fp32 = dtype == JJO_DTYPE_F32, weight = mode == kRowsWeight, input = mode == kRowsInput;
@@ -67,12 +68,12 @@ RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int hal
     // and sums.  By the estimate's own rounds a stage took 0.42 to 0.67, 0.98 to 1.48 and 1.1 to 1.9.  Tiles of 160 rows
     // were the best by 4% at most (4096 x 4096, 1024 rows: 291, 302 otherwise), and are left to one matrix.
     constexpr float kExperts[] = {0.42f, 0.96f, 0.0f, 1.5f};
-    constexpr Cost k32[] = {{64, 64, 2, 2.2f, 0.62f, 1.05f}, {128, 128, 2, 2.9f, 2.0f, 4.0f}};
+    constexpr Cost k32[] = {{64, 64, 2, 2.2f, 0.62f, 1.05f}, {128, 128, 2, 2.9f, 2.0f, 3.5f}};
     // The same of rows that are not aligned.  fp32 by words, 1.01 to 1.2 times the above.  16 bits through registers, of
     // forward, input and weight (4095 x 4095, aligned 4096 x 4096 in brackets: 256 rows 26.5 (23.5), 2047 rows 99 (63);
     // rows' gradients 35.5 (29) and 122 (71), weights' 31 (17) and 133 (58).  All rows at addresses of an odd number of
     // elements cost half as much again as those at multiples of four bytes: 512 rows 70, 44 and, staged but aligned, 37).
-    constexpr Cost k32Odd[] = {{64, 64, 2, 2.2f, 0.8f, 1.12f}, {128, 128, 2, 2.9f, 2.25f, 3.9f}};
+    constexpr Cost k32Odd[] = {{64, 64, 2, 2.2f, 0.8f, 1.12f}, {128, 128, 2, 2.9f, 2.25f, 3.7f}};
     constexpr Cost k16Odd[][2] = {{{64, 64, 2, 2.2f, 0.4f, 0.74f}, {128, 128, 2, 2.9f, 1.0f, 1.5f}},
                                   {{64, 64, 2, 2.2f, 0.62f, 0.8f}, {128, 128, 2, 2.9f, 1.33f, 1.87f}},
                                   {{64, 64, 2, 2.2f, 0.73f, 0.76f}, {128, 128, 2, 2.9f, 1.55f, 2.0f}}};
@@ -100,7 +101,7 @@ RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int hal
             tiles_q *= experts;
         }
         const double tiles = tiles_q * ((cols + c.p - 1) / c.p);
-        for (int slices : {1, 2, 3, 4, 6, 8}) {
+        for (int slices : {1, 2, 3, 4, 5, 6, 8}) {
             const double per = std::ceil(stages / slices), n = std::ceil(tiles * slices), slots = (double)kCus * c.a_cu;
             if (slices > 1 && (per < 8 || tile > kRowsTile128)) break;
             double us;
