@@ -46,8 +46,8 @@ int check_ptr(const char *who, const char *name, const void *p, int align, bool 
 
 int check_stride(const char *who, const char *name, int64_t stride, int cols, int rows) {
     if (rows > 1 && (stride < cols || stride > kMaxStride / rows))
-        return set_error(JJO_ERR_INVALID_ARG, "%s: %s=%lld must be at least %d, %d rows within 2^40 elements", who, name,
-                         (long long)stride, cols, rows);
+        return set_error(JJO_ERR_INVALID_ARG, "%s: %s=%lld must be at least %d, %d rows within 2^40 elements", who,
+                         name, (long long)stride, cols, rows);
     return JJO_OK;
 }
 
@@ -139,7 +139,8 @@ constexpr Wanted kAll{true, true, true};
 // Sums in slices of the products asked for, one after the other in the same place (n_experts 0: one matrix).
 int64_t part_bytes(int dtype, int K, int N, int rows, int n_experts, int halves, Wanted want) {
     const int64_t a = want.rows ? rows_part_bytes(kRowsInput, input(dtype, K, N, rows, n_experts, halves)) : 0;
-    const int64_t b = want.weights ? rows_part_bytes(kRowsWeight, weight(dtype, K, N, rows, n_experts, halves, false)) : 0;
+    const int64_t b =
+        want.weights ? rows_part_bytes(kRowsWeight, weight(dtype, K, N, rows, n_experts, halves, false)) : 0;
     return up256(std::max(a, b));
 }
 
@@ -255,8 +256,9 @@ int linear_rows_backward_device(void *stream, const void *grad_y, int64_t grad_y
     const void *gz = grad_y;
     int64_t gz_stride = stride_of(grad_y_stride, N, T);
     if (act || grad_bias != nullptr) {
-        const hipError_t e = launch_rows_act_backward(grad_y, gz_stride, pre, base + ws.gz, planes, ws.plane / es, dtype, activation,
-                                                      grad_bias, wide, (float *)(base + ws.columns), T, N, s);
+        const hipError_t e =
+            launch_rows_act_backward(grad_y, gz_stride, pre, base + ws.gz, planes, ws.plane / es, dtype, activation,
+                                     grad_bias, wide, (float *)(base + ws.columns), T, N, s);
         if (e != hipSuccess) return launched(e, "linear_rows_backward activation");
         if (act) gz = base + ws.gz, gz_stride = N;
     }
@@ -431,7 +433,8 @@ int moe_rows_gate_up_swiglu_backward_device(void *stream, const void *grad_mid, 
     uint8_t *const gz = (uint8_t *)workspace;
     const int64_t plane = gz_plane_bytes(dtype, 2LL * R * I);
     float *const part = (float *)(gz + planes * plane);
-    hipError_t e = launch_rows_swiglu_backward(grad_mid, gate_up, gz, planes, plane / es, dtype, expert_offsets, E, I, R, s);
+    hipError_t e =
+        launch_rows_swiglu_backward(grad_mid, gate_up, gz, planes, plane / es, dtype, expert_offsets, E, I, R, s);
     if (e != hipSuccess) return launched(e, "moe_rows_gate_up_swiglu_backward activation");
     if (grad_x_sorted != nullptr) {
         RowsMm m = input(dtype, H, I, R, E, 2);

@@ -39,11 +39,12 @@ RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int hal
     // slices; 11008 x 4095 42 / 75 against 29 / 39; fp32 15.3 / 20.4 against 30 / 31).
     // Of experts fp32, whose matrix instructions are slow on rows that are not there, up to 8 rows (8 experts' 4096 x
     // 2048 and 4096 x 4096, 1 row each: 54 and 99 against 75 and 146; 8 rows 65 and 119 against 75 and 145; 16 rows 78
-    // and 141 against 75 and 147).  16 bits up to 4 rows: where the tiles are fewer than the CUs (8 experts of 704 and 1408
-    // columns over 2048: 8.5 and 14.2 against 11.8 and 14.5; over 4096: 13 and 20 against 16 and 25; over 512 all
+    // and 141 against 75 and 147).  16 bits up to 4 rows: where the tiles are fewer than the CUs (8 experts of 704 and
+    // 1408 columns over 2048: 8.5 and 14.2 against 11.8 and 14.5; over 4096: 13 and 20 against 16 and 25; over 512 all
     // within 3%), and, about even on average and ahead where few experts have rows, where sums are long and the tiles
-    // leave CUs without a third workgroup (4096 x 14336, 8, 4 and 1 experts of 8 active: 214, 153 and 62 against 219, 144
-    // and 54 to 87; 4096 x 4096: 97, 53 and 22 against 98, 54 and 21 to 28; over 2048 29 against 30, over 2560 32 and 32).
+    // leave CUs without a third workgroup (4096 x 14336, 8, 4 and 1 experts of 8 active: 214, 153 and 62 against 219,
+    // 144 and 54 to 87; 4096 x 4096: 97, 53 and 22 against 98, 54 and 21 to 28; over 2048 29 against 30, over 2560 32
+    // and 32).
     const int64_t tiles64 = (cols + 63) / 64;
     const double in_all = experts * (double)tiles64;
     const bool few = n_experts == 0 ? Q <= (fp32 || tiles64 < kCus / 2 ? 16 : 12)
@@ -65,14 +66,15 @@ RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int hal
     // A stage of experts' rows, where few tiles share a matrix's rows and wait for memory: the tile with the least
     // estimate was within 4% of the best one's time on average, 30% at most (16 experts' 4096 x 4096, 64 rows: 153 us,
     // 118 on tiles of 256), over 53 products of 8 to 128 experts with 25 to 1024 rows on average, 704 to 14336 columns
-    // and sums.  By the estimate's own rounds a stage took 0.42 to 0.67, 0.98 to 1.48 and 1.1 to 1.9.  Tiles of 160 rows
-    // were the best by 4% at most (4096 x 4096, 1024 rows: 291, 302 otherwise), and are left to one matrix.
+    // and sums.  By the estimate's own rounds a stage took 0.42 to 0.67, 0.98 to 1.48 and 1.1 to 1.9.  Tiles of 160
+    // rows were the best by 4% at most (4096 x 4096, 1024 rows: 291, 302 otherwise), and are left to one matrix.
     constexpr float kExperts[] = {0.42f, 0.96f, 0.0f, 1.5f};
     constexpr Cost k32[] = {{64, 64, 2, 2.2f, 0.62f, 1.05f}, {128, 128, 2, 2.9f, 2.0f, 3.5f}};
-    // The same of rows that are not aligned.  fp32 by words, 1.01 to 1.2 times the above.  16 bits through registers, of
-    // forward, input and weight (4095 x 4095, aligned 4096 x 4096 in brackets: 256 rows 26.5 (23.5), 2047 rows 99 (63);
-    // rows' gradients 35.5 (29) and 122 (71), weights' 31 (17) and 133 (58).  All rows at addresses of an odd number of
-    // elements cost half as much again as those at multiples of four bytes: 512 rows 70, 44 and, staged but aligned, 37).
+    // The same of rows that are not aligned.  fp32 by words, 1.01 to 1.2 times the above.  16 bits through registers,
+    // of forward, input and weight (4095 x 4095, aligned 4096 x 4096 in brackets: 256 rows 26.5 (23.5), 2047 rows 99
+    // (63); rows' gradients 35.5 (29) and 122 (71), weights' 31 (17) and 133 (58).  All rows at addresses of an odd
+    // number of elements cost half as much again as those at multiples of four bytes: 512 rows 70, 44 and, staged but
+    // aligned, 37).
     constexpr Cost k32Odd[] = {{64, 64, 2, 2.2f, 0.8f, 1.12f}, {128, 128, 2, 2.9f, 2.25f, 3.7f}};
     constexpr Cost k16Odd[][2] = {{{64, 64, 2, 2.2f, 0.4f, 0.74f}, {128, 128, 2, 2.9f, 1.0f, 1.5f}},
                                   {{64, 64, 2, 2.2f, 0.62f, 0.8f}, {128, 128, 2, 2.9f, 1.33f, 1.87f}},
@@ -119,8 +121,8 @@ RowsChoice rows_mm_choose(RowsMode mode, int dtype, int P, int Q, int K, int hal
     return best;
 }
 
-// About four workgroups a CU, two rows a wave at least.  bf16, us with the join: 2048 x 4096 silu 15.9, 4096 x 14336 83,
-// 4096 x 4096 without an activation 9.4; with two a CU 19.5, 133, 11.4; with eight 15.9, 77, 11.7.  Two or four of
+// About four workgroups a CU, two rows a wave at least.  bf16, us with the join: 2048 x 4096 silu 15.9, 4096 x 14336
+// 83, 4096 x 4096 without an activation 9.4; with two a CU 19.5, 133, 11.4; with eight 15.9, 77, 11.7.  Two or four of
 // a wave's rows loaded at once are no faster (two a CU: 19.8 and 20.3, 134 and 137).
 int rows_column_chunks(int T, int N) {
     const int64_t across = ((int64_t)N + kRowsColumns - 1) / kRowsColumns;

@@ -61,7 +61,8 @@ template <class T>
 __device__ __forceinline__ float rows_erfc(float x) {
     if constexpr (sizeof(T) == 4) return erfcf(x);
     const float a = fabsf(x), t = __builtin_amdgcn_rcpf(1.0f + 0.375f * a);
-    constexpr float kP[] = {0.21133944f, 0.21568918f, 0.16666459f, 0.28306147f, -0.12959719f, 0.38793775f, -0.13509588f};
+    constexpr float kP[] = {0.21133944f,  0.21568918f, 0.16666459f, 0.28306147f,
+                            -0.12959719f, 0.38793775f, -0.13509588f};
     float poly = kP[6];
 #pragma unroll
     for (int i = 5; i >= 0; --i) poly = poly * t + kP[i];
@@ -222,10 +223,11 @@ constexpr float kRowsRestScale = 2048.0f;
 constexpr int kRowsColumns = 512;  // of a workgroup
 int rows_column_chunks(int T, int N);
 hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, const void *pre, void *gz, int planes,
-                                    int64_t plane, int dtype, int act, void *sums, bool sums_wide, float *column_part, int T, int N,
-                                    hipStream_t stream);
+                                    int64_t plane, int dtype, int act, void *sums, bool sums_wide,
+                                     float *column_part, int T, int N, hipStream_t stream);
 // grad_gate_up [R][2I] from grad_mid and the saved gate|up, rows below offsets[n_experts].
-hipError_t launch_rows_swiglu_backward(const void *grad_mid, const void *gate_up, void *grad_gate_up, int planes, int64_t plane, int dtype,
-                                       const int32_t *offsets, int n_experts, int I, int R, hipStream_t stream);
+hipError_t launch_rows_swiglu_backward(const void *grad_mid, const void *gate_up, void *grad_gate_up, int planes,
+                                       int64_t plane, int dtype, const int32_t *offsets, int n_experts, int I, int R,
+                                       hipStream_t stream);
 
 }  // namespace jjo

@@ -37,7 +37,8 @@ __global__ __launch_bounds__(512) void rows_direct_kernel(RowsMm p) {
     f32x4v acc[kMats];
 #pragma unroll
     for (int m = 0; m < kMats; ++m) {
-        wrow[m] = (const T *)(m == 0 ? p.p : p.p2) + expert * p.expert_stride + min(p0 + r16, p.P - 1) * p.ldp + q4 * kPiece;
+        const T *const matrix = (const T *)(m == 0 ? p.p : p.p2) + expert * p.expert_stride;
+        wrow[m] = matrix + min(p0 + r16, p.P - 1) * p.ldp + q4 * kPiece;
         acc[m] = f32x4v{0.f, 0.f, 0.f, 0.f};
     }
     const T *const xrow = (const T *)p.q + min(q0 + r16, end - 1) * p.ldq + q4 * kPiece;

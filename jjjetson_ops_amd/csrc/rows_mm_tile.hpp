@@ -236,8 +236,9 @@ __device__ __forceinline__ void rows_dma(uint32_t off, uint64_t from, uint32_t l
 // Workgroups go to the eight XCDs in turn.  Each XCD takes a contiguous run of the tiles, its workgroups
 // neighbours of it, so that tiles that read the same rows are read into one L2; or (tiles of unequal length) the
 // XCDs take turns at chunks of 32, an XCD's workgroups (gradients of 8 experts' 28672 x 4096 matrices, one
-// expert a run: as long as the one with the most tokens, 444 of 2048, 1036 us, 800 to 880 in turn), first to last and last to first, as
-// the experts with the most rows may come first.  A workgroup's places are at, at + step, ... below end.
+// expert a run: as long as the one with the most tokens, 444 of 2048, 1036 us, 800 to 880 in turn), first to last and
+// last to first, as the experts with the most rows may come first.  A workgroup's places are at, at + step, ... below
+// end.
 struct RowsRun {
     int at, step, end, beg, xcd;
     bool chunked;
@@ -384,7 +385,7 @@ struct RowsTiles {
         }
         c.p0 = tile_p * kOutP;
         const int half_stages = (c.length + STEP - 1) / STEP;
-        const int stages = MODE == kRowsInput ? p.halves * half_stages : MODE == kRowsWeight ? p.terms * half_stages : half_stages;
+        const int stages = half_stages * (MODE == kRowsInput ? p.halves : MODE == kRowsWeight ? p.terms : 1);
         c.s_beg = p.slices == 1 ? 0 : (int)((int64_t)stages * c.slice / p.slices);
         c.s_end = p.slices == 1 ? stages : (int)((int64_t)stages * (c.slice + 1) / p.slices);
         if (c.s_beg == c.s_end) c.s_beg = c.s_end = stages;  // a slice without stages: behind the sums' end
@@ -394,8 +395,8 @@ struct RowsTiles {
 };
 
 // Four of them, to places 1 KB apart.  What a stage's requests cost a wave in instructions is a slot of
-// rows_stream_kernel that is longer than the other's products: 8192 cubed 849 us for 861 to 874 with the addresses computed
-// anew for each, gradients of the weights and rows 820 and 842 for 890.
+// rows_stream_kernel that is longer than the other's products: 8192 cubed 849 us for 861 to 874 with the addresses
+// computed anew for each, gradients of the weights and rows 820 and 842 for 890.
 __device__ __forceinline__ void rows_dma4(const uint32_t *off, uint64_t from, uint32_t lds) {
     uint32_t m0v = __builtin_amdgcn_readfirstlane(lds);
     from = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(from >> 32)) << 32 |
@@ -534,7 +535,8 @@ struct RowsSource {
             rows_dma4(off_q, at_q, at + Tile::kStageP + 1024 * OpQ::run(wave, 0));
         } else {
 #pragma unroll
-            for (int n = 0; n < OpQ::kMine; ++n) rows_dma(off_q[n], at_q, at + Tile::kStageP + 1024 * OpQ::run(wave, n));
+            for (int n = 0; n < OpQ::kMine; ++n)
+                rows_dma(off_q[n], at_q, at + Tile::kStageP + 1024 * OpQ::run(wave, n));
         }
         at_q += QT ? 128 * p.ldq : 128;
     }
@@ -570,8 +572,10 @@ struct RowsSource {
         if (s.left >= kStep) {
             if constexpr (MODE == kRowsSwiglu) {
 #pragma unroll
-                for (int n = 0; n < OpP::kMine; ++n)
-                    in_p[n] = load_any<u32x4v>((const uint8_t *)(is_up(8 * OpP::run(wave, n)) ? s.from_up : s.from_p) + off_p[n]);
+                for (int n = 0; n < OpP::kMine; ++n) {
+                    const T *const from = is_up(8 * OpP::run(wave, n)) ? s.from_up : s.from_p;
+                    in_p[n] = load_any<u32x4v>((const uint8_t *)from + off_p[n]);
+                }
             } else {
                 OpP::fetch(in_p, s.from_p, off_p);
             }
@@ -654,9 +658,9 @@ struct RowsSource {
 //
 // The code of every epilogue unrolled over a wave's sums would be 150 KB, more than the instruction cache, and
 // cost a tile of 256 x 256 some 8 us.  So plain outputs (whole groups of eight columns) have a path of
-// their own.  kRowsFull has one for each activation, for whole groups too; kRowsAny takes one row of tiles at a time, in a loop that moves the next one's sums into the same
-// registers (which costs registers that the large tiles do not have).
-// Of weights' gradients kRowsPlain has rows at multiples of 64 bytes, kRowsFull others.
+// their own.  kRowsFull has one for each activation, for whole groups too; kRowsAny takes one row of tiles at a time,
+// in a loop that moves the next one's sums into the same registers (which costs registers that the large tiles do not
+// have). Of weights' gradients kRowsPlain has rows at multiples of 64 bytes, kRowsFull others.
 enum RowsOutput { kRowsPlain, kRowsFull, kRowsAny };
 
 // 16 bytes of a row, values col.. of P, through the caches.  Of 16 bits at an odd place whole words, from the second
@@ -688,8 +692,8 @@ __device__ __forceinline__ void rows_store_line(Out *to, u32x4v v, uint32_t next
 }
 
 template <class T, RowsMode MODE, RowsOutput KIND, class Tile>
-__device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c, f32x4v (&acc)[Tile::RT][Tile::TT], int wp,
-                                            int wq) {
+__device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c, f32x4v (&acc)[Tile::RT][Tile::TT],
+                                            int wp, int wq) {
     constexpr int RT = Tile::RT, TT = Tile::TT;
     constexpr int kWaveP = MODE == kRowsSwiglu ? 8 * RT : 16 * RT;  // columns of a wave
     // Pairs of tiles side by side, or (the small tile's gate and up) of two rows of tiles.
@@ -717,7 +721,8 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
     auto take = [&](int tt, int pair, float *v, float *up) {
         if constexpr (kBeside) {
             rows_exchange(acc[2 * pair][tt], acc[2 * pair + 1][tt], v);
-            if constexpr (MODE == kRowsSwiglu) rows_exchange(acc[RT / 2 + 2 * pair][tt], acc[RT / 2 + 2 * pair + 1][tt], up);
+            if constexpr (MODE == kRowsSwiglu)
+                rows_exchange(acc[RT / 2 + 2 * pair][tt], acc[RT / 2 + 2 * pair + 1][tt], up);
         } else {
             rows_exchange(acc[0][tt], acc[0][tt + 1], v);
             rows_exchange(acc[1][tt], acc[1][tt + 1], up);
@@ -763,12 +768,13 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
         return all(std::integral_constant<int, JJO_ACT_NONE>{});
     }
     // Weights' gradients go past the caches, in whole lines: nothing near reads them, and they would push out what
-    // the tiles beside read (64 experts of 2048 x 1408, 244 tokens each: 160 us, 195 through the caches).  Stores of 64 bytes a row
-    // reach 3.0 to 4.0 TB/s that way, of 128 bytes 5.6 to 6.3, as through the caches.  So lanes 8..15 of each 16
-    // exchange with 0..7: an instruction writes 128 bytes of eight rows.  Rows that do not begin at multiples of 64 bytes
-    // go through the caches, which join the lines that two stores share (64 experts of 2048 x 1408 with 25 rows each, 4
-    // bytes beside: 128 us, past the caches 188; at a multiple 110).  Rows of 16 bits at odd places are written in
-    // whole words but for their ends, each lane taking the next one's first value (odd sizes: 250 us, 302 otherwise).
+    // the tiles beside read (64 experts of 2048 x 1408, 244 tokens each: 160 us, 195 through the caches).  Stores of 64
+    // bytes a row reach 3.0 to 4.0 TB/s that way, of 128 bytes 5.6 to 6.3, as through the caches.  So lanes 8..15 of
+    // each 16 exchange with 0..7: an instruction writes 128 bytes of eight rows.  Rows that do not begin at multiples
+    // of 64 bytes go through the caches, which join the lines that two stores share (64 experts of 2048 x 1408 with 25
+    // rows each, 4 bytes beside: 128 us, past the caches 188; at a multiple 110).  Rows of 16 bits at odd places are
+    // written in whole words but for their ends, each lane taking the next one's first value (odd sizes: 250 us, 302
+    // otherwise).
     if constexpr (MODE == kRowsWeight && RT == 4) {
         const bool high = (lane & 8) != 0;
         auto all = [&](auto past_tag) {
@@ -777,7 +783,8 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
                 using Out = decltype(out);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t x = __builtin_amdgcn_update_dpp(0, high ? a[i] : b[i], 0x128, 0xf, 0xf, false);  // row_ror:8
+                    const uint32_t mine = high ? a[i] : b[i];
+                    const uint32_t x = __builtin_amdgcn_update_dpp(0, mine, 0x128, 0xf, 0xf, false);  // row_ror:8
                     a[i] = high ? x : a[i], b[i] = high ? b[i] : x;
                 }
                 const int in_tile = 16 * (TT * wq + tt) + (r16 & 7);
@@ -790,7 +797,8 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
                     uint32_t next_a = 0, next_b = 0;
                     if constexpr (sizeof(Out) == 2) {  // of the columns' next eight: lanes + 32, then + 16, then + 8
                         const int next = 4 * (upper == 0 ? lane ^ 32 : odd == 0 ? lane ^ 48 : lane ^ 56);
-                        next_a = __builtin_amdgcn_ds_bpermute(next, a[0]), next_b = __builtin_amdgcn_ds_bpermute(next, b[0]);
+                        next_a = __builtin_amdgcn_ds_bpermute(next, a[0]);
+                        next_b = __builtin_amdgcn_ds_bpermute(next, b[0]);
                     }
                     if (in_tile < c.rows_q) rows_store_line(to, a, next_a, col, p.P);
                     if (in_tile + 8 < c.rows_q) rows_store_line(to + 8 * ld, b, next_b, col, p.P);
@@ -816,7 +824,8 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
         if (((uintptr_t)y | (uint64_t)ld * (to32 ? 4 : sizeof(T))) % 64 == 0) return all(std::true_type{});
         return all(std::false_type{});
     }
-    if (KIND != kRowsAny || (p.P % 8 == 0 && (parts || (e.bias == nullptr && e.residual == nullptr && e.pre == nullptr && e.act == JJO_ACT_NONE)))) {
+    const bool bare = e.bias == nullptr && e.residual == nullptr && e.pre == nullptr && e.act == JJO_ACT_NONE;
+    if (KIND != kRowsAny || (p.P % 8 == 0 && (parts || bare))) {
         auto all = [&](auto wide_tag) {
             constexpr bool WIDE = decltype(wide_tag)::value;
             using Out = std::conditional_t<WIDE, float, T>;
@@ -891,9 +900,9 @@ __device__ __forceinline__ void rows_turn(const RowsMm &p, const RowsPlace &c, i
 }
 
 // ---- four waves, a tile a workgroup, two or more workgroups a CU: one stages while another multiplies.
-// Stages that the staged way holds in registers.  bf16, odd K and N, us: tiles of 64, 64 x 4095 over 4095 with one 18.0,
-// with three 15.9 (of four waves their loads are most of what a CU waits for); tiles of 128, 2047 rows, forward 98 with
-// one and 109 with two, rows' gradients 128 and 123, weights' 136 and 136.
+// Stages that the staged way holds in registers.  bf16, odd K and N, us: tiles of 64, 64 x 4095 over 4095 with one
+// 18.0, with three 15.9 (of four waves their loads are most of what a CU waits for); tiles of 128, 2047 rows, forward
+// 98 with one and 109 with two, rows' gradients 128 and 123, weights' 136 and 136.
 template <RowsMode MODE, int RT>
 constexpr int kRowsHeld = RT == 2 ? 3 : MODE == kRowsInput ? 2 : 1;
 template <class E, RowsMode MODE, class Tile, RowsWay WAY>
@@ -984,7 +993,8 @@ __global__ __launch_bounds__(Tile::kThreads) void rows_mm_kernel(RowsMm p, int m
         for (int st = c.s_beg; st < c.s_end; ++st) {
             // Stage st has landed, and no wave reads the buffer of stage st - 1 any more.
             if (st + kAhead - 1 < c.s_end)
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((kAhead - 1) * Source::kDma) : "memory");
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((kAhead - 1) * Source::kDma)
+                             : "memory");
             else
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (st + kAhead < c.s_end)
@@ -1161,7 +1171,8 @@ hipError_t run_rows(RowsMm p, hipStream_t stream) {
         const int wgs = (int)std::min<int64_t>(blocks, device_cu_count());
         const RowsEpilogue &e = p.epi;
         if constexpr (MODE == kRowsForward || MODE == kRowsSwiglu)
-            if (p.slices == 1 && (e.bias != nullptr || e.residual != nullptr || e.pre != nullptr || e.act != JJO_ACT_NONE))
+            if (p.slices == 1 &&
+                (e.bias != nullptr || e.residual != nullptr || e.pre != nullptr || e.act != JJO_ACT_NONE))
                 return go(rows_stream_kernel<E, MODE, kRowsFull, Tile>, wgs);
         if constexpr (MODE == kRowsWeight) {
             const int es = p.wide ? 4 : (int)sizeof(typename E::type);
@@ -1202,7 +1213,8 @@ hipError_t rows_by_tile(const RowsMm &p, int tile, hipStream_t stream) {
         // The large tiles write whole groups of eight columns.
         if (tile == kRowsTile256 && p.P % 8 == 0) return run_rows<E, MODE, RowsTile<4, 8, 4, 2>, kRowsDma>(p, stream);
         if constexpr (MODE == kRowsForward || MODE == kRowsInput)
-            if (tile == kRowsTile160 && p.P % 8 == 0) return run_rows<E, MODE, RowsTile<4, 5, 4, 2, 3>, kRowsDma>(p, stream);
+            if (tile == kRowsTile160 && p.P % 8 == 0)
+                return run_rows<E, MODE, RowsTile<4, 5, 4, 2, 3>, kRowsDma>(p, stream);
     }
     return run_rows<E, MODE, RowsTile<4, 4, 2, 2>, kRowsDma>(p, stream);
 }

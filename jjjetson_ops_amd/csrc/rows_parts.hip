@@ -72,7 +72,8 @@ __global__ __launch_bounds__(256) void rows_act_backward_kernel(const void *grad
     __shared__ float sums[4][kColumnsAtOnce];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = blockIdx.x * kColumnsAtOnce + 8 * lane, n = min(8, N - col);
-    const int beg = (int)((int64_t)T_ * blockIdx.y / gridDim.y), end = (int)((int64_t)T_ * (blockIdx.y + 1) / gridDim.y);
+    const int beg = (int)((int64_t)T_ * blockIdx.y / gridDim.y);
+    const int end = (int)((int64_t)T_ * (blockIdx.y + 1) / gridDim.y);
     float total[8] = {};
     if (n > 0)
         for (int t = beg + wave; t < end; t += 4) {
@@ -146,7 +147,8 @@ bool grid_of(int64_t threads, dim3 *grid) {
 }  // namespace
 
 hipError_t launch_rows_mm(RowsMode mode, int dtype, const RowsMm &p, hipStream_t stream, const RowsChoice *pinned) {
-    const RowsChoice c = pinned != nullptr ? *pinned : rows_mm_choose(mode, dtype, p.P, p.Q, p.K, p.halves, p.n_experts);
+    const RowsChoice c =
+        pinned != nullptr ? *pinned : rows_mm_choose(mode, dtype, p.P, p.Q, p.K, p.halves, p.n_experts);
     if (c.slices != p.slices) return hipErrorInvalidValue;
     const hipError_t e = mx_by_dtype(dtype, [&](auto tag) {
         return rows_mm_run<decltype(tag)>(mode, p, c, stream);
@@ -171,29 +173,31 @@ hipError_t launch_rows_mm(RowsMode mode, int dtype, const RowsMm &p, hipStream_t
 }
 
 hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, const void *pre, void *gz, int planes,
-                                    int64_t plane, int dtype, int act, void *sums, bool sums_wide, float *column_part, int T, int N,
-                                    hipStream_t stream) {
+                                    int64_t plane, int dtype, int act, void *sums, bool sums_wide,
+                                     float *column_part, int T, int N, hipStream_t stream) {
     const int chunks = rows_column_chunks(T, N);
     const dim3 grid((unsigned)((N + (int64_t)kColumnsAtOnce - 1) / kColumnsAtOnce), (unsigned)chunks);
     float *const part = sums != nullptr ? column_part : nullptr;
     return mx_by_dtype(dtype, [&](auto tag) {
         using E = decltype(tag);
         typedef typename E::type V;
-        hipLaunchKernelGGL(rows_act_backward_kernel<E>, grid, dim3(256), 0, stream, grad_y, grad_y_stride, pre, gz, planes,
-                           plane, act, part, T, N);
+        hipLaunchKernelGGL(rows_act_backward_kernel<E>, grid, dim3(256), 0, stream, grad_y, grad_y_stride, pre, gz,
+                           planes, plane, act, part, T, N);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess || sums == nullptr) return e;
         const dim3 join((unsigned)((N + 63LL) / 64));
         if (sums_wide)
-            hipLaunchKernelGGL(rows_column_join_kernel<float>, join, dim3(256), 0, stream, part, chunks, N, (float *)sums);
+            hipLaunchKernelGGL(rows_column_join_kernel<float>, join, dim3(256), 0, stream, part, chunks, N,
+                               (float *)sums);
         else
             hipLaunchKernelGGL(rows_column_join_kernel<V>, join, dim3(256), 0, stream, part, chunks, N, (V *)sums);
         return hipGetLastError();
     });
 }
 
-hipError_t launch_rows_swiglu_backward(const void *grad_mid, const void *gate_up, void *grad_gate_up, int planes, int64_t plane, int dtype,
-                                       const int32_t *offsets, int n_experts, int I, int R, hipStream_t stream) {
+hipError_t launch_rows_swiglu_backward(const void *grad_mid, const void *gate_up, void *grad_gate_up, int planes,
+                                       int64_t plane, int dtype, const int32_t *offsets, int n_experts, int I, int R,
+                                       hipStream_t stream) {
     const int chunks = (I + 7) / 8;
     dim3 grid;
     if (!grid_of((int64_t)R * chunks, &grid)) return hipErrorInvalidConfiguration;
