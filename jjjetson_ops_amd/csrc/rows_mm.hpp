@@ -224,7 +224,7 @@ constexpr int kRowsColumns = 512;  // of a workgroup
 int rows_column_chunks(int T, int N);
 hipError_t launch_rows_act_backward(const void *grad_y, int64_t grad_y_stride, const void *pre, void *gz, int planes,
                                     int64_t plane, int dtype, int act, void *sums, bool sums_wide,
-                                     float *column_part, int T, int N, hipStream_t stream);
+                                    float *column_part, int T, int N, hipStream_t stream);
 // grad_gate_up [R][2I] from grad_mid and the saved gate|up, rows below offsets[n_experts].
 hipError_t launch_rows_swiglu_backward(const void *grad_mid, const void *gate_up, void *grad_gate_up, int planes,
                                        int64_t plane, int dtype, const int32_t *offsets, int n_experts, int I, int R,

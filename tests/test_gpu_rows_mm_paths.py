@@ -374,3 +374,23 @@ def test_rows_far_apart(dev, name):
         ws = R.workspace(capi.linear_rows_backward_workspace_bytes(CODES[name], K, N, T))
         capi.linear_rows_backward(g, x, None, None, gw, None, K, N, T, ws=ws)
         R.check(gw, *R.mm(g.t(), x.t()), "grad_w")
+
+
+@pytest.mark.parametrize("K,N,T", [(4104, 2056, 100), (4096, 2048, 100), (4104, 4104, 60), (1408, 520, 40)])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+def test_weights_gradients_at_any_place(dev, name, wide, K, N, T):
+    """Outputs of the large tiles at places of one element after the other, aligned operands: the same bits as aligned, and
+    nothing beside them is written."""
+    d = R.DTYPES[name]
+    gd = torch.float32 if wide else d
+    x, g, pre = R.randn(1, T, K, dtype=d), R.randn(2, T, N, dtype=d), R.randn(3, T, N, dtype=d)
+    ws = R.workspace(capi.linear_rows_backward_workspace_bytes(CODES[name], K, N, T))
+    want = torch.empty(N, K, dtype=gd, device="cuda")
+    capi.linear_rows_backward(g, x, None, None, want, None, K, N, T, activation=capi.ACT_RELU, pre=pre, ws=ws)
+    for at in (1, 2, 3, 8, 32):
+        buf = torch.full((N * K + 64,), 7.0, dtype=gd, device="cuda")
+        capi.linear_rows_backward(g, x, None, None, buf[at:at + N * K].view(N, K), None, K, N, T, activation=capi.ACT_RELU, pre=pre,
+                                  ws=ws)
+        assert torch.equal(buf[at:at + N * K].view(N, K), want)
+        assert (buf[:at] == 7.0).all() and (buf[at + N * K:] == 7.0).all()
