@@ -663,32 +663,34 @@ struct RowsSource {
 // have). Of weights' gradients kRowsPlain has rows at multiples of 64 bytes, kRowsFull others.
 enum RowsOutput { kRowsPlain, kRowsFull, kRowsAny };
 
-// 16 bytes of a row, values col.. of P, through the caches.  Of 16 bits at an odd place whole words, from the second
-// value on: `next` holds the first of the lane with the columns behind, which lanes 56 and up have not.
+// 16 bytes of a row, values col.. of P, through the caches.
 template <class Out>
-__device__ __forceinline__ void rows_store_line(Out *to, u32x4v v, uint32_t next, int col, int P) {
+__device__ __forceinline__ void rows_store_line(Out *to, u32x4v v, int col, int P) {
     constexpr int kN = 16 / sizeof(Out);
-    const int lane = threadIdx.x & 63;
     const MxVec<Out, kN> e = __builtin_bit_cast(MxVec<Out, kN>, v);
-    if (col + kN > P) {
+    if (col + kN <= P) return store_any(to, v);
 #pragma unroll
-        for (int i = 0; i < kN - 1; ++i)
-            if (col + i < P) to[i] = e.v[i];
-    } else if (sizeof(Out) == 4 || (uintptr_t)to % 4 == 0) {
-        store_any(to, v);
+    for (int i = 0; i < kN - 1; ++i)
+        if (col + i < P) to[i] = e.v[i];
+}
+// The same of 16 bits where some rows are at odd places, those in whole words from the second value on: `next` holds the
+// first of the lane with the columns behind, which lanes 56 and up have not.
+template <class Out>
+__device__ __forceinline__ void rows_store_words(Out *to, u32x4v v, uint32_t next, int col, int P) {
+    if ((uintptr_t)to % 4 == 0 || col + 8 > P) return rows_store_line(to, v, col, P);
+    typedef uint32_t Words3 __attribute__((ext_vector_type(3), aligned(4)));
+    typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(4)));
+    const int lane = threadIdx.x & 63;
+    const MxVec<Out, 8> e = __builtin_bit_cast(MxVec<Out, 8>, v);
+    const uint32_t w[4] = {v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16,
+                           v[3] >> 16 | next << 16};
+    if (lane < 56 && col + 8 < P) {
+        *(Words4 *)(to + 1) = Words4{w[0], w[1], w[2], w[3]};
     } else {
-        typedef uint32_t Words3 __attribute__((ext_vector_type(3), aligned(4)));
-        typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(4)));
-        const uint32_t w[4] = {v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16,
-                               v[3] >> 16 | next << 16};
-        if (lane < 56 && col + kN < P) {
-            *(Words4 *)(to + 1) = Words4{w[0], w[1], w[2], w[3]};
-        } else {
-            *(Words3 *)(to + 1) = Words3{w[0], w[1], w[2]};
-            to[kN - 1] = e.v[kN - 1];
-        }
-        if (lane < 8) to[0] = e.v[0];
+        *(Words3 *)(to + 1) = Words3{w[0], w[1], w[2]};
+        to[7] = e.v[7];
     }
+    if (lane < 8) to[0] = e.v[0];
 }
 
 template <class T, RowsMode MODE, RowsOutput KIND, class Tile>
@@ -773,8 +775,8 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
     // each 16 exchange with 0..7: an instruction writes 128 bytes of eight rows.  Rows that do not begin at multiples
     // of 64 bytes go through the caches, which join the lines that two stores share (64 experts of 2048 x 1408 with 25
     // rows each, 4 bytes beside: 128 us, past the caches 188; at a multiple 110).  Rows of 16 bits at odd places are
-    // written in whole words but for their ends, each lane taking the next one's first value (odd sizes: 250 us, 302
-    // otherwise).
+    // written in whole words but for their ends, each lane taking the next one's first value (2 bytes beside: 172 us,
+    // 217 otherwise).
     if constexpr (MODE == kRowsWeight && RT == 4) {
         const bool high = (lane & 8) != 0;
         auto all = [&](auto past_tag) {
@@ -794,14 +796,19 @@ __device__ __forceinline__ void rows_output(const RowsMm &p, const RowsPlace &c,
                     if (in_tile < c.rows_q) rows_store_past(to, a);
                     if (in_tile + 8 < c.rows_q) rows_store_past(to + 8 * ld, b);
                 } else {
-                    uint32_t next_a = 0, next_b = 0;
-                    if constexpr (sizeof(Out) == 2) {  // of the columns' next eight: lanes + 32, then + 16, then + 8
-                        const int next = 4 * (upper == 0 ? lane ^ 32 : odd == 0 ? lane ^ 48 : lane ^ 56);
-                        next_a = __builtin_amdgcn_ds_bpermute(next, a[0]);
-                        next_b = __builtin_amdgcn_ds_bpermute(next, b[0]);
+                    if constexpr (sizeof(Out) == 2) {
+                        if (((uintptr_t)y | (uint64_t)ld * 2) % 4 != 0) {
+                            // The next eight columns are those of the lane + 32, then + 16, then + 8.
+                            const int next = 4 * (upper == 0 ? lane ^ 32 : odd == 0 ? lane ^ 48 : lane ^ 56);
+                            const uint32_t next_a = __builtin_amdgcn_ds_bpermute(next, a[0]);
+                            const uint32_t next_b = __builtin_amdgcn_ds_bpermute(next, b[0]);
+                            if (in_tile < c.rows_q) rows_store_words(to, a, next_a, col, p.P);
+                            if (in_tile + 8 < c.rows_q) rows_store_words(to + 8 * ld, b, next_b, col, p.P);
+                            return;
+                        }
                     }
-                    if (in_tile < c.rows_q) rows_store_line(to, a, next_a, col, p.P);
-                    if (in_tile + 8 < c.rows_q) rows_store_line(to + 8 * ld, b, next_b, col, p.P);
+                    if (in_tile < c.rows_q) rows_store_line(to, a, col, p.P);
+                    if (in_tile + 8 < c.rows_q) rows_store_line(to + 8 * ld, b, col, p.P);
                 }
             };
 #pragma unroll
