@@ -661,7 +661,7 @@ struct RowsSource {
 // cost a tile of 256 x 256 some 8 us.  So plain outputs (whole groups of eight columns) have a path of
 // their own.  kRowsFull has one for each activation, for whole groups too; kRowsAny takes one row of tiles at a time,
 // in a loop that moves the next one's sums into the same registers (which costs registers that the large tiles do not
-// have). Of weights' gradients kRowsPlain has rows at multiples of 64 bytes, kRowsFull others.
+// have).  Of weights' gradients kRowsPlain has rows at multiples of 64 bytes, kRowsFull others.
 enum RowsOutput { kRowsPlain, kRowsFull, kRowsAny };
 
 // 16 bytes of a row, values col.. of P, through the caches.
